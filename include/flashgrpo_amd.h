@@ -225,6 +225,40 @@ int fg_linear_rope_kv_write(const void* x, int64_t ldx, const void* w_pairs, int
                             int64_t cache_head_stride, int capacity, const int32_t* row_map, int32_t* err_flag,
                             void* stream);
 
+/* Microscaled (MX) rows. A [rows, cols] matrix (cols a multiple of 32) is held as codes, format 0: e4m3, one byte
+ * each, [rows, cols]; 1: e2m1, two to a byte (the earlier element in the low half), [rows, cols / 2]; and scales,
+ * bytes [ceil(cols / 128)][rows][4]: the block of elements 32 b .. 32 b + 31 of a row has the factor 2^(s - 127),
+ * s = scales[b / 4][row][b % 4] (255: the block is NaN; bytes behind the last block are written 0). Codes 16-byte
+ * and scales 4-byte aligned, both contiguous. No counterpart in the reference: 4-bit weights for the decoder MLP.
+ *
+ * fg_mx_quantize: x [rows, cols] (row stride ldx, a multiple of 8; dtype fp32 or bf16) to codes and scales. A block's
+ * scale is the smallest power of two >= 2^-126 that holds its largest magnitude without saturation (448 for e4m3, 6
+ * for e2m1), codes are rounded to nearest, ties to even; a block with an infinity or a NaN becomes NaN.
+ * fg_mx_dequantize: the values, in fp32 or bf16 (row stride ldo, a multiple of 8). */
+int fg_mx_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, int format, void* codes, void* scales,
+                   void* stream);
+int fg_mx_dequantize(const void* codes, const void* scales, int format, int rows, int cols, void* out, int dtype,
+                     int64_t ldo, void* stream);
+
+/* fg_rmsnorm with an MX e4m3 output: s = x (+ delta, rounded to the row dtype and written to sum, which may be x),
+ * MX of s * rsqrt(mean(s^2) + eps) * weight, not rounded in between. x, delta, sum [rows, hidden] and weight contiguous,
+ * in one dtype; delta NULL: sum is not written. hidden a multiple of 32, at most 8192. */
+int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* sum, int dtype, int rows, int hidden,
+                  float eps, void* codes, void* scales, void* stream);
+
+/* out = bf16(x . w^T (+ bias) (+ residual)): MX rows x [rows, hidden] (x_format 0 or 1) times an MX e2m1 weight w
+ * [cols, hidden], fp32 sums rounded once; bias [cols], residual [rows, cols] (row stride ldr) and out (row stride ldo)
+ * bf16; out may be the residual. hidden a multiple of 32; operands under 2 GiB each. */
+int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const void* w_codes, const void* w_scales,
+                 int rows, int cols, int hidden, const void* bias, const void* residual, int64_t ldr, void* out,
+                 int64_t ldo, void* stream);
+
+/* MX e4m3 [rows, inter] of SiLU(x . w[:inter]^T) * (x . w[inter:]^T), in fp32 up to the codes: x as for fg_mx_linear,
+ * w [2 * inter, hidden] MX e2m1 (gate rows, then up rows), inter a multiple of 32. */
+int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format, const void* w_codes,
+                         const void* w_scales, int rows, int inter, int hidden, void* codes, void* scales,
+                         void* stream);
+
 /* dst[i] = src[i] (bytes[i] bytes, a positive multiple of 4, 4-byte aligned device addresses, no
  * overlaps) for i < count <= 8, in one launch; src, dst and bytes are host arrays. No counterpart in the
  * reference: it brings a captured verify forward's inputs into the graph's static buffers. */

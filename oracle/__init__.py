@@ -24,6 +24,8 @@ Modules and the reference code each follows:
                           the decoder arithmetic itself lives in transformers 4.49)
 * ``oracle.decode``    -- one verify step and the generate loop
                           (``flashgrpo/decoding/flash_medusa_decoder.py:550-1166``)
+* ``oracle.mx``        -- microscaled rows: quantisation, values, RMSNorm and the gated MLP input (no
+                          counterpart in the reference)
 
 How each function is pinned (golden vectors, known answers, closed forms,
 library cross-checks) is listed in ``tests/test_oracle_*.py``.

@@ -1,0 +1,254 @@
+// Microscaled rows (fg_mx.h): quantisation, the values they stand for, and the RMSNorm whose output is MX e4m3.
+//
+// All three move each element once and are bound by HBM: a row is read as 16-byte (bf16) or 32-byte (fp32) pieces of
+// eight elements per lane, four lanes hold a block, sixteen a dword of scales.
+#include "fg_mx.h"
+
+namespace {
+
+// A workgroup takes 16 rows x 512 columns: 16 lanes per row, four steps of 128 columns each, whose loads are all
+// issued first. 16 rows, because the scale dwords of a step are neighbours along the rows: 64 bytes per store
+// instruction of the workgroup instead of 4 scattered ones.
+constexpr int kTileRows = 16, kTileSteps = 4;
+
+template <int DT, int FMT>
+__global__ void __launch_bounds__(256) mx_quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int cols,
+                                                          int steps, int step_tiles, uint8_t* __restrict__ codes,
+                                                          uint32_t* __restrict__ scales) {
+  const int rt = blockIdx.x / step_tiles, st = blockIdx.x - rt * step_tiles;
+  const int l = threadIdx.x & 15;
+  const int row = rt * kTileRows + (threadIdx.x >> 4);
+  const bool row_ok = row < rows;
+  float v[kTileSteps][8];
+#pragma unroll
+  for (int u = 0; u < kTileSteps; ++u) {
+    const int col = (st * kTileSteps + u) * fg::kMxStep + l * 8;
+    if (row_ok && col < cols) {
+      fg::load8<DT>(x, (int64_t)row * ldx + col, v[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kTileSteps; ++u) {
+    const int step = st * kTileSteps + u, col = step * fg::kMxStep + l * 8;
+    if (step >= steps) break;  // for the whole workgroup
+    const int64_t at = (int64_t)row * cols + col;
+    fg::mx_store_step<FMT>(v[u], col < cols, l, codes + (FMT == fg::kE4M3 ? at : at / 2),
+                           scales + (int64_t)step * rows + row, row_ok);
+  }
+}
+
+template <int DT, int FMT>
+__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ codes,
+                                                            const uint8_t* __restrict__ scales, int rows, int cols,
+                                                            int step_tiles, void* __restrict__ out, int64_t ldo) {
+  const int rt = blockIdx.x / step_tiles, st = blockIdx.x - rt * step_tiles;
+  const int l = threadIdx.x & 15;
+  const int row = rt * kTileRows + (threadIdx.x >> 4);
+  if (row >= rows) return;
+  uint2 c[kTileSteps];
+  uint32_t s[kTileSteps];
+#pragma unroll
+  for (int u = 0; u < kTileSteps; ++u) {
+    const int step = st * kTileSteps + u, col = step * fg::kMxStep + l * 8;
+    c[u] = make_uint2(0u, 0u);
+    s[u] = 0;
+    if (col < cols) {
+      const int64_t at = (int64_t)row * cols + col;
+      if constexpr (FMT == fg::kE4M3)
+        c[u] = *(const uint2*)(codes + at);
+      else
+        c[u].x = *(const uint32_t*)(codes + at / 2);
+      s[u] = scales[((int64_t)step * rows + row) * 4 + (l >> 2)];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kTileSteps; ++u) {
+    const int col = (st * kTileSteps + u) * fg::kMxStep + l * 8;
+    if (col >= cols) continue;
+    float v[8];
+    if constexpr (FMT == fg::kE4M3) {
+      const fg::f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(c[u].x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(c[u].x, true);
+      const fg::f32x2_t d = __builtin_amdgcn_cvt_pk_f32_fp8(c[u].y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8(c[u].y, true);
+      v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+      v[4] = d.x; v[5] = d.y; v[6] = e.x; v[7] = e.y;
+    } else {
+      const fg::f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u].x, 1.0f, 0);
+      const fg::f32x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u].x, 1.0f, 1);
+      const fg::f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u].x, 1.0f, 2);
+      const fg::f32x2_t e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u].x, 1.0f, 3);
+      v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+      v[4] = d.x; v[5] = d.y; v[6] = e.x; v[7] = e.y;
+    }
+    const float f = fg::mx_scale(s[u]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+    fg::store8<DT>(out, (int64_t)row * ldo + col, v);
+  }
+}
+
+// A double as the float next to it towards zero, with the last bit set where the float is not the double ("round to
+// odd"): a later rounding to fewer bits then gives what rounding the double at once would give, ties included.
+FG_DEVICE float round_odd(double d) {
+  const float f = (float)d;
+  const double r = d - (double)f;
+  uint32_t b = __float_as_uint(f);
+  if (r != 0.0 && (b & 0x7fffffffu) != 0u && (b & 0x7fffffffu) < 0x7f800000u) {
+    b -= (r < 0.0) != (f < 0.0f) ? 1u : 0u;  // back towards zero
+    b |= 1u;
+  }
+  return __uint_as_float(b);
+}
+
+FG_DEVICE double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    v += __longlong_as_double((long long)fg::shfl_xor_u64((uint64_t)__double_as_longlong(v), o));
+  return v;
+}
+
+// s = x + delta (rounded to the row type, written to sum), y = s * rsqrt(mean(s^2) + eps) * w, MX e4m3 of y. One
+// workgroup per row, which stays in registers between the two passes. The sum of squares and y are held in 64 bits
+// (bf16 products are exact there, and so is their sum to 2^-50): an 8-bit code has a rounding border every 1/8 of a
+// value, and with y in 32 bits one value in a million falls on another side of it than the definition's.
+template <int DT, int CHUNKS>
+__global__ void __launch_bounds__(256) rmsnorm_mx_kernel(const void* x, const void* __restrict__ delta,
+                                                         const void* __restrict__ w, void* sum, int rows, int H,
+                                                         float eps, uint8_t* __restrict__ codes,
+                                                         uint32_t* __restrict__ scales) {
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, nch = H / 8;
+  __shared__ double red[4];
+  float v[CHUNKS][8];
+  double ss = 0.0;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = tid + c * 256;
+    if (ch < nch) {
+      fg::load8<DT>(x, row * H + ch * 8, v[c]);
+      if (delta) {
+        float d[8];
+        fg::load8<DT>(delta, row * H + ch * 8, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] = DT == fg::kBF16 ? fg::round_bf16(v[c][j] + d[j]) : v[c][j] + d[j];
+        fg::store8<DT>(sum, row * H + ch * 8, v[c]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += (double)v[c][j] * (double)v[c][j];
+    }
+  }
+  ss = wave_sum(ss);
+  if ((tid & 63) == 0) red[tid >> 6] = ss;
+  __syncthreads();
+  const double rs = rsqrt((red[0] + red[1] + red[2] + red[3]) / (double)H + (double)eps);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int ch = tid + c * 256;
+    if (c * 256 * 8 >= H) break;  // for the whole workgroup
+    float wv[8], y[8];
+    const bool valid = ch < nch;
+    if (valid) {
+      fg::load8<DT>(w, ch * 8, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = round_odd((double)v[c][j] * (double)wv[j] * rs);
+    }
+    const int step = ch / 16;
+    fg::mx_store_step<fg::kE4M3>(y, valid, ch & 15, codes + row * H + ch * 8,
+                                 scales + (int64_t)step * rows + row, (ch & ~15) < nch);
+  }
+}
+
+template <int DT>
+void launch_norm(const void* x, const void* delta, const void* w, void* sum, int rows, int H, float eps, uint8_t* codes,
+                 uint32_t* scales, hipStream_t s) {
+  if (H <= 2048)
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 1>), dim3(rows), dim3(256), 0, s, x, delta, w, sum, rows, H, eps, codes, scales);
+  else if (H <= 4096)
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 2>), dim3(rows), dim3(256), 0, s, x, delta, w, sum, rows, H, eps, codes, scales);
+  else
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 4>), dim3(rows), dim3(256), 0, s, x, delta, w, sum, rows, H, eps, codes, scales);
+}
+
+int64_t tiles_of(int rows, int cols, int* steps, int* step_tiles) {
+  *steps = (cols + fg::kMxStep - 1) / fg::kMxStep;
+  *step_tiles = (*steps + kTileSteps - 1) / kTileSteps;
+  return (int64_t)((rows + kTileRows - 1) / kTileRows) * *step_tiles;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fg_mx_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, int format, void* codes, void* scales,
+                   void* stream) {
+  FG_REQUIRE(x && codes && scales, "fg_mx_quantize: null pointer");
+  FG_REQUIRE(dtype == fg::kF32 || dtype == fg::kBF16, "fg_mx_quantize: bad dtype");
+  FG_REQUIRE(format == fg::kE4M3 || format == fg::kE2M1, "fg_mx_quantize: bad format");
+  FG_REQUIRE(rows > 0 && cols > 0 && ldx >= cols, "fg_mx_quantize: bad shape");
+  FG_REQUIRE(cols % fg::kMxBlock == 0, "fg_mx_quantize: columns must be a multiple of 32");
+  FG_REQUIRE(ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)codes) & 15) == 0 && ((uintptr_t)scales & 3) == 0,
+             "fg_mx_quantize: rows must start 16-byte aligned, scales 4-byte aligned");
+  int steps, st;
+  const int64_t tiles = tiles_of(rows, cols, &steps, &st);
+  FG_REQUIRE(tiles < (1ll << 31), "fg_mx_quantize: bad shape (too many elements for one call)");
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 g((unsigned)tiles), b(256);
+  uint8_t* c = (uint8_t*)codes;
+  uint32_t* sc = (uint32_t*)scales;
+  if (dtype == fg::kBF16 && format == fg::kE4M3)
+    hipLaunchKernelGGL((mx_quantize_kernel<fg::kBF16, fg::kE4M3>), g, b, 0, s, x, ldx, rows, cols, steps, st, c, sc);
+  else if (dtype == fg::kBF16)
+    hipLaunchKernelGGL((mx_quantize_kernel<fg::kBF16, fg::kE2M1>), g, b, 0, s, x, ldx, rows, cols, steps, st, c, sc);
+  else if (format == fg::kE4M3)
+    hipLaunchKernelGGL((mx_quantize_kernel<fg::kF32, fg::kE4M3>), g, b, 0, s, x, ldx, rows, cols, steps, st, c, sc);
+  else
+    hipLaunchKernelGGL((mx_quantize_kernel<fg::kF32, fg::kE2M1>), g, b, 0, s, x, ldx, rows, cols, steps, st, c, sc);
+  return fg::check_launch("fg_mx_quantize");
+}
+
+int fg_mx_dequantize(const void* codes, const void* scales, int format, int rows, int cols, void* out, int dtype,
+                     int64_t ldo, void* stream) {
+  FG_REQUIRE(codes && scales && out, "fg_mx_dequantize: null pointer");
+  FG_REQUIRE(dtype == fg::kF32 || dtype == fg::kBF16, "fg_mx_dequantize: bad dtype");
+  FG_REQUIRE(format == fg::kE4M3 || format == fg::kE2M1, "fg_mx_dequantize: bad format");
+  FG_REQUIRE(rows > 0 && cols > 0 && ldo >= cols, "fg_mx_dequantize: bad shape");
+  FG_REQUIRE(cols % fg::kMxBlock == 0, "fg_mx_dequantize: columns must be a multiple of 32");
+  FG_REQUIRE(ldo % 8 == 0 && (((uintptr_t)out | (uintptr_t)codes) & 15) == 0 && ((uintptr_t)scales & 3) == 0,
+             "fg_mx_dequantize: rows must start 16-byte aligned, scales 4-byte aligned");
+  int steps, st;
+  const int64_t tiles = tiles_of(rows, cols, &steps, &st);
+  FG_REQUIRE(tiles < (1ll << 31), "fg_mx_dequantize: bad shape (too many elements for one call)");
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 g((unsigned)tiles), b(256);
+  const uint8_t *c = (const uint8_t*)codes, *sc = (const uint8_t*)scales;
+  if (dtype == fg::kBF16 && format == fg::kE4M3)
+    hipLaunchKernelGGL((mx_dequantize_kernel<fg::kBF16, fg::kE4M3>), g, b, 0, s, c, sc, rows, cols, st, out, ldo);
+  else if (dtype == fg::kBF16)
+    hipLaunchKernelGGL((mx_dequantize_kernel<fg::kBF16, fg::kE2M1>), g, b, 0, s, c, sc, rows, cols, st, out, ldo);
+  else if (format == fg::kE4M3)
+    hipLaunchKernelGGL((mx_dequantize_kernel<fg::kF32, fg::kE4M3>), g, b, 0, s, c, sc, rows, cols, st, out, ldo);
+  else
+    hipLaunchKernelGGL((mx_dequantize_kernel<fg::kF32, fg::kE2M1>), g, b, 0, s, c, sc, rows, cols, st, out, ldo);
+  return fg::check_launch("fg_mx_dequantize");
+}
+
+int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* sum, int dtype, int rows, int hidden,
+                  float eps, void* codes, void* scales, void* stream) {
+  FG_REQUIRE(x && weight && codes && scales && (!delta || sum), "fg_rmsnorm_mx: null pointer");
+  FG_REQUIRE(dtype == fg::kF32 || dtype == fg::kBF16, "fg_rmsnorm_mx: bad dtype");
+  FG_REQUIRE(rows > 0 && hidden > 0, "fg_rmsnorm_mx: bad shape");
+  FG_REQUIRE(hidden % fg::kMxBlock == 0 && hidden <= 8192,
+             "fg_rmsnorm_mx: hidden must be a multiple of 32, at most 8192");
+  FG_REQUIRE((((uintptr_t)x | (uintptr_t)delta | (uintptr_t)weight | (uintptr_t)sum | (uintptr_t)codes) & 15) == 0 &&
+                 ((uintptr_t)scales & 3) == 0,
+             "fg_rmsnorm_mx: rows must start 16-byte aligned, scales 4-byte aligned");
+  if (dtype == fg::kBF16)
+    launch_norm<fg::kBF16>(x, delta, weight, sum, rows, hidden, eps, (uint8_t*)codes, (uint32_t*)scales, (hipStream_t)stream);
+  else
+    launch_norm<fg::kF32>(x, delta, weight, sum, rows, hidden, eps, (uint8_t*)codes, (uint32_t*)scales, (hipStream_t)stream);
+  return fg::check_launch("fg_rmsnorm_mx");
+}
+
+}  // extern "C"

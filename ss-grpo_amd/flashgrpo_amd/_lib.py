@@ -55,6 +55,11 @@ SIGNATURES = {
     "fg_rope_cos_sin": (_I, [_P, _P, _I64, _P, _I, _I, _I, _P, _P]),
     "fg_linear_rope_kv_write": (_I, [_P, _I64, _P, _I64, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P,
                                     _P, _P, _P, _I64, _I64, _I, _P, _P, _P]),
+    "fg_mx_quantize": (_I, [_P, _I, _I64, _I, _I, _I, _P, _P, _P]),
+    "fg_mx_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _I, _I64, _P]),
+    "fg_rmsnorm_mx": (_I, [_P, _P, _P, _P, _I, _I, _I, _F, _P, _P, _P]),
+    "fg_mx_linear": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _I64, _P, _I64, _P]),
+    "fg_mx_gate_up_swiglu": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P]),
     "fg_sample_workspace": (_SZ, [_I]),
     "fg_sample_tokens": (_I, [_P, _I, _I64, _I, _I, _P, _P, _P, _I, _I, _U64, _U64, _P, _I, _F, _I, _I, _U32, _P,
                               _P, _SZ, _P]),

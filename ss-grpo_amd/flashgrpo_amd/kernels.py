@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -686,6 +687,192 @@ def linear_rope_kv_write(x, w_pairs, bias_pairs, *, tile=(64, 64), stages=0, bat
           x.shape[0], x.shape[1], tm, tn, int(stages), batch, num_nodes, q_heads, kv_heads, head_dim, _ptr(seq_len),
           _ptr(cos_sin), _ptr(q_out), _ptr(k_cache), _ptr(v_cache), k_cache.stride(0), k_cache.stride(1),
           k_cache.shape[-2], _ptr(row_map), _ptr(err_flag), _stream())
+
+
+# ------------------------------------------------------------------ microscaled (MX) rows
+MX_BLOCK = 32                         # elements per scale
+MX_FORMATS = {"e4m3": 0, "e2m1": 1}   # fg_mx_quantize's format codes
+
+
+class MX(NamedTuple):
+    """Microscaled rows [rows, cols] (``mx_quantize``). ``codes``: float8_e4m3fn [rows, cols], or uint8
+    [rows, cols / 2] holding two e2m1 codes to a byte (the earlier element in the low half). ``scales``: uint8
+    [ceil(cols / 128), rows, 4], byte s of the block of 32 elements standing for the factor 2^(s - 127) (255: the
+    block is NaN; bytes behind the last block 0)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def format(self) -> str:
+        return "e2m1" if self.codes.dtype == torch.uint8 else "e4m3"
+
+    @property
+    def shape(self) -> tuple:
+        return self.codes.shape[0], self.codes.shape[1] * (2 if self.codes.dtype == torch.uint8 else 1)
+
+
+def _on(what, *ts):
+    """The one device of the given tensors (None entries aside)."""
+    _dev(*ts)
+    dev = ts[0].device
+    if any(t is not None and t.device != dev for t in ts):
+        raise ValueError(f"{what}: tensors on different devices")
+    return dev
+
+
+def _call_on(dev, name, *args):
+    """The call on ``dev``'s current stream, whichever device is the current one."""
+    if dev.index == _cur_device():
+        _call(name, *args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            _call(name, *args, _stream())
+
+
+def _mx_of(q, what, *, cols=None):
+    """q as an MX pair whose tensors are what the kernels take: (MX, rows, cols)."""
+    codes, scales = q
+    q = MX(codes, scales)
+    if codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or scales.dtype != torch.uint8 or codes.dim() != 2:
+        raise TypeError(f"{what}: MX codes must be float8_e4m3fn or uint8 [rows, ..] with uint8 scales")
+    rows, k = q.shape
+    if k == 0 or k % MX_BLOCK or (cols is not None and k != cols):
+        raise ValueError(f"{what}: MX rows of {k} elements; expected {cols if cols else 'a multiple of 32'}")
+    if tuple(scales.shape) != (-(-k // 128), rows, 4):
+        raise ValueError(f"{what}: MX scales must be [{-(-k // 128)}, {rows}, 4], got {list(scales.shape)}")
+    if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
+        raise ValueError(f"{what}: MX codes and scales must be contiguous, 16- and 4-byte aligned")
+    return q, rows, k
+
+
+def _mx_empty(rows, cols, fmt, dev) -> MX:
+    codes = (torch.empty(rows, cols // 2, dtype=torch.uint8, device=dev) if fmt == "e2m1"
+             else torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device=dev))
+    return MX(codes, torch.empty(-(-cols // 128), rows, 4, dtype=torch.uint8, device=dev))
+
+
+def _mx_out(out, rows, cols, fmt, dev, what) -> MX:
+    if out is None:
+        return _mx_empty(rows, cols, fmt, dev)
+    q, r, k = _mx_of(out, what)
+    if (r, k) != (rows, cols) or q.format != fmt or _on(what, *q) != dev:
+        raise ValueError(f"{what}: out must be an {fmt} MX pair of [{rows}, {cols}] on {dev}")
+    return q
+
+
+def mx_quantize(x, fmt="e2m1", *, out=None) -> MX:
+    """The MX form of x [rows, cols] (``fg_mx_quantize``), cols a multiple of 32: fmt "e4m3" (8 bits) or "e2m1"
+    (4 bits). Each block of 32 elements gets the smallest power-of-two scale >= 2^-126 that holds it without
+    saturation; a block that holds an infinity or a NaN becomes NaN. x bf16 or fp32 with unit column stride and
+    16-byte aligned rows. ``out``: an MX pair to overwrite in place (a weight that is quantised again)."""
+    dev = _on("mx_quantize", x)
+    if fmt not in MX_FORMATS:
+        raise ValueError(f"mx_quantize: fmt must be one of {tuple(MX_FORMATS)}")
+    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % MX_BLOCK:
+        raise ValueError("mx_quantize: x must be [rows, cols] with cols a multiple of 32")
+    dt = dtype_code(x)
+    rows, cols = x.shape
+    q = _mx_out(out, rows, cols, fmt, dev, "mx_quantize")
+    if rows == 0:
+        return q
+    ldx = x.stride(0) if rows > 1 else cols
+    if x.stride(1) != 1 or ldx % 8 or ldx < cols or x.data_ptr() % 16:
+        raise ValueError("mx_quantize: x rows must have unit column stride and start 16-byte aligned")
+    _call_on(dev, "fg_mx_quantize", _ptr(x), dt, ldx, rows, cols, MX_FORMATS[fmt], _ptr(q.codes), _ptr(q.scales))
+    return q
+
+
+def mx_dequantize(q, dtype=torch.bfloat16, *, out=None):
+    """The values that an MX pair stands for, [rows, cols] in bf16 (exact but under 2^-126) or fp32
+    (``fg_mx_dequantize``)."""
+    q, rows, cols = _mx_of(q, "mx_dequantize")
+    dev = _on("mx_dequantize", *q, out)
+    if out is None:
+        if dtype not in _DT:
+            raise TypeError("mx_dequantize: dtype must be bfloat16 or float32")
+        out = torch.empty(rows, cols, dtype=dtype, device=dev)
+    elif tuple(out.shape) != (rows, cols) or out.dtype not in _DT or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"mx_dequantize: out must be a contiguous 16-byte aligned bf16 or fp32 [{rows}, {cols}] tensor")
+    if rows == 0:
+        return out
+    _call_on(dev, "fg_mx_dequantize", _ptr(q.codes), _ptr(q.scales), MX_FORMATS[q.format], rows, cols, _ptr(out),
+             dtype_code(out), cols)
+    return out
+
+
+def rmsnorm_mx(x, weight, eps, *, delta=None, sum_out=None, out=None) -> MX:
+    """``rmsnorm`` with an 8-bit output (``fg_rmsnorm_mx``): MX e4m3 of RMSNorm(x [+ delta]) * weight over the last
+    dimension of x [rows, H], H a multiple of 32 up to 8192. With delta the sum, rounded to x's dtype, is written to
+    ``sum_out`` (x itself when not given). x, delta, weight and sum_out contiguous, one dtype (bf16 or fp32). The
+    norm is not rounded between its steps: the codes are those of the formula in 64 bits."""
+    dev = _on("rmsnorm_mx", x, weight, delta, sum_out)
+    dt = dtype_code(x)
+    if x.dim() != 2:
+        raise ValueError("rmsnorm_mx: x must be [rows, H]")
+    rows, H = x.shape
+    if H == 0 or H % MX_BLOCK or H > 8192:
+        raise ValueError("rmsnorm_mx: H must be a multiple of 32, at most 8192")
+    if weight.numel() != H or weight.dtype != x.dtype or not weight.is_contiguous():
+        raise ValueError("rmsnorm_mx: weight must be a contiguous [H] tensor of x's dtype")
+    if delta is None and sum_out is not None:
+        raise ValueError("rmsnorm_mx: sum_out without delta")
+    if delta is not None and sum_out is None:
+        sum_out = x
+    for t, n in ((x, "x"), (delta, "delta"), (sum_out, "sum_out")):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"rmsnorm_mx: {n} must be a contiguous, 16-byte aligned tensor of x's shape and dtype")
+    if weight.data_ptr() % 16:
+        raise ValueError("rmsnorm_mx: weight must be 16-byte aligned")
+    q = _mx_out(out, rows, H, "e4m3", dev, "rmsnorm_mx")
+    if rows:
+        _call_on(dev, "fg_rmsnorm_mx", _ptr(x), _ptr(delta), _ptr(weight), _ptr(sum_out), dt, rows, H, float(eps),
+                 _ptr(q.codes), _ptr(q.scales))
+    return q
+
+
+def _mx_operands(x, w, what):
+    x, rows, k = _mx_of(x, what)
+    w, n, _ = _mx_of(w, what, cols=k)
+    if w.format != "e2m1":
+        raise TypeError(f"{what}: the weight must be in e2m1 (4 bits)")
+    return x, w, rows, n, k, _on(what, *x, *w)
+
+
+def mx_linear(x, w, *, bias=None, residual=None, out=None):
+    """bf16 [rows, N] = x . w^T (+ bias) (+ residual) of MX rows x [rows, K] (e4m3 or e2m1) and a 4-bit MX weight w
+    [N, K] (``fg_mx_linear``), summed in fp32 and rounded once. bias bf16 [N]; residual bf16 [rows, N] with unit
+    column stride; ``out`` bf16 with unit column stride, which may be the residual (an update in place)."""
+    x, w, rows, N, k, dev = _mx_operands(x, w, "mx_linear")
+    if _on("mx_linear", x.codes, bias, residual, out) != dev:
+        raise ValueError("mx_linear: tensors on different devices")
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != N or not bias.is_contiguous()):
+        raise ValueError(f"mx_linear: bias must be a contiguous bf16 [{N}] tensor")
+    if out is None:
+        out = torch.empty(rows, N, dtype=torch.bfloat16, device=dev)
+    for t, n in ((residual, "residual"), (out, "out")):
+        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (rows, N) or (N > 1 and t.stride(1) != 1)
+                              or (rows > 1 and t.stride(0) < N)):
+            raise ValueError(f"mx_linear: {n} must be bf16 [{rows}, {N}] with unit column stride")
+    if rows == 0 or N == 0:
+        return out
+    ld = lambda t: N if t is None or rows == 1 else t.stride(0)
+    _call_on(dev, "fg_mx_linear", _ptr(x.codes), _ptr(x.scales), MX_FORMATS[x.format], _ptr(w.codes), _ptr(w.scales),
+             rows, N, k, _ptr(bias), _ptr(residual), ld(residual), _ptr(out), ld(out))
+    return out
+
+
+def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
+    """MX e4m3 [rows, I] of SiLU(x . w[:I]^T) * (x . w[I:]^T) (``fg_mx_gate_up_swiglu``): MX rows x [rows, K] (e4m3
+    or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums and the activation in
+    fp32, rounded once, to the 8-bit codes."""
+    x, w, rows, n2, k, dev = _mx_operands(x, w, "mx_gate_up_swiglu")
+    if n2 == 0 or n2 % (2 * MX_BLOCK):
+        raise ValueError("mx_gate_up_swiglu: the weight must have 2 I rows, I a multiple of 32")
+    q = _mx_out(out, rows, n2 // 2, "e4m3", dev, "mx_gate_up_swiglu")
+    if rows:
+        _call_on(dev, "fg_mx_gate_up_swiglu", _ptr(x.codes), _ptr(x.scales), MX_FORMATS[x.format], _ptr(w.codes),
+                 _ptr(w.scales), rows, n2 // 2, k, _ptr(q.codes), _ptr(q.scales))
+    return q
 
 
 # ------------------------------------------------------------------ sampling / acceptance

@@ -1,0 +1,397 @@
+"""Microscaled rows on the GPU against the float64 oracle (``oracle/mx.py``).
+
+Quantisation, values and the norm are compared bit for bit. The products are held to a bound derived from what the
+scaled matrix instruction does with its operands: products of two e2m1 codes are exact and summed with at least 24 bits;
+with an e4m3 operand the products of 8 neighbouring elements are cut to multiples of 2^-13 of the power of two below the
+largest of them. So a sum is off by at most 7 * 2^-13 of the largest product of each group of 8 (e4m3), plus 9 cuts of
+2^-23 of the sum of magnitudes per 64 elements, plus the sum over splits; the bf16 result by half a step, 2^-8 of it.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def K():
+    from flashgrpo_amd import kernels
+
+    return kernels
+
+
+def rows_of(rows, cols, seed, dtype=torch.bfloat16, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(spread * torch.randn(rows, cols // 32, generator=g)).repeat_interleave(32, 1)
+    return x.to(dtype)
+
+
+def random_mx(rows, cols, fmt, seed):
+    """An MX pair of a spread of magnitudes, and its float64 values."""
+    codes, scales = O.quantize(rows_of(rows, cols, seed).double().numpy(), fmt)
+    return device_mx(codes, scales, fmt), O.values(codes, scales, fmt)
+
+
+def device_mx(codes, scales, fmt):
+    c = torch.from_numpy(np.ascontiguousarray(O.pack(codes, fmt))).to(DEV)
+    return K().MX(c if fmt == "e2m1" else c.view(torch.float8_e4m3fn), torch.from_numpy(scales).to(DEV))
+
+
+def held(q):
+    """(codes one to an element, scales) of an MX pair on the host."""
+    return O.unpack(q.codes.view(torch.uint8).cpu().numpy(), q.format), q.scales.cpu().numpy()
+
+
+def host(q):
+    return O.values(*held(q), q.format)
+
+
+# ------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 3584), (3, 96), (16, 512), (17, 544), (33, 160), (130, 1184)])
+def test_quantize_is_the_oracle_bit_for_bit(rows, cols, fmt, dtype):
+    x = rows_of(rows, cols, rows + cols, dtype, spread=3.0)
+    codes, scales = held(K().mx_quantize(x.to(DEV), fmt))
+    want_c, want_s = O.quantize(x.double().numpy(), fmt)
+    assert np.array_equal(scales, want_s)
+    assert np.array_equal(codes, want_c)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_quantize_borders(fmt):
+    """Ties, block maxima at and next to a scale's border, zeros, subnormals, the ends of fp32's range."""
+    big = O.LARGEST[fmt]
+    rng = np.random.default_rng(0)
+    blocks = [np.zeros(32), np.full(32, -0.0)]
+    for n in (-130, -126, -20, 0, 7, 115):
+        for edge in (1.0, 1 - 2.0 ** -23, 1 + 2.0 ** -22):
+            b = rng.uniform(-1, 1, 32) * big * 2.0 ** n
+            b[3] = big * edge * 2.0 ** n
+            blocks.append(b)
+        t = O.TABLE[fmt]
+        mids = (t[1:] + t[:-1]) / 2 * 2.0 ** n
+        for i in range(0, len(mids), 31):
+            b = np.zeros(32)
+            m = mids[i:i + 31]
+            b[:len(m)] = m * np.where(np.arange(len(m)) % 2, -1, 1)
+            b[31] = big * 2.0 ** n
+            blocks.append(b)
+    blocks.append(np.full(32, 3.4028234663852886e38))
+    blocks.append(rng.uniform(-1, 1, 32) * 1e-44)
+    x = torch.from_numpy(np.stack(blocks).astype(np.float32))
+    codes, scales = held(K().mx_quantize(x.to(DEV), fmt))
+    want_c, want_s = O.quantize(x.double().numpy(), fmt)
+    assert np.array_equal(scales, want_s)
+    assert np.array_equal(codes, want_c)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_a_block_with_a_non_finite_element_is_nan_and_no_other(fmt, bad):
+    x = rows_of(5, 160, 3)
+    x[2, 70] = bad
+    q = K().mx_quantize(x.to(DEV), fmt)
+    v, w = host(q), K().mx_dequantize(q, torch.float32).cpu().numpy()
+    nan = np.zeros((5, 160), bool)
+    nan[2, 64:96] = True
+    assert np.array_equal(np.isnan(v), nan) and np.array_equal(np.isnan(w), nan)
+    clean = x.clone()
+    clean[2, 64:96] = 0
+    assert np.array_equal(v[~nan], host(K().mx_quantize(clean.to(DEV), fmt))[~nan])
+
+
+def test_quantize_strided_rows_and_in_place_pair():
+    x = torch.randn(9, 320, device=DEV).to(torch.bfloat16)
+    q = K().mx_quantize(x[:, 64:224], "e2m1")
+    want = K().mx_quantize(x[:, 64:224].contiguous(), "e2m1")
+    assert torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales)
+    again = K().mx_quantize(x[:, :160], "e2m1", out=q)
+    assert again.codes.data_ptr() == q.codes.data_ptr()
+    want = K().mx_quantize(x[:, :160].contiguous(), "e2m1")
+    assert torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (19, 416), (64, 1024)])
+def test_dequantize_every_code_and_scale(fmt, rows, cols):
+    g = np.random.default_rng(rows)
+    codes = g.integers(0, 2 * O.SIGN[fmt], (rows, cols)).astype(np.uint8)
+    scales = g.integers(0, 256, (-(-cols // 128), rows, 4)).astype(np.uint8)
+    v = O.values(codes, scales, fmt)
+    q = device_mx(codes, scales, fmt)
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(v.astype(np.float32))
+    got = K().mx_dequantize(q, torch.float32).cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=1.0, posinf=9e9), want.nan_to_num(nan=1.0, posinf=9e9))
+    got = K().mx_dequantize(q).cpu()
+    want = want.to(torch.bfloat16)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(nan=1.0).view(torch.int16), want.nan_to_num(nan=1.0).view(torch.int16))
+
+
+def test_no_rows():
+    k = K()
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
+    q = k.mx_quantize(x, "e4m3")
+    w, _ = random_mx(64, 64, "e2m1", 0)
+    assert q.codes.shape == (0, 64) and q.scales.shape == (1, 0, 4)
+    assert k.mx_dequantize(q).shape == (0, 64)
+    assert k.rmsnorm_mx(x, torch.ones(64, dtype=torch.bfloat16, device=DEV), 1e-6).codes.shape == (0, 64)
+    assert k.mx_linear(q, w).shape == (0, 64) and k.mx_gate_up_swiglu(q, w).codes.shape == (0, 32)
+
+
+# ------------------------------------------------------------------ norm
+def norm_oracle(x, weight, eps, delta):
+    s = x if delta is None else (x.float() + delta.float()).to(x.dtype)
+    return s, O.quantize(O.rmsnorm(s.double().numpy(), weight.double().numpy(), eps), "e4m3")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (5, 160), (3, 1536), (2, 2080), (17, 3584), (4, 8192)])
+def test_rmsnorm_codes_are_the_formulas(rows, cols, delta, dtype):
+    x, d = rows_of(rows, cols, cols, dtype), rows_of(rows, cols, cols + 1, dtype)
+    w = (1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(cols))).to(dtype)
+    eps = float(np.float32(1e-6))
+    s, (want_c, want_s) = norm_oracle(x, w, eps, d if delta else None)
+    xg = x.to(DEV)
+    total = torch.full_like(xg, 7.0) if delta else None
+    q = K().rmsnorm_mx(xg, w.to(DEV), 1e-6, delta=d.to(DEV) if delta else None, sum_out=total)
+    codes, scales = held(q)
+    assert np.array_equal(scales, want_s) and np.array_equal(codes, want_c)
+    assert torch.equal(xg.cpu(), x)
+    if delta:
+        assert torch.equal(total.cpu(), s)
+        q2 = K().rmsnorm_mx(xg, w.to(DEV), 1e-6, delta=d.to(DEV))  # into x itself
+        assert torch.equal(xg.cpu(), s) and torch.equal(q2.scales, q.scales)
+        assert torch.equal(q2.codes.view(torch.uint8), q.codes.view(torch.uint8))
+
+
+def test_rmsnorm_special_rows():
+    """A row of zeros, one with an infinity, one with a NaN, tiny and huge rows; the others are as without them."""
+    x = rows_of(7, 256, 5, torch.float32)
+    x[1] = 0
+    x[2, 40] = float("inf")
+    x[3, 200] = float("nan")
+    x[4] *= 1e-30
+    x[5] *= 1e18
+    w = torch.ones(256)
+    q = K().rmsnorm_mx(x.to(DEV), w.to(DEV), 1e-6)
+    v = host(q)
+    assert (v[1] == 0).all() and np.isnan(v[3]).all()
+    assert np.isnan(v[2, 32:64]).all() and (v[2, :32] == 0).all() and (v[2, 64:] == 0).all()
+    fine = [0, 4, 5, 6]
+    want_c, want_s = O.quantize(O.rmsnorm(x[fine].double().numpy(), w.double().numpy(), float(np.float32(1e-6))), "e4m3")
+    codes, scales = held(q)
+    assert np.array_equal(codes[fine], want_c) and np.array_equal(scales[:, fine], want_s)
+
+
+# ------------------------------------------------------------------ products
+def product_bound(xv, wv, fmt):
+    """How far a product's fp32 sums may be off (see the head of this file), and the exact products."""
+    k = xv.shape[1]
+    x, w = torch.from_numpy(xv).to(DEV), torch.from_numpy(wv).to(DEV)
+    exact, mags = x @ w.t(), x.abs() @ w.abs().t()
+    err = (k / 64 + 1) * 9 * 2.0 ** -23 * mags + 256 * 2.0 ** -24 * mags
+    if fmt == "e4m3":
+        big = torch.zeros_like(exact)
+        for g in range(0, k, 8):
+            big += (x[:, None, g:g + 8] * w[None, :, g:g + 8]).abs().amax(-1)
+        err += 7 * 2.0 ** -13 * big
+    return exact, err
+
+
+def check_linear(got, exact, err, bias=None, residual=None):
+    ref = exact
+    if bias is not None:
+        ref = ref + bias.double()
+        err = err + 2.0 ** -23 * (exact.abs() + bias.double().abs())
+    if residual is not None:
+        ref = ref + residual.double()
+        err = err + 2.0 ** -23 * (exact.abs() + residual.double().abs() + (0 if bias is None else bias.double().abs()))
+    far = (got.double() - ref).abs() - (2.0 ** -8 * ref.abs() + (1 + 2.0 ** -8) * err + 1e-38)
+    assert not got.isnan().any()
+    assert float(far.max()) <= 0, f"worst {float(far.max())} over the bound at {int(far.argmax())}"
+
+
+SHAPES = [(1, 1, 32), (1, 2048, 1536), (2, 33, 96), (5, 77, 160), (15, 130, 512), (16, 64, 544), (17, 129, 640), (31, 256, 1184),
+          (64, 200, 2048), (65, 384, 288), (129, 257, 416), (200, 513, 1056), (257, 300, 384), (300, 700, 128)]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("rows,n,k", SHAPES)
+def test_linear_matches_float64(rows, n, k, fmt):
+    x, xv = random_mx(rows, k, fmt, rows + k)
+    w, wv = random_mx(n, k, "e2m1", n + k + 1)
+    exact, err = product_bound(xv, wv, fmt)
+    check_linear(K().mx_linear(x, w), exact, err)
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 40, 160), (3, 2048, 1536), (70, 129, 256), (130, 264, 1024)])
+def test_linear_bias_residual_strides_and_in_place(rows, n, k):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x, xv = random_mx(rows, k, "e4m3", rows)
+    w, wv = random_mx(n, k, "e2m1", n)
+    exact, err = product_bound(xv, wv, "e4m3")
+    scale = float(exact.abs().mean())
+    bias = (scale * torch.randn(n, device=DEV, generator=g)).to(torch.bfloat16)
+    res = (scale * torch.randn(rows, n + 24, device=DEV, generator=g)).to(torch.bfloat16)
+    check_linear(K().mx_linear(x, w, bias=bias), exact, err, bias)
+    for off in (0, 3, 8):  # rows that start anywhere
+        r = res[:, off:off + n]
+        plain = K().mx_linear(x, w, bias=bias, residual=r)
+        check_linear(plain, exact, err, bias, r)
+        wide = torch.full((rows + 2, n + 24), 5.0, dtype=torch.bfloat16, device=DEV)
+        wide[1:-1, off:off + n] = r
+        view = wide[1:-1, off:off + n]
+        assert K().mx_linear(x, w, bias=bias, residual=view, out=view) is view
+        assert torch.equal(view, plain)
+        assert (wide[0] == 5).all() and (wide[-1] == 5).all() and (wide[:, :off] == 5).all() and (wide[:, off + n:] == 5).all()
+
+
+@pytest.mark.parametrize("rows,n,k", [(3, 50, 160), (140, 150, 288)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_nan_blocks_reach_their_own_rows_and_columns_only(rows, n, k, fmt):
+    """Also where K ends inside a step of 128: what lies behind a row's end, here a neighbour's NaN, is not read."""
+    x, _ = random_mx(rows, k, fmt, 1)
+    w, _ = random_mx(n, k, "e2m1", 2)
+    clean = K().mx_linear(x, w)
+    xs, ws = x.scales.clone(), w.scales.clone()
+    xs[0, 1, 0] = 255   # row 1, first block: it follows row 0's end in memory
+    ws[-1, n - 1, 0] = 255
+    codes = x.codes.clone()
+    if fmt == "e4m3":
+        codes.view(torch.uint8)[2, :8] = 127  # e4m3 NaN codes at the start of row 2
+    got = K().mx_linear(K().MX(codes, xs), K().MX(w.codes, ws))
+    nan = torch.zeros(rows, n, dtype=torch.bool, device=DEV)
+    nan[1] = True
+    nan[:, n - 1] = True
+    if fmt == "e4m3":
+        nan[2] = True
+    assert torch.equal(got.isnan(), nan)
+    assert torch.equal(got[~nan], clean[~nan])
+
+
+def check_gate_up(q, xv, wv, fmt, min_equal=0.97):
+    n = wv.shape[0] // 2
+    exact, err = product_bound(xv, wv, fmt)
+    g, u, eg, eu = exact[:, :n], exact[:, n:], err[:, :n], err[:, n:]
+    v = torch.from_numpy(O.silu_mul(g.cpu().numpy(), u.cpu().numpy())).to(DEV)
+    # |SiLU'| <= 1.1; the fp32 exponential, reciprocal and products are within 8 * 2^-23 of the value
+    d = 1.1 * eg * (u.abs() + eu) + g.abs() * eu + 8 * 2.0 ** -23 * v.abs()
+    # a code is within half a step (2^-4 of the value, or of the least step, 2^-10 of the scale; the block's largest
+    # value may move the scale up by one)
+    step = torch.from_numpy(np.repeat(np.exp2(O.scale_exponents(v.cpu().numpy(), "e4m3") + 1.0), 32, 1)).to(DEV)
+    got = torch.from_numpy(host(q)).to(DEV)
+    far = (got - v).abs() - (d + 2.0 ** -4 * (v.abs() + d) + 2.0 ** -10 * step)
+    assert float(far.max()) <= 0, f"worst {float(far.max())} over the bound"
+    codes, scales = held(q)
+    want_c, want_s = O.quantize(v.cpu().numpy(), "e4m3")
+    last = scales[-1].copy()
+    assert (last[:, (n // 32 - 1) % 4 + 1:] == 0).all()  # behind the last block
+    assert (scales == want_s).mean() >= 0.99
+    assert (codes == want_c).mean() >= min_equal
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("rows,inter,k", [(1, 32, 32), (1, 480, 1536), (3, 64, 160), (16, 96, 512), (17, 160, 544), (64, 288, 1056),
+                                          (65, 96, 256), (130, 352, 384), (260, 544, 128)])
+def test_gate_up_matches_float64(rows, inter, k, fmt):
+    # magnitudes as after a norm (the gate has to move through SiLU's bend)
+    codes, scales = O.quantize(rows_of(rows, k, rows + k, spread=0.5).double().numpy(), fmt)
+    x, xv = device_mx(codes, scales, fmt), O.values(codes, scales, fmt)
+    codes, scales = O.quantize((rows_of(2 * inter, k, inter, spread=0.5) * k ** -0.5).double().numpy(), "e2m1")
+    w, wv = device_mx(codes, scales, "e2m1"), O.values(codes, scales, "e2m1")
+    check_gate_up(K().mx_gate_up_swiglu(x, w), xv, wv, fmt)
+
+
+# ------------------------------------------------------------------ together
+def mlp(k, x, delta, norm, gate_up, down):
+    q = k.rmsnorm_mx(x, norm, 1e-6, delta=delta)
+    act = k.mx_gate_up_swiglu(q, gate_up)
+    return q, act, k.mx_linear(act, down, residual=x, out=x)
+
+
+def mlp_state(rows, hidden, inter, seed):
+    k = K()
+    x, d = rows_of(rows, hidden, seed).to(DEV), rows_of(rows, hidden, seed + 1, spread=0.1).to(DEV)
+    norm = torch.ones(hidden, dtype=torch.bfloat16, device=DEV)
+    gu = k.mx_quantize((rows_of(2 * inter, hidden, seed + 2, spread=0.2) * hidden ** -0.5).to(DEV), "e2m1")
+    dn = k.mx_quantize((rows_of(hidden, inter, seed + 3, spread=0.2) * inter ** -0.5).to(DEV), "e2m1")
+    return x, d, norm, gu, dn
+
+
+@pytest.mark.parametrize("rows,hidden,inter", [(1, 256, 480), (29, 512, 1408), (416, 384, 608)])
+def test_mlp_chain(rows, hidden, inter):
+    """norm -> gate/up -> down + residual in place, each stage against the oracle on the stage's own inputs."""
+    x, d, norm, gu, dn = mlp_state(rows, hidden, inter, rows)
+    s, (want_c, want_s) = norm_oracle(x.cpu(), norm.cpu(), float(np.float32(1e-6)), d.cpu())
+    q, act, y = mlp(K(), x, d, norm, gu, dn)
+    codes, scales = held(q)
+    assert np.array_equal(codes, want_c) and np.array_equal(scales, want_s)
+    check_gate_up(act, host(q), host(gu), "e4m3")
+    exact, err = product_bound(host(act), host(dn), "e4m3")
+    assert y is x
+    check_linear(y, exact, err, residual=s.to(DEV))
+
+
+@pytest.mark.parametrize("rows", [1, 64, 150])
+def test_chain_is_the_same_twice_captured_and_on_another_stream(rows):
+    x, d, norm, gu, dn = mlp_state(rows, 512, 992, 3)
+    first, k = x.clone(), K()
+    want = mlp(k, x, d, norm, gu, dn)[2].clone()
+    x.copy_(first)
+    assert torch.equal(mlp(k, x, d, norm, gu, dn)[2], want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x.copy_(first)
+        got = mlp(k, x, d, norm, gu, dn)[2].clone()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    # two graphs of the same calls on rows of their own, replayed in turn with eager work between
+    a, b = first.clone(), first.clone()
+    graphs = []
+    for t in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            mlp(k, t, d, norm, gu, dn)
+        graphs.append(g)
+    for _ in range(3):
+        for t in (a, b, x):
+            t.copy_(first)
+        graphs[0].replay()
+        mlp(k, x, d, norm, gu, dn)
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want) and torch.equal(x, want)
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    k = K()
+    x = torch.zeros(4, 128, dtype=torch.bfloat16, device=DEV)
+    q, w = k.mx_quantize(x, "e4m3"), k.mx_quantize(x, "e2m1")
+    one = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    for call in (lambda: k.mx_quantize(x, "e5m2"), lambda: k.mx_quantize(x[:, :48]), lambda: k.mx_quantize(x[0]),
+                 lambda: k.mx_quantize(x.t()), lambda: k.mx_quantize(x[:, 4:100]), lambda: k.mx_quantize(x, "e2m1", out=q),
+                 lambda: k.mx_linear(q, k.mx_quantize(x[:, :64], "e2m1")), lambda: k.mx_linear(q, w, bias=one),
+                 lambda: k.mx_linear(q, w, residual=x), lambda: k.mx_linear(q, w, out=x), lambda: k.mx_gate_up_swiglu(q, w),
+                 lambda: k.rmsnorm_mx(x, one, 1e-6, sum_out=x), lambda: k.rmsnorm_mx(x, one, 1e-6, delta=x[:2]),
+                 lambda: k.rmsnorm_mx(x[:, :64], one[:64], 1e-6), lambda: k.rmsnorm_mx(x, one[:64], 1e-6),
+                 lambda: k.mx_linear(k.MX(q.codes, q.scales[:, :2]), w)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: k.mx_linear(q, q), lambda: k.mx_quantize(x.half()), lambda: k.mx_dequantize(q, torch.float16),
+                 lambda: k.mx_linear((x, q.scales), w), lambda: k.mx_gate_up_swiglu(w, q)):
+        with pytest.raises(TypeError):
+            call()

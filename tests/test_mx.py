@@ -1,0 +1,110 @@
+"""Microscaled rows without a GPU: the oracle's quantisation against values written out by hand, and what the
+entry points refuse before they launch anything."""
+import ctypes
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx as O
+
+
+def _block(*v):
+    x = np.zeros((1, 32))
+    x[0, :len(v)] = v
+    return x
+
+
+def test_code_tables():
+    assert O.TABLE["e2m1"].tolist() == [0, 0.5, 1, 1.5, 2, 3, 4, 6]
+    t = O.TABLE["e4m3"]
+    assert t[-1] == 448 and t[1] == 2.0 ** -9 and t[8] == 2.0 ** -6 and t[0x38] == 1.0
+    for c in range(127):
+        assert float(torch.tensor([c], dtype=torch.uint8).view(torch.float8_e4m3fn).float()) == t[c]
+
+
+@pytest.mark.parametrize("fmt,largest", [("e4m3", 448.0), ("e2m1", 6.0)])
+def test_scale_is_the_least_power_of_two_that_holds_the_block(fmt, largest):
+    for n in (-20, -1, 0, 3):
+        at = O.quantize(_block(largest * 2.0 ** n), fmt)[1][0, 0]
+        above = O.quantize(_block(largest * 2.0 ** n * (1 + 2.0 ** -7)), fmt)[1][0, 0]
+        assert at.tolist() == [127 + n, 0, 0, 0] and above.tolist() == [128 + n, 0, 0, 0]
+    assert O.quantize(_block(), fmt)[1][0, 0, 0] == 1                 # nothing but zeros: the least scale
+    assert O.quantize(_block(2.0 ** -140), fmt)[1][0, 0, 0] == 1
+    assert O.quantize(_block(1.0, np.inf), fmt)[1][0, 0, 0] == 255 and O.quantize(_block(np.nan), fmt)[1][0, 0, 0] == 255
+
+
+def test_ties_go_to_the_even_code():
+    c, _ = O.quantize(_block(6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.75, -0.25), "e2m1")
+    assert c[0, :10].tolist() == [7, 0, 2, 2, 4, 4, 6, 6, 10, 8]
+    c, _ = O.quantize(_block(448, 1.0625, 1.1875, 2.0 ** -10, 3 * 2.0 ** -10), "e4m3")
+    assert c[0, :5].tolist() == [126, 0x38, 0x3a, 0, 2]
+
+
+def test_oracle_round_trip_and_layout():
+    x = np.random.default_rng(0).standard_normal((3, 160))
+    for fmt, half in (("e4m3", 2.0 ** -4), ("e2m1", 2.0 ** -2)):
+        codes, scales = O.quantize(x, fmt)
+        assert scales.shape == (2, 3, 4) and (scales[1, :, 1:] == 0).all() and (scales[1, :, 0] > 0).all()
+        v = O.values(O.unpack(O.pack(codes, fmt), fmt), scales, fmt)
+        step = np.repeat(np.exp2(O.scale_exponents(x, fmt).astype(float)), 32, 1)
+        assert (np.abs(v - x) <= np.maximum(half * np.abs(x), step * (2.0 ** -10 if fmt == "e4m3" else 0.25))).all()
+
+
+# ------------------------------------------------------------------ refusals
+def _lib():
+    from flashgrpo_amd import _lib as L
+
+    if not os.path.exists(L.library_path()):
+        pytest.skip("native library not built")
+    return L.load()
+
+
+def test_entry_points_refuse_bad_arguments_on_the_host():
+    lib = _lib()
+    p, odd = ctypes.c_void_p(256), ctypes.c_void_p(264)
+
+    def refused(rc, text):
+        assert rc != 0 and text in lib.fg_last_error(), (rc, lib.fg_last_error())
+
+    refused(lib.fg_mx_quantize(None, 1, 64, 1, 64, 0, p, p, None), b"null pointer")
+    refused(lib.fg_mx_quantize(p, 2, 64, 1, 64, 0, p, p, None), b"dtype")
+    refused(lib.fg_mx_quantize(p, 1, 64, 1, 64, 2, p, p, None), b"format")
+    refused(lib.fg_mx_quantize(p, 1, 64, 0, 64, 0, p, p, None), b"shape")
+    refused(lib.fg_mx_quantize(p, 1, 32, 1, 64, 0, p, p, None), b"shape")
+    refused(lib.fg_mx_quantize(p, 1, 48, 1, 48, 0, p, p, None), b"multiple of 32")
+    refused(lib.fg_mx_quantize(p, 1, 68, 1, 64, 0, p, p, None), b"aligned")
+    refused(lib.fg_mx_quantize(odd, 1, 64, 1, 64, 0, p, p, None), b"aligned")
+    refused(lib.fg_mx_dequantize(p, p, 0, 1, 48, p, 1, 48, None), b"multiple of 32")
+    refused(lib.fg_mx_dequantize(p, None, 0, 1, 64, p, 1, 64, None), b"null pointer")
+    refused(lib.fg_rmsnorm_mx(p, p, p, None, 1, 1, 64, 1e-6, p, p, None), b"null pointer")
+    refused(lib.fg_rmsnorm_mx(p, None, p, None, 1, 1, 8224, 1e-6, p, p, None), b"8192")
+    refused(lib.fg_rmsnorm_mx(p, None, p, None, 1, 1, 40, 1e-6, p, p, None), b"multiple of 32")
+    refused(lib.fg_rmsnorm_mx(odd, None, p, None, 1, 1, 64, 1e-6, p, p, None), b"aligned")
+
+
+def test_wrappers_take_device_tensors_only():
+    from flashgrpo_amd import kernels as K
+
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    q = K.MX(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(1, 2, 4, dtype=torch.uint8))
+    assert q.format == "e2m1" and q.shape == (2, 64)
+    for call in (lambda: K.mx_quantize(x), lambda: K.mx_dequantize(q), lambda: K.rmsnorm_mx(x, x[0], 1e-6),
+                 lambda: K.mx_linear(q, q), lambda: K.mx_gate_up_swiglu(q, q)):
+        with pytest.raises(ValueError, match="device tensors"):
+            call()
+
+
+def test_mx_pairs_are_checked():
+    from flashgrpo_amd import kernels as K
+
+    codes, scales = torch.zeros(2, 96, dtype=torch.uint8), torch.zeros(2, 2, 4, dtype=torch.uint8)
+    assert K._mx_of((codes, scales), "t")[1:] == (2, 192)
+    for bad in ((codes.float(), scales), (codes, scales.float())):
+        with pytest.raises(TypeError):
+            K._mx_of(bad, "t")
+    for bad in ((codes[:, :95], scales), (codes[:, :8], scales), (codes, scales[:1]), (codes, scales[:, :1]),
+                (codes.t().contiguous().t(), scales), (codes[:0, :0], scales)):
+        with pytest.raises(ValueError):
+            K._mx_of(bad, "t")
