@@ -248,16 +248,20 @@ int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* su
 
 /* out = bf16(x . w^T (+ bias) (+ residual)): MX rows x [rows, hidden] (x_format 0 or 1) times an MX e2m1 weight w
  * [cols, hidden], fp32 sums rounded once; bias [cols], residual [rows, cols] (row stride ldr) and out (row stride ldo)
- * bf16; out may be the residual. hidden a multiple of 32; operands under 2 GiB each. */
+ * bf16; out may be the residual. hidden a multiple of 32; operands under 2 GiB each. Long reductions over few output
+ * tiles are split over workgroups, whose fp32 sums need workspace >= fg_mx_linear_workspace(...) bytes (0 when no split
+ * is used; a null or smaller workspace runs unsplit). */
+size_t fg_mx_linear_workspace(int rows, int cols, int hidden, int x_format);
 int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const void* w_codes, const void* w_scales,
                  int rows, int cols, int hidden, const void* bias, const void* residual, int64_t ldr, void* out,
-                 int64_t ldo, void* stream);
+                 int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
 
 /* MX e4m3 [rows, inter] of SiLU(x . w[:inter]^T) * (x . w[inter:]^T), in fp32 up to the codes: x as for fg_mx_linear,
- * w [2 * inter, hidden] MX e2m1 (gate rows, then up rows), inter a multiple of 32. */
+ * w [2 * inter, hidden] MX e2m1 (gate rows, then up rows), inter a multiple of 32; workspace as for fg_mx_linear. */
+size_t fg_mx_gate_up_swiglu_workspace(int rows, int inter, int hidden, int x_format);
 int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format, const void* w_codes,
                          const void* w_scales, int rows, int inter, int hidden, void* codes, void* scales,
-                         void* stream);
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* dst[i] = src[i] (bytes[i] bytes, a positive multiple of 4, 4-byte aligned device addresses, no
  * overlaps) for i < count <= 8, in one launch; src, dst and bytes are host arrays. No counterpart in the

@@ -92,7 +92,8 @@ struct MxArgs {
   uint8_t* codes;
   uint32_t* scales;
   // kParts
-  float* part;  // [splits][rows][wrows]
+  float* part;  // [splits][rows][ldp], ldp the weight rows rounded up to a multiple of 4
+  int splits, ldp;
 };
 
 FG_DEVICE float silu_mul(float g, float u) { return fg::silu_f32(g) * u; }
@@ -106,22 +107,30 @@ struct RowLoads {
   static FG_DEVICE int lane_chunk(int lane) { return (lane % kChunks) ^ swizzle(lane / kChunks); }
 };
 
-template <int FMT, int BM, int BN, int WAVES_M, int NS, int EPI>
-__global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
+// Bytes of one ring stage: codes of x and w, scale dwords of x (rounded up to a load of 64) and w.
+constexpr int stage_bytes(int fmt, int bm, int bn) {
+  return bm * (fmt == fg::kE4M3 ? 128 : 64) + bn * 64 + (bm + 63) / 64 * 256 + bn * 4;
+}
+
+template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI>
+__global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, BM, BN) <= 80 * 1024 ? 2 : 1)
+    mx_gemm_kernel(MxArgs p) {
   constexpr int XB = FMT == fg::kE4M3 ? 128 : 64, WB = 64;  // bytes per row and step
-  constexpr int WAVES_N = 4 / WAVES_M;
+  constexpr int WAVES = WAVES_M * WAVES_N;
   constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
   constexpr int FM = WM / 32, FN = WN / 32;  // MFMA tiles per wave
   constexpr int X_BYTES = BM * XB, W_BYTES = BN * WB, SX_BYTES = (BM + 63) / 64 * 256, SW_BYTES = BN * 4;
   constexpr int STAGE = X_BYTES + W_BYTES + SX_BYTES + SW_BYTES;
-  // loads per step over the four waves; a wave without one of its own repeats the last, so that all count alike
+  static_assert(STAGE == stage_bytes(FMT, BM, BN), "stage");
+  // loads per step over the waves; a wave without one of its own repeats the last, so that all count alike
   constexpr int TX = X_BYTES / 1024, TW = W_BYTES / 1024, TS = (SX_BYTES + SW_BYTES) / 256;
-  constexpr int LX = (TX + 3) / 4, LW = (TW + 3) / 4, LS = (TS + 3) / 4, LPW = LX + LW + LS;
+  constexpr int LX = (TX + WAVES - 1) / WAVES, LW = (TW + WAVES - 1) / WAVES, LS = (TS + WAVES - 1) / WAVES;
+  constexpr int LPW = LX + LW + LS;
   static_assert(FM >= 1 && FN >= 1 && TX * 1024 == X_BYTES && TW * 1024 == W_BYTES && BN % 64 == 0, "tile sizes");
   static_assert(EPI != kGateUp || FN % 2 == 0, "a wave holds gate and up of its columns");
   static_assert(NS >= 2 && (NS - 1) * LPW < 64, "vmcnt");
   constexpr int OUT_LD = WN + 4;  // floats per row of the epilogue's staging: 16-byte rows on distinct banks
-  constexpr int EPI_BYTES = EPI == kLinear ? 4 * 32 * OUT_LD * 4 : 0;
+  constexpr int EPI_BYTES = EPI == kLinear ? WAVES * 32 * OUT_LD * 4 : 0;
   static_assert(NS * STAGE <= 160 * 1024 && EPI_BYTES <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) unsigned char smem[NS * STAGE > EPI_BYTES ? NS * STAGE : EPI_BYTES];
 
@@ -158,12 +167,14 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
   const int64_t w_first = EPI == kGateUp ? 0 : (int64_t)n0 * p.wb;
   const __amdgpu_buffer_rsrc_t xrs = rsrc(p.x + (int64_t)m0 * p.xb, (int64_t)(p.rows - m0) * p.xb);
   const __amdgpu_buffer_rsrc_t wrs = rsrc(p.w + w_first, (int64_t)p.wrows * p.wb - w_first);
-  const __amdgpu_buffer_rsrc_t xsrs = rsrc(p.xs, (int64_t)p.steps * p.rows * 4);
-  const __amdgpu_buffer_rsrc_t wsrs = rsrc(p.ws, (int64_t)p.steps * p.wrows * 4);
 
   using XL = RowLoads<XB>;
   using WL = RowLoads<WB>;
   uint32_t xoff[LX], woff[LW], soff[LS];
+  // scales: each load of a wave is of x rows or of weight rows throughout, chosen here and not by a branch between
+  // the matrix instructions, which would part them from the loads they are to cover
+  __amdgpu_buffer_rsrc_t srs[LS];
+  uint32_t sstep[LS];
 #pragma unroll
   for (int u = 0; u < LX; ++u) {
     const int r = min(wave * LX + u, TX - 1) * XL::kRows + XL::lane_row(lane);
@@ -178,7 +189,10 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
   for (int u = 0; u < LS; ++u) {
     const int q = min(wave * LS + u, TS - 1);
     const int j = q * 64 + lane - SX_BYTES / 4;
-    soff[u] = (uint32_t)(q < SX_BYTES / 256 ? min(m0 + q * 64 + lane, p.rows - 1) : weight_row(j)) * 4;
+    const bool of_x = q < SX_BYTES / 256;
+    soff[u] = (uint32_t)(of_x ? min(m0 + q * 64 + lane, p.rows - 1) : weight_row(j)) * 4;
+    sstep[u] = (uint32_t)(of_x ? p.rows : p.wrows) * 4;
+    srs[u] = rsrc(of_x ? p.xs : p.ws, (int64_t)p.steps * sstep[u]);
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem;
   // The last step of a K that is no multiple of 128: chunks behind the row's end read 0.
@@ -201,19 +215,11 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
       asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(wrs), "s"(k), "{m0}"(m0v)
                    : "memory");
     } else {
-      const int e = min(wave * LS + q - LX - LW, TS - 1);
-      const uint32_t m0v = sbase + X_BYTES + W_BYTES + e * 256;
-      if (e < SX_BYTES / 256) {
-        const uint32_t k = (uint32_t)(ks0 + ks) * p.rows * 4;
-        asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(soff[q - LX - LW]), "s"(xsrs), "s"(k),
-                     "{m0}"(m0v)
-                     : "memory");
-      } else {
-        const uint32_t k = (uint32_t)(ks0 + ks) * p.wrows * 4;
-        asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(soff[q - LX - LW]), "s"(wsrs), "s"(k),
-                     "{m0}"(m0v)
-                     : "memory");
-      }
+      const int e = q - LX - LW;
+      const uint32_t m0v = sbase + X_BYTES + W_BYTES + min(wave * LS + e, TS - 1) * 256;
+      const uint32_t k = (uint32_t)(ks0 + ks) * sstep[e];
+      asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, %2 offen lds" ::"v"(soff[e]), "s"(srs[e]), "s"(k), "{m0}"(m0v)
+                   : "memory");
     }
   };
 
@@ -224,40 +230,52 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
     for (int k = 0; k < FM; ++k)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][k][v] = 0.0f;
-  intx8 fx[2][FM], fw[2][FN];
-  int sx[2][FM], sw[2][FN];  // a row's scales of one step, its own half's first block in byte 0, second in byte 2
+  constexpr int XR = FMT == fg::kE4M3 ? 2 : 1;  // 16-byte reads per fragment of x
+  int4 fx[2][FM][XR], fw[2][FN];
+  // a row's scale dword of this step, its own half's first block in byte 0 and second in byte 2; as read for the next
+  uint32_t sx[FM], sw[FN], nx[FM], nw[FN];
   const int xswz = XL::swizzle(l32), wswz = WL::swizzle(l32);
-  auto read = [&](int slot, int s, int buf) __attribute__((always_inline)) {
+  constexpr int kReads = FM * XR + FN, kScaleReads = FM + FN;
+  // One of the LDS reads of sub-step s of a slot; those from kReads on are the step's scales.
+  auto read = [&](int slot, int s, int buf, int q) __attribute__((always_inline)) {
     const unsigned char* st = smem + slot * STAGE;
-#pragma unroll
-    for (int f = 0; f < FM; ++f) {
-      const unsigned char* row = st + (wm * WM + f * 32 + l32) * XB;
-      if constexpr (FMT == fg::kE4M3) {
-        const int4 lo = *(const int4*)(row + ((4 * s + half) ^ xswz) * 16);
-        const int4 hi = *(const int4*)(row + ((4 * s + 2 + half) ^ xswz) * 16);
-        fx[buf][f] = intx8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      } else {
-        const int4 lo = *(const int4*)(row + ((2 * s + half) ^ xswz) * 16);
-        fx[buf][f] = intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
-      }
-    }
-#pragma unroll
-    for (int f = 0; f < FN; ++f) {
-      const int4 lo = *(const int4*)(st + X_BYTES + (wn * WN + f * 32 + l32) * WB + ((2 * s + half) ^ wswz) * 16);
-      fw[buf][f] = intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
+    if (q < FM * XR) {
+      const int f = q / XR, h = q % XR;
+      const int chunk = FMT == fg::kE4M3 ? 4 * s + 2 * h + half : 2 * s + half;
+      fx[buf][f][h] = *(const int4*)(st + (wm * WM + f * 32 + l32) * XB + (chunk ^ xswz) * 16);
+    } else if (q < kReads) {
+      const int f = q - FM * XR;
+      fw[buf][f] = *(const int4*)(st + X_BYTES + (wn * WN + f * 32 + l32) * WB + ((2 * s + half) ^ wswz) * 16);
+    } else {
+      const uint32_t* sc = (const uint32_t*)(st + X_BYTES + W_BYTES);
+      const int f = q - kReads;
+      if (f < FM) nx[f] = sc[wm * WM + f * 32 + l32];
+      else nw[f - FM] = sc[SX_BYTES / 4 + wn * WN + (f - FM) * 32 + l32];
     }
   };
-  auto read_scales = [&](int slot, int buf) __attribute__((always_inline)) {
-    const uint32_t* sc = (const uint32_t*)(smem + slot * STAGE + X_BYTES + W_BYTES);
+  auto take_scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int f = 0; f < FM; ++f) sx[buf][f] = (int)(sc[wm * WM + f * 32 + l32] >> (8 * half));
+    for (int f = 0; f < FM; ++f) sx[f] = nx[f] >> (8 * half);
 #pragma unroll
-    for (int f = 0; f < FN; ++f) sw[buf][f] = (int)(sc[SX_BYTES / 4 + wn * WN + f * 32 + l32] >> (8 * half));
+    for (int f = 0; f < FN; ++f) sw[f] = nw[f] >> (8 * half);
+  };
+  auto x_frag = [&](int buf, int f) __attribute__((always_inline)) {
+    const int4 lo = fx[buf][f][0];
+    if constexpr (XR == 2) {
+      const int4 hi = fx[buf][f][1];
+      return intx8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    } else {
+      return intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
+    }
+  };
+  auto w_frag = [&](int buf, int f) __attribute__((always_inline)) {
+    const int4 lo = fw[buf][f];
+    return intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
   };
   constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;  // the instruction's code of x's format; 4 is e2m1
-#define FG_MX_MFMA(i, k, buf, sel, sb)                                                                              \
-  acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[buf][i], fx[buf][k], acc[i][k], 4, kBF, sel,       \
-                                                              sw[sb][i], sel, sx[sb][k])
+#define FG_MX_MFMA(i, k, buf, sel)                                                                                  \
+  acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w_frag(buf, i), x_frag(buf, k), acc[i][k], 4, kBF,     \
+                                                              sel, (int)sw[i], sel, (int)sx[k])
 
   // Prologue: steps 0 .. min(NS, nk) - 1 in flight, wait for step 0.
   const int first = min(NS, nk);
@@ -270,19 +288,26 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
   wait_steps<LPW, NS - 1>(first - 1);
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
-  read(0, 0, 0);
-  read_scales(0, 0);
+#pragma unroll
+  for (int q = 0; q < kReads + kScaleReads; ++q) read(0, 0, 0, q);
+  take_scales();
 
-  // Step t in slot t % NS, which takes step t + NS once consumed; sb: which of the two scale registers it uses.
-  auto step = [&](int t, int slot, int next, auto sbc, auto with_load) __attribute__((always_inline)) {
-    constexpr int sb = decltype(sbc)::value;
+  // Step t in slot t % NS, which takes step t + NS once consumed.
+  int slot = 0;
+  auto step = [&](int t, auto with_load) __attribute__((always_inline)) {
     constexpr bool load = decltype(with_load)::value;
-    read(slot, 1, 1);
+    const int next = slot + 1 == NS ? 0 : slot + 1;
+    constexpr int NM = FM * FN;
+    constexpr int R1 = (kReads + NM - 1) / NM, R2 = (kReads + kScaleReads + NM - 1) / NM;  // reads per MFMA, at least
+    // First sub-step: the second's fragments are read between its matrix instructions.
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+    for (int j = 0; j < NM; ++j) {
+      FG_MX_MFMA(j / FM, j % FM, 0, 0);
 #pragma unroll
-      for (int k = 0; k < FM; ++k) FG_MX_MFMA(i, k, 0, 0, sb);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int q = j * R1; q < (j + 1) * R1; ++q)
+        if (q < kReads) read(slot, 1, 1, q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     wait_lgkmcnt0();  // this wave's reads of the slot are done
     // step t + 1 has landed for this wave; t + 2 .. min(t + NS - 1, nk - 1) may still load
     if constexpr (load)
@@ -291,62 +316,37 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
       wait_steps<LPW, NS - 2>(min(NS - 2, nk - 2 - t));
     __builtin_amdgcn_s_barrier();  // ... and for every wave, and no wave still reads slot t
     __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 < nk) {
-      read(next, 0, 0);
-      read_scales(next, 1 - sb);
-    }
+    // Second sub-step: the next step's first fragments and scales are read, and the loads of step t + NS issued.
+    // (Behind the last step the ring holds nothing newer, and what is read is not used.)
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+    for (int j = 0; j < NM; ++j) {
+      FG_MX_MFMA(j / FM, j % FM, 1, 2);
 #pragma unroll
-      for (int k = 0; k < FM; ++k) {
-        FG_MX_MFMA(i, k, 1, 2, sb);
-        if constexpr (load) {
-          if (i * FM + k < LPW) {
-            __builtin_amdgcn_sched_barrier(0);
-            issue(t + NS, slot, i * FM + k);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
+      for (int q = j * R2; q < (j + 1) * R2; ++q)
+        if (q < kReads + kScaleReads) read(next, 0, 0, q);
+      if constexpr (load) {
+        if (j < LPW) issue(t + NS, slot, j);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (load) {
 #pragma unroll
-      for (int q = FM * FN; q < LPW; ++q) issue(t + NS, slot, q);
+      for (int q = NM; q < LPW; ++q) issue(t + NS, slot, q);
     }
+    take_scales();
     __builtin_amdgcn_sched_barrier(0);
-  };
-  int t = 0, slot = 0;
-  auto advance = [&](auto sbc, auto with_load) __attribute__((always_inline)) {
-    const int next = slot + 1 == NS ? 0 : slot + 1;
-    step(t, slot, next, sbc, with_load);
     slot = next;
-    ++t;
   };
-  using S0 = std::integral_constant<int, 0>;
-  using S1 = std::integral_constant<int, 1>;
-  // two steps per round, as the scale registers alternate; the tail has no more loads to issue
-  while (t + 1 + NS < nk) {
-    advance(S0{}, std::true_type{});
-    advance(S1{}, std::true_type{});
-  }
-  if (t + NS < nk) {
-    advance(S0{}, std::true_type{});
-    while (t < nk) {
-      advance(S1{}, std::false_type{});
-      if (t < nk) advance(S0{}, std::false_type{});
-    }
-  } else {
-    while (t < nk) {
-      advance(S0{}, std::false_type{});
-      if (t < nk) advance(S1{}, std::false_type{});
-    }
-  }
+  int t = 0;
+  for (; t + NS < nk; ++t) step(t, std::true_type{});  // NS - 1 steps in flight at each wait
+  for (; t < nk; ++t) step(t, std::false_type{});      // the tail: no more loads to issue
   wait_vmcnt<0>();  // no load still writes LDS when the workgroup ends
 #undef FG_MX_MFMA
 
   // Epilogue: acc[i][k] lane l holds output row m0 + wm * WM + k * 32 + l % 32 and the columns wn * WN + i * 32 + 8g +
   // 4 * half + 0..3 of the tile in elements 4g .. 4g + 3.
   if constexpr (EPI == kParts) {
-    float* dst = p.part + (int64_t)split * p.rows * p.wrows;
+    float* dst = p.part + (int64_t)split * p.rows * p.ldp;
 #pragma unroll
     for (int k = 0; k < FM; ++k) {
       const int m = m0 + wm * WM + k * 32 + l32;
@@ -356,13 +356,12 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int n = n0 + wn * WN + i * 32 + 8 * g + 4 * half;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < p.wrows) dst[(int64_t)m * p.wrows + n + e] = acc[i][k][4 * g + e];
+          if (n < p.ldp)  // whole groups of four: what lies behind the last column is never read
+            *(float4*)(dst + (int64_t)m * p.ldp + n) =
+                make_float4(acc[i][k][4 * g], acc[i][k][4 * g + 1], acc[i][k][4 * g + 2], acc[i][k][4 * g + 3]);
         }
     }
   } else if constexpr (EPI == kGateUp) {
-    const int out_steps = (p.cols + kStep - 1) / kStep;
 #pragma unroll
     for (int k = 0; k < FM; ++k) {
       const int m = m0 + wm * WM + k * 32 + l32;
@@ -400,7 +399,6 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
         }
       }
     }
-    (void)out_steps;
   } else {
     __syncthreads();  // no wave still reads the ring: each stages 32 of its rows at a time in it
     float* stage = (float*)smem + wave * 32 * OUT_LD;
@@ -449,14 +447,327 @@ __global__ void __launch_bounds__(256, 1) mx_gemm_kernel(MxArgs p) {
   }
 }
 
-template <int FMT, int BM, int BN, int WAVES_M, int NS, int EPI>
+// Up to 16 rows: the weights are streamed once, straight into registers, and the rows are read beside them. A
+// workgroup takes NT tiles of 16 weight rows (gate_up: 32 gate and 32 up rows, one block of 32 output columns) and its
+// waves take every waves-th step of 128 elements, so that together they read each row's bytes in order; v_mfma_scale_
+// f32_16x16x128_f8f6f4 multiplies a step (lane l: row l % 16; e2m1 elements 32 (l / 16) .. + 31, e4m3 elements
+// 16 (l / 16) .. + 15 and 64 further; scale of block l / 16 from a byte of its register; D: column l % 16 of the second
+// operand, rows 4 (l / 16) + 0..3 of the first). The waves' sums meet in LDS, added in wave order.
+// There are no loads to wait for but the weights, so the loop only keeps U steps of them in flight per wave; long
+// reductions over few columns take more waves per workgroup instead of a second launch.
+constexpr int kStreamLd = 20;  // floats per x row and tile in LDS: 16-byte stores on distinct banks
+
+template <int FMT, int NT, int U, int EPI>
+__global__ void __launch_bounds__(1024) mx_stream_kernel(MxArgs p) {
+  typedef float floatx4 __attribute__((ext_vector_type(4)));
+  constexpr int XR = FMT == fg::kE4M3 ? 2 : 1, XB = FMT == fg::kE4M3 ? 128 : 64;
+  constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;
+  static_assert(EPI != kGateUp || NT == 4, "gate_up: two tiles of gate rows and two of up rows");
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [waves][NT][16 x rows][16 weight rows]
+  constexpr int RLD = kStreamLd;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+  const int n0 = blockIdx.x * (EPI == kGateUp ? 32 : NT * 16);
+
+  const uint8_t* wrow[NT];
+  uint32_t wscale[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    int n = n0 + (EPI == kGateUp ? (i & 1) * 16 : i * 16) + r;
+    n = min(n, (EPI == kGateUp ? p.cols : p.wrows) - 1) + (EPI == kGateUp && i >= 2 ? p.cols : 0);
+    wrow[i] = p.w + (int64_t)n * p.wb;
+    wscale[i] = n;
+  }
+  const int m = min(r, p.rows - 1);
+  const uint8_t* xrow = p.x + (int64_t)m * p.xb;
+
+  floatx4 acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  int4 wv[U][NT], xv[U][XR];
+  uint32_t ws[U][NT], xs[U];
+  // A step's loads; chunks behind the rows' end (the last step of a K that is no multiple of 128) read the row's
+  // first bytes and count as zeros.
+  auto load = [&](int u, int t) __attribute__((always_inline)) {
+    const int wo = t * 64 + g * 16;
+    const bool w_in = wo < p.wb;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int4 v = *(const int4*)(wrow[i] + (w_in ? wo : 0));
+      wv[u][i] = w_in ? v : make_int4(0, 0, 0, 0);
+      ws[u][i] = p.ws[(int64_t)t * p.wrows + wscale[i]];
+    }
+#pragma unroll
+    for (int h = 0; h < XR; ++h) {
+      const int xo = t * XB + g * 16 + h * 64;
+      const bool x_in = xo < p.xb;
+      const int4 v = *(const int4*)(xrow + (x_in ? xo : 0));
+      xv[u][h] = x_in ? v : make_int4(0, 0, 0, 0);
+    }
+    xs[u] = p.xs[(int64_t)t * p.rows + m];
+  };
+  auto multiply = [&](int u) __attribute__((always_inline)) {
+    intx8 x = intx8{xv[u][0].x, xv[u][0].y, xv[u][0].z, xv[u][0].w, 0, 0, 0, 0};
+    if constexpr (XR == 2) {
+      x[4] = xv[u][1].x; x[5] = xv[u][1].y; x[6] = xv[u][1].z; x[7] = xv[u][1].w;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const intx8 w = intx8{wv[u][i].x, wv[u][i].y, wv[u][i].z, wv[u][i].w, 0, 0, 0, 0};
+      acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[i], 4, kBF, 0, (int)(ws[u][i] >> (8 * g)), 0,
+                                                                (int)(xs[u] >> (8 * g)));
+    }
+  };
+  int t = wave;
+  for (; t + (U - 1) * waves < p.steps; t += U * waves) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u, t + u * waves);
+#pragma unroll
+    for (int u = 0; u < U; ++u) multiply(u);
+  }
+  for (; t < p.steps; t += waves) {
+    load(0, t);
+    multiply(0);
+  }
+
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+    *(floatx4*)(red + ((wave * NT + i) * 16 + r) * RLD + 4 * g) = acc[i];  // x row r, weight rows 4g .. 4g + 3
+  __syncthreads();
+  auto sum = [&](int i, int row, int c) __attribute__((always_inline)) {
+    float v = 0.0f;
+    for (int w = 0; w < waves; ++w) v += red[((w * NT + i) * 16 + row) * RLD + c];
+    return v;
+  };
+  if constexpr (EPI == kGateUp) {
+    for (int e = tid; e < ((p.rows * 32 + 63) & ~63); e += blockDim.x) {  // whole waves
+      const int row = min(e >> 5, p.rows - 1), c = e & 31;
+      const float v = silu_mul(sum(c >> 4, row, c & 15), sum(2 + (c >> 4), row, c & 15));
+      uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
+      const uint32_t s = fg::mx_scale_byte<fg::kE4M3>(a);
+      const float y = s == 255u ? 0.0f : v * fg::mx_inverse_scale(s);
+      if ((e >> 5) >= p.rows) continue;
+      p.codes[(int64_t)row * p.cols + n0 + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+      if (c == 0) {
+        uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(n0 / kStep) * p.rows + row);
+        const int b = (n0 / 32) & 3;
+        sc[b] = (uint8_t)s;
+        if (n0 + 32 >= p.cols)  // the last block also writes the zeros behind it
+          for (int q = b + 1; q < 4; ++q) sc[q] = 0;
+      }
+    }
+  } else {
+    for (int e = tid; e < p.rows * NT * 16; e += blockDim.x) {
+      const int row = e / (NT * 16), c = e - row * (NT * 16), n = n0 + c;
+      if (n >= p.wrows) continue;
+      float v = sum(c >> 4, row, c & 15);
+      if (p.bias) v += fg::bf16_to_f32(p.bias[n]);
+      if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)row * p.ldr + n]);
+      p.out[(int64_t)row * p.ldo + n] = fg::f32_to_bf16(v);
+    }
+  }
+}
+
+// The sums of a split product, added in split order, with what the epilogue of an unsplit one does: four columns per
+// thread, or (gate_up) eight, sixteen threads to a dword of scales.
+__global__ void __launch_bounds__(256) mx_finish_linear_kernel(MxArgs p) {
+  const int groups = p.ldp / 4;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = e / groups;
+  if (row >= p.rows) return;
+  const int n = (int)(e - row * groups) * 4;
+  const float* src = p.part + row * p.ldp + n;
+  const int64_t stride = (int64_t)p.rows * p.ldp;
+  float4 a = *(const float4*)src;
+  for (int s = 1; s < p.splits; ++s) {
+    const float4 b = *(const float4*)(src + s * stride);
+    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+  }
+  const float v[4] = {a.x, a.y, a.z, a.w};
+  uint16_t* dst = p.out + row * p.ldo + n;
+  const uint16_t* res = p.residual ? p.residual + row * p.ldr + n : nullptr;
+  float o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    o[j] = v[j];
+    if (n + j < p.wrows) {
+      if (p.bias) o[j] += fg::bf16_to_f32(p.bias[n + j]);
+      if (res) o[j] += fg::bf16_to_f32(res[j]);
+    }
+  }
+  if (p.wide && n + 4 <= p.wrows) {
+    *(uint2*)dst = make_uint2(fg::pack_bf16x2(o[0], o[1]), fg::pack_bf16x2(o[2], o[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.wrows) dst[j] = fg::f32_to_bf16(o[j]);
+  }
+}
+
+__global__ void __launch_bounds__(256) mx_finish_gate_up_kernel(MxArgs p) {
+  const int out_steps = (p.cols + kStep - 1) / kStep;
+  const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, step) of these 16 threads
+  const int l = threadIdx.x & 15;
+  const int64_t row = g / out_steps;
+  const int step = (int)(g - row * out_steps), n = step * kStep + l * 8;
+  const bool row_ok = row < p.rows, valid = row_ok && n < p.cols;
+  float v[8];
+  if (valid) {
+    const int64_t stride = (int64_t)p.rows * p.ldp;
+    float gt[8], up[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) gt[j] = up[j] = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float* src = p.part + s * stride + row * p.ldp + n;
+      float a[8], b[8];
+      fg::load8<fg::kF32>(src, 0, a);
+      fg::load8<fg::kF32>(src + p.cols, 0, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        gt[j] += a[j];
+        up[j] += b[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = silu_mul(gt[j], up[j]);
+  }
+  fg::mx_store_step<fg::kE4M3>(v, valid, l, p.codes + row * p.cols + n, p.scales + (int64_t)step * p.rows + row, row_ok);
+}
+
+// ------------------------------------------------------------------ which kernel
+struct Tile {
+  int bm, bn;
+  float step_us;   // one step of one workgroup, a CU to itself (two at a time where two fit)
+  float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
+  bool pairs;      // two workgroups per CU
+};
+// Measured with e4m3 rows over 17 .. 1856 rows x 1536 .. 37888 columns x 1536 .. 18944.
+constexpr Tile kTiles[] = {
+    {64, 128, 0.29f, 2.0f, true},
+    {128, 128, 0.39f, 2.0f, true},
+    {128, 256, 0.66f, 2.5f, false},
+    {256, 256, 1.04f, 4.0f, false},
+};
+constexpr int kTileCount = 4, kMaxSplits = 16;
+
+struct Plan {
+  int tile;    // of kTiles; -1: the stream of few rows
+  int splits;
+};
+
+// Estimated microseconds of a plan: whole rounds of 256 workgroups (pairs fill the last one better), not under what
+// the card sustains in matrix work (power sets it: 2.8 PFLOP/s on random operands, 4.0 where both are e2m1) or reads;
+// a split product also writes and reads its fp32 sums and takes a second launch.
+float plan_us(const Tile& t, int splits, int fmt, int rows, int wrows, int steps) {
+  const int64_t tiles = (int64_t)((rows + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn);
+  const float n = (float)(tiles * splits);
+  const float rounds = t.pairs && n > 256 ? n / 256 : (float)((tiles * splits + 255) / 256);
+  const float work = rounds * ((steps + splits - 1) / splits) * t.step_us * (fmt == fg::kE4M3 ? 1.0f : 0.7f);
+  const float flops = 2.0f * tiles * t.bm * t.bn * steps * kStep / (fmt == fg::kE4M3 ? 2.8e9f : 4.0e9f);
+  const float bytes = ((float)wrows * steps * 68 + (float)rows * steps * 132) / 4.8e6f;
+  const float parts = splits == 1 ? 0.0f : 2.5f + (float)splits * rows * wrows * 4 * 2 / 4.5e6f;
+  return 4.0f + std::max(work, std::max(flops, bytes)) + rounds * t.tile_us + parts;
+}
+
+bool splits_ok(int steps, int splits) {
+  const int per = (steps + splits - 1) / splits;
+  return (steps + per - 1) / per == splits;
+}
+
+Plan make_plan(int fmt, int rows, int wrows, int steps, bool may_split) {
+  if (rows <= 8) return Plan{-1, 1};
+  Plan best{0, 1};
+  float least = 1e30f;
+  for (int c = 0; c < kTileCount; ++c)
+    for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
+      if (s > 1 && (steps / s < 3 || !splits_ok(steps, s))) continue;
+      const float us = plan_us(kTiles[c], s, fmt, rows, wrows, steps);
+      if (us < least) {
+        least = us;
+        best = Plan{c, s};
+      }
+    }
+  return best;
+}
+
+size_t parts_bytes(const Plan& plan, int rows, int wrows) {
+  return plan.splits > 1 ? (size_t)plan.splits * rows * ((wrows + 3) & ~3) * 4 : 0;
+}
+
+// ------------------------------------------------------------------ launches
+template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI>
 void launch(MxArgs p, int splits, hipStream_t s) {
   constexpr int kOutCols = EPI == kGateUp ? BN / 2 : BN;
   p.tiles_m = (p.rows + BM - 1) / BM;
   p.tiles_n = ((EPI == kGateUp ? p.cols : p.wrows) + kOutCols - 1) / kOutCols;
   p.tiles = p.tiles_m * p.tiles_n * splits;
   p.per_xcd = (p.tiles + 7) / 8;
-  hipLaunchKernelGGL((mx_gemm_kernel<FMT, BM, BN, WAVES_M, NS, EPI>), dim3(8 * p.per_xcd), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((mx_gemm_kernel<FMT, BM, BN, WAVES_M, WAVES_N, NS, EPI>), dim3(8 * p.per_xcd),
+                     dim3(64 * WAVES_M * WAVES_N), 0, s, p);
+}
+
+template <int FMT, int EPI>
+void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
+  switch (plan.tile) {
+    case 0: launch<FMT, 64, 128, 2, 2, 4, EPI>(p, plan.splits, s); break;
+    case 1: launch<FMT, 128, 128, 2, 2, 3, EPI>(p, plan.splits, s); break;
+    case 2: launch<FMT, 128, 256, 2, 4, 4, EPI>(p, plan.splits, s); break;
+    default: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
+  }
+}
+
+template <int FMT, int NT, int EPI>
+void launch_stream(const MxArgs& p, int waves, hipStream_t s) {
+  const int per = EPI == kGateUp ? 32 : NT * 16, cols = EPI == kGateUp ? p.cols : p.wrows;
+  hipLaunchKernelGGL((mx_stream_kernel<FMT, NT, 2, EPI>), dim3((cols + per - 1) / per), dim3(64 * waves),
+                     waves * NT * 16 * kStreamLd * 4, s, p);
+}
+
+template <int FMT, int EPI>
+void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
+  if (plan.tile < 0) {
+    // Eight waves per workgroup; twelve where a wave would have more than a dozen steps and columns are few.
+    const int waves = std::max(1, std::min(8, p.steps));
+    if constexpr (EPI == kGateUp) {
+      launch_stream<FMT, 4, EPI>(p, waves, s);
+    } else {
+      if (p.wrows >= 16384)
+        launch_stream<FMT, 4, EPI>(p, waves, s);
+      else
+        launch_stream<FMT, 1, EPI>(p, p.steps >= 96 ? 12 : waves, s);
+    }
+    return;
+  }
+  if (plan.splits == 1) {
+    launch_tile<FMT, EPI>(p, plan, s);
+    return;
+  }
+  launch_tile<FMT, kParts>(p, plan, s);
+  if constexpr (EPI == kGateUp) {
+    const int64_t groups = (int64_t)p.rows * ((p.cols + kStep - 1) / kStep);
+    hipLaunchKernelGGL(mx_finish_gate_up_kernel, dim3((unsigned)((groups + 15) / 16)), dim3(256), 0, s, p);
+  } else {
+    const int64_t n = (int64_t)p.rows * (p.ldp / 4);
+    hipLaunchKernelGGL(mx_finish_linear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p);
+  }
+}
+
+template <int EPI>
+void run(MxArgs p, int x_format, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  p.steps = (p.wb * 2 + kStep - 1) / kStep;
+  Plan plan = make_plan(x_format, p.rows, p.wrows, p.steps, true);
+  if (plan.splits > 1 && (!workspace || workspace_bytes < parts_bytes(plan, p.rows, p.wrows)))
+    plan = make_plan(x_format, p.rows, p.wrows, p.steps, false);
+  p.splits = plan.splits;
+  p.steps_per_split = (p.steps + plan.splits - 1) / plan.splits;
+  p.part = (float*)workspace;
+  p.ldp = (p.wrows + 3) & ~3;
+  if (x_format == fg::kE4M3)
+    run_format<fg::kE4M3, EPI>(p, plan, s);
+  else
+    run_format<fg::kE2M1, EPI>(p, plan, s);
 }
 
 int check(const char* what, const void* x_codes, const void* x_scales, int x_format, const void* w_codes,
@@ -480,13 +791,19 @@ int check(const char* what, const void* x_codes, const void* x_scales, int x_for
 
 extern "C" {
 
+size_t fg_mx_linear_workspace(int rows, int cols, int hidden, int x_format) {
+  if (rows <= 0 || cols <= 0 || hidden <= 0) return 0;
+  return parts_bytes(make_plan(x_format, rows, cols, (hidden + kStep - 1) / kStep, true), rows, cols);
+}
+
 int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const void* w_codes, const void* w_scales,
                  int rows, int cols, int hidden, const void* bias, const void* residual, int64_t ldr, void* out,
-                 int64_t ldo, void* stream) {
+                 int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check("fg_mx_linear", x_codes, x_scales, x_format, w_codes, w_scales, rows, cols, hidden)) return rc;
   FG_REQUIRE(out, "fg_mx_linear: null pointer");
   FG_REQUIRE(ldo >= cols && (!residual || ldr >= cols), "fg_mx_linear: bad row strides");
   FG_REQUIRE((((uintptr_t)out | (uintptr_t)bias | (uintptr_t)residual) & 1) == 0, "fg_mx_linear: outputs must be 2-byte aligned");
+  FG_REQUIRE(((uintptr_t)workspace & 15) == 0, "fg_mx_linear: workspace must be 16-byte aligned");
   MxArgs p{};
   p.x = (const uint8_t*)x_codes;
   p.xs = (const uint32_t*)x_scales;
@@ -497,31 +814,31 @@ int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const 
   p.rows = rows;
   p.cols = cols;
   p.wrows = cols;
-  p.steps = (hidden + kStep - 1) / kStep;
-  p.steps_per_split = p.steps;
   p.bias = (const uint16_t*)bias;
   p.residual = (const uint16_t*)residual;
   p.ldr = ldr;
   p.out = (uint16_t*)out;
   p.ldo = ldo;
   p.wide = ldo % 8 == 0 && ((uintptr_t)out & 15) == 0 && (!residual || (ldr % 8 == 0 && ((uintptr_t)residual & 15) == 0));
-  hipStream_t s = (hipStream_t)stream;
-  if (x_format == fg::kE4M3)
-    launch<fg::kE4M3, 128, 128, 2, 4, kLinear>(p, 1, s);
-  else
-    launch<fg::kE2M1, 128, 128, 2, 4, kLinear>(p, 1, s);
+  run<kLinear>(p, x_format, workspace, workspace_bytes, (hipStream_t)stream);
   return fg::check_launch("fg_mx_linear");
+}
+
+size_t fg_mx_gate_up_swiglu_workspace(int rows, int inter, int hidden, int x_format) {
+  if (rows <= 0 || inter <= 0 || hidden <= 0 || inter > (1 << 21)) return 0;
+  return parts_bytes(make_plan(x_format, rows, 2 * inter, (hidden + kStep - 1) / kStep, true), rows, 2 * inter);
 }
 
 int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format, const void* w_codes,
                          const void* w_scales, int rows, int inter, int hidden, void* codes, void* scales,
-                         void* stream) {
+                         void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check("fg_mx_gate_up_swiglu", x_codes, x_scales, x_format, w_codes, w_scales, rows, 2 * (int64_t)inter, hidden))
     return rc;
   FG_REQUIRE(codes && scales, "fg_mx_gate_up_swiglu: null pointer");
   FG_REQUIRE(inter % fg::kMxBlock == 0, "fg_mx_gate_up_swiglu: inter must be a multiple of 32");
   FG_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 3) == 0,
              "fg_mx_gate_up_swiglu: codes must be 16-byte aligned, scales 4-byte aligned");
+  FG_REQUIRE(((uintptr_t)workspace & 15) == 0, "fg_mx_gate_up_swiglu: workspace must be 16-byte aligned");
   MxArgs p{};
   p.x = (const uint8_t*)x_codes;
   p.xs = (const uint32_t*)x_scales;
@@ -532,15 +849,9 @@ int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format
   p.rows = rows;
   p.cols = inter;
   p.wrows = 2 * inter;
-  p.steps = (hidden + kStep - 1) / kStep;
-  p.steps_per_split = p.steps;
   p.codes = (uint8_t*)codes;
   p.scales = (uint32_t*)scales;
-  hipStream_t s = (hipStream_t)stream;
-  if (x_format == fg::kE4M3)
-    launch<fg::kE4M3, 128, 128, 2, 4, kGateUp>(p, 1, s);
-  else
-    launch<fg::kE2M1, 128, 128, 2, 4, kGateUp>(p, 1, s);
+  run<kGateUp>(p, x_format, workspace, workspace_bytes, (hipStream_t)stream);
   return fg::check_launch("fg_mx_gate_up_swiglu");
 }
 

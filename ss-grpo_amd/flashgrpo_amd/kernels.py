@@ -838,6 +838,13 @@ def _mx_operands(x, w, what):
     return x, w, rows, n, k, _on(what, *x, *w)
 
 
+def _mx_workspace(name, rows, cols, k, x, dev):
+    """A split product's sums: a buffer of the call's own, so that calls on two streams, or two captured graphs, share
+    none (torch's allocator keeps it until the stream, or the graph, is done with it)."""
+    n = getattr(_lib.load(), name)(rows, cols, k, MX_FORMATS[x.format])
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
 def mx_linear(x, w, *, bias=None, residual=None, out=None):
     """bf16 [rows, N] = x . w^T (+ bias) (+ residual) of MX rows x [rows, K] (e4m3 or e2m1) and a 4-bit MX weight w
     [N, K] (``fg_mx_linear``), summed in fp32 and rounded once. bias bf16 [N]; residual bf16 [rows, N] with unit
@@ -856,8 +863,10 @@ def mx_linear(x, w, *, bias=None, residual=None, out=None):
     if rows == 0 or N == 0:
         return out
     ld = lambda t: N if t is None or rows == 1 else t.stride(0)
+    ws = _mx_workspace("fg_mx_linear_workspace", rows, N, k, x, dev)
     _call_on(dev, "fg_mx_linear", _ptr(x.codes), _ptr(x.scales), MX_FORMATS[x.format], _ptr(w.codes), _ptr(w.scales),
-             rows, N, k, _ptr(bias), _ptr(residual), ld(residual), _ptr(out), ld(out))
+             rows, N, k, _ptr(bias), _ptr(residual), ld(residual), _ptr(out), ld(out), _ptr(ws),
+             0 if ws is None else ws.numel())
     return out
 
 
@@ -870,8 +879,9 @@ def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
         raise ValueError("mx_gate_up_swiglu: the weight must have 2 I rows, I a multiple of 32")
     q = _mx_out(out, rows, n2 // 2, "e4m3", dev, "mx_gate_up_swiglu")
     if rows:
+        ws = _mx_workspace("fg_mx_gate_up_swiglu_workspace", rows, n2 // 2, k, x, dev)
         _call_on(dev, "fg_mx_gate_up_swiglu", _ptr(x.codes), _ptr(x.scales), MX_FORMATS[x.format], _ptr(w.codes),
-                 _ptr(w.scales), rows, n2 // 2, k, _ptr(q.codes), _ptr(q.scales))
+                 _ptr(w.scales), rows, n2 // 2, k, _ptr(q.codes), _ptr(q.scales), _ptr(ws), 0 if ws is None else ws.numel())
     return q
 
 

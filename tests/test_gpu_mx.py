@@ -224,7 +224,10 @@ def check_linear(got, exact, err, bias=None, residual=None):
 
 
 SHAPES = [(1, 1, 32), (1, 2048, 1536), (2, 33, 96), (5, 77, 160), (15, 130, 512), (16, 64, 544), (17, 129, 640), (31, 256, 1184),
-          (64, 200, 2048), (65, 384, 288), (129, 257, 416), (200, 513, 1056), (257, 300, 384), (300, 700, 128)]
+          (64, 200, 2048), (65, 384, 288), (129, 257, 416), (200, 513, 1056), (257, 300, 384), (300, 700, 128),
+          # long reductions over few tiles (split over workgroups), and outputs of every tile size
+          (8, 16400, 160), (9, 50, 8192), (40, 300, 9600), (130, 520, 6016), (400, 1031, 4448), (700, 2050, 1120),
+          (1030, 4100, 576), (1900, 6000, 160)]
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
@@ -304,7 +307,8 @@ def check_gate_up(q, xv, wv, fmt, min_equal=0.97):
 
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("rows,inter,k", [(1, 32, 32), (1, 480, 1536), (3, 64, 160), (16, 96, 512), (17, 160, 544), (64, 288, 1056),
-                                          (65, 96, 256), (130, 352, 384), (260, 544, 128)])
+                                          (65, 96, 256), (130, 352, 384), (260, 544, 128), (20, 288, 4128), (300, 1056, 2080),
+                                          (1000, 2080, 288)])
 def test_gate_up_matches_float64(rows, inter, k, fmt):
     # magnitudes as after a norm (the gate has to move through SiLU's bend)
     codes, scales = O.quantize(rows_of(rows, k, rows + k, spread=0.5).double().numpy(), fmt)
@@ -312,6 +316,27 @@ def test_gate_up_matches_float64(rows, inter, k, fmt):
     codes, scales = O.quantize((rows_of(2 * inter, k, inter, spread=0.5) * k ** -0.5).double().numpy(), "e2m1")
     w, wv = device_mx(codes, scales, "e2m1"), O.values(codes, scales, "e2m1")
     check_gate_up(K().mx_gate_up_swiglu(x, w), xv, wv, fmt)
+
+
+@pytest.mark.parametrize("rows,n,k", [(40, 300, 9600), (400, 1031, 4448)])
+def test_without_workspace_a_split_product_runs_unsplit(rows, n, k):
+    from flashgrpo_amd import _lib
+
+    lib, kk = _lib.load(), K()
+    x, xv = random_mx(rows, k, "e4m3", rows)
+    w, wv = random_mx(n, k, "e2m1", n)
+    need = lib.fg_mx_linear_workspace(rows, n, k, 0)
+    assert need >= 2 * rows * n * 4
+    exact, err = product_bound(xv, wv, "e4m3")
+    for given in (0, need - 16, need):
+        ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)
+        out = torch.empty(rows, n, dtype=torch.bfloat16, device=DEV)
+        rc = lib.fg_mx_linear(x.codes.data_ptr(), x.scales.data_ptr(), 0, w.codes.data_ptr(), w.scales.data_ptr(), rows, n, k,
+                              None, None, n, out.data_ptr(), n, ws.data_ptr() if given else None, given, kk._stream())
+        assert rc == 0, lib.fg_last_error()
+        check_linear(out, exact, err)
+        assert (ws[need:] == 255).all() and ((ws == 255).all() or given == need)
+    assert torch.equal(out, kk.mx_linear(x, w))
 
 
 # ------------------------------------------------------------------ together
