@@ -294,18 +294,21 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
 
   // Step t in slot t % NS, which takes step t + NS once consumed.
   int slot = 0;
-  auto step = [&](int t, auto with_load) __attribute__((always_inline)) {
+  auto step = [&](int t, auto with_load, auto with_math) __attribute__((always_inline)) {
     constexpr bool load = decltype(with_load)::value;
+    constexpr bool math = decltype(with_math)::value;
     const int next = slot + 1 == NS ? 0 : slot + 1;
     constexpr int NM = FM * FN;
     constexpr int R1 = (kReads + NM - 1) / NM, R2 = (kReads + kScaleReads + NM - 1) / NM;  // reads per MFMA, at least
     // First sub-step: the second's fragments are read between its matrix instructions.
 #pragma unroll
     for (int j = 0; j < NM; ++j) {
-      FG_MX_MFMA(j / FM, j % FM, 0, 0);
+      if constexpr (math) {
+        FG_MX_MFMA(j / FM, j % FM, 0, 0);
 #pragma unroll
-      for (int q = j * R1; q < (j + 1) * R1; ++q)
-        if (q < kReads) read(slot, 1, 1, q);
+        for (int q = j * R1; q < (j + 1) * R1; ++q)
+          if (q < kReads) read(slot, 1, 1, q);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_lgkmcnt0();  // this wave's reads of the slot are done
@@ -320,10 +323,12 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     // (Behind the last step the ring holds nothing newer, and what is read is not used.)
 #pragma unroll
     for (int j = 0; j < NM; ++j) {
-      FG_MX_MFMA(j / FM, j % FM, 1, 2);
+      if constexpr (math) {
+        FG_MX_MFMA(j / FM, j % FM, 1, 2);
 #pragma unroll
-      for (int q = j * R2; q < (j + 1) * R2; ++q)
-        if (q < kReads + kScaleReads) read(next, 0, 0, q);
+        for (int q = j * R2; q < (j + 1) * R2; ++q)
+          if (q < kReads + kScaleReads) read(next, 0, 0, q);
+      }
       if constexpr (load) {
         if (j < LPW) issue(t + NS, slot, j);
       }
@@ -333,13 +338,21 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
 #pragma unroll
       for (int q = NM; q < LPW; ++q) issue(t + NS, slot, q);
     }
-    take_scales();
+    if constexpr (math) take_scales();
     __builtin_amdgcn_sched_barrier(0);
     slot = next;
   };
-  int t = 0;
-  for (; t + NS < nk; ++t) step(t, std::true_type{});  // NS - 1 steps in flight at each wait
-  for (; t < nk; ++t) step(t, std::false_type{});      // the tail: no more loads to issue
+  auto steps = [&](auto with_math) __attribute__((always_inline)) {
+    int t = 0;
+    for (; t + NS < nk; ++t) step(t, std::true_type{}, with_math);  // NS - 1 steps in flight at each wait
+    for (; t < nk; ++t) step(t, std::false_type{}, with_math);      // the tail: no more loads to issue
+  };
+  // A wave whose rows are all behind the last one loads its share and multiplies nothing: the card's power, which
+  // bounds large products, goes to the others.
+  if (m0 + wm * WM < p.rows)
+    steps(std::true_type{});
+  else
+    steps(std::false_type{});
   wait_vmcnt<0>();  // no load still writes LDS when the workgroup ends
 #undef FG_MX_MFMA
 
@@ -419,6 +432,22 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
           *(float4*)(stage + l32 * OUT_LD + i * 32 + 8 * g + 4 * half) =
               make_float4(acc[i][k][4 * g], acc[i][k][4 * g + 1], acc[i][k][4 * g + 2], acc[i][k][4 * g + 3]);
       __builtin_amdgcn_wave_barrier();
+      if (!p.wide) {  // rows that start anywhere: two bytes per lane, side by side
+        for (int r0 = 0; r0 < 32; ++r0) {
+          const int m = m0 + wm * WM + k * 32 + r0;
+          if (m >= p.rows) break;
+#pragma unroll
+          for (int c0 = 0; c0 < WN; c0 += 64) {
+            const int nn = n0 + wn * WN + c0 + lane;
+            if (c0 + lane >= WN || nn >= p.wrows) continue;
+            float v = stage[r0 * OUT_LD + c0 + lane];
+            if (p.bias) v += fg::bf16_to_f32(p.bias[nn]);
+            if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)m * p.ldr + nn]);
+            p.out[(int64_t)m * p.ldo + nn] = fg::f32_to_bf16(v);
+          }
+        }
+        continue;
+      }
 #pragma unroll
       for (int r0 = 0; r0 < 32; r0 += ROWS) {
         const int m = m0 + wm * WM + k * 32 + r0 + rr;
@@ -430,7 +459,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
         for (int e = 0; e < 8; ++e) v[e] += bv[e];
         uint16_t* dst = p.out + (int64_t)m * p.ldo + n;
         const uint16_t* res = p.residual ? p.residual + (int64_t)m * p.ldr + n : nullptr;
-        if (p.wide && n + 8 <= p.wrows) {
+        if (n + 8 <= p.wrows) {
           if (res) {
             float rv[8];
             fg::load8<fg::kBF16>(res, 0, rv);
@@ -455,6 +484,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
 // operand, rows 4 (l / 16) + 0..3 of the first). The waves' sums meet in LDS, added in wave order.
 // There are no loads to wait for but the weights, so the loop only keeps U steps of them in flight per wave; long
 // reductions over few columns take more waves per workgroup instead of a second launch.
+constexpr int kStreamRows = 16;
 constexpr int kStreamLd = 20;  // floats per x row and tile in LDS: 16-byte stores on distinct banks
 
 template <int FMT, int NT, int U, int EPI>
@@ -581,7 +611,8 @@ __global__ void __launch_bounds__(256) mx_finish_linear_kernel(MxArgs p) {
   const float* src = p.part + row * p.ldp + n;
   const int64_t stride = (int64_t)p.rows * p.ldp;
   float4 a = *(const float4*)src;
-  for (int s = 1; s < p.splits; ++s) {
+#pragma unroll 4
+  for (int s = 1; s < p.splits; ++s) {  // (several loads in flight)
     const float4 b = *(const float4*)(src + s * stride);
     a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
   }
@@ -619,6 +650,7 @@ __global__ void __launch_bounds__(256) mx_finish_gate_up_kernel(MxArgs p) {
     float gt[8], up[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) gt[j] = up[j] = 0.0f;
+#pragma unroll 2
     for (int s = 0; s < p.splits; ++s) {
       const float* src = p.part + s * stride + row * p.ldp + n;
       float a[8], b[8];
@@ -638,37 +670,53 @@ __global__ void __launch_bounds__(256) mx_finish_gate_up_kernel(MxArgs p) {
 
 // ------------------------------------------------------------------ which kernel
 struct Tile {
-  int bm, bn;
-  float step_us;   // one step of one workgroup, a CU to itself (two at a time where two fit)
+  int bm, bn, wave_rows;  // rows and weight rows of a workgroup, rows of a wave
+  float step_us;   // one step of one workgroup, a CU to itself
   float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
+  float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
   bool pairs;      // two workgroups per CU
 };
-// Measured with e4m3 rows over 17 .. 1856 rows x 1536 .. 37888 columns x 1536 .. 18944.
+// Fitted to times of every tile and several splits with e4m3 rows over 1 .. 3500 rows x 700 .. 37888 columns x 640 ..
+// 18944: what the estimate picks is 3 % behind the fastest in the geometric mean, 25 % at worst.
 constexpr Tile kTiles[] = {
-    {64, 128, 0.29f, 2.0f, true},
-    {128, 128, 0.39f, 2.0f, true},
-    {128, 256, 0.66f, 2.5f, false},
-    {256, 256, 1.04f, 4.0f, false},
+    {64, 128, 32, 0.31f, 2.0f, 1.6f, true},
+    {128, 128, 64, 0.42f, 2.0f, 1.9f, true},
+    {128, 256, 64, 0.66f, 2.5f, 2.35f, false},
+    {192, 256, 96, 0.86f, 3.5f, 2.6f, false},
+    {256, 256, 64, 1.04f, 4.0f, 2.75f, false},
 };
-constexpr int kTileCount = 4, kMaxSplits = 16;
+constexpr int kTileCount = 5, kMaxSplits = 16;
 
 struct Plan {
   int tile;    // of kTiles; -1: the stream of few rows
   int splits;
 };
 
-// Estimated microseconds of a plan: whole rounds of 256 workgroups (pairs fill the last one better), not under what
-// the card sustains in matrix work (power sets it: 2.8 PFLOP/s on random operands, 4.0 where both are e2m1) or reads;
-// a split product also writes and reads its fp32 sums and takes a second launch.
+constexpr float kReadRate = 5.5e6f;  // bytes per us that the weights are read at
+
+// Estimated microseconds of a plan: whole rounds of 256 workgroups (a second one beside the first takes 0.7 of its
+// time, more of them 0.95), not under what the card sustains in matrix work (1.45 times as much where both operands are
+// e2m1) or reads; a split product also writes and reads its fp32 sums and takes a second launch.
 float plan_us(const Tile& t, int splits, int fmt, int rows, int wrows, int steps) {
-  const int64_t tiles = (int64_t)((rows + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn);
+  const int64_t tiles_n = (wrows + t.bn - 1) / t.bn, tiles = (int64_t)((rows + t.bm - 1) / t.bm) * tiles_n;
   const float n = (float)(tiles * splits);
-  const float rounds = t.pairs && n > 256 ? n / 256 : (float)((tiles * splits + 255) / 256);
+  const float rounds = t.pairs && n > 256 ? std::max(1.7f, 0.95f * n / 256) : (float)((tiles * splits + 255) / 256);
   const float work = rounds * ((steps + splits - 1) / splits) * t.step_us * (fmt == fg::kE4M3 ? 1.0f : 0.7f);
-  const float flops = 2.0f * tiles * t.bm * t.bn * steps * kStep / (fmt == fg::kE4M3 ? 2.8e9f : 4.0e9f);
-  const float bytes = ((float)wrows * steps * 68 + (float)rows * steps * 132) / 4.8e6f;
-  const float parts = splits == 1 ? 0.0f : 2.5f + (float)splits * rows * wrows * 4 * 2 / 4.5e6f;
-  return 4.0f + std::max(work, std::max(flops, bytes)) + rounds * t.tile_us + parts;
+  const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
+  const float flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (fmt == fg::kE4M3 ? 1e9f : 1.45e9f));
+  const float bytes = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
+  const float sums = (float)splits * rows * wrows * 4 * 2;
+  const float parts = splits == 1 ? 0.0f : 2.5f + sums / (sums < 16e6f ? 9e6f : 5e6f);
+  return 2.0f + std::max(work, std::max(flops, bytes)) + rounds * t.tile_us + parts;
+}
+
+// The same for the stream of up to 16 rows, which has no second launch and no ring to fill but reads the rows again for
+// every 16 weight rows (gate_up and wide outputs, four tiles to a workgroup: every 64), and gains nothing from its
+// waves where the steps are fewer than they.
+constexpr int kWideCols = 16384;
+float stream_us(bool wide, int rows, int wrows, int steps) {
+  const float wgs = (float)wrows / (wide ? 64 : 16);
+  return (wide ? 3.0f : 4.5f) + (float)wrows * steps * 68 / kReadRate + rows * wgs * steps * 1.3e-5f + (steps < 8 ? 1.5f : 0.0f);
 }
 
 bool splits_ok(int steps, int splits) {
@@ -676,8 +724,7 @@ bool splits_ok(int steps, int splits) {
   return (steps + per - 1) / per == splits;
 }
 
-Plan make_plan(int fmt, int rows, int wrows, int steps, bool may_split) {
-  if (rows <= 8) return Plan{-1, 1};
+Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_split) {
   Plan best{0, 1};
   float least = 1e30f;
   for (int c = 0; c < kTileCount; ++c)
@@ -689,6 +736,7 @@ Plan make_plan(int fmt, int rows, int wrows, int steps, bool may_split) {
         best = Plan{c, s};
       }
     }
+  if (rows <= kStreamRows && stream_us(gate_up || wrows >= kWideCols, rows, wrows, steps) <= least) return Plan{-1, 1};
   return best;
 }
 
@@ -714,6 +762,7 @@ void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
     case 0: launch<FMT, 64, 128, 2, 2, 4, EPI>(p, plan.splits, s); break;
     case 1: launch<FMT, 128, 128, 2, 2, 3, EPI>(p, plan.splits, s); break;
     case 2: launch<FMT, 128, 256, 2, 4, 4, EPI>(p, plan.splits, s); break;
+    case 3: launch<FMT, 192, 256, 2, 4, 3, EPI>(p, plan.splits, s); break;
     default: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
   }
 }
@@ -733,7 +782,7 @@ void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
     if constexpr (EPI == kGateUp) {
       launch_stream<FMT, 4, EPI>(p, waves, s);
     } else {
-      if (p.wrows >= 16384)
+      if (p.wrows >= kWideCols)
         launch_stream<FMT, 4, EPI>(p, waves, s);
       else
         launch_stream<FMT, 1, EPI>(p, p.steps >= 96 ? 12 : waves, s);
@@ -757,9 +806,9 @@ void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
 template <int EPI>
 void run(MxArgs p, int x_format, void* workspace, size_t workspace_bytes, hipStream_t s) {
   p.steps = (p.wb * 2 + kStep - 1) / kStep;
-  Plan plan = make_plan(x_format, p.rows, p.wrows, p.steps, true);
+  Plan plan = make_plan(EPI == kGateUp, x_format, p.rows, p.wrows, p.steps, true);
   if (plan.splits > 1 && (!workspace || workspace_bytes < parts_bytes(plan, p.rows, p.wrows)))
-    plan = make_plan(x_format, p.rows, p.wrows, p.steps, false);
+    plan = make_plan(EPI == kGateUp, x_format, p.rows, p.wrows, p.steps, false);
   p.splits = plan.splits;
   p.steps_per_split = (p.steps + plan.splits - 1) / plan.splits;
   p.part = (float*)workspace;
@@ -793,7 +842,7 @@ extern "C" {
 
 size_t fg_mx_linear_workspace(int rows, int cols, int hidden, int x_format) {
   if (rows <= 0 || cols <= 0 || hidden <= 0) return 0;
-  return parts_bytes(make_plan(x_format, rows, cols, (hidden + kStep - 1) / kStep, true), rows, cols);
+  return parts_bytes(make_plan(false, x_format, rows, cols, (hidden + kStep - 1) / kStep, true), rows, cols);
 }
 
 int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const void* w_codes, const void* w_scales,
@@ -826,7 +875,7 @@ int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const 
 
 size_t fg_mx_gate_up_swiglu_workspace(int rows, int inter, int hidden, int x_format) {
   if (rows <= 0 || inter <= 0 || hidden <= 0 || inter > (1 << 21)) return 0;
-  return parts_bytes(make_plan(x_format, rows, 2 * inter, (hidden + kStep - 1) / kStep, true), rows, 2 * inter);
+  return parts_bytes(make_plan(true, x_format, rows, 2 * inter, (hidden + kStep - 1) / kStep, true), rows, 2 * inter);
 }
 
 int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format, const void* w_codes,

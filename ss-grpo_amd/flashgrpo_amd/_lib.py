@@ -112,9 +112,9 @@ def load() -> C.CDLL:
 
 
 def call(name: str, *args) -> int:
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
-    if SIGNATURES[name][0] is _I and rc != 0:
+    if rc != 0 and SIGNATURES[name][0] is _I:
         msg = lib.fg_last_error().decode(errors="replace")
         if "null pointer" in msg or "bad" in msg or "must" in msg or "shape" in msg:
             raise ValueError(msg)

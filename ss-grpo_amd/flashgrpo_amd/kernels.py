@@ -692,6 +692,7 @@ def linear_rope_kv_write(x, w_pairs, bias_pairs, *, tile=(64, 64), stages=0, bat
 # ------------------------------------------------------------------ microscaled (MX) rows
 MX_BLOCK = 32                         # elements per scale
 MX_FORMATS = {"e4m3": 0, "e2m1": 1}   # fg_mx_quantize's format codes
+_U8, _FP8, _BF16 = torch.uint8, torch.float8_e4m3fn, torch.bfloat16
 
 
 class MX(NamedTuple):
@@ -711,53 +712,63 @@ class MX(NamedTuple):
         return self.codes.shape[0], self.codes.shape[1] * (2 if self.codes.dtype == torch.uint8 else 1)
 
 
-def _on(what, *ts):
-    """The one device of the given tensors (None entries aside)."""
-    _dev(*ts)
-    dev = ts[0].device
-    if any(t is not None and t.device != dev for t in ts):
-        raise ValueError(f"{what}: tensors on different devices")
-    return dev
+# The calls below serve single tokens, where a launch costs 3.5 us of host time and every check counts: devices are
+# compared as indices and shapes in one expression each, and what is wrong is worked out after a check has failed.
+def _same_device(what, dev, *ts) -> None:
+    """Raises unless every given tensor (None aside) is on GPU ``dev`` (a device index, -1 for the CPU)."""
+    if dev < 0:
+        raise ValueError("flashgrpo_amd kernels take device tensors (got a CPU tensor)")
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on different devices")
 
 
 def _call_on(dev, name, *args):
-    """The call on ``dev``'s current stream, whichever device is the current one."""
-    if dev.index == _cur_device():
-        _call(name, *args, _stream())
+    """The call on GPU ``dev``'s current stream, whichever device is the current one."""
+    if dev == _cur_device():
+        _call(name, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            _call(name, *args, _stream())
+            _call(name, *args, _raw_stream(dev))
 
 
-def _mx_of(q, what, *, cols=None):
-    """q as an MX pair whose tensors are what the kernels take: (MX, rows, cols)."""
-    codes, scales = q
-    q = MX(codes, scales)
-    if codes.dtype not in (torch.uint8, torch.float8_e4m3fn) or scales.dtype != torch.uint8 or codes.dim() != 2:
+def _mx_bad(codes, scales, what):
+    if codes.dtype not in (_U8, _FP8) or scales.dtype != _U8 or codes.dim() != 2:
         raise TypeError(f"{what}: MX codes must be float8_e4m3fn or uint8 [rows, ..] with uint8 scales")
-    rows, k = q.shape
-    if k == 0 or k % MX_BLOCK or (cols is not None and k != cols):
-        raise ValueError(f"{what}: MX rows of {k} elements; expected {cols if cols else 'a multiple of 32'}")
+    rows, k = MX(codes, scales).shape
+    if k == 0 or k % MX_BLOCK:
+        raise ValueError(f"{what}: MX rows of {k} elements; expected a multiple of 32")
     if tuple(scales.shape) != (-(-k // 128), rows, 4):
         raise ValueError(f"{what}: MX scales must be [{-(-k // 128)}, {rows}, 4], got {list(scales.shape)}")
-    if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
-        raise ValueError(f"{what}: MX codes and scales must be contiguous, 16- and 4-byte aligned")
-    return q, rows, k
+    raise ValueError(f"{what}: MX codes and scales must be contiguous, 16- and 4-byte aligned, on one device")
 
 
-def _mx_empty(rows, cols, fmt, dev) -> MX:
-    codes = (torch.empty(rows, cols // 2, dtype=torch.uint8, device=dev) if fmt == "e2m1"
-             else torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device=dev))
-    return MX(codes, torch.empty(-(-cols // 128), rows, 4, dtype=torch.uint8, device=dev))
+def _mx_of(q, what):
+    """(codes, scales, format code, rows, cols, device index) of an MX pair as the kernels take it."""
+    codes, scales = q
+    dt = codes.dtype
+    if (dt is not _U8 and dt is not _FP8) or codes.dim() != 2:
+        _mx_bad(codes, scales, what)
+    rows, k = codes.shape
+    fmt = 0
+    if dt is _U8:
+        fmt, k = 1, 2 * k
+    dev = codes.get_device()
+    if (k % 32 or k == 0 or scales.dtype is not _U8 or scales.shape != ((k + 127) // 128, rows, 4)
+            or not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 4
+            or scales.get_device() != dev):
+        _mx_bad(codes, scales, what)
+    return codes, scales, fmt, rows, k, dev
 
 
-def _mx_out(out, rows, cols, fmt, dev, what) -> MX:
+def _mx_out(out, rows, cols, fmt, device, what) -> MX:
     if out is None:
-        return _mx_empty(rows, cols, fmt, dev)
-    q, r, k = _mx_of(out, what)
-    if (r, k) != (rows, cols) or q.format != fmt or _on(what, *q) != dev:
-        raise ValueError(f"{what}: out must be an {fmt} MX pair of [{rows}, {cols}] on {dev}")
-    return q
+        return MX(torch.empty(rows, cols // 2 if fmt else cols, dtype=_U8 if fmt else _FP8, device=device),
+                  torch.empty((cols + 127) // 128, rows, 4, dtype=_U8, device=device))
+    codes, scales, f, r, k, dev = _mx_of(out, what)
+    if (r, k, f, dev) != (rows, cols, fmt, device.index):
+        raise ValueError(f"{what}: out must be an {'e2m1' if fmt else 'e4m3'} MX pair of [{rows}, {cols}] on {device}")
+    return MX(codes, scales)
 
 
 def mx_quantize(x, fmt="e2m1", *, out=None) -> MX:
@@ -765,38 +776,44 @@ def mx_quantize(x, fmt="e2m1", *, out=None) -> MX:
     (4 bits). Each block of 32 elements gets the smallest power-of-two scale >= 2^-126 that holds it without
     saturation; a block that holds an infinity or a NaN becomes NaN. x bf16 or fp32 with unit column stride and
     16-byte aligned rows. ``out``: an MX pair to overwrite in place (a weight that is quantised again)."""
-    dev = _on("mx_quantize", x)
-    if fmt not in MX_FORMATS:
+    dev = x.get_device()
+    _same_device("mx_quantize", dev)
+    f = MX_FORMATS.get(fmt)
+    if f is None:
         raise ValueError(f"mx_quantize: fmt must be one of {tuple(MX_FORMATS)}")
-    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % MX_BLOCK:
-        raise ValueError("mx_quantize: x must be [rows, cols] with cols a multiple of 32")
     dt = dtype_code(x)
-    rows, cols = x.shape
-    q = _mx_out(out, rows, cols, fmt, dev, "mx_quantize")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0 or shape[1] % MX_BLOCK:
+        raise ValueError("mx_quantize: x must be [rows, cols] with cols a multiple of 32")
+    rows, cols = shape
+    q = _mx_out(out, rows, cols, f, x.device, "mx_quantize")
     if rows == 0:
         return q
-    ldx = x.stride(0) if rows > 1 else cols
-    if x.stride(1) != 1 or ldx % 8 or ldx < cols or x.data_ptr() % 16:
-        raise ValueError("mx_quantize: x rows must have unit column stride and start 16-byte aligned")
-    _call_on(dev, "fg_mx_quantize", _ptr(x), dt, ldx, rows, cols, MX_FORMATS[fmt], _ptr(q.codes), _ptr(q.scales))
+    ldx = cols
+    if not x.is_contiguous():
+        ldx = x.stride(0) if rows > 1 else cols
+        if x.stride(1) != 1 or ldx < cols:
+            raise ValueError("mx_quantize: x rows must have unit column stride")
+    if ldx % 8 or x.data_ptr() % 16:
+        raise ValueError("mx_quantize: x rows must start 16-byte aligned")
+    _call_on(dev, "fg_mx_quantize", x.data_ptr(), dt, ldx, rows, cols, f, q[0].data_ptr(), q[1].data_ptr())
     return q
 
 
 def mx_dequantize(q, dtype=torch.bfloat16, *, out=None):
     """The values that an MX pair stands for, [rows, cols] in bf16 (exact but under 2^-126) or fp32
     (``fg_mx_dequantize``)."""
-    q, rows, cols = _mx_of(q, "mx_dequantize")
-    dev = _on("mx_dequantize", *q, out)
+    codes, scales, f, rows, cols, dev = _mx_of(q, "mx_dequantize")
+    _same_device("mx_dequantize", dev, out)
     if out is None:
         if dtype not in _DT:
             raise TypeError("mx_dequantize: dtype must be bfloat16 or float32")
-        out = torch.empty(rows, cols, dtype=dtype, device=dev)
+        out = torch.empty(rows, cols, dtype=dtype, device=codes.device)
     elif tuple(out.shape) != (rows, cols) or out.dtype not in _DT or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"mx_dequantize: out must be a contiguous 16-byte aligned bf16 or fp32 [{rows}, {cols}] tensor")
-    if rows == 0:
-        return out
-    _call_on(dev, "fg_mx_dequantize", _ptr(q.codes), _ptr(q.scales), MX_FORMATS[q.format], rows, cols, _ptr(out),
-             dtype_code(out), cols)
+    if rows:
+        _call_on(dev, "fg_mx_dequantize", codes.data_ptr(), scales.data_ptr(), f, rows, cols, out.data_ptr(),
+                 dtype_code(out), cols)
     return out
 
 
@@ -805,83 +822,109 @@ def rmsnorm_mx(x, weight, eps, *, delta=None, sum_out=None, out=None) -> MX:
     dimension of x [rows, H], H a multiple of 32 up to 8192. With delta the sum, rounded to x's dtype, is written to
     ``sum_out`` (x itself when not given). x, delta, weight and sum_out contiguous, one dtype (bf16 or fp32). The
     norm is not rounded between its steps: the codes are those of the formula in 64 bits."""
-    dev = _on("rmsnorm_mx", x, weight, delta, sum_out)
+    dev = x.get_device()
+    _same_device("rmsnorm_mx", dev, weight, delta, sum_out)
     dt = dtype_code(x)
-    if x.dim() != 2:
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2:
         raise ValueError("rmsnorm_mx: x must be [rows, H]")
-    rows, H = x.shape
+    rows, H = shape
     if H == 0 or H % MX_BLOCK or H > 8192:
         raise ValueError("rmsnorm_mx: H must be a multiple of 32, at most 8192")
-    if weight.numel() != H or weight.dtype != x.dtype or not weight.is_contiguous():
-        raise ValueError("rmsnorm_mx: weight must be a contiguous [H] tensor of x's dtype")
-    if delta is None and sum_out is not None:
-        raise ValueError("rmsnorm_mx: sum_out without delta")
-    if delta is not None and sum_out is None:
+    if weight.numel() != H or weight.dtype is not dtype or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError("rmsnorm_mx: weight must be a contiguous 16-byte aligned [H] tensor of x's dtype")
+    if delta is None:
+        if sum_out is not None:
+            raise ValueError("rmsnorm_mx: sum_out without delta")
+        rest = (x,)
+    elif sum_out is None:
         sum_out = x
-    for t, n in ((x, "x"), (delta, "delta"), (sum_out, "sum_out")):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16):
-            raise ValueError(f"rmsnorm_mx: {n} must be a contiguous, 16-byte aligned tensor of x's shape and dtype")
-    if weight.data_ptr() % 16:
-        raise ValueError("rmsnorm_mx: weight must be 16-byte aligned")
-    q = _mx_out(out, rows, H, "e4m3", dev, "rmsnorm_mx")
+        rest = (x, delta)
+    else:
+        rest = (x, delta, sum_out)
+    for t in rest:
+        if not t.is_contiguous() or t.data_ptr() % 16 or (t is not x and (t.shape != shape or t.dtype is not dtype)):
+            raise ValueError("rmsnorm_mx: x, delta and sum_out must be contiguous, 16-byte aligned and of one shape and "
+                             "dtype")
+    q = _mx_out(out, rows, H, 0, x.device, "rmsnorm_mx")
     if rows:
-        _call_on(dev, "fg_rmsnorm_mx", _ptr(x), _ptr(delta), _ptr(weight), _ptr(sum_out), dt, rows, H, float(eps),
-                 _ptr(q.codes), _ptr(q.scales))
+        _call_on(dev, "fg_rmsnorm_mx", x.data_ptr(), _ptr(delta), weight.data_ptr(), _ptr(sum_out), dt, rows, H,
+                 float(eps), q[0].data_ptr(), q[1].data_ptr())
     return q
 
 
 def _mx_operands(x, w, what):
-    x, rows, k = _mx_of(x, what)
-    w, n, _ = _mx_of(w, what, cols=k)
-    if w.format != "e2m1":
+    """Both operands of a product as addresses and sizes: x's and w's pointers and x's format in the entry points'
+    order, then rows, weight rows, K and the device index."""
+    xc, xs, f, rows, k, dev = _mx_of(x, what)
+    wc, ws, wf, n, kw, wdev = _mx_of(w, what)
+    if dev != wdev or dev < 0:
+        _same_device(what, dev, wc)
+    if kw != k:
+        raise ValueError(f"{what}: x has {k} columns and the weight {kw}")
+    if wf != 1:
         raise TypeError(f"{what}: the weight must be in e2m1 (4 bits)")
-    return x, w, rows, n, k, _on(what, *x, *w)
+    return (xc.data_ptr(), xs.data_ptr(), f, wc.data_ptr(), ws.data_ptr()), rows, n, k, dev
 
 
-def _mx_workspace(name, rows, cols, k, x, dev):
-    """A split product's sums: a buffer of the call's own, so that calls on two streams, or two captured graphs, share
-    none (torch's allocator keeps it until the stream, or the graph, is done with it)."""
-    n = getattr(_lib.load(), name)(rows, cols, k, MX_FORMATS[x.format])
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+def _mx_workspace(name, rows, cols, k, fmt, device):
+    """(tensor, address, bytes) for a split product's sums: a buffer of the call's own, so that calls on two streams, or
+    two captured graphs, share none (torch's allocator keeps it until the stream, or the graph, is done with it)."""
+    n = getattr(_lib.load(), name)(rows, cols, k, fmt)
+    if n == 0:
+        return None, None, 0
+    ws = torch.empty(n, dtype=_U8, device=device)
+    return ws, ws.data_ptr(), n
 
 
 def mx_linear(x, w, *, bias=None, residual=None, out=None):
     """bf16 [rows, N] = x . w^T (+ bias) (+ residual) of MX rows x [rows, K] (e4m3 or e2m1) and a 4-bit MX weight w
     [N, K] (``fg_mx_linear``), summed in fp32 and rounded once. bias bf16 [N]; residual bf16 [rows, N] with unit
     column stride; ``out`` bf16 with unit column stride, which may be the residual (an update in place)."""
-    x, w, rows, N, k, dev = _mx_operands(x, w, "mx_linear")
-    if _on("mx_linear", x.codes, bias, residual, out) != dev:
-        raise ValueError("mx_linear: tensors on different devices")
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.numel() != N or not bias.is_contiguous()):
+    operands, rows, N, k, dev = _mx_operands(x, w, "mx_linear")
+    _same_device("mx_linear", dev, bias, residual, out)
+    if bias is not None and (bias.dtype is not _BF16 or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError(f"mx_linear: bias must be a contiguous bf16 [{N}] tensor")
+    device = w[0].device
     if out is None:
-        out = torch.empty(rows, N, dtype=torch.bfloat16, device=dev)
-    for t, n in ((residual, "residual"), (out, "out")):
-        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (rows, N) or (N > 1 and t.stride(1) != 1)
-                              or (rows > 1 and t.stride(0) < N)):
-            raise ValueError(f"mx_linear: {n} must be bf16 [{rows}, {N}] with unit column stride")
+        out = torch.empty(rows, N, dtype=_BF16, device=device)
+        ldo = N
+    else:
+        ldo = _mx_rows(out, rows, N, "out")
+    ldr = N if residual is None else _mx_rows(residual, rows, N, "residual")
     if rows == 0 or N == 0:
         return out
-    ld = lambda t: N if t is None or rows == 1 else t.stride(0)
-    ws = _mx_workspace("fg_mx_linear_workspace", rows, N, k, x, dev)
-    _call_on(dev, "fg_mx_linear", _ptr(x.codes), _ptr(x.scales), MX_FORMATS[x.format], _ptr(w.codes), _ptr(w.scales),
-             rows, N, k, _ptr(bias), _ptr(residual), ld(residual), _ptr(out), ld(out), _ptr(ws),
-             0 if ws is None else ws.numel())
+    ws, ws_ptr, ws_bytes = _mx_workspace("fg_mx_linear_workspace", rows, N, k, operands[2], device)
+    _call_on(dev, "fg_mx_linear", *operands, rows, N, k, _ptr(bias), _ptr(residual), ldr, out.data_ptr(), ldo, ws_ptr,
+             ws_bytes)
     return out
+
+
+def _mx_rows(t, rows, n, what):
+    """The row stride of a bf16 [rows, n] tensor with unit column stride."""
+    if t.dtype is not _BF16 or t.shape != (rows, n):
+        raise ValueError(f"mx_linear: {what} must be bf16 [{rows}, {n}]")
+    if t.is_contiguous() or rows == 1 and (n == 1 or t.stride(1) == 1):
+        return n
+    if (n > 1 and t.stride(1) != 1) or t.stride(0) < n:
+        raise ValueError(f"mx_linear: {what} must have unit column stride and rows apart")
+    return t.stride(0)
 
 
 def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
     """MX e4m3 [rows, I] of SiLU(x . w[:I]^T) * (x . w[I:]^T) (``fg_mx_gate_up_swiglu``): MX rows x [rows, K] (e4m3
     or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums and the activation in
     fp32, rounded once, to the 8-bit codes."""
-    x, w, rows, n2, k, dev = _mx_operands(x, w, "mx_gate_up_swiglu")
+    operands, rows, n2, k, dev = _mx_operands(x, w, "mx_gate_up_swiglu")
     if n2 == 0 or n2 % (2 * MX_BLOCK):
         raise ValueError("mx_gate_up_swiglu: the weight must have 2 I rows, I a multiple of 32")
-    q = _mx_out(out, rows, n2 // 2, "e4m3", dev, "mx_gate_up_swiglu")
+    device = w[0].device
+    inter = n2 // 2
+    q = _mx_out(out, rows, inter, 0, device, "mx_gate_up_swiglu")
     if rows:
-        ws = _mx_workspace("fg_mx_gate_up_swiglu_workspace", rows, n2 // 2, k, x, dev)
-        _call_on(dev, "fg_mx_gate_up_swiglu", _ptr(x.codes), _ptr(x.scales), MX_FORMATS[x.format], _ptr(w.codes),
-                 _ptr(w.scales), rows, n2 // 2, k, _ptr(q.codes), _ptr(q.scales), _ptr(ws), 0 if ws is None else ws.numel())
+        ws, ws_ptr, ws_bytes = _mx_workspace("fg_mx_gate_up_swiglu_workspace", rows, inter, k, operands[2], device)
+        _call_on(dev, "fg_mx_gate_up_swiglu", *operands, rows, inter, k, q[0].data_ptr(), q[1].data_ptr(), ws_ptr,
+                 ws_bytes)
     return q
 
 

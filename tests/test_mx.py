@@ -100,8 +100,8 @@ def test_mx_pairs_are_checked():
     from flashgrpo_amd import kernels as K
 
     codes, scales = torch.zeros(2, 96, dtype=torch.uint8), torch.zeros(2, 2, 4, dtype=torch.uint8)
-    assert K._mx_of((codes, scales), "t")[1:] == (2, 192)
-    for bad in ((codes.float(), scales), (codes, scales.float())):
+    assert K._mx_of((codes, scales), "t")[2:] == (1, 2, 192, -1)
+    for bad in ((codes.float(), scales), (codes, scales.float()), (codes[0], scales)):
         with pytest.raises(TypeError):
             K._mx_of(bad, "t")
     for bad in ((codes[:, :95], scales), (codes[:, :8], scales), (codes, scales[:1]), (codes, scales[:, :1]),
