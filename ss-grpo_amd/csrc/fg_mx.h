@@ -29,7 +29,7 @@ FG_DEVICE uint32_t mx_scale_byte(uint32_t amax_bits) {  // amax_bits: of the lar
 }
 
 // 2^(127 - s), the factor that takes a block's values to its codes' grid (exact: s in [1, 247]); 0 for a NaN block,
-// whose codes then hold 0 (or NaN, which its scale says anyway).
+// whose codes are of no account.
 FG_DEVICE float mx_inverse_scale(uint32_t s) { return __uint_as_float(s == 255u ? 0u : (254u - s) << 23); }
 
 // 2^(s - 127), NaN for 255. s = 0, 2^-127, is a subnormal float.
@@ -63,7 +63,7 @@ FG_DEVICE uint2 mx_pack8(const float (&v)[8]) {
 FG_DEVICE uint32_t mx_amax8(const float (&v)[8]) {
   uint32_t a = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(v[j]) & 0x7fffffffu);
+  for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(v[j]) & 0x7fffffffu);  // (v_max3_u32 takes two)
   return a;
 }
 
@@ -83,7 +83,7 @@ FG_DEVICE void mx_store_step(const float (&v)[8], bool valid, int l, uint8_t* co
     const float inv = mx_inverse_scale(s);
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = s == 255u ? 0.0f : v[j] * inv;
+    for (int j = 0; j < 8; ++j) y[j] = v[j] * inv;
     const uint2 c = mx_pack8<FMT>(y);
     if constexpr (FMT == kE4M3)
       *(uint2*)code = c;

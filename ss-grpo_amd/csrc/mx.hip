@@ -6,37 +6,36 @@
 
 namespace {
 
-// A workgroup takes 16 rows x 512 columns: 16 lanes per row, four steps of 128 columns each, whose loads are all
-// issued first. 16 rows, because the scale dwords of a step are neighbours along the rows: 64 bytes per store
-// instruction of the workgroup instead of 4 scattered ones.
-constexpr int kTileRows = 16, kTileSteps = 4;
+// A workgroup takes 16 rows x 512 columns, a wave four of the rows: each load instruction reads 1 KB of one row, and
+// all four are issued before the first is used. 16 rows, because the scale dwords of a step are neighbours along the
+// rows: the workgroup's make 64 bytes.
+constexpr int kTileRows = 16, kWaveRows = 4, kTileSteps = 4;
 
 template <int DT, int FMT>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int cols,
                                                           int steps, int step_tiles, uint8_t* __restrict__ codes,
                                                           uint32_t* __restrict__ scales) {
   const int rt = blockIdx.x / step_tiles, st = blockIdx.x - rt * step_tiles;
-  const int l = threadIdx.x & 15;
-  const int row = rt * kTileRows + (threadIdx.x >> 4);
-  const bool row_ok = row < rows;
-  float v[kTileSteps][8];
+  const int lane = threadIdx.x & 63, l = lane & 15;
+  const int row0 = rt * kTileRows + (threadIdx.x >> 6) * kWaveRows;
+  const int step = st * kTileSteps + (lane >> 4), col = step * fg::kMxStep + l * 8;
+  float v[kWaveRows][8];
 #pragma unroll
-  for (int u = 0; u < kTileSteps; ++u) {
-    const int col = (st * kTileSteps + u) * fg::kMxStep + l * 8;
-    if (row_ok && col < cols) {
-      fg::load8<DT>(x, (int64_t)row * ldx + col, v[u]);
+  for (int u = 0; u < kWaveRows; ++u) {
+    if (row0 + u < rows && col < cols) {
+      fg::load8<DT>(x, (int64_t)(row0 + u) * ldx + col, v[u]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
     }
   }
 #pragma unroll
-  for (int u = 0; u < kTileSteps; ++u) {
-    const int step = st * kTileSteps + u, col = step * fg::kMxStep + l * 8;
-    if (step >= steps) break;  // for the whole workgroup
+  for (int u = 0; u < kWaveRows; ++u) {
+    const int row = row0 + u;
+    if (row >= rows) break;  // for the whole wave
     const int64_t at = (int64_t)row * cols + col;
     fg::mx_store_step<FMT>(v[u], col < cols, l, codes + (FMT == fg::kE4M3 ? at : at / 2),
-                           scales + (int64_t)step * rows + row, row_ok);
+                           scales + (int64_t)step * rows + row, step < steps);
   }
 }
 
@@ -45,29 +44,29 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
                                                             const uint8_t* __restrict__ scales, int rows, int cols,
                                                             int step_tiles, void* __restrict__ out, int64_t ldo) {
   const int rt = blockIdx.x / step_tiles, st = blockIdx.x - rt * step_tiles;
-  const int l = threadIdx.x & 15;
-  const int row = rt * kTileRows + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  uint2 c[kTileSteps];
-  uint32_t s[kTileSteps];
+  const int lane = threadIdx.x & 63, l = lane & 15;
+  const int row0 = rt * kTileRows + (threadIdx.x >> 6) * kWaveRows;
+  const int step = st * kTileSteps + (lane >> 4), col = step * fg::kMxStep + l * 8;
+  if (col >= cols) return;
+  uint2 c[kWaveRows];
+  uint32_t s[kWaveRows];
 #pragma unroll
-  for (int u = 0; u < kTileSteps; ++u) {
-    const int step = st * kTileSteps + u, col = step * fg::kMxStep + l * 8;
+  for (int u = 0; u < kWaveRows; ++u) {
     c[u] = make_uint2(0u, 0u);
     s[u] = 0;
-    if (col < cols) {
-      const int64_t at = (int64_t)row * cols + col;
+    if (row0 + u < rows) {
+      const int64_t at = (int64_t)(row0 + u) * cols + col;
       if constexpr (FMT == fg::kE4M3)
         c[u] = *(const uint2*)(codes + at);
       else
         c[u].x = *(const uint32_t*)(codes + at / 2);
-      s[u] = scales[((int64_t)step * rows + row) * 4 + (l >> 2)];
+      s[u] = scales[((int64_t)step * rows + row0 + u) * 4 + (l >> 2)];
     }
   }
 #pragma unroll
-  for (int u = 0; u < kTileSteps; ++u) {
-    const int col = (st * kTileSteps + u) * fg::kMxStep + l * 8;
-    if (col >= cols) continue;
+  for (int u = 0; u < kWaveRows; ++u) {
+    const int row = row0 + u;
+    if (row >= rows) break;
     float v[8];
     if constexpr (FMT == fg::kE4M3) {
       const fg::f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(c[u].x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(c[u].x, true);
@@ -98,24 +97,40 @@ FG_DEVICE float round_odd(float hi, float lo) {
   return __uint_as_float(b);
 }
 
+// The sum over the wave's 64 lanes, in every lane: six additions of what the data-parallel moves bring (within rows
+// of 16 lanes, then from row to row), where shuffles through LDS would put six round trips in front of the norm.
+template <int CTRL, int ROWS>
+FG_DEVICE double moved(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, true);
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
 FG_DEVICE double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-    v += __longlong_as_double((long long)fg::shfl_xor_u64((uint64_t)__double_as_longlong(v), o));
-  return v;
+  v += moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8: lane 15 of each row has the row's sum
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+  v += moved<0x143, 0xc>(v);
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 
 // s = x + delta (rounded to the row type, written to sum), y = s * rsqrt(mean(s^2) + eps) * w, MX e4m3 of y. One
-// workgroup per row, eight columns per thread and chunk; the row stays in registers between the two passes. The
-// squares are summed in 64 bits (bf16's are exact there, and so is their sum to 2^-50), and y is the product of s, of
-// the factor as two floats and of w with the rounding errors of both products carried beside it (fused multiply-adds
-// give them exactly): an 8-bit code has a rounding border every 1/8 of a value, and with y in 32 bits one value in a
-// million falls on another side of it than the definition's. In 64-bit multiplications and conversions, the same took
-// 15.4 instead of %US% us for 1856 rows of 3584 with an addend.
+// workgroup per row, eight columns per thread and chunk; the row stays in registers between the two passes. An 8-bit
+// code has a rounding border every 1/8 of a value, and with plain 32-bit arithmetic one value in a million falls on
+// another side of it than the definition's. So the squares are summed in 64 bits (bf16's are exact there, and so is
+// their sum to 2^-50), and where a product is so near a tie that its two roundings decide (by the 19 bits at its end:
+// one wave in 400), it is taken again with the rounding errors of both multiplications, which fused multiply-adds
+// give exactly. For 1856 rows of 3584 with an addend, 46.6 MB: 12.5 us (3.7 TB/s; 5.0 for 8192 x 4096); with every
+// product in 64 bits and the sums shuffled through LDS 15.4.
 template <int DT, int CHUNKS>
 __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const void* __restrict__ delta,
                                                          const void* __restrict__ w, void* sum, int rows, int H,
-                                                         float eps, uint8_t* __restrict__ codes,
+                                                         double inv_h, float eps, uint8_t* __restrict__ codes,
                                                          uint32_t* __restrict__ scales) {
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, nch = H / 8, threads = blockDim.x;
@@ -143,7 +158,7 @@ __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const vo
   __syncthreads();
   ss = 0.0;
   for (int i = 0; i < threads / 64; ++i) ss += red[i];
-  const double rs = rsqrt(ss / (double)H + (double)eps);
+  const double rs = rsqrt(ss * inv_h + (double)eps);
   const float rs_hi = (float)rs, rs_lo = (float)(rs - (double)rs_hi);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
@@ -152,12 +167,21 @@ __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const vo
     const bool valid = ch < nch;
     if (valid) {
       fg::load8<DT>(w, ch * 8, wv);
+      uint32_t low = ~0u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = v[c][j] * rs_hi;
-        const float tl = __builtin_fmaf(v[c][j], rs_lo, __builtin_fmaf(v[c][j], rs_hi, -t));
-        const float p = t * wv[j];
-        y[j] = round_odd(p, __builtin_fmaf(tl, wv[j], __builtin_fmaf(t, wv[j], -p)));
+        y[j] = v[c][j] * rs_hi * wv[j];
+        low = min(low, (__float_as_uint(y[j]) + 2u) << 13);
+      }
+      if (low <= 4u << 13) {  // within two units of its last place of a multiple of 2^19 of them
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float t = v[c][j] * rs_hi;
+          const float tl = __builtin_fmaf(v[c][j], rs_lo, __builtin_fmaf(v[c][j], rs_hi, -t));
+          const float r = __builtin_fmaf(tl, wv[j], __builtin_fmaf(t, wv[j], -y[j]));  // what y[j] lacks
+          const float hi = y[j] + r;
+          y[j] = round_odd(hi, r - (hi - y[j]));
+        }
       }
     }
     fg::mx_store_step<fg::kE4M3>(y, valid, ch & 15, codes + row * H + ch * 8,
@@ -168,13 +192,15 @@ __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const vo
 template <int DT>
 void launch_norm(const void* x, const void* delta, const void* w, void* sum, int rows, int H, float eps, uint8_t* codes,
                  uint32_t* scales, hipStream_t s) {
-  // as few chunks per thread as 512 threads allow, then no more threads than those chunks need
-  const int nch = H / 8, chunks = (nch + 511) / 512;
+  // one chunk per thread up to 256 threads, then two (one chunk and 448 threads, 1856 rows of 3584 without an
+  // addend: 8.5 against 8.0 us)
+  const int nch = H / 8, chunks = nch <= 256 ? 1 : 2;
   const dim3 g(rows), b(((nch + chunks - 1) / chunks + 63) / 64 * 64);
+  const double inv_h = 1.0 / H;
   if (chunks == 1)
-    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 1>), g, b, 0, s, x, delta, w, sum, rows, H, eps, codes, scales);
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 1>), g, b, 0, s, x, delta, w, sum, rows, H, inv_h, eps, codes, scales);
   else
-    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 2>), g, b, 0, s, x, delta, w, sum, rows, H, eps, codes, scales);
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 2>), g, b, 0, s, x, delta, w, sum, rows, H, inv_h, eps, codes, scales);
 }
 
 int64_t tiles_of(int rows, int cols, int* steps, int* step_tiles) {

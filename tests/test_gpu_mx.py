@@ -176,6 +176,30 @@ def test_rmsnorm_codes_are_the_formulas(rows, cols, delta, dtype):
         assert torch.equal(q2.codes.view(torch.uint8), q.codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("eps", [0.0, 1e-10, 3e-8])
+def test_rmsnorm_next_to_ties(eps, dtype):
+    """Rows of +-1 have a mean square of 1: the norm is the weight itself, an eighth of whose values are ties between
+    two codes, or a part in 10^10 less, which 32 bits cannot hold and which takes a tie to the smaller magnitude."""
+    g = torch.Generator().manual_seed(4)
+    cols = 4096
+    x = (torch.randint(0, 2, (9, cols), generator=g) * 2 - 1).to(dtype)
+    w = torch.exp(torch.randn(cols, generator=g)).to(torch.bfloat16).to(dtype)
+    want_c, want_s = O.quantize(O.rmsnorm(x.double().numpy(), w.double().numpy(), float(np.float32(eps))), "e4m3")
+    codes, scales = held(K().rmsnorm_mx(x.to(DEV), w.to(DEV), eps))
+    assert np.array_equal(scales, want_s) and np.array_equal(codes, want_c)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rmsnorm_codes_of_many_values(dtype):
+    """Enough values for those that 32-bit arithmetic would round differently (one in a million) to be among them."""
+    x = rows_of(1500, 4096, 11, dtype, spread=0.3)
+    w = (1 + 0.2 * torch.randn(4096, generator=torch.Generator().manual_seed(1))).to(dtype)
+    want_c, want_s = O.quantize(O.rmsnorm(x.double().numpy(), w.double().numpy(), float(np.float32(1e-6))), "e4m3")
+    codes, scales = held(K().rmsnorm_mx(x.to(DEV), w.to(DEV), 1e-6))
+    assert np.array_equal(scales, want_s) and np.array_equal(codes, want_c)
+
+
 def test_rmsnorm_special_rows():
     """A row of zeros, one with an infinity, one with a NaN, tiny and huge rows; the others are as without them."""
     x = rows_of(7, 256, 5, torch.float32)
