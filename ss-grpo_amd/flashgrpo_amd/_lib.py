@@ -115,11 +115,16 @@ def call(name: str, *args) -> int:
     lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0 and SIGNATURES[name][0] is _I:
-        msg = lib.fg_last_error().decode(errors="replace")
-        if "null pointer" in msg or "bad" in msg or "must" in msg or "shape" in msg:
-            raise ValueError(msg)
-        raise NativeError(msg)
+        raise_last_error()
     return rc
+
+
+def raise_last_error() -> None:
+    """The error of the call that just returned a code other than 0: ValueError for arguments, else NativeError."""
+    msg = load().fg_last_error().decode(errors="replace")
+    if "null pointer" in msg or "bad" in msg or "must" in msg or "shape" in msg:
+        raise ValueError(msg)
+    raise NativeError(msg)
 
 
 def exported_symbols() -> list:

@@ -726,7 +726,11 @@ def _same_device(what, dev, *ts) -> None:
 def _call_on(dev, name, *args):
     """The call on GPU ``dev``'s current stream, whichever device is the current one."""
     if dev == _cur_device():
-        _call(name, *args, _raw_stream(dev))
+        if timing.idle():
+            if getattr(_lib.load(), name)(*args, _raw_stream(dev)):
+                _lib.raise_last_error()
+        else:
+            _call(name, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
             _call(name, *args, _raw_stream(dev))

@@ -487,6 +487,8 @@ class TargetModel:
         # wherever the operands allow (the shape's best measured split-K plan, else
         # default_linear_plan), False never; drop_graphs() after a change
         self.split_k_linear = None
+        # 4-bit copies (gate/up, down) of every layer's MLP weights, which its MLP then runs on (quantize_mlp)
+        self.mlp_mx = None
         if self.device.type == "cuda":
             use_tuned_gemms()
 
@@ -592,6 +594,9 @@ class TargetModel:
                     if lw.get("qkv_b_pairs") is not None:
                         lw["qkv_b_pairs"].copy_(K.rope_pair_rows(lw["qkv_b"], cfg.q_heads, cfg.kv_heads,
                                                                  cfg.head_dim))
+            for lw, (gate_up, down) in zip(self.w["layers"], self.mlp_mx or ()):
+                K.mx_quantize(lw["gate_up_w"], "e2m1", out=gate_up)
+                K.mx_quantize(lw["down_w"], "e2m1", out=down)
         self._hf_key = key
         return True
 
@@ -602,6 +607,30 @@ class TargetModel:
     @property
     def embed_weight(self) -> torch.Tensor:
         return self.w["embed"]
+
+    def quantize_mlp(self, enable: bool = True) -> "TargetModel":
+        """Run every layer's MLP on 4-bit copies of its weights (MX e2m1) with 8-bit rows (MX e4m3): the norm writes
+        its output quantised (``rmsnorm_mx``), ``mx_gate_up_swiglu`` takes it to the quantised activation, and
+        ``mx_linear`` adds the down projection to the residual stream. ``enable=False`` goes back to the weights as
+        they are (and frees the copies). Returns self.
+
+        The copies are made here and again, in place, by ``sync_from_hf``. Attention, the projections around it and
+        the LM head are unchanged. The rollout then samples from the quantised model, exactly; a trainer that takes
+        its tokens for the full model's has to weigh them (its log probabilities are not the full model's). bf16
+        models whose hidden size (at most 8192) and intermediate size are multiples of 32."""
+        cfg = self.cfg
+        if enable and (self.dtype != torch.bfloat16 or cfg.hidden % K.MX_BLOCK or cfg.hidden > 8192
+                       or cfg.intermediate % K.MX_BLOCK):
+            raise ValueError("quantize_mlp: needs a bf16 model with hidden (at most 8192) and intermediate sizes that "
+                             "are multiples of 32")
+        self.mlp_mx = [(K.mx_quantize(lw["gate_up_w"], "e2m1"), K.mx_quantize(lw["down_w"], "e2m1"))
+                       for lw in self.w["layers"]] if enable else None
+        self.drop_graphs()
+        return self
+
+    def _mx_buf(self, name, rows, cols) -> K.MX:
+        return K.MX(self._buf(name, (rows, cols), torch.float8_e4m3fn),
+                    self._buf(name + "_scales", (-(-cols // 128), rows, 4), torch.uint8))
 
     def new_cache(self, batch: int, capacity: int) -> KVCache:
         return KVCache(self.cfg, batch, capacity, dtype=self.dtype, device=self.device)
@@ -731,6 +760,12 @@ class TargetModel:
             K.tree_attention(q, cache.k(l), cache.v(l), seq_len=seq_len, anc=anc, num_nodes=N, q_heads=cfg.q_heads,
                              kv_heads=cfg.kv_heads, head_dim=d, out=attn, row_map=row_map)
             a2 = attn.view(T, cfg.q_heads * d)
+            if self.mlp_mx is not None:  # the residual add inside the library GEMM, then norm to residual on MX rows
+                x.addmm_(a2, lw["o_w"].t())
+                q2 = K.rmsnorm_mx(x, lw["post_norm"], cfg.rms_eps, out=self._mx_buf("h_mx", T, H))
+                act = K.mx_gate_up_swiglu(q2, self.mlp_mx[l][0], out=self._mx_buf("act_mx", T, cfg.intermediate))
+                K.mx_linear(act, self.mlp_mx[l][1], residual=x, out=x)
+                continue
             plan = self._linear_plan("o", a2, lw["o_w"])
             if plan:
                 # bf16(x + bf16(o_proj)) and the post-attention norm from the parts

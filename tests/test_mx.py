@@ -108,3 +108,14 @@ def test_mx_pairs_are_checked():
                 (codes.t().contiguous().t(), scales), (codes[:0, :0], scales)):
         with pytest.raises(ValueError):
             K._mx_of(bad, "t")
+
+
+def test_only_bf16_models_of_whole_blocks_are_quantised():
+    from flashgrpo_amd.models.target import TargetConfig, TargetModel
+
+    for hidden, inter, dtype in ((256, 512, torch.float32), (272, 512, torch.bfloat16), (256, 520, torch.bfloat16),
+                                 (8224, 512, torch.bfloat16)):
+        m = TargetModel(TargetConfig(1, hidden, 4, 2, 64, inter, 100), {"layers": []}, dtype=dtype, device="cpu")
+        with pytest.raises(ValueError, match="multiples of 32"):
+            m.quantize_mlp()
+        assert m.quantize_mlp(False).mlp_mx is None
