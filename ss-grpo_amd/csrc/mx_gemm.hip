@@ -273,9 +273,11 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     return intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
   };
   constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;  // the instruction's code of x's format; 4 is e2m1
-#define FG_MX_MFMA(i, k, buf, sel)                                                                                  \
-  acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w_frag(buf, i), x_frag(buf, k), acc[i][k], 4, kBF,     \
-                                                              sel, (int)sw[i], sel, (int)sx[k])
+  // matrix instruction j of a sub-step
+#define FG_MX_MFMA(j, buf, sel)                                                                                     \
+  acc[(j) / FM][(j) % FM] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                         \
+      w_frag(buf, (j) / FM), x_frag(buf, (j) % FM), acc[(j) / FM][(j) % FM], 4, kBF, sel, (int)sw[(j) / FM], sel,    \
+      (int)sx[(j) % FM])
 
   // Prologue: steps 0 .. min(NS, nk) - 1 in flight, wait for step 0.
   const int first = min(NS, nk);
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
 #pragma unroll
     for (int j = 0; j < NM; ++j) {
       if constexpr (math) {
-        FG_MX_MFMA(j / FM, j % FM, 0, 0);
+        FG_MX_MFMA(j, 0, 0);
 #pragma unroll
         for (int q = j * R1; q < (j + 1) * R1; ++q)
           if (q < kReads) read(slot, 1, 1, q);
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
 #pragma unroll
     for (int j = 0; j < NM; ++j) {
       if constexpr (math) {
-        FG_MX_MFMA(j / FM, j % FM, 1, 2);
+        FG_MX_MFMA(j, 1, 2);
 #pragma unroll
         for (int q = j * R2; q < (j + 1) * R2; ++q)
           if (q < kReads + kScaleReads) read(next, 0, 0, q);
@@ -476,6 +478,20 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
   }
 }
 
+// The e4m3 codes of magnitude 4 and up (0x48 ..; part 0) or those below (part 1), zeros in place of the others. The
+// products of either with e2m1 codes span 13 bits (2^-2 .. 2^11 and 2^-10 .. 2^4), so the matrix instruction loses
+// nothing of them but the last bit of subnormal codes'.
+FG_DEVICE intx8 part_of(const intx8& x, int part) {
+  intx8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t v = (uint32_t)x[j], big = ((v & 0x7f7f7f7fu) + 0x38383838u) & 0x80808080u;
+    const uint32_t mask = (big << 1) - (big >> 7);  // 0xff for each such byte
+    r[j] = (int)(part == 0 ? v & mask : v & ~mask);
+  }
+  return r;
+}
+
 // Up to 16 rows: the weights are streamed once, straight into registers, and the rows are read beside them. A
 // workgroup takes NT tiles of 16 weight rows (gate_up: 32 gate and 32 up rows, one block of 32 output columns) and its
 // waves take every waves-th step of 128 elements, so that together they read each row's bytes in order; v_mfma_scale_
@@ -488,7 +504,7 @@ constexpr int kStreamRows = 16;
 constexpr int kStreamLd = 20;  // floats per x row and tile in LDS: 16-byte stores on distinct banks
 
 template <int FMT, int NT, int U, int EPI>
-__global__ void __launch_bounds__(1024) mx_stream_kernel(MxArgs p) {
+__global__ void __launch_bounds__(NT == 4 ? 512 : 1024) mx_stream_kernel(MxArgs p) {
   typedef float floatx4 __attribute__((ext_vector_type(4)));
   constexpr int XR = FMT == fg::kE4M3 ? 2 : 1, XB = FMT == fg::kE4M3 ? 128 : 64;
   constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;
@@ -536,17 +552,24 @@ __global__ void __launch_bounds__(1024) mx_stream_kernel(MxArgs p) {
     }
     xs[u] = p.xs[(int64_t)t * p.rows + m];
   };
-  auto multiply = [&](int u) __attribute__((always_inline)) {
-    intx8 x = intx8{xv[u][0].x, xv[u][0].y, xv[u][0].z, xv[u][0].w, 0, 0, 0, 0};
-    if constexpr (XR == 2) {
-      x[4] = xv[u][1].x; x[5] = xv[u][1].y; x[6] = xv[u][1].z; x[7] = xv[u][1].w;
-    }
+  auto multiply_part = [&](int u, const intx8& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const intx8 w = intx8{wv[u][i].x, wv[u][i].y, wv[u][i].z, wv[u][i].w, 0, 0, 0, 0};
       acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[i], 4, kBF, 0, (int)(ws[u][i] >> (8 * g)), 0,
                                                                 (int)(xs[u] >> (8 * g)));
     }
+  };
+  auto multiply = [&](int u) __attribute__((always_inline)) {
+    intx8 x = intx8{xv[u][0].x, xv[u][0].y, xv[u][0].z, xv[u][0].w, 0, 0, 0, 0};
+    if constexpr (XR == 2) {
+      x[4] = xv[u][1].x; x[5] = xv[u][1].y; x[6] = xv[u][1].z; x[7] = xv[u][1].w;
+    }
+    if constexpr (EPI == kGateUp && FMT == fg::kE4M3) {  // an 8-bit code follows: lose nothing (it is free here)
+      multiply_part(u, part_of(x, 1));
+      x = part_of(x, 0);
+    }
+    multiply_part(u, x);
   };
   int t = wave;
   for (; t + (U - 1) * waves < p.steps; t += U * waves) {
@@ -770,7 +793,10 @@ void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
 template <int FMT, int NT, int EPI>
 void launch_stream(const MxArgs& p, int waves, hipStream_t s) {
   const int per = EPI == kGateUp ? 32 : NT * 16, cols = EPI == kGateUp ? p.cols : p.wrows;
-  hipLaunchKernelGGL((mx_stream_kernel<FMT, NT, 2, EPI>), dim3((cols + per - 1) / per), dim3(64 * waves),
+  // One step per wave in flight with x in two parts (8B gate/up of one row: 14.4 us, two steps' registers 16.8; not in
+  // parts 13.9), else two.
+  constexpr int U = EPI == kGateUp ? 1 : 2;
+  hipLaunchKernelGGL((mx_stream_kernel<FMT, NT, U, EPI>), dim3((cols + per - 1) / per), dim3(64 * waves),
                      waves * NT * 16 * kStreamLd * 4, s, p);
 }
 
