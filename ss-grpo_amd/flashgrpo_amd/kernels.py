@@ -7,6 +7,7 @@ device work happens in the HIP kernels of ``ss-grpo_amd/csrc``.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple
 
@@ -748,31 +749,30 @@ def _mx_bad(codes, scales, what):
 
 
 def _mx_of(q, what):
-    """(codes, scales, format code, rows, cols, device index) of an MX pair as the kernels take it."""
+    """(codes' address, scales' address, format code, rows, cols, device index) of an MX pair that the kernels take."""
     codes, scales = q
-    dt = codes.dtype
-    if (dt is not _U8 and dt is not _FP8) or codes.dim() != 2:
+    dt, shape = codes.dtype, codes.shape
+    if (dt is not _U8 and dt is not _FP8) or len(shape) != 2:
         _mx_bad(codes, scales, what)
-    rows, k = codes.shape
+    rows, k = shape
     fmt = 0
     if dt is _U8:
         fmt, k = 1, 2 * k
     dev = codes.get_device()
-    if (k % 32 or k == 0 or scales.dtype is not _U8 or scales.shape != ((k + 127) // 128, rows, 4)
-            or not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 4
-            or scales.get_device() != dev):
+    c, s = codes.data_ptr(), scales.data_ptr()
+    if (k % 32 or k == 0 or c % 16 or s % 4 or scales.dtype is not _U8 or scales.shape != ((k + 127) // 128, rows, 4)
+            or not codes.is_contiguous() or not scales.is_contiguous() or scales.get_device() != dev):
         _mx_bad(codes, scales, what)
-    return codes, scales, fmt, rows, k, dev
+    return c, s, fmt, rows, k, dev
 
 
 def _mx_out(out, rows, cols, fmt, device, what) -> MX:
     if out is None:
         return MX(torch.empty(rows, cols // 2 if fmt else cols, dtype=_U8 if fmt else _FP8, device=device),
                   torch.empty((cols + 127) // 128, rows, 4, dtype=_U8, device=device))
-    codes, scales, f, r, k, dev = _mx_of(out, what)
-    if (r, k, f, dev) != (rows, cols, fmt, device.index):
+    if _mx_of(out, what)[2:] != (fmt, rows, cols, device.index):
         raise ValueError(f"{what}: out must be an {'e2m1' if fmt else 'e4m3'} MX pair of [{rows}, {cols}] on {device}")
-    return MX(codes, scales)
+    return MX(*out)
 
 
 def mx_quantize(x, fmt="e2m1", *, out=None) -> MX:
@@ -812,12 +812,11 @@ def mx_dequantize(q, dtype=torch.bfloat16, *, out=None):
     if out is None:
         if dtype not in _DT:
             raise TypeError("mx_dequantize: dtype must be bfloat16 or float32")
-        out = torch.empty(rows, cols, dtype=dtype, device=codes.device)
+        out = torch.empty(rows, cols, dtype=dtype, device=q[0].device)
     elif tuple(out.shape) != (rows, cols) or out.dtype not in _DT or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"mx_dequantize: out must be a contiguous 16-byte aligned bf16 or fp32 [{rows}, {cols}] tensor")
     if rows:
-        _call_on(dev, "fg_mx_dequantize", codes.data_ptr(), scales.data_ptr(), f, rows, cols, out.data_ptr(),
-                 dtype_code(out), cols)
+        _call_on(dev, "fg_mx_dequantize", codes, scales, f, rows, cols, out.data_ptr(), dtype_code(out), cols)
     return out
 
 
@@ -863,18 +862,23 @@ def _mx_operands(x, w, what):
     xc, xs, f, rows, k, dev = _mx_of(x, what)
     wc, ws, wf, n, kw, wdev = _mx_of(w, what)
     if dev != wdev or dev < 0:
-        _same_device(what, dev, wc)
+        _same_device(what, dev, w[0])
     if kw != k:
         raise ValueError(f"{what}: x has {k} columns and the weight {kw}")
     if wf != 1:
         raise TypeError(f"{what}: the weight must be in e2m1 (4 bits)")
-    return (xc.data_ptr(), xs.data_ptr(), f, wc.data_ptr(), ws.data_ptr()), rows, n, k, dev
+    return (xc, xs, f, wc, ws), rows, n, k, dev
+
+
+@functools.lru_cache(maxsize=4096)
+def _mx_workspace_bytes(name, rows, cols, k, fmt):
+    return getattr(_lib.load(), name)(rows, cols, k, fmt)
 
 
 def _mx_workspace(name, rows, cols, k, fmt, device):
     """(tensor, address, bytes) for a split product's sums: a buffer of the call's own, so that calls on two streams, or
     two captured graphs, share none (torch's allocator keeps it until the stream, or the graph, is done with it)."""
-    n = getattr(_lib.load(), name)(rows, cols, k, fmt)
+    n = _mx_workspace_bytes(name, rows, cols, k, fmt)
     if n == 0:
         return None, None, 0
     ws = torch.empty(n, dtype=_U8, device=device)
