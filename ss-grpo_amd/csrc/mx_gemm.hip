@@ -113,7 +113,9 @@ constexpr int stage_bytes(int fmt, int bm, int bn) {
 }
 
 template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI>
-__global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, BM, BN) <= 80 * 1024 ? 2 : 1)
+__global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, BM, BN) <= 40 * 1024   ? 4
+                                                          : NS * stage_bytes(FMT, BM, BN) <= 80 * 1024 ? 2
+                                                                                                       : 1)
     mx_gemm_kernel(MxArgs p) {
   constexpr int XB = FMT == fg::kE4M3 ? 128 : 64, WB = 64;  // bytes per row and step
   constexpr int WAVES = WAVES_M * WAVES_N;
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
   static_assert(EPI != kGateUp || FN % 2 == 0, "a wave holds gate and up of its columns");
   static_assert(NS >= 2 && (NS - 1) * LPW < 64, "vmcnt");
   constexpr int OUT_LD = WN + 4;  // floats per row of the epilogue's staging: 16-byte rows on distinct banks
-  constexpr int EPI_BYTES = EPI == kLinear ? WAVES * 32 * OUT_LD * 4 : 0;
+  constexpr int EPI_BYTES = EPI == kLinear ? WAVES * 32 * OUT_LD * 4 + BN * 4 : 0;
   static_assert(NS * STAGE <= 160 * 1024 && EPI_BYTES <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) unsigned char smem[NS * STAGE > EPI_BYTES ? NS * STAGE : EPI_BYTES];
 
@@ -223,6 +225,11 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     }
   };
 
+  float bias_v = 0.0f;  // of the tile's column tid, on its way while the sums are made
+  if constexpr (EPI == kLinear) {
+    static_assert(64 * WAVES >= BN, "a thread per column");
+    if (p.bias && tid < BN && n0 + tid < p.wrows) bias_v = fg::bf16_to_f32(p.bias[n0 + tid]);
+  }
   floatx16 acc[FN][FM];
 #pragma unroll
   for (int i = 0; i < FN; ++i)
@@ -377,9 +384,18 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
         }
     }
   } else if constexpr (EPI == kGateUp) {
+    // Each wave's codes go out through LDS, its rows of WN / 2 bytes as 16-byte chunks side by side (stored from the
+    // accumulators, four bytes of 32 rows at a time: 1.5 us more per 256 x 256 tile).
+    __syncthreads();  // no wave still reads the ring
+    constexpr int OB = WN / 2, CH = OB / 16;  // bytes and chunks of an output row
+    unsigned char* stage = smem + wave * WM * OB;
+    auto place = [&](int r, int q) __attribute__((always_inline)) { return r * OB + ((q ^ ((r >> 1) & (CH - 1))) * 16); };
+    const int cw = n0 + wn * OB;  // the wave's first output column
+    if (m0 + wm * WM >= p.rows || cw >= p.cols) return;
 #pragma unroll
     for (int k = 0; k < FM; ++k) {
-      const int m = m0 + wm * WM + k * 32 + l32;
+      const int r = k * 32 + l32, m = m0 + wm * WM + r;
+      uint32_t bytes = 0;  // the scales of the wave's blocks
 #pragma unroll
       for (int i = 0; i < FN / 2; ++i) {
         float v[16];
@@ -392,86 +408,104 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
         a = max(a, (uint32_t)__shfl_xor((int)a, 32, 64));
         const uint32_t s = fg::mx_scale_byte<fg::kE4M3>(a);
         const float inv = fg::mx_inverse_scale(s);
-        const int c = n0 + wn * (WN / 2) + i * 32;  // the block's first output column
-        if (m >= p.rows || c >= p.cols) continue;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          float y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = s == 255u ? 0.0f : v[4 * g + e] * inv;
           int q = 0;
-          q = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], q, false);
-          q = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], q, true);
-          *(int*)(p.codes + (int64_t)m * p.cols + c + 8 * g + 4 * half) = q;
+          q = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * g] * inv, v[4 * g + 1] * inv, q, false);
+          q = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * g + 2] * inv, v[4 * g + 3] * inv, q, true);
+          *(int*)(stage + place(r, i * 2 + g / 2) + (g % 2) * 8 + half * 4) = q;
         }
-        if (half == 0) {
-          uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(c / kStep) * p.rows + m);
-          const int b = (c / 32) & 3;
-          sc[b] = (uint8_t)s;
-          if (c + 32 >= p.cols) {  // the last block also writes the zeros behind it
-            for (int e = b + 1; e < 4; ++e) sc[e] = 0;
-          }
-        }
+        if (cw + i * 32 < p.cols) bytes |= s << (8 * i);  // zeros behind the last block
       }
+      if (half == 0 && m < p.rows) {
+        uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(cw / kStep) * p.rows + m) + ((cw / 32) & 3);
+        if constexpr (FN / 2 == 2) *(uint16_t*)sc = (uint16_t)bytes;
+        else *sc = (uint8_t)bytes;
+        if (cw + OB >= p.cols)  // the last wave of the row also writes the zeros behind its blocks
+          for (int e = ((cw / 32) & 3) + FN / 2; e < 4; ++e) sc[e - ((cw / 32) & 3)] = 0;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < WM * CH / 64; ++it) {
+      const int r = it * (64 / CH) + lane / CH, q = lane % CH;
+      const int m = m0 + wm * WM + r, c = cw + q * 16;
+      const uint4 v = *(const uint4*)(stage + place(r, q));
+      if (m < p.rows && c < p.cols) *(uint4*)(p.codes + (int64_t)m * p.cols + c) = v;
     }
   } else {
     __syncthreads();  // no wave still reads the ring: each stages 32 of its rows at a time in it
     float* stage = (float*)smem + wave * 32 * OUT_LD;
-    constexpr int LANES = WN / 8;          // lanes per row when reading back, 8 columns each
-    constexpr int ROWS = 64 / LANES;       // rows per pass
-    const int rr = lane / LANES, cc = (lane % LANES) * 8;
-    const int n = n0 + wn * WN + cc;
-    float bv[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bv[e] = p.bias && n + e < p.wrows ? fg::bf16_to_f32(p.bias[n + e]) : 0.0f;
-#pragma unroll
+    float* s_bias = (float*)smem + WAVES * 32 * OUT_LD;
+    if (tid < BN) s_bias[tid] = bias_v;
+    __syncthreads();
+    s_bias += wn * WN;
+    const int nb = n0 + wn * WN, cols = min(WN, p.wrows - nb);  // the wave's first column, how many it has
+    // One copy of the code behind the accumulators' stores for all k: a workgroup runs it once, and instructions that
+    // have to be fetched cost more than those of a loop.
+#pragma clang loop unroll(disable)
     for (int k = 0; k < FM; ++k) {
+      const int mk = m0 + wm * WM + k * 32;
+      if (mk >= p.rows || cols <= 0) break;
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
+      for (int kk = 0; kk < FM; ++kk)
+        if (kk == k) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *(float4*)(stage + l32 * OUT_LD + i * 32 + 8 * g + 4 * half) =
-              make_float4(acc[i][k][4 * g], acc[i][k][4 * g + 1], acc[i][k][4 * g + 2], acc[i][k][4 * g + 3]);
+          for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              *(float4*)(stage + l32 * OUT_LD + i * 32 + 8 * g + 4 * half) =
+                  make_float4(acc[i][kk][4 * g], acc[i][kk][4 * g + 1], acc[i][kk][4 * g + 2], acc[i][kk][4 * g + 3]);
+        }
       __builtin_amdgcn_wave_barrier();
-      if (!p.wide) {  // rows that start anywhere: two bytes per lane, side by side
-        for (int r0 = 0; r0 < 32; ++r0) {
-          const int m = m0 + wm * WM + k * 32 + r0;
-          if (m >= p.rows) break;
+      if (p.wide) {  // 8 columns per lane
+        constexpr int PER = WN / 8, AT_ONCE = 64 / PER;  // lanes per row, rows per pass
+        const int c = (lane % PER) * 8, r = lane / PER;
+        if (c >= cols) continue;
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+          const int m = mk + r0 + r;
+          if (m >= p.rows) continue;
+          float v[8], bv[8], rv[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          fg::load8<fg::kF32>(stage + (r0 + r) * OUT_LD + c, 0, v);
+          fg::load8<fg::kF32>(s_bias + c, 0, bv);
+          uint16_t* dst = p.out + (int64_t)m * p.ldo + nb + c;
+          const uint16_t* res = p.residual + (int64_t)m * p.ldr + nb + c;
+          if (c + 8 <= cols) {
+            if (p.residual) fg::load8<fg::kBF16>(res, 0, rv);
 #pragma unroll
-          for (int c0 = 0; c0 < WN; c0 += 64) {
-            const int nn = n0 + wn * WN + c0 + lane;
-            if (c0 + lane >= WN || nn >= p.wrows) continue;
-            float v = stage[r0 * OUT_LD + c0 + lane];
-            if (p.bias) v += fg::bf16_to_f32(p.bias[nn]);
-            if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)m * p.ldr + nn]);
-            p.out[(int64_t)m * p.ldo + nn] = fg::f32_to_bf16(v);
+            for (int e = 0; e < 8; ++e) v[e] = v[e] + bv[e] + rv[e];
+            fg::store8<fg::kBF16>(dst, 0, v);
+          } else {
+            for (int e = 0; c + e < cols; ++e)
+              dst[e] = fg::f32_to_bf16(stage[(r0 + r) * OUT_LD + c + e] + s_bias[c + e] +
+                                       (p.residual ? fg::bf16_to_f32(res[e]) : 0.0f));
           }
         }
-        continue;
-      }
+      } else {
+        // Rows that start anywhere: a column per lane, one row at a time (its address is the wave's), eight rows' loads in
+        // flight. (Pairs of columns in the row's aligned dwords took more instructions than they saved stores.)
 #pragma unroll
-      for (int r0 = 0; r0 < 32; r0 += ROWS) {
-        const int m = m0 + wm * WM + k * 32 + r0 + rr;
-        const float4 a = *(const float4*)(stage + (r0 + rr) * OUT_LD + cc);
-        const float4 b = *(const float4*)(stage + (r0 + rr) * OUT_LD + cc + 4);
-        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        if (m >= p.rows || n >= p.wrows) continue;
+        for (int c0 = 0; c0 < WN; c0 += 64) {
+          const int c = c0 + lane;
+          if (c >= cols) continue;
+          const float bias = s_bias[c];
+#pragma clang loop unroll(disable)
+          for (int r0 = 0; r0 < 32 && mk + r0 < p.rows; r0 += 8) {
+            float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += bv[e];
-        uint16_t* dst = p.out + (int64_t)m * p.ldo + n;
-        const uint16_t* res = p.residual ? p.residual + (int64_t)m * p.ldr + n : nullptr;
-        if (n + 8 <= p.wrows) {
-          if (res) {
-            float rv[8];
-            fg::load8<fg::kBF16>(res, 0, rv);
+            for (int u = 0; u < 8; ++u) v[u] = stage[(r0 + u) * OUT_LD + c] + bias;
+            if (p.residual) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += rv[e];
+              for (int u = 0; u < 8; ++u)
+                v[u] += fg::bf16_to_f32((p.residual + (int64_t)min(mk + r0 + u, p.rows - 1) * p.ldr + nb)[c]);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              if (mk + r0 + u < p.rows)
+                (p.out + (int64_t)(mk + r0 + u) * p.ldo + nb)[c] = (uint16_t)fg::pack_bf16x2(v[u], 0.0f);
           }
-          fg::store8<fg::kBF16>(dst, 0, v);
-        } else {
-          for (int e = 0; e < 8 && n + e < p.wrows; ++e)
-            dst[e] = fg::f32_to_bf16(v[e] + (res ? fg::bf16_to_f32(res[e]) : 0.0f));
         }
       }
     }
@@ -697,18 +731,20 @@ struct Tile {
   float step_us;   // one step of one workgroup, a CU to itself
   float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
   float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
-  bool pairs;      // two workgroups per CU
+  float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
 };
-// Fitted to times of every tile and several splits with e4m3 rows over 1 .. 3500 rows x 700 .. 37888 columns x 640 ..
-// 18944: what the estimate picks is 3 % behind the fastest in the geometric mean, 25 % at worst.
+// Fitted to times of every tile and several splits with e4m3 rows over 1 .. 3500 rows x 200 .. 37888 columns x 192 ..
+// 18944: what the estimate picks is 3 % behind the fastest in the geometric mean, 20 % at worst.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 0.31f, 2.0f, 1.6f, true},
-    {128, 128, 64, 0.42f, 2.0f, 1.9f, true},
-    {128, 256, 64, 0.66f, 2.5f, 2.35f, false},
-    {192, 256, 96, 0.86f, 3.5f, 2.6f, false},
-    {256, 256, 64, 1.04f, 4.0f, 2.75f, false},
+    {64, 128, 32, 0.31f, 2.5f, 1.6f, 0.95f},
+    {128, 128, 64, 0.42f, 3.5f, 1.9f, 0.95f},
+    {128, 256, 64, 0.66f, 4.0f, 2.35f, 0},
+    {192, 256, 96, 0.86f, 5.5f, 2.8f, 0},
+    {256, 256, 64, 1.04f, 6.0f, 2.9f, 0},
+    {128, 256, 64, 1.05f, 4.5f, 2.6f, 0.8f},
+    {64, 128, 32, 0.35f, 2.5f, 1.45f, 0.4f},
 };
-constexpr int kTileCount = 5, kMaxSplits = 16;
+constexpr int kTileCount = 7, kMaxSplits = 16;
 
 struct Plan {
   int tile;    // of kTiles; -1: the stream of few rows
@@ -717,20 +753,25 @@ struct Plan {
 
 constexpr float kReadRate = 5.5e6f;  // bytes per us that the weights are read at
 
-// Estimated microseconds of a plan: whole rounds of 256 workgroups (a second one beside the first takes 0.7 of its
-// time, more of them 0.95), not under what the card sustains in matrix work (1.45 times as much where both operands are
-// e2m1) or reads; a split product also writes and reads its fp32 sums and takes a second launch.
-float plan_us(const Tile& t, int splits, int fmt, int rows, int wrows, int steps) {
+// Estimated microseconds of a plan: whole rounds of 256 workgroups (of which a second one beside the first takes 0.7
+// of its time, or 0.2 where four fit), not under what the card sustains in matrix work (1.45 times as much where both
+// operands are e2m1) or in bytes; the output's bytes on top where nothing else runs meanwhile. A split product writes
+// and reads its fp32 sums instead and takes a second launch.
+float plan_us(const Tile& t, int splits, bool gate_up, int fmt, int rows, int wrows, int steps) {
   const int64_t tiles_n = (wrows + t.bn - 1) / t.bn, tiles = (int64_t)((rows + t.bm - 1) / t.bm) * tiles_n;
   const float n = (float)(tiles * splits);
-  const float rounds = t.pairs && n > 256 ? std::max(1.7f, 0.95f * n / 256) : (float)((tiles * splits + 255) / 256);
+  const bool beside = t.pair > 0 && n > 256;
+  const float rounds = beside ? std::max(t.pair < 0.5f ? 1.2f : 1.7f, t.pair * n / 256) : (float)((tiles * splits + 255) / 256);
   const float work = rounds * ((steps + splits - 1) / splits) * t.step_us * (fmt == fg::kE4M3 ? 1.0f : 0.7f);
   const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
   const float flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (fmt == fg::kE4M3 ? 1e9f : 1.45e9f));
-  const float bytes = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
+  const float in = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
+  const float out = splits > 1 ? 0.0f : (float)rows * wrows * (gate_up ? 0.5f : 2.0f) / kReadRate;
   const float sums = (float)splits * rows * wrows * 4 * 2;
   const float parts = splits == 1 ? 0.0f : 2.5f + sums / (sums < 16e6f ? 9e6f : 5e6f);
-  return 2.0f + std::max(work, std::max(flops, bytes)) + rounds * t.tile_us + parts;
+  const float ends = rounds * t.tile_us;
+  if (beside) return 2.0f + std::max(work + ends, std::max(flops, in + out)) + parts;
+  return 2.0f + std::max(work, std::max(flops, in)) + ends + out + parts;
 }
 
 // The same for the stream of up to 16 rows, which has no second launch and no ring to fill but reads the rows again for
@@ -752,14 +793,19 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
   float least = 1e30f;
   for (int c = 0; c < kTileCount; ++c)
     for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
-      if (s > 1 && (steps / s < 3 || !splits_ok(steps, s))) continue;
-      const float us = plan_us(kTiles[c], s, fmt, rows, wrows, steps);
+      // (the two-stage ring of the last tile keeps too little in flight for a long reduction)
+      if (s > 1 && (steps / s < 3 || !splits_ok(steps, s) || c == kTileCount - 1)) continue;
+      const float us = plan_us(kTiles[c], s, gate_up, fmt, rows, wrows, steps);
       if (us < least) {
         least = us;
         best = Plan{c, s};
       }
     }
-  if (rows <= kStreamRows && stream_us(gate_up || wrows >= kWideCols, rows, wrows, steps) <= least) return Plan{-1, 1};
+  // The stream of a gate_up with e4m3 rows loses nothing of their products, so it takes all up to its 16 rows (at 16
+  // and 8B's sizes 17.5 us against the smallest tile's 15.1).
+  if (rows <= kStreamRows && ((gate_up && fmt == fg::kE4M3) ||
+                              stream_us(gate_up || wrows >= kWideCols, rows, wrows, steps) <= least))
+    return Plan{-1, 1};
   return best;
 }
 
@@ -786,7 +832,9 @@ void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
     case 1: launch<FMT, 128, 128, 2, 2, 3, EPI>(p, plan.splits, s); break;
     case 2: launch<FMT, 128, 256, 2, 4, 4, EPI>(p, plan.splits, s); break;
     case 3: launch<FMT, 192, 256, 2, 4, 3, EPI>(p, plan.splits, s); break;
-    default: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
+    case 4: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
+    case 5: launch<FMT, 128, 256, 2, 2, 2, EPI>(p, plan.splits, s); break;
+    default: launch<FMT, 64, 128, 2, 2, 2, EPI>(p, plan.splits, s); break;
   }
 }
 
