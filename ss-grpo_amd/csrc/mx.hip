@@ -158,7 +158,15 @@ __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const vo
   __syncthreads();
   ss = 0.0;
   for (int i = 0; i < threads / 64; ++i) ss += red[i];
-  const double rs = rsqrt(ss * inv_h + (double)eps);
+  double rs = rsqrt(ss * inv_h + (double)eps);
+  if (!(rs > 0x1p-64 && rs < 0x1p64)) {  // fp32 rows near the type's ends: both factors where 32 bits hold them in full
+    const float f = rs < 1.0 ? 0x1p-64f : 0x1p64f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[c][j] *= f;
+    rs /= (double)f;
+  }
   const float rs_hi = (float)rs, rs_lo = (float)(rs - (double)rs_hi);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
@@ -203,11 +211,12 @@ void launch_norm(const void* x, const void* delta, const void* w, void* sum, int
     hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 2>), g, b, 0, s, x, delta, w, sum, rows, H, inv_h, eps, codes, scales);
 }
 
-int64_t tiles_of(int rows, int cols, int* steps, int* step_tiles) {
-  *steps = (cols + fg::kMxStep - 1) / fg::kMxStep;
+int64_t tiles_of(int64_t rows, int64_t cols, int* steps, int* step_tiles) {
+  *steps = (int)((cols + fg::kMxStep - 1) / fg::kMxStep);
   *step_tiles = (*steps + kTileSteps - 1) / kTileSteps;
-  return (int64_t)((rows + kTileRows - 1) / kTileRows) * *step_tiles;
+  return (rows + kTileRows - 1) / kTileRows * *step_tiles;
 }
+constexpr int64_t kMaxThreads = (1ll << 32) - 1;  // of a launch
 
 }  // namespace
 
@@ -224,7 +233,7 @@ int fg_mx_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, in
              "fg_mx_quantize: rows must start 16-byte aligned, scales 4-byte aligned");
   int steps, st;
   const int64_t tiles = tiles_of(rows, cols, &steps, &st);
-  FG_REQUIRE(tiles < (1ll << 31), "fg_mx_quantize: bad shape (too many elements for one call)");
+  FG_REQUIRE(tiles * 256 <= kMaxThreads, "fg_mx_quantize: bad shape (too many rows for one call)");
   hipStream_t s = (hipStream_t)stream;
   const dim3 g((unsigned)tiles), b(256);
   uint8_t* c = (uint8_t*)codes;
@@ -251,7 +260,7 @@ int fg_mx_dequantize(const void* codes, const void* scales, int format, int rows
              "fg_mx_dequantize: rows must start 16-byte aligned, scales 4-byte aligned");
   int steps, st;
   const int64_t tiles = tiles_of(rows, cols, &steps, &st);
-  FG_REQUIRE(tiles < (1ll << 31), "fg_mx_dequantize: bad shape (too many elements for one call)");
+  FG_REQUIRE(tiles * 256 <= kMaxThreads, "fg_mx_dequantize: bad shape (too many rows for one call)");
   hipStream_t s = (hipStream_t)stream;
   const dim3 g((unsigned)tiles), b(256);
   const uint8_t *c = (const uint8_t*)codes, *sc = (const uint8_t*)scales;
@@ -273,6 +282,7 @@ int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* su
   FG_REQUIRE(rows > 0 && hidden > 0, "fg_rmsnorm_mx: bad shape");
   FG_REQUIRE(hidden % fg::kMxBlock == 0 && hidden <= 8192,
              "fg_rmsnorm_mx: hidden must be a multiple of 32, at most 8192");
+  FG_REQUIRE((int64_t)rows * 512 <= kMaxThreads, "fg_rmsnorm_mx: bad shape (too many rows for one call)");
   FG_REQUIRE((((uintptr_t)x | (uintptr_t)delta | (uintptr_t)weight | (uintptr_t)sum | (uintptr_t)codes) & 15) == 0 &&
                  ((uintptr_t)scales & 3) == 0,
              "fg_rmsnorm_mx: rows must start 16-byte aligned, scales 4-byte aligned");

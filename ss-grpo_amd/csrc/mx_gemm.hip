@@ -6,9 +6,10 @@
 // x [rows, K] in e4m3 or e2m1, w [cols, K] in e2m1, fp32 sums. v_mfma_scale_f32_32x32x64_f8f6f4 multiplies codes of
 // both formats as they are and applies each block's two scales itself, so nothing is decoded on the way: a byte of
 // weights is two operands. It does 2048 (e4m3 x e2m1) or 4096 (e2m1 x e2m1) multiply-adds per clock and SIMD.
-// Products of e2m1 codes are exact; with e4m3 codes the instruction aligns the products of a few neighbouring
-// elements to their largest before it adds them in 32 bits, and bits under 2^-14 of that one are lost (measured:
-// 1e-5 of the sum of magnitudes on random codes), a hundredth of the rounding that the bf16 output makes.
+// Products of e2m1 codes are exact; with e4m3 codes the instruction adds the products of eight neighbouring elements
+// cut (towards zero) to multiples of 2^-13 of the power of two at or below the largest of them, and carries 24 bits
+// from there on (found by comparison; 1e-5 of the sum of magnitudes on random codes), a hundredth of the rounding that
+// the bf16 output makes.
 //
 // Operand layout (lane l, r = l % 32, h = l / 32, 64 elements of K per instruction), found by exact comparison over
 // random codes and scales: e2m1 lanes hold row r, elements 32h .. 32h + 31 (16 bytes); e4m3 lanes hold row r,
@@ -17,7 +18,7 @@
 // the first in registers 4g .. 4g + 3. The weights are the first operand, so that a lane ends with four consecutive
 // output columns of one row.
 //
-// Tiling: a workgroup of 4 waves per output tile of BM rows x BN weight rows. K advances 128 elements (one dword of
+// Tiling: a workgroup of 4 or 8 waves per output tile of BM rows x BN weight rows. K advances 128 elements (one dword of
 // scales per row) per step through an NS-stage ring in LDS that direct HBM->LDS loads fill: x rows of 128 (or 64)
 // bytes, weight rows of 64, and the step's scale dwords of both, which lie side by side in memory. Chunks of 16
 // bytes are XOR-swizzled by row so that the fragment reads of neighbouring rows hit distinct banks. A step is two
@@ -734,7 +735,7 @@ struct Tile {
   float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
 };
 // Fitted to times of every tile and several splits with e4m3 rows over 1 .. 3500 rows x 200 .. 37888 columns x 192 ..
-// 18944: what the estimate picks is 3 % behind the fastest in the geometric mean, 20 % at worst.
+// 18944: what the estimate picks is 2 % behind the fastest in the geometric mean, 20 % at worst.
 constexpr Tile kTiles[] = {
     {64, 128, 32, 0.31f, 2.5f, 1.6f, 0.95f},
     {128, 128, 64, 0.42f, 3.5f, 1.9f, 0.95f},
@@ -744,7 +745,7 @@ constexpr Tile kTiles[] = {
     {128, 256, 64, 1.05f, 4.5f, 2.6f, 0.8f},
     {64, 128, 32, 0.35f, 2.5f, 1.45f, 0.4f},
 };
-constexpr int kTileCount = 7, kMaxSplits = 16;
+constexpr int kTileCount = 7, kTwoStages = 5, kMaxSplits = 16;  // from kTwoStages on: rings of two stages
 
 struct Plan {
   int tile;    // of kTiles; -1: the stream of few rows
@@ -753,12 +754,16 @@ struct Plan {
 
 constexpr float kReadRate = 5.5e6f;  // bytes per us that the weights are read at
 
+int64_t tiles_of(const Tile& t, int rows, int wrows) {
+  return (int64_t)((rows + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn);
+}
+
 // Estimated microseconds of a plan: whole rounds of 256 workgroups (of which a second one beside the first takes 0.7
 // of its time, or 0.2 where four fit), not under what the card sustains in matrix work (1.45 times as much where both
 // operands are e2m1) or in bytes; the output's bytes on top where nothing else runs meanwhile. A split product writes
 // and reads its fp32 sums instead and takes a second launch.
 float plan_us(const Tile& t, int splits, bool gate_up, int fmt, int rows, int wrows, int steps) {
-  const int64_t tiles_n = (wrows + t.bn - 1) / t.bn, tiles = (int64_t)((rows + t.bm - 1) / t.bm) * tiles_n;
+  const int64_t tiles_n = (wrows + t.bn - 1) / t.bn, tiles = tiles_of(t, rows, wrows);
   const float n = (float)(tiles * splits);
   const bool beside = t.pair > 0 && n > 256;
   const float rounds = beside ? std::max(t.pair < 0.5f ? 1.2f : 1.7f, t.pair * n / 256) : (float)((tiles * splits + 255) / 256);
@@ -793,8 +798,9 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
   float least = 1e30f;
   for (int c = 0; c < kTileCount; ++c)
     for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
-      // (the two-stage ring of the last tile keeps too little in flight for a long reduction)
-      if (s > 1 && (steps / s < 3 || !splits_ok(steps, s) || c == kTileCount - 1)) continue;
+      // (two stages keep too little in flight for a long reduction; what fills the card four times is not split)
+      if (s > 1 && (steps / s < 3 || !splits_ok(steps, s) || c >= kTwoStages || tiles_of(kTiles[c], rows, wrows) > 1024))
+        continue;
       const float us = plan_us(kTiles[c], s, gate_up, fmt, rows, wrows, steps);
       if (us < least) {
         least = us;
@@ -833,8 +839,11 @@ void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
     case 2: launch<FMT, 128, 256, 2, 4, 4, EPI>(p, plan.splits, s); break;
     case 3: launch<FMT, 192, 256, 2, 4, 3, EPI>(p, plan.splits, s); break;
     case 4: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
-    case 5: launch<FMT, 128, 256, 2, 2, 2, EPI>(p, plan.splits, s); break;
-    default: launch<FMT, 64, 128, 2, 2, 2, EPI>(p, plan.splits, s); break;
+    default:
+      if constexpr (EPI != kParts) {  // from kTwoStages on: never split
+        if (plan.tile == 5) launch<FMT, 128, 256, 2, 2, 2, EPI>(p, 1, s);
+        else launch<FMT, 64, 128, 2, 2, 2, EPI>(p, 1, s);
+      }
   }
 }
 
@@ -893,20 +902,25 @@ void run(MxArgs p, int x_format, void* workspace, size_t workspace_bytes, hipStr
     run_format<fg::kE2M1, EPI>(p, plan, s);
 }
 
+// Row counts whose grids (up to 512 threads for each 128 x 256 tile, 256 for each 64 x 128) stay under 2^32 threads.
+bool sizes_ok(int rows, int64_t wrows, int hidden) {
+  return rows > 0 && rows <= (1 << 22) && wrows > 0 && wrows <= (1 << 22) && hidden > 0 && hidden <= (1 << 20) &&
+         (int64_t)((rows + 63) / 64) * ((wrows + 127) / 128) < (1 << 23);
+}
+
 int check(const char* what, const void* x_codes, const void* x_scales, int x_format, const void* w_codes,
           const void* w_scales, int rows, int64_t wrows, int hidden) {
   const std::string f(what);
   FG_REQUIRE(x_codes && x_scales && w_codes && w_scales, f + ": null pointer");
   FG_REQUIRE(x_format == fg::kE4M3 || x_format == fg::kE2M1, f + ": bad format");
-  FG_REQUIRE(rows > 0 && rows <= (1 << 22) && wrows > 0 && wrows <= (1 << 22) && hidden > 0 && hidden <= (1 << 20),
-             f + ": bad shape");
+  FG_REQUIRE(sizes_ok(rows, wrows, hidden), f + ": bad shape");
   FG_REQUIRE(hidden % fg::kMxBlock == 0, f + ": hidden must be a multiple of 32");
   FG_REQUIRE((((uintptr_t)x_codes | (uintptr_t)w_codes) & 15) == 0 && (((uintptr_t)x_scales | (uintptr_t)w_scales) & 3) == 0,
              f + ": codes must be 16-byte aligned, scales 4-byte aligned");
   const int64_t steps = (hidden + kStep - 1) / kStep;
-  // 32-bit offsets within one operand
-  FG_REQUIRE(wrows * hidden / 2 < (1ll << 31) && steps * wrows * 4 < (1ll << 31) && steps * rows * 4 < (1ll << 31),
-             f + ": operands must be smaller than 2 GiB");
+  // 32-bit offsets within the weights and the scales, and up to a step of codes behind them (which reads as 0)
+  FG_REQUIRE(wrows * hidden / 2 <= (1ll << 31) - 256 && steps * wrows * 4 < (1ll << 31) && steps * rows * 4 < (1ll << 31),
+             f + ": the weight and the scales must be smaller than 2 GiB each");
   return 0;
 }
 
@@ -915,7 +929,7 @@ int check(const char* what, const void* x_codes, const void* x_scales, int x_for
 extern "C" {
 
 size_t fg_mx_linear_workspace(int rows, int cols, int hidden, int x_format) {
-  if (rows <= 0 || cols <= 0 || hidden <= 0) return 0;
+  if (!sizes_ok(rows, cols, hidden)) return 0;
   return parts_bytes(make_plan(false, x_format, rows, cols, (hidden + kStep - 1) / kStep, true), rows, cols);
 }
 
@@ -948,7 +962,7 @@ int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const 
 }
 
 size_t fg_mx_gate_up_swiglu_workspace(int rows, int inter, int hidden, int x_format) {
-  if (rows <= 0 || inter <= 0 || hidden <= 0 || inter > (1 << 21)) return 0;
+  if (!sizes_ok(rows, 2 * (int64_t)inter, hidden)) return 0;
   return parts_bytes(make_plan(true, x_format, rows, 2 * inter, (hidden + kStep - 1) / kStep, true), rows, 2 * inter);
 }
 

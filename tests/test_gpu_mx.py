@@ -219,6 +219,20 @@ def test_rmsnorm_special_rows():
     assert np.array_equal(codes[fine], want_c) and np.array_equal(scales[:, fine], want_s)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [2.0 ** -149, 2.0 ** -126, 1e-30, 1e-19, 1e19, 1e30, 2.0 ** 124])
+def test_rmsnorm_near_the_ends_of_the_type(size, dtype):
+    """Rows so small or large that the norm's factor (eps 0) or its rounding error has no place in 32 bits."""
+    x = rows_of(40, 2080, 21, torch.float32, spread=0.2).clamp(-8, 8)
+    x = (x.double() * size).to(dtype)
+    x[:, 0] = size
+    w = torch.exp(torch.randn(2080, generator=torch.Generator().manual_seed(2))).to(dtype)
+    want_c, want_s = O.quantize(O.rmsnorm(x.double().numpy(), w.double().numpy(), 0.0), "e4m3")
+    codes, scales = held(K().rmsnorm_mx(x.to(DEV), w.to(DEV), 0.0))
+    assert np.array_equal(scales, want_s)  # (bf16 rows of 2^-149 are zeros: 0 / 0, NaN blocks, whose codes are free)
+    assert np.array_equal(O.values(codes, scales, "e4m3"), O.values(want_c, want_s, "e4m3"), equal_nan=True)
+
+
 # ------------------------------------------------------------------ products
 def product_bound(xv, wv, fmt):
     """How far a product's fp32 sums may be off (see the head of this file), and the exact products."""
@@ -363,6 +377,59 @@ def test_without_workspace_a_split_product_runs_unsplit(rows, n, k):
     assert torch.equal(out, kk.mx_linear(x, w))
 
 
+def strips(rows, n, at_once=32):
+    """Rows and columns that meet every tile of an output: a pair of index lists, first and last ones included."""
+    pick = lambda size: sorted({0, size - 1, *range(7, size, max(size // at_once, 1))})
+    return torch.tensor(pick(rows), device=DEV), torch.tensor(pick(n), device=DEV)
+
+
+def device_pair(rows, cols, fmt, seed, scale=1.0, spread=1.0):
+    """An MX pair made on the device (bit for bit the oracle's, by the tests above) and its float64 values there."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g, device=DEV) * scale
+    x *= torch.exp(spread * torch.randn(rows, cols // 32, generator=g, device=DEV)).repeat_interleave(32, 1)
+    q = K().mx_quantize(x, fmt)
+    return q, K().mx_dequantize(q, torch.float32)
+
+
+# Sizes at which the choice takes each tile, whole and in parts; odd sizes where it allows them.
+LARGE = [(777, 1280, 8960), (1408, 1533, 13824), (2311, 2048, 18944), (1856, 2045, 28672), (3500, 2047, 2048),
+         (2311, 2559, 3584), (2311, 4607, 2080), (2311, 5119, 2080), (1856, 18943, 3584)]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("rows,n,k", LARGE)
+def test_linear_of_every_tile_with_bias_and_residual_in_place(rows, n, k, fmt):
+    g = torch.Generator(device=DEV).manual_seed(n)
+    (x, xv), (w, wv) = device_pair(rows, k, fmt, rows), device_pair(n, k, "e2m1", n)
+    bias = torch.randn(n, device=DEV, generator=g).to(torch.bfloat16)
+    res = (k ** 0.5 * torch.randn(rows, n, device=DEV, generator=g)).to(torch.bfloat16)
+    out = res.clone()
+    assert K().mx_linear(x, w, bias=bias, residual=out, out=out) is out
+    rr, cc = strips(rows, n)
+    for r, c in ((rr, slice(None)), (slice(None), cc)):
+        exact, err = product_bound(xv[r].double().cpu().numpy(), wv[c].double().cpu().numpy(), fmt)
+        check_linear(out[r][:, c], exact, err, bias[c], res[r][:, c])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("rows,inter,k", [(2311, 768, 5120), (1856, 1792, 2080), (4096, 1280, 1376), (2048, 4096, 1056),
+                                          (500, 18944, 1536), (1408, 768, 13824)])
+def test_gate_up_of_every_tile(rows, inter, k, fmt):
+    (x, xv), (w, wv) = device_pair(rows, k, fmt, rows, spread=0.5), device_pair(2 * inter, k, "e2m1", k, k ** -0.5, 0.5)
+    q = K().mx_gate_up_swiglu(x, w)
+    rr = strips(rows, 1, 24)[0]
+    cc = torch.tensor(sorted({0, inter // 32 - 1, *range(1, inter // 32, max(inter // 320, 1))}), device=DEV)  # whole blocks
+    cols = (cc[:, None] * 32 + torch.arange(32, device=DEV)).flatten()
+    every = torch.arange(rows, device=DEV)
+    for r, b, c in ((rr, torch.arange(inter // 32, device=DEV), torch.arange(inter, device=DEV)), (every, cc, cols)):
+        flat = torch.zeros(len(r), -(-len(b) // 4) * 4, dtype=torch.uint8, device=DEV)
+        flat[:, :len(b)] = q.scales.transpose(0, 1).reshape(rows, -1)[r][:, b]
+        part = K().MX(q.codes.view(torch.uint8)[r][:, c].contiguous().view(torch.float8_e4m3fn),
+                      flat.view(len(r), -1, 4).transpose(0, 1).contiguous())
+        check_gate_up(part, xv[r].double().cpu().numpy(), torch.cat([wv[c], wv[inter + c]]).double().cpu().numpy(), fmt)
+
+
 # ------------------------------------------------------------------ together
 def mlp(k, x, delta, norm, gate_up, down):
     q = k.rmsnorm_mx(x, norm, 1e-6, delta=delta)
@@ -423,6 +490,38 @@ def test_chain_is_the_same_twice_captured_and_on_another_stream(rows):
         graphs[1].replay()
         torch.cuda.synchronize()
         assert torch.equal(a, want) and torch.equal(b, want) and torch.equal(x, want)
+
+
+def test_split_products_of_two_streams_at_once():
+    """Two products whose sums go through workspaces, in flight together: each has its own."""
+    k = K()
+    pairs = [(random_mx(40, 9600, "e4m3", i)[0], random_mx(300, 9600, "e2m1", i + 5)[0]) for i in (1, 2)]
+    want = [k.mx_linear(x, w) for x, w in pairs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(k.mx_linear(*pairs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in (0, 1) for o in got[i])
+
+
+def test_calls_under_a_kernel_timer_are_timed_and_the_same():
+    from flashgrpo_amd import timing
+
+    k = K()
+    x, d, norm, gu, dn = mlp_state(5, 256, 320, 9)
+    first = x.clone()
+    want = mlp(k, x, d, norm, gu, dn)[2].clone()
+    x.copy_(first)
+    t = timing.KernelTimer()
+    with timing.active(t):
+        assert torch.equal(mlp(k, x, d, norm, gu, dn)[2], want)
+    torch.cuda.synchronize()
+    assert {"fg_rmsnorm_mx", "fg_mx_gate_up_swiglu", "fg_mx_linear"} <= set(t.summary())
 
 
 # ------------------------------------------------------------------ refusals

@@ -84,6 +84,70 @@ def test_entry_points_refuse_bad_arguments_on_the_host():
     refused(lib.fg_rmsnorm_mx(odd, None, p, None, 1, 1, 64, 1e-6, p, p, None), b"aligned")
 
 
+def test_products_refuse_bad_arguments_on_the_host():
+    lib = _lib()
+    p, off8, off1, n = ctypes.c_void_p(256), ctypes.c_void_p(264), ctypes.c_void_p(257), None
+
+    def refused(rc, text):
+        assert rc != 0 and text in lib.fg_last_error(), (rc, lib.fg_last_error())
+
+    def linear(xc=p, xs=p, f=0, wc=p, ws=p, rows=4, cols=64, hidden=64, bias=n, res=n, ldr=64, out=p, ldo=64, wksp=n, size=0):
+        return lib.fg_mx_linear(xc, xs, f, wc, ws, rows, cols, hidden, bias, res, ldr, out, ldo, wksp, size, None)
+
+    def gate_up(xc=p, xs=p, f=0, wc=p, ws=p, rows=4, inter=64, hidden=64, codes=p, scales=p, wksp=n, size=0):
+        return lib.fg_mx_gate_up_swiglu(xc, xs, f, wc, ws, rows, inter, hidden, codes, scales, wksp, size, None)
+
+    for call in (linear, gate_up):
+        for name in ("xc", "xs", "wc", "ws"):
+            refused(call(**{name: n}), b"null pointer")
+        refused(call(f=2), b"format")
+        refused(call(f=-1), b"format")
+        refused(call(rows=0), b"shape")
+        refused(call(rows=(1 << 22) + 1), b"shape")
+        refused(call(hidden=0), b"shape")
+        refused(call(hidden=48), b"multiple of 32")
+        refused(call(xc=off8), b"aligned")
+        refused(call(wc=off8), b"aligned")
+        refused(call(xs=off1), b"aligned")
+        refused(call(wksp=off8), b"workspace")
+    refused(linear(cols=-1), b"shape")
+    refused(linear(rows=1 << 22, cols=1 << 22, hidden=32, ldo=1 << 22), b"shape")  # more tiles than a launch takes
+    refused(linear(cols=1 << 16, hidden=1 << 16, ldo=1 << 16), b"2 GiB")
+    refused(linear(rows=1 << 22, hidden=1 << 16), b"2 GiB")   # the rows' scales
+    refused(linear(out=n), b"null pointer")
+    refused(linear(out=off1), b"aligned")
+    refused(linear(bias=off1), b"aligned")
+    refused(linear(ldo=63), b"strides")
+    refused(linear(res=p, ldr=63), b"strides")
+    refused(gate_up(codes=n), b"null pointer")
+    refused(gate_up(scales=n), b"null pointer")
+    refused(gate_up(inter=48), b"multiple of 32")
+    refused(gate_up(inter=1 << 30), b"shape")
+    refused(gate_up(codes=off8), b"aligned")
+    refused(gate_up(scales=off1), b"aligned")
+
+
+def test_more_rows_than_a_launch_takes_are_refused():
+    lib = _lib()
+    p = ctypes.c_void_p(256)
+    most = 2 ** 31 - 1
+    for rc in (lib.fg_mx_quantize(p, 1, 32, most, 32, 0, p, p, None), lib.fg_mx_dequantize(p, p, 1, most, 32, p, 1, 32, None),
+               lib.fg_rmsnorm_mx(p, None, p, None, 1, 1 << 23, 32, 1e-6, p, p, None)):
+        assert rc != 0 and b"too many rows" in lib.fg_last_error()
+
+
+def test_workspace_sizes():
+    """Sums of split products only; 0 for sizes that the calls refuse."""
+    lib = _lib()
+    assert lib.fg_mx_linear_workspace(1, 64, 64, 0) == 0
+    need = lib.fg_mx_linear_workspace(40, 301, 9600, 0)
+    assert need >= 2 * 40 * 304 * 4 and need % (40 * 304 * 4) == 0
+    assert lib.fg_mx_gate_up_swiglu_workspace(20, 288, 4128, 0) % (20 * 576 * 4) == 0
+    for bad in (0, -1, 2 ** 31 - 1):
+        assert lib.fg_mx_linear_workspace(bad, 64, 64, 0) == lib.fg_mx_linear_workspace(64, bad, 64, 0) == 0
+        assert lib.fg_mx_linear_workspace(64, 64, bad, 0) == lib.fg_mx_gate_up_swiglu_workspace(64, bad, 64, 0) == 0
+
+
 def test_wrappers_take_device_tensors_only():
     from flashgrpo_amd import kernels as K
 
