@@ -5,7 +5,7 @@
 //
 // x [rows, K] in e4m3 or e2m1, w [cols, K] in e2m1, fp32 sums. v_mfma_scale_f32_32x32x64_f8f6f4 multiplies codes of
 // both formats as they are and applies each block's two scales itself, so nothing is decoded on the way: a byte of
-// weights is two operands. It does 2048 (e4m3 x e2m1) or 4096 (e2m1 x e2m1) multiply-adds per clock and SIMD.
+// weights is two operands. It does 1024 (e4m3 x e2m1) or 2048 (e2m1 x e2m1) multiply-adds per clock and SIMD.
 // Products of e2m1 codes are exact; with e4m3 codes the instruction adds the products of eight neighbouring elements
 // cut (towards zero) to multiples of 2^-13 of the power of two at or below the largest of them, and carries 24 bits
 // from there on (found by comparison; 1e-5 of the sum of magnitudes on random codes), a hundredth of the rounding that
