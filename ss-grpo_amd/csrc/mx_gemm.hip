@@ -527,84 +527,103 @@ FG_DEVICE intx8 part_of(const intx8& x, int part) {
   return r;
 }
 
-// Up to 16 rows: the weights are streamed once, straight into registers, and the rows are read beside them. A
+// Few rows (up to 16 MT): the weights are streamed once, straight into registers, and the rows are read beside them. A
 // workgroup takes NT tiles of 16 weight rows (gate_up: 32 gate and 32 up rows, one block of 32 output columns) and its
 // waves take every waves-th step of 128 elements, so that together they read each row's bytes in order; v_mfma_scale_
 // f32_16x16x128_f8f6f4 multiplies a step (lane l: row l % 16; e2m1 elements 32 (l / 16) .. + 31, e4m3 elements
 // 16 (l / 16) .. + 15 and 64 further; scale of block l / 16 from a byte of its register; D: column l % 16 of the second
-// operand, rows 4 (l / 16) + 0..3 of the first). The waves' sums meet in LDS, added in wave order.
-// There are no loads to wait for but the weights, so the loop only keeps U steps of them in flight per wave; long
-// reductions over few columns take more waves per workgroup instead of a second launch.
-constexpr int kStreamRows = 16;
+// operand, rows 4 (l / 16) + 0..3 of the first) for each of MT tiles of 16 rows. The waves' sums meet in LDS, a few
+// tiles at a time, added in wave order.
+// There are no loads to wait for but the weights and (from L2) the rows, so the loop only keeps U steps of them in
+// flight per wave; long reductions over few columns take more waves per workgroup instead of a second launch.
 constexpr int kStreamLd = 20;  // floats per x row and tile in LDS: 16-byte stores on distinct banks
+constexpr int kStreamLds = 64 * 1024;
+// tiles of 16 rows whose sums meet at once
+constexpr int stream_pass(int nt, int mt) { return nt == 4 ? 1 : mt < 4 ? mt : 4; }
 
-template <int FMT, int NT, int U, int EPI>
-__global__ void __launch_bounds__(NT == 4 ? 512 : 1024) mx_stream_kernel(MxArgs p) {
+constexpr int stream_waves(int nt) { return nt == 1 ? 12 : 8; }  // at most
+
+template <int FMT, int NT, int MT, int U, int EPI>
+__global__ void __launch_bounds__(64 * stream_waves(NT)) mx_stream_kernel(MxArgs p) {
   typedef float floatx4 __attribute__((ext_vector_type(4)));
   constexpr int XR = FMT == fg::kE4M3 ? 2 : 1, XB = FMT == fg::kE4M3 ? 128 : 64;
   constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;
   static_assert(EPI != kGateUp || NT == 4, "gate_up: two tiles of gate rows and two of up rows");
-  extern __shared__ __attribute__((aligned(16))) float red[];  // [waves][NT][16 x rows][16 weight rows]
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [tiles of a pass][waves][NT][16 x rows][16 weight rows]
   constexpr int RLD = kStreamLd;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
   const int n0 = blockIdx.x * (EPI == kGateUp ? 32 : NT * 16);
 
-  const uint8_t* wrow[NT];
+  uint32_t wrow[NT];  // offsets: the weight, and so few rows, are under 2 GiB
   uint32_t wscale[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     int n = n0 + (EPI == kGateUp ? (i & 1) * 16 : i * 16) + r;
     n = min(n, (EPI == kGateUp ? p.cols : p.wrows) - 1) + (EPI == kGateUp && i >= 2 ? p.cols : 0);
-    wrow[i] = p.w + (int64_t)n * p.wb;
+    wrow[i] = (uint32_t)n * p.wb;
     wscale[i] = n;
   }
-  const int m = min(r, p.rows - 1);
-  const uint8_t* xrow = p.x + (int64_t)m * p.xb;
-
-  floatx4 acc[NT];
+  uint32_t xrow[MT], xm[MT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  int4 wv[U][NT], xv[U][XR];
-  uint32_t ws[U][NT], xs[U];
+  for (int k = 0; k < MT; ++k) {
+    xm[k] = (uint32_t)min(k * 16 + r, p.rows - 1);
+    xrow[k] = xm[k] * p.xb;
+  }
+
+  floatx4 acc[MT][NT];
+#pragma unroll
+  for (int k = 0; k < MT; ++k)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[k][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  int4 wv[U][NT], xv[U][MT][XR];
+  uint32_t ws[U][NT], xs[U][MT];
   // A step's loads; chunks behind the rows' end (the last step of a K that is no multiple of 128) read the row's
   // first bytes and count as zeros.
   auto load = [&](int u, int t) __attribute__((always_inline)) {
-    const int wo = t * 64 + g * 16;
-    const bool w_in = wo < p.wb;
+    const uint32_t wo = t * 64 + g * 16;
+    const bool w_in = wo < (uint32_t)p.wb;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int4 v = *(const int4*)(wrow[i] + (w_in ? wo : 0));
+      const int4 v = *(const int4*)(p.w + (wrow[i] + (w_in ? wo : 0)));
       wv[u][i] = w_in ? v : make_int4(0, 0, 0, 0);
-      ws[u][i] = p.ws[(int64_t)t * p.wrows + wscale[i]];
+      ws[u][i] = p.ws[(uint32_t)t * p.wrows + wscale[i]];
     }
 #pragma unroll
-    for (int h = 0; h < XR; ++h) {
-      const int xo = t * XB + g * 16 + h * 64;
-      const bool x_in = xo < p.xb;
-      const int4 v = *(const int4*)(xrow + (x_in ? xo : 0));
-      xv[u][h] = x_in ? v : make_int4(0, 0, 0, 0);
+    for (int k = 0; k < MT; ++k) {
+#pragma unroll
+      for (int h = 0; h < XR; ++h) {
+        const uint32_t xo = t * XB + g * 16 + h * 64;
+        const bool x_in = xo < (uint32_t)p.xb;
+        const int4 v = *(const int4*)(p.x + (xrow[k] + (x_in ? xo : 0)));
+        xv[u][k][h] = x_in ? v : make_int4(0, 0, 0, 0);
+      }
+      xs[u][k] = p.xs[(uint32_t)t * p.rows + xm[k]];
     }
-    xs[u] = p.xs[(int64_t)t * p.rows + m];
   };
-  auto multiply_part = [&](int u, const intx8& x) __attribute__((always_inline)) {
+  auto multiply_part = [&](int u, int k, const intx8& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const intx8 w = intx8{wv[u][i].x, wv[u][i].y, wv[u][i].z, wv[u][i].w, 0, 0, 0, 0};
-      acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[i], 4, kBF, 0, (int)(ws[u][i] >> (8 * g)), 0,
-                                                                (int)(xs[u] >> (8 * g)));
+      acc[k][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc[k][i], 4, kBF, 0,
+                                                                   (int)(ws[u][i] >> (8 * g)), 0, (int)(xs[u][k] >> (8 * g)));
     }
   };
   auto multiply = [&](int u) __attribute__((always_inline)) {
-    intx8 x = intx8{xv[u][0].x, xv[u][0].y, xv[u][0].z, xv[u][0].w, 0, 0, 0, 0};
-    if constexpr (XR == 2) {
-      x[4] = xv[u][1].x; x[5] = xv[u][1].y; x[6] = xv[u][1].z; x[7] = xv[u][1].w;
+#pragma unroll
+    for (int k = 0; k < MT; ++k) {
+      const int4 lo = xv[u][k][0];
+      intx8 x = intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
+      if constexpr (XR == 2) {
+        const int4 hi = xv[u][k][1];
+        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+      }
+      if constexpr (EPI == kGateUp && FMT == fg::kE4M3) {  // an 8-bit code follows: lose nothing (it is nearly free here)
+        multiply_part(u, k, part_of(x, 1));
+        x = part_of(x, 0);
+      }
+      multiply_part(u, k, x);
     }
-    if constexpr (EPI == kGateUp && FMT == fg::kE4M3) {  // an 8-bit code follows: lose nothing (it is free here)
-      multiply_part(u, part_of(x, 1));
-      x = part_of(x, 0);
-    }
-    multiply_part(u, x);
   };
   int t = wave;
   for (; t + (U - 1) * waves < p.steps; t += U * waves) {
@@ -618,42 +637,51 @@ __global__ void __launch_bounds__(NT == 4 ? 512 : 1024) mx_stream_kernel(MxArgs 
     multiply(0);
   }
 
+  constexpr int PASS = stream_pass(NT, MT);
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-    *(floatx4*)(red + ((wave * NT + i) * 16 + r) * RLD + 4 * g) = acc[i];  // x row r, weight rows 4g .. 4g + 3
-  __syncthreads();
-  auto sum = [&](int i, int row, int c) __attribute__((always_inline)) {
-    float v = 0.0f;
-    for (int w = 0; w < waves; ++w) v += red[((w * NT + i) * 16 + row) * RLD + c];
-    return v;
-  };
-  if constexpr (EPI == kGateUp) {
-    for (int e = tid; e < ((p.rows * 32 + 63) & ~63); e += blockDim.x) {  // whole waves
-      const int row = min(e >> 5, p.rows - 1), c = e & 31;
-      const float v = silu_mul(sum(c >> 4, row, c & 15), sum(2 + (c >> 4), row, c & 15));
-      uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+  for (int k0 = 0; k0 < MT; k0 += PASS) {
+    const int rows = min(p.rows - k0 * 16, PASS * 16);
+    if (rows <= 0) break;  // for the whole workgroup
+    if (k0) __syncthreads();
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
-      const uint32_t s = fg::mx_scale_byte<fg::kE4M3>(a);
-      const float y = s == 255u ? 0.0f : v * fg::mx_inverse_scale(s);
-      if ((e >> 5) >= p.rows) continue;
-      p.codes[(int64_t)row * p.cols + n0 + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
-      if (c == 0) {
-        uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(n0 / kStep) * p.rows + row);
-        const int b = (n0 / 32) & 3;
-        sc[b] = (uint8_t)s;
-        if (n0 + 32 >= p.cols)  // the last block also writes the zeros behind it
-          for (int q = b + 1; q < 4; ++q) sc[q] = 0;
+    for (int k = 0; k < PASS; ++k)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)  // x row r, weight rows 4g .. 4g + 3
+        *(floatx4*)(red + (((k * waves + wave) * NT + i) * 16 + r) * RLD + 4 * g) = acc[k0 + k][i];
+    __syncthreads();
+    auto sum = [&](int i, int row, int c) __attribute__((always_inline)) {
+      float v = 0.0f;
+      for (int w = 0; w < waves; ++w) v += red[((((row >> 4) * waves + w) * NT + i) * 16 + (row & 15)) * RLD + c];
+      return v;
+    };
+    if constexpr (EPI == kGateUp) {
+      for (int e = tid; e < ((rows * 32 + 63) & ~63); e += blockDim.x) {  // whole waves
+        const int in = min(e >> 5, rows - 1), row = k0 * 16 + in, c = e & 31;
+        const float v = silu_mul(sum(c >> 4, in, c & 15), sum(2 + (c >> 4), in, c & 15));
+        uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
+        const uint32_t s = fg::mx_scale_byte<fg::kE4M3>(a);
+        const float y = s == 255u ? 0.0f : v * fg::mx_inverse_scale(s);
+        if ((e >> 5) >= rows) continue;
+        p.codes[(int64_t)row * p.cols + n0 + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+        if (c == 0) {
+          uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(n0 / kStep) * p.rows + row);
+          const int b = (n0 / 32) & 3;
+          sc[b] = (uint8_t)s;
+          if (n0 + 32 >= p.cols)  // the last block also writes the zeros behind it
+            for (int q = b + 1; q < 4; ++q) sc[q] = 0;
+        }
       }
-    }
-  } else {
-    for (int e = tid; e < p.rows * NT * 16; e += blockDim.x) {
-      const int row = e / (NT * 16), c = e - row * (NT * 16), n = n0 + c;
-      if (n >= p.wrows) continue;
-      float v = sum(c >> 4, row, c & 15);
-      if (p.bias) v += fg::bf16_to_f32(p.bias[n]);
-      if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)row * p.ldr + n]);
-      p.out[(int64_t)row * p.ldo + n] = fg::f32_to_bf16(v);
+    } else {
+      for (int e = tid; e < rows * NT * 16; e += blockDim.x) {
+        const int in = e / (NT * 16), row = k0 * 16 + in, c = e - in * (NT * 16), n = n0 + c;
+        if (n >= p.wrows) continue;
+        float v = sum(c >> 4, in, c & 15);
+        if (p.bias) v += fg::bf16_to_f32(p.bias[n]);
+        if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)row * p.ldr + n]);
+        p.out[(int64_t)row * p.ldo + n] = fg::f32_to_bf16(v);
+      }
     }
   }
 }
@@ -729,21 +757,23 @@ __global__ void __launch_bounds__(256) mx_finish_gate_up_kernel(MxArgs p) {
 // ------------------------------------------------------------------ which kernel
 struct Tile {
   int bm, bn, wave_rows;  // rows and weight rows of a workgroup, rows of a wave
-  float step_us;   // one step of one workgroup, a CU to itself
+  float step_us;   // one step of one workgroup, a CU to itself, with e4m3 rows
+  float e2m1;      // what a step takes of that with e2m1 rows
   float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
   float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
   float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
 };
-// Fitted to times of every tile and several splits with e4m3 rows over 1 .. 3500 rows x 200 .. 37888 columns x 192 ..
-// 18944: what the estimate picks is 2 % behind the fastest in the geometric mean, 20 % at worst.
+// Fitted to times of every tile and many splits with rows of both formats over some 1400 sizes, 1 .. 4096 rows x 64 ..
+// 152000 columns x 160 .. 19000. Over 1850 others what the estimates pick is 1 to 2 % behind the fastest in the geometric
+// mean, 35 % at worst.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 0.31f, 2.5f, 1.6f, 0.95f},
-    {128, 128, 64, 0.42f, 3.5f, 1.9f, 0.95f},
-    {128, 256, 64, 0.66f, 4.0f, 2.35f, 0},
-    {192, 256, 96, 0.86f, 5.5f, 2.8f, 0},
-    {256, 256, 64, 1.04f, 6.0f, 2.9f, 0},
-    {128, 256, 64, 1.05f, 4.5f, 2.6f, 0.8f},
-    {64, 128, 32, 0.35f, 2.5f, 1.45f, 0.4f},
+    {64, 128, 32, 0.34f, 0.99f, 2.65f, 1.6f, 0.76f},
+    {128, 128, 64, 0.42f, 0.96f, 3.75f, 2.03f, 0.94f},
+    {128, 256, 64, 0.68f, 0.76f, 4.2f, 2.7f, 0},
+    {192, 256, 96, 0.79f, 0.75f, 5.55f, 2.8f, 0},
+    {256, 256, 64, 1.04f, 0.71f, 6.0f, 2.76f, 0},
+    {128, 256, 64, 1.08f, 0.85f, 4.0f, 2.6f, 0.73f},
+    {64, 128, 32, 0.36f, 1.0f, 2.5f, 1.0f, 0.37f},
 };
 constexpr int kTileCount = 7, kTwoStages = 5, kMaxSplits = 16;  // from kTwoStages on: rings of two stages
 
@@ -758,34 +788,44 @@ int64_t tiles_of(const Tile& t, int rows, int wrows) {
   return (int64_t)((rows + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn);
 }
 
-// Estimated microseconds of a plan: whole rounds of 256 workgroups (of which a second one beside the first takes 0.7
-// of its time, or 0.2 where four fit), not under what the card sustains in matrix work (1.45 times as much where both
-// operands are e2m1) or in bytes; the output's bytes on top where nothing else runs meanwhile. A split product writes
-// and reads its fp32 sums instead and takes a second launch.
+// Estimated microseconds of a plan: whole rounds of 256 workgroups (where more than one fit a CU, the share that each
+// takes, and not under what a first full round of them was found to take), not under what the card sustains in matrix work
+// (1.6 times as much where both operands are e2m1) or in bytes; the output's bytes on top where nothing else runs
+// meanwhile. A split product writes and reads its fp32 sums instead and takes a second launch.
 float plan_us(const Tile& t, int splits, bool gate_up, int fmt, int rows, int wrows, int steps) {
   const int64_t tiles_n = (wrows + t.bn - 1) / t.bn, tiles = tiles_of(t, rows, wrows);
+  const bool e4m3 = fmt == fg::kE4M3;
   const float n = (float)(tiles * splits);
   const bool beside = t.pair > 0 && n > 256;
-  const float rounds = beside ? std::max(t.pair < 0.5f ? 1.2f : 1.7f, t.pair * n / 256) : (float)((tiles * splits + 255) / 256);
-  const float work = rounds * ((steps + splits - 1) / splits) * t.step_us * (fmt == fg::kE4M3 ? 1.0f : 0.7f);
+  const float rounds = beside ? std::max(t.pair < 0.5f ? 1.37f : 3.08f, t.pair * n / 256) : (float)((tiles * splits + 255) / 256);
+  const float work = rounds * ((steps + splits - 1) / splits) * t.step_us * (e4m3 ? 1.0f : t.e2m1);
   const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
-  const float flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (fmt == fg::kE4M3 ? 1e9f : 1.45e9f));
+  const float flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.62e9f));
   const float in = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
   const float out = splits > 1 ? 0.0f : (float)rows * wrows * (gate_up ? 0.5f : 2.0f) / kReadRate;
   const float sums = (float)splits * rows * wrows * 4 * 2;
-  const float parts = splits == 1 ? 0.0f : 2.5f + sums / (sums < 16e6f ? 9e6f : 5e6f);
+  const float parts = splits == 1 ? 0.0f : 3.65f + sums / (sums < 16e6f ? 4.6e6f : 5.4e6f);
   const float ends = rounds * t.tile_us;
   if (beside) return 2.0f + std::max(work + ends, std::max(flops, in + out)) + parts;
   return 2.0f + std::max(work, std::max(flops, in)) + ends + out + parts;
 }
 
-// The same for the stream of up to 16 rows, which has no second launch and no ring to fill but reads the rows again for
-// every 16 weight rows (gate_up and wide outputs, four tiles to a workgroup: every 64), and gains nothing from its
-// waves where the steps are fewer than they.
-constexpr int kWideCols = 16384;
-float stream_us(bool wide, int rows, int wrows, int steps) {
-  const float wgs = (float)wrows / (wide ? 64 : 16);
-  return (wide ? 3.0f : 4.5f) + (float)wrows * steps * 68 / kReadRate + rows * wgs * steps * 1.3e-5f + (steps < 8 ? 1.5f : 0.0f);
+// The stream of few rows: tiles of 16 weight rows per workgroup as many as leave a workgroup per CU, up to four (the rows
+// are read again for each workgroup, which costs little for up to four of them: two tiles then), and up to 64, 32 and 16
+// rows with one, two and four tiles: beyond, the rows' bytes from L2 cost more than a tile's loads into LDS (4096 x 4096,
+// 32 rows: 7.7 against 10.1 us, 64 rows 12.2 against 12.3; 8192 x 4096, 32 rows: 8.9 against 11.3).
+int stream_tiles(bool gate_up, int rows, int wrows) {
+  return gate_up ? 4 : wrows <= 4096 ? 1 : wrows <= 8192 || rows <= 4 ? 2 : 4;
+}
+int stream_rows(int nt) { return 64 / nt; }
+
+// Estimated microseconds: a workgroup's steps (the weights' loads or the rows', whichever takes longer; with more
+// workgroups than CUs both), not under the weights' bytes.
+float stream_us(int nt, int fmt, int rows, int wrows, int steps) {
+  const float load = (float)((wrows + 16 * nt - 1) / (16 * nt)) / 256;
+  const float x = rows * (fmt == fg::kE4M3 ? 3.3e-3f : 1.5e-3f), w = nt == 1 ? 0.055f : nt == 2 ? 0.091f : 0.15f;
+  const float step = load <= 1 ? std::max(w, 0.055f + x) : (w + x) * std::max(load, 2.3f);
+  return std::max(2.5f + 6 * x + steps * step, 2.0f + (float)wrows * steps * 68 / kReadRate);
 }
 
 bool splits_ok(int steps, int splits) {
@@ -807,10 +847,11 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
         best = Plan{c, s};
       }
     }
-  // The stream of a gate_up with e4m3 rows loses nothing of their products, so it takes all up to its 16 rows (at 16
-  // and 8B's sizes 17.5 us against the smallest tile's 15.1).
-  if (rows <= kStreamRows && ((gate_up && fmt == fg::kE4M3) ||
-                              stream_us(gate_up || wrows >= kWideCols, rows, wrows, steps) <= least))
+  // The stream of a gate_up with e4m3 rows loses nothing of their products, so it may take a quarter longer (16 rows at
+  // 1.5B's and 8B's sizes: 8.6 and 17.5 us against the smallest tile's 7.8 and 15.1).
+  const int nt = stream_tiles(gate_up, rows, wrows);
+  if (rows <= stream_rows(nt) &&
+      stream_us(nt, fmt, rows, wrows, steps) <= least * (gate_up && fmt == fg::kE4M3 ? 1.25f : 1.0f))
     return Plan{-1, 1};
   return best;
 }
@@ -847,14 +888,24 @@ void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
   }
 }
 
-template <int FMT, int NT, int EPI>
-void launch_stream(const MxArgs& p, int waves, hipStream_t s) {
+template <int FMT, int NT, int MT, int EPI>
+void launch_stream_rows(const MxArgs& p, int waves, hipStream_t s) {
   const int per = EPI == kGateUp ? 32 : NT * 16, cols = EPI == kGateUp ? p.cols : p.wrows;
   // One step per wave in flight with x in two parts (8B gate/up of one row: 14.4 us, two steps' registers 16.8; not in
   // parts 13.9), else two.
-  constexpr int U = EPI == kGateUp ? 1 : 2;
-  hipLaunchKernelGGL((mx_stream_kernel<FMT, NT, U, EPI>), dim3((cols + per - 1) / per), dim3(64 * waves),
-                     waves * NT * 16 * kStreamLd * 4, s, p);
+  constexpr int U = EPI == kGateUp || MT > 1 ? 1 : 2;
+  constexpr int PASS = stream_pass(NT, MT);
+  static_assert(stream_waves(NT) * PASS * NT * 16 * kStreamLd * 4 <= kStreamLds, "LDS");
+  hipLaunchKernelGGL((mx_stream_kernel<FMT, NT, MT, U, EPI>), dim3((cols + per - 1) / per), dim3(64 * waves),
+                     PASS * waves * NT * 16 * kStreamLd * 4, s, p);
+}
+template <int FMT, int NT, int EPI>
+void launch_stream(const MxArgs& p, int waves, hipStream_t s) {
+  if constexpr (NT == 1)
+    if (p.rows > 32) return launch_stream_rows<FMT, NT, 4, EPI>(p, waves, s);
+  if constexpr (NT <= 2)
+    if (p.rows > 16) return launch_stream_rows<FMT, NT, 2, EPI>(p, waves, s);
+  launch_stream_rows<FMT, NT, 1, EPI>(p, waves, s);
 }
 
 template <int FMT, int EPI>
@@ -865,10 +916,11 @@ void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
     if constexpr (EPI == kGateUp) {
       launch_stream<FMT, 4, EPI>(p, waves, s);
     } else {
-      if (p.wrows >= kWideCols)
-        launch_stream<FMT, 4, EPI>(p, waves, s);
-      else
-        launch_stream<FMT, 1, EPI>(p, p.steps >= 96 ? 12 : waves, s);
+      switch (stream_tiles(false, p.rows, p.wrows)) {
+        case 1: launch_stream<FMT, 1, EPI>(p, p.steps >= 96 ? 12 : waves, s); break;
+        case 2: launch_stream<FMT, 2, EPI>(p, waves, s); break;
+        default: launch_stream<FMT, 4, EPI>(p, waves, s);
+      }
     }
     return;
   }
