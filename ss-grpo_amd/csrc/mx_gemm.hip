@@ -836,7 +836,10 @@ bool splits_ok(int steps, int splits) {
 Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_split) {
   Plan best{0, 1};
   float least = 1e30f;
-  for (int c = 0; c < kTileCount; ++c)
+  for (int c = 0; c < kTileCount; ++c) {
+    // One workgroup of the last tile's two stages per CU cannot cover a long reduction's loads (against the first tile, up
+    // to 8 steps 0.95 .. 1.05 of its time, 9 to 12 steps 1.2, 41 and more 1.6).
+    if (c == kTileCount - 1 && steps > 8 && tiles_of(kTiles[c], rows, wrows) <= 256) continue;
     for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
       // (two stages keep too little in flight for a long reduction; what fills the card four times is not split)
       if (s > 1 && (steps / s < 3 || !splits_ok(steps, s) || c >= kTwoStages || tiles_of(kTiles[c], rows, wrows) > 1024))
@@ -847,6 +850,7 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
         best = Plan{c, s};
       }
     }
+  }
   // The stream of a gate_up with e4m3 rows loses nothing of their products, so it may take a quarter longer (16 rows at
   // 1.5B's and 8B's sizes: 8.6 and 17.5 us against the smallest tile's 7.8 and 15.1).
   const int nt = stream_tiles(gate_up, rows, wrows);
