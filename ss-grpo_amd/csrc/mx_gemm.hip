@@ -763,17 +763,17 @@ struct Tile {
   float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
   float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
 };
-// Fitted to times of every tile and many splits with rows of both formats over some 1400 sizes, 1 .. 4096 rows x 64 ..
-// 152000 columns x 160 .. 19000. Over 1850 others what the estimates pick is 1 to 2 % behind the fastest in the geometric
-// mean, 35 % at worst.
+// Fitted to times of every tile and many splits with rows of both formats over some 2000 sizes, 1 .. 8192 rows x 64 ..
+// 152000 columns x 160 .. 19000. Over 2300 others what the estimates pick is 1 to 2 % behind the fastest in the geometric
+// mean, 26 % at worst.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 0.34f, 0.99f, 2.65f, 1.6f, 0.76f},
-    {128, 128, 64, 0.42f, 0.96f, 3.75f, 2.03f, 0.94f},
-    {128, 256, 64, 0.68f, 0.76f, 4.2f, 2.7f, 0},
-    {192, 256, 96, 0.79f, 0.75f, 5.55f, 2.8f, 0},
-    {256, 256, 64, 1.04f, 0.71f, 6.0f, 2.76f, 0},
-    {128, 256, 64, 1.08f, 0.85f, 4.0f, 2.6f, 0.73f},
-    {64, 128, 32, 0.36f, 1.0f, 2.5f, 1.0f, 0.37f},
+    {64, 128, 32, 0.34f, 0.99f, 2.65f, 1.62f, 0.763f},
+    {128, 128, 64, 0.42f, 0.92f, 3.73f, 2.06f, 0.955f},
+    {128, 256, 64, 0.68f, 0.88f, 4.2f, 2.76f, 0},
+    {192, 256, 96, 0.787f, 0.916f, 5.6f, 2.8f, 0},
+    {256, 256, 64, 1.08f, 0.725f, 5.63f, 2.76f, 0},
+    {128, 256, 64, 1.15f, 1.15f, 3.3f, 2.13f, 0.737f},
+    {64, 128, 32, 0.361f, 1.0f, 2.5f, 1.0f, 0.376f},
 };
 constexpr int kTileCount = 7, kTwoStages = 5, kMaxSplits = 16;  // from kTwoStages on: rings of two stages
 
@@ -784,31 +784,37 @@ struct Plan {
 
 constexpr float kReadRate = 5.5e6f;  // bytes per us that the weights are read at
 
-int64_t tiles_of(const Tile& t, int rows, int wrows) {
-  return (int64_t)((rows + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn);
-}
-
 // Estimated microseconds of a plan: whole rounds of 256 workgroups (where more than one fit a CU, the share that each
 // takes, and not under what a first full round of them was found to take), not under what the card sustains in matrix work
-// (1.6 times as much where both operands are e2m1) or in bytes; the output's bytes on top where nothing else runs
-// meanwhile. A split product writes and reads its fp32 sums instead and takes a second launch.
-float plan_us(const Tile& t, int splits, bool gate_up, int fmt, int rows, int wrows, int steps) {
-  const int64_t tiles_n = (wrows + t.bn - 1) / t.bn, tiles = tiles_of(t, rows, wrows);
-  const bool e4m3 = fmt == fg::kE4M3;
-  const float n = (float)(tiles * splits);
-  const bool beside = t.pair > 0 && n > 256;
-  const float rounds = beside ? std::max(t.pair < 0.5f ? 1.37f : 3.08f, t.pair * n / 256) : (float)((tiles * splits + 255) / 256);
-  const float work = rounds * ((steps + splits - 1) / splits) * t.step_us * (e4m3 ? 1.0f : t.e2m1);
-  const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
-  const float flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.62e9f));
-  const float in = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
-  const float out = splits > 1 ? 0.0f : (float)rows * wrows * (gate_up ? 0.5f : 2.0f) / kReadRate;
-  const float sums = (float)splits * rows * wrows * 4 * 2;
-  const float parts = splits == 1 ? 0.0f : 3.65f + sums / (sums < 16e6f ? 4.6e6f : 5.4e6f);
-  const float ends = rounds * t.tile_us;
-  if (beside) return 2.0f + std::max(work + ends, std::max(flops, in + out)) + parts;
-  return 2.0f + std::max(work, std::max(flops, in)) + ends + out + parts;
-}
+// (1.44 times as much where both operands are e2m1) or in bytes; the output's bytes on top where nothing else runs
+// meanwhile. A split product writes and reads its fp32 sums instead and takes a second launch. (A call of few rows waits for
+// these lines on the host, so what does not depend on the split is computed once per tile.)
+struct TileCost {
+  const Tile& t;
+  int steps;
+  int64_t tiles;
+  float step, flops, in, out, sums;
+  TileCost(const Tile& tile, bool gate_up, int fmt, int rows, int wrows, int ksteps) : t(tile), steps(ksteps) {
+    const int tiles_n = (wrows + t.bn - 1) / t.bn;
+    tiles = (int64_t)((rows + t.bm - 1) / t.bm) * tiles_n;
+    const bool e4m3 = fmt == fg::kE4M3;
+    step = t.step_us * (e4m3 ? 1.0f : t.e2m1);
+    const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
+    flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.44e9f));
+    in = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
+    out = (float)rows * wrows * (gate_up ? 0.5f : 2.0f) / kReadRate;
+    sums = (float)rows * wrows * 4 * 2;
+  }
+  float us(int splits, int per_split) const {
+    const int64_t n = tiles * splits;
+    const bool beside = t.pair > 0 && n > 256;
+    const float rounds = beside ? std::max(t.pair < 0.5f ? 1.4f : 2.45f, t.pair * n / 256) : (float)((n + 255) / 256);
+    const float work = rounds * per_split * step, ends = rounds * t.tile_us, o = splits > 1 ? 0.0f : out;
+    const float bytes = sums * splits, parts = splits == 1 ? 0.0f : 3.55f + bytes / (bytes < 16e6f ? 4.6e6f : 5.4e6f);
+    if (beside) return 2.0f + std::max(work + ends, std::max(flops, in + o)) + parts;
+    return 2.0f + std::max(work, std::max(flops, in)) + ends + o + parts;
+  }
+};
 
 // The stream of few rows: tiles of 16 weight rows per workgroup as many as leave a workgroup per CU, up to four (the rows
 // are read again for each workgroup, which costs little for up to four of them: two tiles then), and up to 64, 32 and 16
@@ -823,28 +829,26 @@ int stream_rows(int nt) { return 64 / nt; }
 // workgroups than CUs both), not under the weights' bytes.
 float stream_us(int nt, int fmt, int rows, int wrows, int steps) {
   const float load = (float)((wrows + 16 * nt - 1) / (16 * nt)) / 256;
-  const float x = rows * (fmt == fg::kE4M3 ? 3.3e-3f : 1.5e-3f), w = nt == 1 ? 0.055f : nt == 2 ? 0.091f : 0.15f;
-  const float step = load <= 1 ? std::max(w, 0.055f + x) : (w + x) * std::max(load, 2.3f);
-  return std::max(2.5f + 6 * x + steps * step, 2.0f + (float)wrows * steps * 68 / kReadRate);
-}
-
-bool splits_ok(int steps, int splits) {
-  const int per = (steps + splits - 1) / splits;
-  return (steps + per - 1) / per == splits;
+  const float x = rows * (fmt == fg::kE4M3 ? 3.3e-3f : 1.5e-3f), w = nt == 1 ? 0.054f : nt == 2 ? 0.085f : 0.147f;
+  const float step = load <= 1 ? std::max(w, 0.054f + x) : (w + x) * std::max(load, 2.5f);
+  return std::max(2.45f + 6 * x + steps * step, 2.0f + (float)wrows * steps * 68 / kReadRate);
 }
 
 Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_split) {
   Plan best{0, 1};
   float least = 1e30f;
   for (int c = 0; c < kTileCount; ++c) {
+    const TileCost cost(kTiles[c], gate_up, fmt, rows, wrows, steps);
     // One workgroup of the last tile's two stages per CU cannot cover a long reduction's loads (against the first tile, up
     // to 8 steps 0.95 .. 1.05 of its time, 9 to 12 steps 1.2, 41 and more 1.6).
-    if (c == kTileCount - 1 && steps > 8 && tiles_of(kTiles[c], rows, wrows) <= 256) continue;
-    for (int s = 1; s <= (may_split ? kMaxSplits : 1); ++s) {
-      // (two stages keep too little in flight for a long reduction; what fills the card four times is not split)
-      if (s > 1 && (steps / s < 3 || !splits_ok(steps, s) || c >= kTwoStages || tiles_of(kTiles[c], rows, wrows) > 1024))
-        continue;
-      const float us = plan_us(kTiles[c], s, gate_up, fmt, rows, wrows, steps);
+    if (c == kTileCount - 1 && steps > 8 && cost.tiles <= 256) continue;
+    // No splits of less than three steps, with two stages (they keep too little in flight) or of what fills the card
+    // four times.
+    const int most = !may_split || c >= kTwoStages || cost.tiles > 1024 ? 1 : std::max(1, std::min(kMaxSplits, steps / 3));
+    for (int s = 1; s <= most; ++s) {
+      const int per = (steps + s - 1) / s;
+      if ((steps + per - 1) / per != s) continue;  // one split would be empty
+      const float us = cost.us(s, per);
       if (us < least) {
         least = us;
         best = Plan{c, s};

@@ -395,7 +395,7 @@ def device_pair(rows, cols, fmt, seed, scale=1.0, spread=1.0):
 # Sizes at which the choice takes each tile, whole and in parts; odd sizes where it allows them.
 LARGE = [(777, 1280, 8960), (1408, 1533, 13824), (2311, 2048, 18944), (1856, 2045, 28672), (3500, 2047, 2048),
          (2311, 2559, 3584), (2311, 4607, 2080), (2311, 5119, 2080), (1856, 18943, 3584), (1194, 3584, 18944), (1194, 4608, 18944),
-         (1856, 1536, 13824), (1856, 321, 5120), (1408, 1536, 2048), (2311, 897, 1536), (4096, 6145, 512), (777, 37888, 32),
+         (1856, 1536, 13824), (1856, 321, 5120), (1408, 1536, 2048), (2311, 897, 1536), (4096, 6145, 512), (777, 37888, 32), (2311, 2559, 28672),
          # a few rows beside streamed weights
          (1, 2047, 1536), (17, 33, 160), (30, 4090, 1376), (33, 1000, 416), (64, 3584, 3584), (16, 8190, 1056), (31, 7001, 416),
          (32, 8192, 2048), (3, 20000, 288), (12, 9001, 1376), (16, 151936, 128)]
