@@ -247,10 +247,12 @@ int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* su
                   float eps, void* codes, void* scales, void* stream);
 
 /* out = bf16(x . w^T (+ bias) (+ residual)): MX rows x [rows, hidden] (x_format 0 or 1) times an MX e2m1 weight w
- * [cols, hidden], fp32 sums rounded once; bias [cols], residual [rows, cols] (row stride ldr) and out (row stride ldo)
- * bf16; out may be the residual. hidden a multiple of 32; operands under 2 GiB each. Long reductions over few output
+ * [cols, hidden], fp32 sums rounded once (with e4m3 rows the matrix instruction cuts the products of eight neighbouring
+ * elements to multiples of 2^-13 of the power of two at or below the largest of them); bias [cols], residual
+ * [rows, cols] (row stride ldr) and out (row stride ldo) bf16; out may be the residual. hidden a multiple of 32; rows
+ * and cols at most 2^22, the weight's codes and either operand's scales under 2 GiB. Long reductions over few output
  * tiles are split over workgroups, whose fp32 sums need workspace >= fg_mx_linear_workspace(...) bytes (0 when no split
- * is used; a null or smaller workspace runs unsplit). */
+ * is used; a null or smaller workspace runs unsplit), 16-byte aligned and one call's at a time. */
 size_t fg_mx_linear_workspace(int rows, int cols, int hidden, int x_format);
 int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const void* w_codes, const void* w_scales,
                  int rows, int cols, int hidden, const void* bias, const void* residual, int64_t ldr, void* out,

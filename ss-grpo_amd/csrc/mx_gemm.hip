@@ -532,14 +532,12 @@ FG_DEVICE intx8 part_of(const intx8& x, int part) {
 // waves take every waves-th step of 128 elements, so that together they read each row's bytes in order; v_mfma_scale_
 // f32_16x16x128_f8f6f4 multiplies a step (lane l: row l % 16; e2m1 elements 32 (l / 16) .. + 31, e4m3 elements
 // 16 (l / 16) .. + 15 and 64 further; scale of block l / 16 from a byte of its register; D: column l % 16 of the second
-// operand, rows 4 (l / 16) + 0..3 of the first) for each of MT tiles of 16 rows. The waves' sums meet in LDS, a few
-// tiles at a time, added in wave order.
+// operand, rows 4 (l / 16) + 0..3 of the first) for each of MT tiles of 16 rows. The waves' sums meet in LDS, added in
+// wave order.
 // There are no loads to wait for but the weights and (from L2) the rows, so the loop only keeps U steps of them in
 // flight per wave; long reductions over few columns take more waves per workgroup instead of a second launch.
 constexpr int kStreamLd = 20;  // floats per x row and tile in LDS: 16-byte stores on distinct banks
 constexpr int kStreamLds = 64 * 1024;
-// tiles of 16 rows whose sums meet at once
-constexpr int stream_pass(int nt, int mt) { return nt == 4 ? 1 : mt < 4 ? mt : 4; }
 
 constexpr int stream_waves(int nt) { return nt == 1 ? 12 : 8; }  // at most
 
@@ -549,7 +547,7 @@ __global__ void __launch_bounds__(64 * stream_waves(NT)) mx_stream_kernel(MxArgs
   constexpr int XR = FMT == fg::kE4M3 ? 2 : 1, XB = FMT == fg::kE4M3 ? 128 : 64;
   constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;
   static_assert(EPI != kGateUp || NT == 4, "gate_up: two tiles of gate rows and two of up rows");
-  extern __shared__ __attribute__((aligned(16))) float red[];  // [tiles of a pass][waves][NT][16 x rows][16 weight rows]
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [MT][waves][NT][16 x rows][16 weight rows]
   constexpr int RLD = kStreamLd;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
@@ -637,51 +635,44 @@ __global__ void __launch_bounds__(64 * stream_waves(NT)) mx_stream_kernel(MxArgs
     multiply(0);
   }
 
-  constexpr int PASS = stream_pass(NT, MT);
 #pragma unroll
-  for (int k0 = 0; k0 < MT; k0 += PASS) {
-    const int rows = min(p.rows - k0 * 16, PASS * 16);
-    if (rows <= 0) break;  // for the whole workgroup
-    if (k0) __syncthreads();
+  for (int k = 0; k < MT; ++k)
 #pragma unroll
-    for (int k = 0; k < PASS; ++k)
+    for (int i = 0; i < NT; ++i)  // x row r, weight rows 4g .. 4g + 3
+      *(floatx4*)(red + (((k * waves + wave) * NT + i) * 16 + r) * RLD + 4 * g) = acc[k][i];
+  __syncthreads();
+  auto sum = [&](int i, int row, int c) __attribute__((always_inline)) {
+    float v = 0.0f;
+    for (int w = 0; w < waves; ++w) v += red[((((row >> 4) * waves + w) * NT + i) * 16 + (row & 15)) * RLD + c];
+    return v;
+  };
+  if constexpr (EPI == kGateUp) {
+    for (int e = tid; e < ((p.rows * 32 + 63) & ~63); e += blockDim.x) {  // whole waves
+      const int row = min(e >> 5, p.rows - 1), c = e & 31;
+      const float v = silu_mul(sum(c >> 4, row, c & 15), sum(2 + (c >> 4), row, c & 15));
+      uint32_t a = __float_as_uint(v) & 0x7fffffffu;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)  // x row r, weight rows 4g .. 4g + 3
-        *(floatx4*)(red + (((k * waves + wave) * NT + i) * 16 + r) * RLD + 4 * g) = acc[k0 + k][i];
-    __syncthreads();
-    auto sum = [&](int i, int row, int c) __attribute__((always_inline)) {
-      float v = 0.0f;
-      for (int w = 0; w < waves; ++w) v += red[((((row >> 4) * waves + w) * NT + i) * 16 + (row & 15)) * RLD + c];
-      return v;
-    };
-    if constexpr (EPI == kGateUp) {
-      for (int e = tid; e < ((rows * 32 + 63) & ~63); e += blockDim.x) {  // whole waves
-        const int in = min(e >> 5, rows - 1), row = k0 * 16 + in, c = e & 31;
-        const float v = silu_mul(sum(c >> 4, in, c & 15), sum(2 + (c >> 4), in, c & 15));
-        uint32_t a = __float_as_uint(v) & 0x7fffffffu;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
-        const uint32_t s = fg::mx_scale_byte<fg::kE4M3>(a);
-        const float y = s == 255u ? 0.0f : v * fg::mx_inverse_scale(s);
-        if ((e >> 5) >= rows) continue;
-        p.codes[(int64_t)row * p.cols + n0 + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
-        if (c == 0) {
-          uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(n0 / kStep) * p.rows + row);
-          const int b = (n0 / 32) & 3;
-          sc[b] = (uint8_t)s;
-          if (n0 + 32 >= p.cols)  // the last block also writes the zeros behind it
-            for (int q = b + 1; q < 4; ++q) sc[q] = 0;
-        }
+      for (int o = 16; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
+      const uint32_t s = fg::mx_scale_byte<fg::kE4M3>(a);
+      const float y = s == 255u ? 0.0f : v * fg::mx_inverse_scale(s);
+      if ((e >> 5) >= p.rows) continue;
+      p.codes[(int64_t)row * p.cols + n0 + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+      if (c == 0) {
+        uint8_t* sc = (uint8_t*)(p.scales + (int64_t)(n0 / kStep) * p.rows + row);
+        const int b = (n0 / 32) & 3;
+        sc[b] = (uint8_t)s;
+        if (n0 + 32 >= p.cols)  // the last block also writes the zeros behind it
+          for (int q = b + 1; q < 4; ++q) sc[q] = 0;
       }
-    } else {
-      for (int e = tid; e < rows * NT * 16; e += blockDim.x) {
-        const int in = e / (NT * 16), row = k0 * 16 + in, c = e - in * (NT * 16), n = n0 + c;
-        if (n >= p.wrows) continue;
-        float v = sum(c >> 4, in, c & 15);
-        if (p.bias) v += fg::bf16_to_f32(p.bias[n]);
-        if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)row * p.ldr + n]);
-        p.out[(int64_t)row * p.ldo + n] = fg::f32_to_bf16(v);
-      }
+    }
+  } else {
+    for (int e = tid; e < p.rows * NT * 16; e += blockDim.x) {
+      const int row = e / (NT * 16), c = e - row * (NT * 16), n = n0 + c;
+      if (n >= p.wrows) continue;
+      float v = sum(c >> 4, row, c & 15);
+      if (p.bias) v += fg::bf16_to_f32(p.bias[n]);
+      if (p.residual) v += fg::bf16_to_f32(p.residual[(int64_t)row * p.ldr + n]);
+      p.out[(int64_t)row * p.ldo + n] = fg::f32_to_bf16(v);
     }
   }
 }
@@ -902,10 +893,9 @@ void launch_stream_rows(const MxArgs& p, int waves, hipStream_t s) {
   // One step per wave in flight with x in two parts (8B gate/up of one row: 14.4 us, two steps' registers 16.8; not in
   // parts 13.9), else two.
   constexpr int U = EPI == kGateUp || MT > 1 ? 1 : 2;
-  constexpr int PASS = stream_pass(NT, MT);
-  static_assert(stream_waves(NT) * PASS * NT * 16 * kStreamLd * 4 <= kStreamLds, "LDS");
+  static_assert(stream_waves(NT) * MT * NT * 16 * kStreamLd * 4 <= kStreamLds, "LDS");
   hipLaunchKernelGGL((mx_stream_kernel<FMT, NT, MT, U, EPI>), dim3((cols + per - 1) / per), dim3(64 * waves),
-                     PASS * waves * NT * 16 * kStreamLd * 4, s, p);
+                     MT * waves * NT * 16 * kStreamLd * 4, s, p);
 }
 template <int FMT, int NT, int EPI>
 void launch_stream(const MxArgs& p, int waves, hipStream_t s) {

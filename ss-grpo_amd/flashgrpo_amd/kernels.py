@@ -887,7 +887,8 @@ def _mx_workspace(name, rows, cols, k, fmt, device):
 
 def mx_linear(x, w, *, bias=None, residual=None, out=None):
     """bf16 [rows, N] = x . w^T (+ bias) (+ residual) of MX rows x [rows, K] (e4m3 or e2m1) and a 4-bit MX weight w
-    [N, K] (``fg_mx_linear``), summed in fp32 and rounded once. bias bf16 [N]; residual bf16 [rows, N] with unit
+    [N, K] (``fg_mx_linear``), summed in fp32 and rounded once (of e4m3 rows' products, the bits below 2^-13 of the
+    largest of eight neighbours are lost: 1e-5 of the sum of magnitudes). bias bf16 [N]; residual bf16 [rows, N] with unit
     column stride; ``out`` bf16 with unit column stride, which may be the residual (an update in place)."""
     operands, rows, N, k, dev = _mx_operands(x, w, "mx_linear")
     _same_device("mx_linear", dev, bias, residual, out)
@@ -921,8 +922,8 @@ def _mx_rows(t, rows, n, what):
 
 def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
     """MX e4m3 [rows, I] of SiLU(x . w[:I]^T) * (x . w[I:]^T) (``fg_mx_gate_up_swiglu``): MX rows x [rows, K] (e4m3
-    or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums and the activation in
-    fp32, rounded once, to the 8-bit codes."""
+    or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums (of
+    products as in ``mx_linear``) and the activation in fp32, rounded once, to the 8-bit codes."""
     operands, rows, n2, k, dev = _mx_operands(x, w, "mx_gate_up_swiglu")
     if n2 == 0 or n2 % (2 * MX_BLOCK):
         raise ValueError("mx_gate_up_swiglu: the weight must have 2 I rows, I a multiple of 32")
