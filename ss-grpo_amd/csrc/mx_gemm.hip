@@ -18,7 +18,7 @@
 // the first in registers 4g .. 4g + 3. The weights are the first operand, so that a lane ends with four consecutive
 // output columns of one row.
 //
-// Tiling: a workgroup of 4 or 8 waves per output tile of BM rows x BN weight rows. K advances 128 elements (one dword of
+// Tiling: a workgroup of 4 or 8 waves (1 for the smallest) per output tile of BM rows x BN weight rows. K advances 128 elements (one dword of
 // scales per row) per step through an NS-stage ring in LDS that direct HBM->LDS loads fill: x rows of 128 (or 64)
 // bytes, weight rows of 64, and the step's scale dwords of both, which lie side by side in memory. Chunks of 16
 // bytes are XOR-swizzled by row so that the fragment reads of neighbouring rows hit distinct banks. A step is two
@@ -753,20 +753,24 @@ struct Tile {
   float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
   float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
   float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
+  float least;     // and what more than 256 of them take at least, in lone ones' times
 };
-// Fitted to times of every tile and many splits with rows of both formats over some 2000 sizes, 1 .. 8192 rows x 64 ..
-// 152000 columns x 160 .. 19000. Over 2300 others what the estimates pick is 1 to 2 % behind the fastest in the geometric
-// mean, 26 % at worst.
+// Fitted to times of every tile and many splits with rows of both formats over some 1900 sizes, 1 .. 8192 rows x 64 ..
+// 152000 columns x 160 .. 19000. Over 860 others what the estimates pick is 1.3 % behind the fastest in the geometric
+// mean, 35 % at worst.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 0.34f, 0.99f, 2.65f, 1.62f, 0.763f},
-    {128, 128, 64, 0.42f, 0.92f, 3.73f, 2.06f, 0.955f},
-    {128, 256, 64, 0.68f, 0.88f, 4.2f, 2.76f, 0},
-    {192, 256, 96, 0.787f, 0.916f, 5.6f, 2.8f, 0},
-    {256, 256, 64, 1.08f, 0.725f, 5.63f, 2.76f, 0},
-    {128, 256, 64, 1.15f, 1.15f, 3.3f, 2.13f, 0.737f},
-    {64, 128, 32, 0.361f, 1.0f, 2.5f, 1.0f, 0.376f},
+    {64, 128, 32, 0.329f, 1.02f, 2.42f, 1.63f, 0.762f, 2.95f},
+    {128, 128, 64, 0.424f, 0.922f, 4.49f, 2.08f, 0.906f, 2.47f},
+    {128, 256, 64, 0.68f, 0.881f, 4.36f, 2.73f, 0, 0},
+    {192, 256, 96, 0.787f, 0.946f, 5.48f, 2.8f, 0, 0},
+    {256, 256, 64, 1.08f, 0.725f, 5.61f, 2.77f, 0, 0},
+    // up to 32 rows by more columns than the first tile has a CU for: the weights' loads spread over all of them (37888 x
+    // 3584, 32 rows: 22.1 us, the first tile 29.9 and the last 26.3; 28672 x 4096, 224 of the first tile: all 17)
+    {32, 64, 32, 0.434f, 0.962f, 1.85f, 0.703f, 0.627f, 1.08f},
+    {128, 256, 64, 1.02f, 1.2f, 3.06f, 2.06f, 0.749f, 2.21f},
+    {64, 128, 32, 0.328f, 1.03f, 1.97f, 0.96f, 0.381f, 1.89f},
 };
-constexpr int kTileCount = 7, kTwoStages = 5, kMaxSplits = 16;  // from kTwoStages on: rings of two stages
+constexpr int kTileCount = 8, kUnsplit = 5, kMaxSplits = 16;  // from kUnsplit on: never split
 
 struct Plan {
   int tile;    // of kTiles; -1: the stream of few rows
@@ -799,9 +803,9 @@ struct TileCost {
   float us(int splits, int per_split) const {
     const int64_t n = tiles * splits;
     const bool beside = t.pair > 0 && n > 256;
-    const float rounds = beside ? std::max(t.pair < 0.5f ? 1.4f : 2.45f, t.pair * n / 256) : (float)((n + 255) / 256);
+    const float rounds = beside ? std::max(t.least, t.pair * n / 256) : (float)((n + 255) / 256);
     const float work = rounds * per_split * step, ends = rounds * t.tile_us, o = splits > 1 ? 0.0f : out;
-    const float bytes = sums * splits, parts = splits == 1 ? 0.0f : 3.55f + bytes / (bytes < 16e6f ? 4.6e6f : 5.4e6f);
+    const float bytes = sums * splits, parts = splits == 1 ? 0.0f : 3.74f + bytes / (bytes < 16e6f ? 4.3e6f : 5.34e6f);
     if (beside) return 2.0f + std::max(work + ends, std::max(flops, in + o)) + parts;
     return 2.0f + std::max(work, std::max(flops, in)) + ends + o + parts;
   }
@@ -820,8 +824,8 @@ int stream_rows(int nt) { return 64 / nt; }
 // workgroups than CUs both), not under the weights' bytes.
 float stream_us(int nt, int fmt, int rows, int wrows, int steps) {
   const float load = (float)((wrows + 16 * nt - 1) / (16 * nt)) / 256;
-  const float x = rows * (fmt == fg::kE4M3 ? 3.3e-3f : 1.5e-3f), w = nt == 1 ? 0.054f : nt == 2 ? 0.085f : 0.147f;
-  const float step = load <= 1 ? std::max(w, 0.054f + x) : (w + x) * std::max(load, 2.5f);
+  const float x = rows * (fmt == fg::kE4M3 ? 3e-3f : 1.5e-3f), w = nt == 1 ? 0.054f : nt == 2 ? 0.085f : 0.163f;
+  const float step = load <= 1 ? std::max(w, 0.054f + x) : (w + x) * std::max(load, 2.36f);
   return std::max(2.45f + 6 * x + steps * step, 2.0f + (float)wrows * steps * 68 / kReadRate);
 }
 
@@ -833,9 +837,9 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
     // One workgroup of the last tile's two stages per CU cannot cover a long reduction's loads (against the first tile, up
     // to 8 steps 0.95 .. 1.05 of its time, 9 to 12 steps 1.2, 41 and more 1.6).
     if (c == kTileCount - 1 && steps > 8 && cost.tiles <= 256) continue;
-    // No splits of less than three steps, with two stages (they keep too little in flight) or of what fills the card
-    // four times.
-    const int most = !may_split || c >= kTwoStages || cost.tiles > 1024 ? 1 : std::max(1, std::min(kMaxSplits, steps / 3));
+    // No splits of less than three steps, of the last tiles (two stages keep too little in flight, and few columns leave the
+    // smallest nothing to spread) or of what fills the card four times.
+    const int most = !may_split || c >= kUnsplit || cost.tiles > 1024 ? 1 : std::max(1, std::min(kMaxSplits, steps / 3));
     for (int s = 1; s <= most; ++s) {
       const int per = (steps + s - 1) / s;
       if ((steps + per - 1) / per != s) continue;  // one split would be empty
@@ -880,8 +884,9 @@ void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
     case 3: launch<FMT, 192, 256, 2, 4, 3, EPI>(p, plan.splits, s); break;
     case 4: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
     default:
-      if constexpr (EPI != kParts) {  // from kTwoStages on: never split
-        if (plan.tile == 5) launch<FMT, 128, 256, 2, 2, 2, EPI>(p, 1, s);
+      if constexpr (EPI != kParts) {
+        if (plan.tile == 5) launch<FMT, 32, 64, 1, 1, 4, EPI>(p, 1, s);
+        else if (plan.tile == 6) launch<FMT, 128, 256, 2, 2, 2, EPI>(p, 1, s);
         else launch<FMT, 64, 128, 2, 2, 2, EPI>(p, 1, s);
       }
   }
@@ -952,7 +957,7 @@ void run(MxArgs p, int x_format, void* workspace, size_t workspace_bytes, hipStr
     run_format<fg::kE2M1, EPI>(p, plan, s);
 }
 
-// Row counts whose grids (up to 512 threads for each 128 x 256 tile, 256 for each 64 x 128) stay under 2^32 threads.
+// Row counts whose grids (up to 512 threads for each 128 x 256 tile, 256 for each 64 x 128, 64 for each 32 x 64) stay under 2^32 threads.
 bool sizes_ok(int rows, int64_t wrows, int hidden) {
   return rows > 0 && rows <= (1 << 22) && wrows > 0 && wrows <= (1 << 22) && hidden > 0 && hidden <= (1 << 20) &&
          (int64_t)((rows + 63) / 64) * ((wrows + 127) / 128) < (1 << 23);

@@ -398,7 +398,7 @@ LARGE = [(777, 1280, 8960), (1408, 1533, 13824), (2311, 2048, 18944), (1856, 204
          (1856, 1536, 13824), (1856, 321, 5120), (1408, 1536, 2048), (2311, 897, 1536), (4096, 6145, 512), (777, 37888, 32), (2311, 2559, 28672),
          # a few rows beside streamed weights
          (1, 2047, 1536), (17, 33, 160), (30, 4090, 1376), (33, 1000, 416), (64, 3584, 3584), (16, 8190, 1056), (31, 7001, 416),
-         (32, 8192, 2048), (3, 20000, 288), (12, 9001, 1376), (16, 151936, 128)]
+         (32, 8192, 2048), (3, 20000, 288), (12, 9001, 1376), (16, 151936, 128), (31, 37887, 1376)]
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
@@ -419,7 +419,8 @@ def test_linear_of_every_tile_with_bias_and_residual_in_place(rows, n, k, fmt):
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("rows,inter,k", [(2311, 768, 5120), (1856, 1792, 2080), (4096, 1280, 1376), (2048, 4096, 1056),
                                           (500, 18944, 1536), (1408, 768, 13824), (777, 18944, 32), (3500, 768, 896),
-                                          (2311, 2560, 512), (777, 1280, 896), (2311, 1792, 640), (16, 8960, 1536), (7, 416, 9632)])
+                                          (2311, 2560, 512), (777, 1280, 896), (2311, 1792, 640), (16, 8960, 1536), (7, 416, 9632),
+                                          (29, 18944, 3584)])
 def test_gate_up_of_every_tile(rows, inter, k, fmt):
     (x, xv), (w, wv) = device_pair(rows, k, fmt, rows, spread=0.5), device_pair(2 * inter, k, "e2m1", k, k ** -0.5, 0.5)
     q = K().mx_gate_up_swiglu(x, w)
