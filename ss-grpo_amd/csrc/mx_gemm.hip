@@ -765,7 +765,7 @@ constexpr Tile kTiles[] = {
     {192, 256, 96, 0.787f, 0.946f, 5.48f, 2.8f, 0, 0},
     {256, 256, 64, 1.08f, 0.725f, 5.61f, 2.77f, 0, 0},
     // up to 32 rows by more columns than the first tile has a CU for: the weights' loads spread over all of them (37888 x
-    // 3584, 32 rows: 22.1 us, the first tile 29.9 and the last 26.3; 28672 x 4096, 224 of the first tile: all 17)
+    // 3584, 32 rows: 22.0 us, the first tile 25.0 and the last 26.0; 28672 x 4096, 224 of the first tile: both 17.4)
     {32, 64, 32, 0.434f, 0.962f, 1.85f, 0.703f, 0.627f, 1.08f},
     {128, 256, 64, 1.02f, 1.2f, 3.06f, 2.06f, 0.749f, 2.21f},
     {64, 128, 32, 0.328f, 1.03f, 1.97f, 0.96f, 0.381f, 1.89f},
