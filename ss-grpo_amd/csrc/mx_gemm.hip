@@ -851,7 +851,7 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
     }
   }
   // The stream of a gate_up with e4m3 rows loses nothing of their products, so it may take a quarter longer (16 rows at
-  // 1.5B's and 8B's sizes: 8.6 and 17.5 us against the smallest tile's 7.8 and 15.1).
+  // 1.5B's and 8B's sizes: 8.7 and 19.5 us against the first tile's 7.8 and 17.4).
   const int nt = stream_tiles(gate_up, rows, wrows);
   if (rows <= stream_rows(nt) &&
       stream_us(nt, fmt, rows, wrows, steps) <= least * (gate_up && fmt == fg::kE4M3 ? 1.25f : 1.0f))
