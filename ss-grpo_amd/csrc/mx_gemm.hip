@@ -7,9 +7,13 @@
 // both formats as they are and applies each block's two scales itself, so nothing is decoded on the way: a byte of
 // weights is two operands. It does 1024 (e4m3 x e2m1) or 2048 (e2m1 x e2m1) multiply-adds per clock and SIMD.
 // Products of e2m1 codes are exact; with e4m3 codes the instruction adds the products of eight neighbouring elements
-// cut (towards zero) to multiples of 2^-13 of the power of two at or below the largest of them, and carries 24 bits
-// from there on (found by comparison; 1e-5 of the sum of magnitudes on random codes), a hundredth of the rounding that
-// the bf16 output makes.
+// cut (towards zero) to multiples of 2^-13 of 2^e, e the largest sum of the two factors' exponents among them, and carries
+// 24 bits from there on (found by comparison; 1e-5 of the sum of magnitudes on random codes). That is a hundredth of the
+// rounding that a bf16 output makes, so the products with one (kLinear) take it. Codes of 8 bits show it: one in 1,000 to
+// 2,000 goes to its neighbour, 1.5e-3 to 1.8e-3 of the output. The gate/up product therefore multiplies e4m3 rows' codes in
+// two parts of fewer bits (take_low), of whose products the instruction loses nothing, at twice the matrix instructions
+// (1856 rows at 7B 340 us, in one part 196; 416 rows at 1.5B 23.6 and 16.9; 64 rows at 7B 31 and 28; one token at 8B 14.4
+// and 13.9).
 //
 // Operand layout (lane l, r = l % 32, h = l / 32, 64 elements of K per instruction), found by exact comparison over
 // random codes and scales: e2m1 lanes hold row r, elements 32h .. 32h + 31 (16 bytes); e4m3 lanes hold row r,
@@ -113,7 +117,23 @@ constexpr int stage_bytes(int fmt, int bm, int bn) {
   return bm * (fmt == fg::kE4M3 ? 128 : 64) + bn * 64 + (bm + 63) / 64 * 256 + bn * 4;
 }
 
-template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI>
+// Takes the e4m3 codes of magnitude below 4 (up to 0x47) out of x, zeros in their places, and returns them. The products
+// of either part with e2m1 codes are multiples of 2^-13 of the largest power of two that their factors' exponents add up to
+// (2^-2 beside 2^10, and 2^-10 beside 2^3), so the matrix instruction loses nothing of them. Bit 7 of a magnitude plus 0x38
+// tells the parts apart; v_perm_b32's selectors 8 .. 11 make a byte of it (bit 15, 31, 47 or 63 of the pair of dwords).
+FG_DEVICE intx8 take_low(intx8& x) {
+  intx8 low;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t v = (uint32_t)x[j], t = (v & 0x7f7f7f7fu) + 0x38383838u;
+    const uint32_t high = v & __builtin_amdgcn_perm(t, t << 8, 0x0b090a08u);
+    low[j] = (int)(v ^ high);
+    x[j] = (int)high;
+  }
+  return low;
+}
+
+template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI, int PARTS>
 __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, BM, BN) <= 40 * 1024   ? 4
                                                           : NS * stage_bytes(FMT, BM, BN) <= 80 * 1024 ? 2
                                                                                                        : 1)
@@ -281,11 +301,25 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     return intx8{lo.x, lo.y, lo.z, lo.w, 0, 0, 0, 0};
   };
   constexpr int kBF = FMT == fg::kE4M3 ? 0 : 4;  // the instruction's code of x's format; 4 is e2m1
-  // matrix instruction j of a sub-step
+  intx8 low[FM];  // (PARTS 2) the part of a sub-step's x that is taken out of fx
+  auto part_frag = [&](int buf, int f) __attribute__((always_inline)) {
+    if constexpr (PARTS == 2) {
+      intx8 x = x_frag(buf, f);
+      low[f] = take_low(x);
+      fx[buf][f][0] = make_int4(x[0], x[1], x[2], x[3]);
+      fx[buf][f][XR - 1] = make_int4(x[4], x[5], x[6], x[7]);
+    }
+  };
+  // matrix instruction j of a sub-step's FM * FN * PARTS, those of the low parts first
 #define FG_MX_MFMA(j, buf, sel)                                                                                     \
-  acc[(j) / FM][(j) % FM] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                         \
-      w_frag(buf, (j) / FM), x_frag(buf, (j) % FM), acc[(j) / FM][(j) % FM], 4, kBF, sel, (int)sw[(j) / FM], sel,    \
-      (int)sx[(j) % FM])
+  do {                                                                                                              \
+    constexpr int NM_ = FM * FN;                                                                                    \
+    const int i_ = (j) % NM_ / FM, k_ = (j) % FM;                                                                   \
+    if ((j) < FM) part_frag(buf, k_);                                                                               \
+    const intx8 x_ = PARTS == 2 && (j) < NM_ ? low[k_] : x_frag(buf, k_);                                           \
+    acc[i_][k_] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w_frag(buf, i_), x_, acc[i_][k_], 4, kBF, sel,     \
+                                                                  (int)sw[i_], sel, (int)sx[k_]);                    \
+  } while (0)
 
   // Prologue: steps 0 .. min(NS, nk) - 1 in flight, wait for step 0.
   const int first = min(NS, nk);
@@ -308,11 +342,11 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     constexpr bool load = decltype(with_load)::value;
     constexpr bool math = decltype(with_math)::value;
     const int next = slot + 1 == NS ? 0 : slot + 1;
-    constexpr int NM = FM * FN;
-    constexpr int R1 = (kReads + NM - 1) / NM, R2 = (kReads + kScaleReads + NM - 1) / NM;  // reads per MFMA, at least
+    constexpr int NM = FM * FN, NJ = NM * PARTS;
+    constexpr int R1 = (kReads + NJ - 1) / NJ, R2 = (kReads + kScaleReads + NJ - 1) / NJ;  // reads per MFMA, at least
     // First sub-step: the second's fragments are read between its matrix instructions.
 #pragma unroll
-    for (int j = 0; j < NM; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       if constexpr (math) {
         FG_MX_MFMA(j, 0, 0);
 #pragma unroll
@@ -332,7 +366,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     // Second sub-step: the next step's first fragments and scales are read, and the loads of step t + NS issued.
     // (Behind the last step the ring holds nothing newer, and what is read is not used.)
 #pragma unroll
-    for (int j = 0; j < NM; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       if constexpr (math) {
         FG_MX_MFMA(j, 1, 2);
 #pragma unroll
@@ -346,7 +380,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
     }
     if constexpr (load) {
 #pragma unroll
-      for (int q = NM; q < LPW; ++q) issue(t + NS, slot, q);
+      for (int q = NJ; q < LPW; ++q) issue(t + NS, slot, q);
     }
     if constexpr (math) take_scales();
     __builtin_amdgcn_sched_barrier(0);
@@ -513,20 +547,6 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N, NS * stage_bytes(FMT, 
   }
 }
 
-// The e4m3 codes of magnitude 4 and up (0x48 ..; part 0) or those below (part 1), zeros in place of the others. The
-// products of either with e2m1 codes span 13 bits (2^-2 .. 2^11 and 2^-10 .. 2^4), so the matrix instruction loses
-// nothing of them but the last bit of subnormal codes'.
-FG_DEVICE intx8 part_of(const intx8& x, int part) {
-  intx8 r;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t v = (uint32_t)x[j], big = ((v & 0x7f7f7f7fu) + 0x38383838u) & 0x80808080u;
-    const uint32_t mask = (big << 1) - (big >> 7);  // 0xff for each such byte
-    r[j] = (int)(part == 0 ? v & mask : v & ~mask);
-  }
-  return r;
-}
-
 // Few rows (up to 16 MT): the weights are streamed once, straight into registers, and the rows are read beside them. A
 // workgroup takes NT tiles of 16 weight rows (gate_up: 32 gate and 32 up rows, one block of 32 output columns) and its
 // waves take every waves-th step of 128 elements, so that together they read each row's bytes in order; v_mfma_scale_
@@ -616,10 +636,7 @@ __global__ void __launch_bounds__(64 * stream_waves(NT)) mx_stream_kernel(MxArgs
         const int4 hi = xv[u][k][1];
         x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
       }
-      if constexpr (EPI == kGateUp && FMT == fg::kE4M3) {  // an 8-bit code follows: lose nothing (it is nearly free here)
-        multiply_part(u, k, part_of(x, 1));
-        x = part_of(x, 0);
-      }
+      if constexpr (EPI == kGateUp && FMT == fg::kE4M3) multiply_part(u, k, take_low(x));
       multiply_part(u, k, x);
     }
   };
@@ -750,6 +767,7 @@ struct Tile {
   int bm, bn, wave_rows;  // rows and weight rows of a workgroup, rows of a wave
   float step_us;   // one step of one workgroup, a CU to itself, with e4m3 rows
   float e2m1;      // what a step takes of that with e2m1 rows
+  float parts;     // and with e4m3 rows in two parts (gate_up)
   float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
   float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
   float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
@@ -757,18 +775,18 @@ struct Tile {
 };
 // Fitted to times of every tile and many splits with rows of both formats over some 1900 sizes, 1 .. 8192 rows x 64 ..
 // 152000 columns x 160 .. 19000. Over 860 others what the estimates pick is 1.3 % behind the fastest in the geometric
-// mean, 35 % at worst.
+// mean, 35 % at worst. `parts` alone was fitted to 1950 sizes of the gate/up in two parts; over 1000 others 1 % and 66 %.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 0.329f, 1.02f, 2.42f, 1.63f, 0.762f, 2.95f},
-    {128, 128, 64, 0.424f, 0.922f, 4.49f, 2.08f, 0.906f, 2.47f},
-    {128, 256, 64, 0.68f, 0.881f, 4.36f, 2.73f, 0, 0},
-    {192, 256, 96, 0.787f, 0.946f, 5.48f, 2.8f, 0, 0},
-    {256, 256, 64, 1.08f, 0.725f, 5.61f, 2.77f, 0, 0},
+    {64, 128, 32, 0.329f, 1.02f, 1.74f, 2.42f, 1.63f, 0.762f, 2.95f},
+    {128, 128, 64, 0.424f, 0.922f, 2.06f, 4.49f, 2.08f, 0.906f, 2.47f},
+    {128, 256, 64, 0.68f, 0.881f, 2.1f, 4.36f, 2.73f, 0, 0},
+    {192, 256, 96, 0.787f, 0.946f, 2.35f, 5.48f, 2.8f, 0, 0},
+    {256, 256, 64, 1.08f, 0.725f, 1.74f, 5.61f, 2.77f, 0, 0},
     // up to 32 rows by more columns than the first tile has a CU for: the weights' loads spread over all of them (37888 x
     // 3584, 32 rows: 22.0 us, the first tile 25.0 and the last 26.0; 28672 x 4096, 224 of the first tile: both 17.4)
-    {32, 64, 32, 0.434f, 0.962f, 1.85f, 0.703f, 0.627f, 1.08f},
-    {128, 256, 64, 1.02f, 1.2f, 3.06f, 2.06f, 0.749f, 2.21f},
-    {64, 128, 32, 0.328f, 1.03f, 1.97f, 0.96f, 0.381f, 1.89f},
+    {32, 64, 32, 0.434f, 0.962f, 1.55f, 1.85f, 0.703f, 0.627f, 1.08f},
+    {128, 256, 64, 1.02f, 1.2f, 1.24f, 3.06f, 2.06f, 0.749f, 2.21f},
+    {64, 128, 32, 0.328f, 1.03f, 1.37f, 1.97f, 0.96f, 0.381f, 1.89f},
 };
 constexpr int kTileCount = 8, kUnsplit = 5, kMaxSplits = 16;  // from kUnsplit on: never split
 
@@ -793,7 +811,7 @@ struct TileCost {
     const int tiles_n = (wrows + t.bn - 1) / t.bn;
     tiles = (int64_t)((rows + t.bm - 1) / t.bm) * tiles_n;
     const bool e4m3 = fmt == fg::kE4M3;
-    step = t.step_us * (e4m3 ? 1.0f : t.e2m1);
+    step = t.step_us * (!e4m3 ? t.e2m1 : gate_up ? t.parts : 1.0f);
     const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
     flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.44e9f));
     in = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
@@ -850,12 +868,8 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
       }
     }
   }
-  // The stream of a gate_up with e4m3 rows loses nothing of their products, so it may take a quarter longer (16 rows at
-  // 1.5B's and 8B's sizes: 8.7 and 19.5 us against the first tile's 7.8 and 17.4).
   const int nt = stream_tiles(gate_up, rows, wrows);
-  if (rows <= stream_rows(nt) &&
-      stream_us(nt, fmt, rows, wrows, steps) <= least * (gate_up && fmt == fg::kE4M3 ? 1.25f : 1.0f))
-    return Plan{-1, 1};
+  if (rows <= stream_rows(nt) && stream_us(nt, fmt, rows, wrows, steps) <= least) return Plan{-1, 1};
   return best;
 }
 
@@ -864,30 +878,30 @@ size_t parts_bytes(const Plan& plan, int rows, int wrows) {
 }
 
 // ------------------------------------------------------------------ launches
-template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI>
+template <int FMT, int BM, int BN, int WAVES_M, int WAVES_N, int NS, int EPI, int PARTS>
 void launch(MxArgs p, int splits, hipStream_t s) {
   constexpr int kOutCols = EPI == kGateUp ? BN / 2 : BN;
   p.tiles_m = (p.rows + BM - 1) / BM;
   p.tiles_n = ((EPI == kGateUp ? p.cols : p.wrows) + kOutCols - 1) / kOutCols;
   p.tiles = p.tiles_m * p.tiles_n * splits;
   p.per_xcd = (p.tiles + 7) / 8;
-  hipLaunchKernelGGL((mx_gemm_kernel<FMT, BM, BN, WAVES_M, WAVES_N, NS, EPI>), dim3(8 * p.per_xcd),
+  hipLaunchKernelGGL((mx_gemm_kernel<FMT, BM, BN, WAVES_M, WAVES_N, NS, EPI, PARTS>), dim3(8 * p.per_xcd),
                      dim3(64 * WAVES_M * WAVES_N), 0, s, p);
 }
 
-template <int FMT, int EPI>
+template <int FMT, int EPI, int PARTS>
 void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
   switch (plan.tile) {
-    case 0: launch<FMT, 64, 128, 2, 2, 4, EPI>(p, plan.splits, s); break;
-    case 1: launch<FMT, 128, 128, 2, 2, 3, EPI>(p, plan.splits, s); break;
-    case 2: launch<FMT, 128, 256, 2, 4, 4, EPI>(p, plan.splits, s); break;
-    case 3: launch<FMT, 192, 256, 2, 4, 3, EPI>(p, plan.splits, s); break;
-    case 4: launch<FMT, 256, 256, 4, 2, 3, EPI>(p, plan.splits, s); break;
+    case 0: launch<FMT, 64, 128, 2, 2, 4, EPI, PARTS>(p, plan.splits, s); break;
+    case 1: launch<FMT, 128, 128, 2, 2, 3, EPI, PARTS>(p, plan.splits, s); break;
+    case 2: launch<FMT, 128, 256, 2, 4, 4, EPI, PARTS>(p, plan.splits, s); break;
+    case 3: launch<FMT, 192, 256, 2, 4, 3, EPI, PARTS>(p, plan.splits, s); break;
+    case 4: launch<FMT, 256, 256, 4, 2, 3, EPI, PARTS>(p, plan.splits, s); break;
     default:
       if constexpr (EPI != kParts) {
-        if (plan.tile == 5) launch<FMT, 32, 64, 1, 1, 4, EPI>(p, 1, s);
-        else if (plan.tile == 6) launch<FMT, 128, 256, 2, 2, 2, EPI>(p, 1, s);
-        else launch<FMT, 64, 128, 2, 2, 2, EPI>(p, 1, s);
+        if (plan.tile == 5) launch<FMT, 32, 64, 1, 1, 4, EPI, PARTS>(p, 1, s);
+        else if (plan.tile == 6) launch<FMT, 128, 256, 2, 2, 2, EPI, PARTS>(p, 1, s);
+        else launch<FMT, 64, 128, 2, 2, 2, EPI, PARTS>(p, 1, s);
       }
   }
 }
@@ -913,6 +927,7 @@ void launch_stream(const MxArgs& p, int waves, hipStream_t s) {
 
 template <int FMT, int EPI>
 void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
+  constexpr int PARTS = EPI == kGateUp && FMT == fg::kE4M3 ? 2 : 1;
   if (plan.tile < 0) {
     // Eight waves per workgroup; twelve where a wave would have more than a dozen steps and columns are few.
     const int waves = std::max(1, std::min(8, p.steps));
@@ -928,10 +943,10 @@ void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
     return;
   }
   if (plan.splits == 1) {
-    launch_tile<FMT, EPI>(p, plan, s);
+    launch_tile<FMT, EPI, PARTS>(p, plan, s);
     return;
   }
-  launch_tile<FMT, kParts>(p, plan, s);
+  launch_tile<FMT, kParts, PARTS>(p, plan, s);
   if constexpr (EPI == kGateUp) {
     const int64_t groups = (int64_t)p.rows * ((p.cols + kStep - 1) / kStep);
     hipLaunchKernelGGL(mx_finish_gate_up_kernel, dim3((unsigned)((groups + 15) / 16)), dim3(256), 0, s, p);

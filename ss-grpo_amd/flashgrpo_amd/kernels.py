@@ -922,8 +922,8 @@ def _mx_rows(t, rows, n, what):
 
 def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
     """MX e4m3 [rows, I] of SiLU(x . w[:I]^T) * (x . w[I:]^T) (``fg_mx_gate_up_swiglu``): MX rows x [rows, K] (e4m3
-    or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums (of
-    products as in ``mx_linear``) and the activation in fp32, rounded once, to the 8-bit codes."""
+    or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums (of whole products, where
+    ``mx_linear`` cuts those of e4m3 rows) and the activation in fp32, rounded once, to the 8-bit codes."""
     operands, rows, n2, k, dev = _mx_operands(x, w, "mx_gate_up_swiglu")
     if n2 == 0 or n2 % (2 * MX_BLOCK):
         raise ValueError("mx_gate_up_swiglu: the weight must have 2 I rows, I a multiple of 32")
