@@ -246,6 +246,12 @@ int fg_mx_dequantize(const void* codes, const void* scales, int format, int rows
 int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* sum, int dtype, int rows, int hidden,
                   float eps, void* codes, void* scales, void* stream);
 
+/* fg_residual_rmsnorm_parts with an MX e4m3 output: x[r] = bf16(x[r] + bf16(sum_s part[s][r])) in place (bf16 x, row
+ * stride ldx), then MX of x[r] * rsqrt(mean(x[r]^2) + eps) * weight as fg_rmsnorm_mx makes it. part fp32
+ * [splits][rows][hidden]. */
+int fg_residual_rmsnorm_mx_parts(const float* part, int splits, int rows, int hidden, void* x, int64_t ldx,
+                                 const void* weight, float eps, void* codes, void* scales, void* stream);
+
 /* out = bf16(x . w^T (+ bias) (+ residual)): MX rows x [rows, hidden] (x_format 0 or 1) times an MX e2m1 weight w
  * [cols, hidden], fp32 sums rounded once (with e4m3 rows the matrix instruction cuts the products of eight neighbouring
  * elements to multiples of 2^-13 of the largest power of two that two factors' exponents add up to); bias [cols], residual

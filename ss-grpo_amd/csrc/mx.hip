@@ -127,10 +127,12 @@ FG_DEVICE double wave_sum(double v) {
 // one wave in 400), it is taken again with the rounding errors of both multiplications, which fused multiply-adds
 // give exactly. For 1856 rows of 3584 with an addend, 46.6 MB: 12.5 us (3.7 TB/s; 5.0 for 8192 x 4096); with every
 // product in 64 bits and the sums shuffled through LDS 15.4.
-template <int DT, int CHUNKS>
-__global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const void* __restrict__ delta,
-                                                         const void* __restrict__ w, void* sum, int rows, int H,
-                                                         double inv_h, float eps, uint8_t* __restrict__ codes,
+//
+// PARTS: delta is a projection's split-K parts, fp32 [splits][rows][H], added in split order and rounded to bf16.
+template <int DT, int CHUNKS, bool PARTS>
+__global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, int64_t ldx, const void* __restrict__ delta,
+                                                         int splits, const void* __restrict__ w, void* sum, int rows,
+                                                         int H, double inv_h, float eps, uint8_t* __restrict__ codes,
                                                          uint32_t* __restrict__ scales) {
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, nch = H / 8, threads = blockDim.x;
@@ -141,13 +143,27 @@ __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const vo
   for (int c = 0; c < CHUNKS; ++c) {
     const int ch = tid + c * threads;
     if (ch < nch) {
-      fg::load8<DT>(x, row * H + ch * 8, v[c]);
-      if (delta) {
+      fg::load8<DT>(x, row * ldx + ch * 8, v[c]);
+      if (PARTS || delta) {
         float d[8];
-        fg::load8<DT>(delta, row * H + ch * 8, d);
+        if constexpr (PARTS) {
+          const float* part = (const float*)delta + row * H + ch * 8;
+          fg::load8<fg::kF32>(part, 0, d);
+#pragma unroll 4
+          for (int s = 1; s < splits; ++s) {
+            float e[8];
+            fg::load8<fg::kF32>(part + s * ((int64_t)rows * H), 0, e);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] += e[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[j] = fg::round_bf16(d[j]);
+        } else {
+          fg::load8<DT>(delta, row * H + ch * 8, d);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[c][j] = DT == fg::kBF16 ? fg::round_bf16(v[c][j] + d[j]) : v[c][j] + d[j];
-        fg::store8<DT>(sum, row * H + ch * 8, v[c]);
+        fg::store8<DT>(sum, row * ldx + ch * 8, v[c]);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fma((double)v[c][j], (double)v[c][j], ss);
@@ -197,18 +213,21 @@ __global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, const vo
   }
 }
 
-template <int DT>
-void launch_norm(const void* x, const void* delta, const void* w, void* sum, int rows, int H, float eps, uint8_t* codes,
-                 uint32_t* scales, hipStream_t s) {
+template <int DT, bool PARTS>
+void launch_norm(const void* x, int64_t ldx, const void* delta, int splits, const void* w, void* sum, int rows, int H,
+                 float eps, void* codes, void* scales, void* stream) {
   // one chunk per thread up to 256 threads, then two (one chunk and 448 threads, 1856 rows of 3584 without an
   // addend: 8.5 against 8.0 us)
   const int nch = H / 8, chunks = nch <= 256 ? 1 : 2;
   const dim3 g(rows), b(((nch + chunks - 1) / chunks + 63) / 64 * 64);
   const double inv_h = 1.0 / H;
+  hipStream_t s = (hipStream_t)stream;
+  uint8_t* c = (uint8_t*)codes;
+  uint32_t* sc = (uint32_t*)scales;
   if (chunks == 1)
-    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 1>), g, b, 0, s, x, delta, w, sum, rows, H, inv_h, eps, codes, scales);
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 1, PARTS>), g, b, 0, s, x, ldx, delta, splits, w, sum, rows, H, inv_h, eps, c, sc);
   else
-    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 2>), g, b, 0, s, x, delta, w, sum, rows, H, inv_h, eps, codes, scales);
+    hipLaunchKernelGGL((rmsnorm_mx_kernel<DT, 2, PARTS>), g, b, 0, s, x, ldx, delta, splits, w, sum, rows, H, inv_h, eps, c, sc);
 }
 
 int64_t tiles_of(int64_t rows, int64_t cols, int* steps, int* step_tiles) {
@@ -287,10 +306,25 @@ int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* su
                  ((uintptr_t)scales & 3) == 0,
              "fg_rmsnorm_mx: rows must start 16-byte aligned, scales 4-byte aligned");
   if (dtype == fg::kBF16)
-    launch_norm<fg::kBF16>(x, delta, weight, sum, rows, hidden, eps, (uint8_t*)codes, (uint32_t*)scales, (hipStream_t)stream);
+    launch_norm<fg::kBF16, false>(x, hidden, delta, 0, weight, sum, rows, hidden, eps, codes, scales, stream);
   else
-    launch_norm<fg::kF32>(x, delta, weight, sum, rows, hidden, eps, (uint8_t*)codes, (uint32_t*)scales, (hipStream_t)stream);
+    launch_norm<fg::kF32, false>(x, hidden, delta, 0, weight, sum, rows, hidden, eps, codes, scales, stream);
   return fg::check_launch("fg_rmsnorm_mx");
+}
+
+int fg_residual_rmsnorm_mx_parts(const float* part, int splits, int rows, int hidden, void* x, int64_t ldx,
+                                 const void* weight, float eps, void* codes, void* scales, void* stream) {
+  FG_REQUIRE(part && x && weight && codes && scales, "fg_residual_rmsnorm_mx_parts: null pointer");
+  FG_REQUIRE(rows > 0 && splits >= 1 && hidden > 0, "fg_residual_rmsnorm_mx_parts: bad shape");
+  FG_REQUIRE(hidden % fg::kMxBlock == 0 && hidden <= 8192,
+             "fg_residual_rmsnorm_mx_parts: hidden must be a multiple of 32, at most 8192");
+  FG_REQUIRE(ldx >= hidden && ldx % 8 == 0,
+             "fg_residual_rmsnorm_mx_parts: the row stride must be a multiple of 8, at least hidden");
+  FG_REQUIRE((int64_t)rows * 512 <= kMaxThreads, "fg_residual_rmsnorm_mx_parts: bad shape (too many rows for one call)");
+  FG_REQUIRE((((uintptr_t)part | (uintptr_t)x | (uintptr_t)weight | (uintptr_t)codes) & 15) == 0 && ((uintptr_t)scales & 3) == 0,
+             "fg_residual_rmsnorm_mx_parts: rows must start 16-byte aligned, scales 4-byte aligned");
+  launch_norm<fg::kBF16, true>(x, ldx, part, splits, weight, x, rows, hidden, eps, codes, scales, stream);
+  return fg::check_launch("fg_residual_rmsnorm_mx_parts");
 }
 
 }  // extern "C"

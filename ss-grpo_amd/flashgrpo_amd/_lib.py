@@ -58,6 +58,7 @@ SIGNATURES = {
     "fg_mx_quantize": (_I, [_P, _I, _I64, _I, _I, _I, _P, _P, _P]),
     "fg_mx_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _I, _I64, _P]),
     "fg_rmsnorm_mx": (_I, [_P, _P, _P, _P, _I, _I, _I, _F, _P, _P, _P]),
+    "fg_residual_rmsnorm_mx_parts": (_I, [_P, _I, _I, _I, _P, _I64, _P, _F, _P, _P, _P]),
     "fg_mx_linear_workspace": (_SZ, [_I, _I, _I, _I]),
     "fg_mx_linear": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _I64, _P, _I64, _P, _SZ, _P]),
     "fg_mx_gate_up_swiglu_workspace": (_SZ, [_I, _I, _I, _I]),

@@ -856,6 +856,31 @@ def rmsnorm_mx(x, weight, eps, *, delta=None, sum_out=None, out=None) -> MX:
     return q
 
 
+def residual_rmsnorm_mx_parts(parts, x, weight, eps, *, out=None) -> MX:
+    """``residual_rmsnorm_parts`` with an 8-bit output (``fg_residual_rmsnorm_mx_parts``): x <- bf16(x +
+    bf16(parts.sum(0))) in place, then MX e4m3 of RMSNorm(x) * weight as ``rmsnorm_mx`` makes it. parts fp32
+    [S, rows, H], H a multiple of 32 up to 8192, x bf16 [rows, H] with unit column stride and 16-byte aligned rows."""
+    dev = x.get_device()
+    _same_device("residual_rmsnorm_mx_parts", dev, parts, weight)
+    if parts.dim() != 3 or parts.dtype != torch.float32 or not parts.is_contiguous() or parts.shape[0] == 0:
+        raise ValueError("residual_rmsnorm_mx_parts: parts must be contiguous fp32 [S, rows, H]")
+    S, rows, H = parts.shape
+    if H == 0 or H % MX_BLOCK or H > 8192:
+        raise ValueError("residual_rmsnorm_mx_parts: H must be a multiple of 32, at most 8192")
+    if x.dtype is not _BF16 or x.shape != (rows, H) or x.stride(1) != 1:
+        raise ValueError(f"residual_rmsnorm_mx_parts: x must be bf16 [{rows}, {H}] with unit column stride")
+    ldx = x.stride(0) if rows > 1 else H
+    if ldx < H or ldx % 8 or x.data_ptr() % 16 or parts.data_ptr() % 16:
+        raise ValueError("residual_rmsnorm_mx_parts: rows must be apart and start 16-byte aligned")
+    if weight.dtype is not _BF16 or weight.numel() != H or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError("residual_rmsnorm_mx_parts: weight must be a contiguous 16-byte aligned bf16 [H] tensor")
+    q = _mx_out(out, rows, H, 0, x.device, "residual_rmsnorm_mx_parts")
+    if rows:
+        _call_on(dev, "fg_residual_rmsnorm_mx_parts", parts.data_ptr(), S, rows, H, x.data_ptr(), ldx, weight.data_ptr(),
+                 float(eps), q[0].data_ptr(), q[1].data_ptr())
+    return q
+
+
 def _mx_operands(x, w, what):
     """Both operands of a product as addresses and sizes: x's and w's pointers and x's format in the entry points'
     order, then rows, weight rows, K and the device index."""

@@ -614,10 +614,10 @@ class TargetModel:
         ``mx_linear`` adds the down projection to the residual stream. ``enable=False`` goes back to the weights as
         they are (and frees the copies). Returns self.
 
-        The copies are made here and again, in place, by ``sync_from_hf``. Attention, the projections around it and
-        the LM head are unchanged. The rollout then samples from the quantised model, exactly; a trainer that takes
-        its tokens for the full model's has to weigh them (its log probabilities are not the full model's). bf16
-        models whose hidden size (at most 8192) and intermediate size are multiples of 32."""
+        The copies are made here and again, in place, by ``sync_from_hf``. Attention, the projections around it (run as
+        ``split_k_linear`` says) and the LM head are unchanged. The rollout then samples from the quantised model,
+        exactly; a trainer that takes its tokens for the full model's has to weigh them (its log probabilities are not
+        the full model's). bf16 models whose hidden size (at most 8192) and intermediate size are multiples of 32."""
         cfg = self.cfg
         if enable and (self.dtype != torch.bfloat16 or cfg.hidden % K.MX_BLOCK or cfg.hidden > 8192
                        or cfg.intermediate % K.MX_BLOCK):
@@ -760,13 +760,18 @@ class TargetModel:
             K.tree_attention(q, cache.k(l), cache.v(l), seq_len=seq_len, anc=anc, num_nodes=N, q_heads=cfg.q_heads,
                              kv_heads=cfg.kv_heads, head_dim=d, out=attn, row_map=row_map)
             a2 = attn.view(T, cfg.q_heads * d)
-            if self.mlp_mx is not None:  # the residual add inside the library GEMM, then norm to residual on MX rows
-                x.addmm_(a2, lw["o_w"].t())
-                q2 = K.rmsnorm_mx(x, lw["post_norm"], cfg.rms_eps, out=self._mx_buf("h_mx", T, H))
+            plan = self._linear_plan("o", a2, lw["o_w"])
+            if self.mlp_mx is not None:  # from the post-attention norm to the residual stream on MX rows
+                h_mx = self._mx_buf("h_mx", T, H)
+                if plan:
+                    q2 = K.residual_rmsnorm_mx_parts(self._linear_parts(a2, lw["o_w"], plan), x, lw["post_norm"],
+                                                     cfg.rms_eps, out=h_mx)
+                else:
+                    x.addmm_(a2, lw["o_w"].t())
+                    q2 = K.rmsnorm_mx(x, lw["post_norm"], cfg.rms_eps, out=h_mx)
                 act = K.mx_gate_up_swiglu(q2, self.mlp_mx[l][0], out=self._mx_buf("act_mx", T, cfg.intermediate))
                 K.mx_linear(act, self.mlp_mx[l][1], residual=x, out=x)
                 continue
-            plan = self._linear_plan("o", a2, lw["o_w"])
             if plan:
                 # bf16(x + bf16(o_proj)) and the post-attention norm from the parts
                 h2 = K.residual_rmsnorm_parts(self._linear_parts(a2, lw["o_w"], plan), x, lw["post_norm"],

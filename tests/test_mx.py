@@ -183,3 +183,25 @@ def test_only_bf16_models_of_whole_blocks_are_quantised():
         with pytest.raises(ValueError, match="multiples of 32"):
             m.quantize_mlp()
         assert m.quantize_mlp(False).mlp_mx is None
+
+
+def test_residual_norm_of_parts_refuses_bad_arguments_on_the_host():
+    lib = _lib()
+    p, off8, off1, n = ctypes.c_void_p(256), ctypes.c_void_p(264), ctypes.c_void_p(257), None
+
+    def refused(text, part=p, splits=2, rows=4, hidden=64, x=p, ldx=64, w=p, codes=p, scales=p):
+        rc = lib.fg_residual_rmsnorm_mx_parts(part, splits, rows, hidden, x, ldx, w, 1e-6, codes, scales, None)
+        assert rc != 0 and text in lib.fg_last_error(), (rc, lib.fg_last_error())
+
+    for name in ("part", "x", "w", "codes", "scales"):
+        refused(b"null pointer", **{name: n})
+    for name in ("part", "x", "w", "codes"):
+        refused(b"aligned", **{name: off8})
+    refused(b"aligned", scales=off1)
+    refused(b"shape", rows=0)
+    refused(b"shape", splits=0)
+    refused(b"multiple of 32", hidden=48, ldx=48)
+    refused(b"8192", hidden=8224, ldx=8224)
+    refused(b"stride", ldx=56)
+    refused(b"stride", ldx=68)
+    refused(b"too many rows", rows=1 << 23)
