@@ -272,6 +272,11 @@ int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format
                          const void* w_scales, int rows, int inter, int hidden, void* codes, void* scales,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* Which kernel an fg_mx_linear (gate_up 0) or fg_mx_gate_up_swiglu (1, cols its inter) of these sizes runs, given its
+ * workspace: rows and weight rows of a workgroup, steps of 128 in its ring and splits of the reduction, or, where the
+ * weights are streamed past few rows, 0 in place of the steps and then the waves that share the reduction. */
+int fg_mx_plan(int gate_up, int rows, int cols, int hidden, int x_format, int plan[4]);
+
 /* dst[i] = src[i] (bytes[i] bytes, a positive multiple of 4, 4-byte aligned device addresses, no
  * overlaps) for i < count <= 8, in one launch; src, dst and bytes are host arrays. No counterpart in the
  * reference: it brings a captured verify forward's inputs into the graph's static buffers. */

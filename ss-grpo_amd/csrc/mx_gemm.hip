@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(256) mx_finish_gate_up_kernel(MxArgs p) {
 
 // ------------------------------------------------------------------ which kernel
 struct Tile {
-  int bm, bn, wave_rows;  // rows and weight rows of a workgroup, rows of a wave
+  int bm, bn, wave_rows, stages;  // rows and weight rows of a workgroup, rows of a wave, steps in the ring
   float step_us;   // one step of one workgroup, a CU to itself, with e4m3 rows
   float e2m1;      // what a step takes of that with e2m1 rows
   float parts;     // and with e4m3 rows in two parts (gate_up)
@@ -775,18 +775,18 @@ struct Tile {
 };
 // Fitted to times of every tile and many splits with rows of both formats over some 1900 sizes, 1 .. 8192 rows x 64 ..
 // 152000 columns x 160 .. 19000. Over 860 others what the estimates pick is 1.3 % behind the fastest in the geometric
-// mean, 35 % at worst. `parts` alone was fitted to 1950 sizes of the gate/up in two parts; over 1000 others 1 % and 66 %.
+// mean, 35 % at worst. `parts` alone was fitted to 3600 sizes of the gate/up in two parts; over 1950 others 1 % and 66 %.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 0.329f, 1.02f, 1.74f, 2.42f, 1.63f, 0.762f, 2.95f},
-    {128, 128, 64, 0.424f, 0.922f, 2.06f, 4.49f, 2.08f, 0.906f, 2.47f},
-    {128, 256, 64, 0.68f, 0.881f, 2.1f, 4.36f, 2.73f, 0, 0},
-    {192, 256, 96, 0.787f, 0.946f, 2.35f, 5.48f, 2.8f, 0, 0},
-    {256, 256, 64, 1.08f, 0.725f, 1.74f, 5.61f, 2.77f, 0, 0},
+    {64, 128, 32, 4, 0.329f, 1.02f, 1.74f, 2.42f, 1.63f, 0.762f, 2.95f},
+    {128, 128, 64, 3, 0.424f, 0.922f, 2.06f, 4.49f, 2.08f, 0.906f, 2.47f},
+    {128, 256, 64, 4, 0.68f, 0.881f, 2.1f, 4.36f, 2.73f, 0, 0},
+    {192, 256, 96, 3, 0.787f, 0.946f, 2.35f, 5.48f, 2.8f, 0, 0},
+    {256, 256, 64, 3, 1.08f, 0.725f, 1.74f, 5.61f, 2.77f, 0, 0},
     // up to 32 rows by more columns than the first tile has a CU for: the weights' loads spread over all of them (37888 x
     // 3584, 32 rows: 22.0 us, the first tile 25.0 and the last 26.0; 28672 x 4096, 224 of the first tile: both 17.4)
-    {32, 64, 32, 0.434f, 0.962f, 1.55f, 1.85f, 0.703f, 0.627f, 1.08f},
-    {128, 256, 64, 1.02f, 1.2f, 1.24f, 3.06f, 2.06f, 0.749f, 2.21f},
-    {64, 128, 32, 0.328f, 1.03f, 1.37f, 1.97f, 0.96f, 0.381f, 1.89f},
+    {32, 64, 32, 4, 0.434f, 0.962f, 1.55f, 1.85f, 0.703f, 0.627f, 1.08f},
+    {128, 256, 64, 2, 1.02f, 1.2f, 1.24f, 3.06f, 2.06f, 0.749f, 2.21f},
+    {64, 128, 32, 2, 0.328f, 1.03f, 1.37f, 1.97f, 0.96f, 0.381f, 1.89f},
 };
 constexpr int kTileCount = 8, kUnsplit = 5, kMaxSplits = 16;  // from kUnsplit on: never split
 
@@ -857,8 +857,10 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
     if (c == kTileCount - 1 && steps > 8 && cost.tiles <= 256) continue;
     // No splits of less than three steps, of the last tiles (two stages keep too little in flight, and few columns leave the
     // smallest nothing to spread) or of what fills the card four times.
+    // The third tile is never taken whole with rows in two parts: of 5500 sizes it was the fastest at none.
+    const int fewest = c == 2 && gate_up && fmt == fg::kE4M3 ? 2 : 1;
     const int most = !may_split || c >= kUnsplit || cost.tiles > 1024 ? 1 : std::max(1, std::min(kMaxSplits, steps / 3));
-    for (int s = 1; s <= most; ++s) {
+    for (int s = fewest; s <= most; ++s) {
       const int per = (steps + s - 1) / s;
       if ((steps + per - 1) / per != s) continue;  // one split would be empty
       const float us = cost.us(s, per);
@@ -889,22 +891,37 @@ void launch(MxArgs p, int splits, hipStream_t s) {
                      dim3(64 * WAVES_M * WAVES_N), 0, s, p);
 }
 
+// kTiles[TILE] with its waves.
+template <int TILE, int WAVES_M, int WAVES_N, int FMT, int EPI, int PARTS>
+void launch_one(const MxArgs& p, int splits, hipStream_t s) {
+  constexpr Tile t = kTiles[TILE];
+  static_assert(t.bm == WAVES_M * t.wave_rows, "waves");
+  launch<FMT, t.bm, t.bn, WAVES_M, WAVES_N, t.stages, EPI, PARTS>(p, splits, s);
+}
+
 template <int FMT, int EPI, int PARTS>
 void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
   switch (plan.tile) {
-    case 0: launch<FMT, 64, 128, 2, 2, 4, EPI, PARTS>(p, plan.splits, s); break;
-    case 1: launch<FMT, 128, 128, 2, 2, 3, EPI, PARTS>(p, plan.splits, s); break;
-    case 2: launch<FMT, 128, 256, 2, 4, 4, EPI, PARTS>(p, plan.splits, s); break;
-    case 3: launch<FMT, 192, 256, 2, 4, 3, EPI, PARTS>(p, plan.splits, s); break;
-    case 4: launch<FMT, 256, 256, 4, 2, 3, EPI, PARTS>(p, plan.splits, s); break;
+    case 0: launch_one<0, 2, 2, FMT, EPI, PARTS>(p, plan.splits, s); break;
+    case 1: launch_one<1, 2, 2, FMT, EPI, PARTS>(p, plan.splits, s); break;
+    case 2:  // (make_plan)
+      if constexpr (EPI != kGateUp || PARTS == 1) launch_one<2, 2, 4, FMT, EPI, PARTS>(p, plan.splits, s);
+      break;
+    case 3: launch_one<3, 2, 4, FMT, EPI, PARTS>(p, plan.splits, s); break;
+    case 4: launch_one<4, 4, 2, FMT, EPI, PARTS>(p, plan.splits, s); break;
     default:
       if constexpr (EPI != kParts) {
-        if (plan.tile == 5) launch<FMT, 32, 64, 1, 1, 4, EPI, PARTS>(p, 1, s);
-        else if (plan.tile == 6) launch<FMT, 128, 256, 2, 2, 2, EPI, PARTS>(p, 1, s);
-        else launch<FMT, 64, 128, 2, 2, 2, EPI, PARTS>(p, 1, s);
+        if (plan.tile == 5) launch_one<5, 1, 1, FMT, EPI, PARTS>(p, 1, s);
+        else if (plan.tile == 6) launch_one<6, 2, 2, FMT, EPI, PARTS>(p, 1, s);
+        else launch_one<7, 2, 2, FMT, EPI, PARTS>(p, 1, s);
       }
   }
 }
+
+// Tiles of 16 rows that the stream holds, and its waves: eight per workgroup, twelve where a wave would have more than a
+// dozen steps and columns are few.
+int stream_row_tiles(int nt, int rows) { return nt == 1 && rows > 32 ? 4 : nt <= 2 && rows > 16 ? 2 : 1; }
+int stream_wave_count(int nt, int steps) { return nt == 1 && steps >= 96 ? 12 : std::max(1, std::min(8, steps)); }
 
 template <int FMT, int NT, int MT, int EPI>
 void launch_stream_rows(const MxArgs& p, int waves, hipStream_t s) {
@@ -917,11 +934,12 @@ void launch_stream_rows(const MxArgs& p, int waves, hipStream_t s) {
                      MT * waves * NT * 16 * kStreamLd * 4, s, p);
 }
 template <int FMT, int NT, int EPI>
-void launch_stream(const MxArgs& p, int waves, hipStream_t s) {
+void launch_stream(const MxArgs& p, hipStream_t s) {
+  const int waves = stream_wave_count(NT, p.steps), mt = stream_row_tiles(NT, p.rows);
   if constexpr (NT == 1)
-    if (p.rows > 32) return launch_stream_rows<FMT, NT, 4, EPI>(p, waves, s);
+    if (mt == 4) return launch_stream_rows<FMT, NT, 4, EPI>(p, waves, s);
   if constexpr (NT <= 2)
-    if (p.rows > 16) return launch_stream_rows<FMT, NT, 2, EPI>(p, waves, s);
+    if (mt == 2) return launch_stream_rows<FMT, NT, 2, EPI>(p, waves, s);
   launch_stream_rows<FMT, NT, 1, EPI>(p, waves, s);
 }
 
@@ -929,15 +947,13 @@ template <int FMT, int EPI>
 void run_format(MxArgs p, const Plan& plan, hipStream_t s) {
   constexpr int PARTS = EPI == kGateUp && FMT == fg::kE4M3 ? 2 : 1;
   if (plan.tile < 0) {
-    // Eight waves per workgroup; twelve where a wave would have more than a dozen steps and columns are few.
-    const int waves = std::max(1, std::min(8, p.steps));
     if constexpr (EPI == kGateUp) {
-      launch_stream<FMT, 4, EPI>(p, waves, s);
+      launch_stream<FMT, 4, EPI>(p, s);
     } else {
       switch (stream_tiles(false, p.rows, p.wrows)) {
-        case 1: launch_stream<FMT, 1, EPI>(p, p.steps >= 96 ? 12 : waves, s); break;
-        case 2: launch_stream<FMT, 2, EPI>(p, waves, s); break;
-        default: launch_stream<FMT, 4, EPI>(p, waves, s);
+        case 1: launch_stream<FMT, 1, EPI>(p, s); break;
+        case 2: launch_stream<FMT, 2, EPI>(p, s); break;
+        default: launch_stream<FMT, 4, EPI>(p, s);
       }
     }
     return;
@@ -1060,6 +1076,28 @@ int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format
   p.scales = (uint32_t*)scales;
   run<kGateUp>(p, x_format, workspace, workspace_bytes, (hipStream_t)stream);
   return fg::check_launch("fg_mx_gate_up_swiglu");
+}
+
+int fg_mx_plan(int gate_up, int rows, int cols, int hidden, int x_format, int plan[4]) {
+  const int64_t wrows = (gate_up ? 2 : 1) * (int64_t)cols;
+  FG_REQUIRE(plan, "fg_mx_plan: null pointer");
+  FG_REQUIRE(x_format == fg::kE4M3 || x_format == fg::kE2M1, "fg_mx_plan: bad format");
+  FG_REQUIRE(sizes_ok(rows, wrows, hidden) && hidden % fg::kMxBlock == 0, "fg_mx_plan: bad shape");
+  const int steps = (hidden + kStep - 1) / kStep;
+  const Plan p = make_plan(gate_up, x_format, rows, (int)wrows, steps, true);
+  if (p.tile < 0) {
+    const int nt = stream_tiles(gate_up, rows, (int)wrows);
+    plan[0] = 16 * stream_row_tiles(nt, rows);
+    plan[1] = 16 * nt;
+    plan[2] = 0;
+    plan[3] = stream_wave_count(nt, steps);
+  } else {
+    plan[0] = kTiles[p.tile].bm;
+    plan[1] = kTiles[p.tile].bn;
+    plan[2] = kTiles[p.tile].stages;
+    plan[3] = p.splits;
+  }
+  return 0;
 }
 
 }  // extern "C"

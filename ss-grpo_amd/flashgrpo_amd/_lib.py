@@ -63,6 +63,7 @@ SIGNATURES = {
     "fg_mx_linear": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _I64, _P, _I64, _P, _SZ, _P]),
     "fg_mx_gate_up_swiglu_workspace": (_SZ, [_I, _I, _I, _I]),
     "fg_mx_gate_up_swiglu": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _SZ, _P]),
+    "fg_mx_plan": (_I, [_I, _I, _I, _I, _I, _P]),
     "fg_sample_workspace": (_SZ, [_I]),
     "fg_sample_tokens": (_I, [_P, _I, _I64, _I, _I, _P, _P, _P, _I, _I, _U64, _U64, _P, _I, _F, _I, _I, _U32, _P,
                               _P, _SZ, _P]),

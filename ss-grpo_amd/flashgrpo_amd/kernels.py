@@ -962,6 +962,25 @@ def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
     return q
 
 
+class MXPlan(NamedTuple):
+    """The kernel of an MX product (``mx_plan``): rows and weight rows of a workgroup; steps in its LDS ring and splits of
+    the reduction, or, with 0 stages, the stream of the weights and its waves per workgroup."""
+    rows: int
+    cols: int
+    stages: int
+    splits_or_waves: int
+
+
+def mx_plan(rows, cols, k, *, fmt="e4m3", gate_up=False) -> MXPlan:
+    """Which kernel ``mx_linear`` (or ``mx_gate_up_swiglu``, cols its I) runs for x [rows, k] of a format
+    (``fg_mx_plan``); for profiles and tests. Needs no GPU."""
+    if fmt not in MX_FORMATS:
+        raise ValueError(f"mx_plan: fmt must be one of {tuple(MX_FORMATS)}")
+    p = (C.c_int * 4)()
+    _lib.call("fg_mx_plan", int(gate_up), rows, cols, k, MX_FORMATS[fmt], p)
+    return MXPlan(*p)
+
+
 # ------------------------------------------------------------------ sampling / acceptance
 def sample_workspace(rows, device):
     """Scratch that lets draws of long rows run split over several workgroups per row."""
