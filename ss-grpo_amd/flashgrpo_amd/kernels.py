@@ -737,12 +737,18 @@ def _call_on(dev, name, *args):
             _call(name, *args, _raw_stream(dev))
 
 
+def _too_large(what):
+    raise ValueError(f"{what}: rows and columns must be less than 2^31")
+
+
 def _mx_bad(codes, scales, what):
     if codes.dtype not in (_U8, _FP8) or scales.dtype != _U8 or codes.dim() != 2:
         raise TypeError(f"{what}: MX codes must be float8_e4m3fn or uint8 [rows, ..] with uint8 scales")
     rows, k = MX(codes, scales).shape
     if k == 0 or k % MX_BLOCK:
         raise ValueError(f"{what}: MX rows of {k} elements; expected a multiple of 32")
+    if (rows | k) >> 31:
+        _too_large(what)
     if tuple(scales.shape) != (-(-k // 128), rows, 4):
         raise ValueError(f"{what}: MX scales must be [{-(-k // 128)}, {rows}, 4], got {list(scales.shape)}")
     raise ValueError(f"{what}: MX codes and scales must be contiguous, 16- and 4-byte aligned, on one device")
@@ -760,13 +766,16 @@ def _mx_of(q, what):
         fmt, k = 1, 2 * k
     dev = codes.get_device()
     c, s = codes.data_ptr(), scales.data_ptr()
-    if (k % 32 or k == 0 or c % 16 or s % 4 or scales.dtype is not _U8 or scales.shape != ((k + 127) // 128, rows, 4)
-            or not codes.is_contiguous() or not scales.is_contiguous() or scales.get_device() != dev):
+    if (k % 32 or k == 0 or (rows | k) >> 31 or c % 16 or s % 4 or scales.dtype is not _U8
+            or scales.shape != ((k + 127) // 128, rows, 4) or not codes.is_contiguous() or not scales.is_contiguous()
+            or scales.get_device() != dev):
         _mx_bad(codes, scales, what)
     return c, s, fmt, rows, k, dev
 
 
 def _mx_out(out, rows, cols, fmt, device, what) -> MX:
+    if (rows | cols) >> 31:
+        _too_large(what)
     if out is None:
         return MX(torch.empty(rows, cols // 2 if fmt else cols, dtype=_U8 if fmt else _FP8, device=device),
                   torch.empty((cols + 127) // 128, rows, 4, dtype=_U8, device=device))

@@ -205,3 +205,17 @@ def test_residual_norm_of_parts_refuses_bad_arguments_on_the_host():
     refused(b"stride", ldx=56)
     refused(b"stride", ldx=68)
     refused(b"too many rows", rows=1 << 23)
+
+
+def test_pairs_of_more_than_an_int_counts_are_refused():
+    """Sizes are C ints behind the wrappers: one over them would arrive as its last 32 bits."""
+    from flashgrpo_amd import kernels as K
+
+    big = 2 ** 32 + 4
+    meta = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device="meta")
+    for codes, scales in ((meta(big, 16), meta(1, big, 4)), (meta(1, 2 ** 31), meta(2 ** 25, 1, 4)), (meta(2 ** 31, 16), meta(1, 2 ** 31, 4))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            K._mx_of((codes, scales), "t")
+    for rows, cols in ((big, 32), (1, 2 ** 32 + 64), (2 ** 31, 32)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            K._mx_out(None, rows, cols, 0, torch.device("meta"), "t")
