@@ -228,8 +228,9 @@ int fg_linear_rope_kv_write(const void* x, int64_t ldx, const void* w_pairs, int
 /* Microscaled (MX) rows. A [rows, cols] matrix (cols a multiple of 32) is held as codes, format 0: e4m3, one byte
  * each, [rows, cols]; 1: e2m1, two to a byte (the earlier element in the low half), [rows, cols / 2]; and scales,
  * bytes [ceil(cols / 128)][rows][4]: the block of elements 32 b .. 32 b + 31 of a row has the factor 2^(s - 127),
- * s = scales[b / 4][row][b % 4] (255: the block is NaN; bytes behind the last block are written 0). Codes 16-byte
- * and scales 4-byte aligned, both contiguous. No counterpart in the reference: 4-bit weights for the decoder MLP.
+ * s = scales[b / 4][row][b % 4] (255: the block is NaN; bytes behind the last block are written 0 and must be 0 in an
+ * input). Codes 16-byte and scales 4-byte aligned, both contiguous. Outputs must not overlap operands but where it is said
+ * that they may be one. No counterpart in the reference: 4-bit weights for the decoder MLP.
  *
  * fg_mx_quantize: x [rows, cols] (row stride ldx, a multiple of 8; dtype fp32 or bf16) to codes and scales. A block's
  * scale is the smallest power of two >= 2^-126 that holds its largest magnitude without saturation (448 for e4m3, 6

@@ -737,6 +737,19 @@ def _call_on(dev, name, *args):
             _call(name, *args, _raw_stream(dev))
 
 
+def _apart(what, outs, ins) -> None:
+    """Raises where the memory of an output that the caller gave meets an operand's, each as (address, bytes)."""
+    for a, n in outs:
+        for b, m in ins:
+            if b < a + n and a < b + m:
+                raise ValueError(f"{what}: an output overlaps an operand")
+
+
+def _mx_spans(c, s, fmt, rows, cols):
+    """(address, bytes) of an MX pair's codes and scales."""
+    return (c, rows * cols >> fmt), (s, (cols + 127 >> 7) * rows * 4)
+
+
 def _too_large(what):
     raise ValueError(f"{what}: rows and columns must be less than 2^31")
 
@@ -773,14 +786,17 @@ def _mx_of(q, what):
     return c, s, fmt, rows, k, dev
 
 
-def _mx_out(out, rows, cols, fmt, device, what) -> MX:
+def _mx_out(out, rows, cols, fmt, device, what, operands=()) -> MX:
+    """out, checked against what it has to be and (address, bytes) of the operands, or a new pair."""
     if (rows | cols) >> 31:
         _too_large(what)
     if out is None:
         return MX(torch.empty(rows, cols // 2 if fmt else cols, dtype=_U8 if fmt else _FP8, device=device),
                   torch.empty((cols + 127) // 128, rows, 4, dtype=_U8, device=device))
-    if _mx_of(out, what)[2:] != (fmt, rows, cols, device.index):
+    held = _mx_of(out, what)
+    if held[2:] != (fmt, rows, cols, device.index):
         raise ValueError(f"{what}: out must be an {'e2m1' if fmt else 'e4m3'} MX pair of [{rows}, {cols}] on {device}")
+    _apart(what, _mx_spans(*held[:5]), operands)
     return MX(*out)
 
 
@@ -788,7 +804,7 @@ def mx_quantize(x, fmt="e2m1", *, out=None) -> MX:
     """The MX form of x [rows, cols] (``fg_mx_quantize``), cols a multiple of 32: fmt "e4m3" (8 bits) or "e2m1"
     (4 bits). Each block of 32 elements gets the smallest power-of-two scale >= 2^-126 that holds it without
     saturation; a block that holds an infinity or a NaN becomes NaN. x bf16 or fp32 with unit column stride and
-    16-byte aligned rows. ``out``: an MX pair to overwrite in place (a weight that is quantised again)."""
+    16-byte aligned rows. ``out``: an MX pair to overwrite (a weight that is quantised again), apart from x."""
     dev = x.get_device()
     _same_device("mx_quantize", dev)
     f = MX_FORMATS.get(fmt)
@@ -799,14 +815,15 @@ def mx_quantize(x, fmt="e2m1", *, out=None) -> MX:
     if len(shape) != 2 or shape[1] == 0 or shape[1] % MX_BLOCK:
         raise ValueError("mx_quantize: x must be [rows, cols] with cols a multiple of 32")
     rows, cols = shape
-    q = _mx_out(out, rows, cols, f, x.device, "mx_quantize")
-    if rows == 0:
-        return q
     ldx = cols
     if not x.is_contiguous():
         ldx = x.stride(0) if rows > 1 else cols
         if x.stride(1) != 1 or ldx < cols:
             raise ValueError("mx_quantize: x rows must have unit column stride")
+    q = _mx_out(out, rows, cols, f, x.device, "mx_quantize", () if out is None else
+                ((x.data_ptr(), ((rows - 1) * ldx + cols) * x.element_size()),))
+    if rows == 0:
+        return q
     if ldx % 8 or x.data_ptr() % 16:
         raise ValueError("mx_quantize: x rows must start 16-byte aligned")
     _call_on(dev, "fg_mx_quantize", x.data_ptr(), dt, ldx, rows, cols, f, q[0].data_ptr(), q[1].data_ptr())
@@ -824,6 +841,9 @@ def mx_dequantize(q, dtype=torch.bfloat16, *, out=None):
         out = torch.empty(rows, cols, dtype=dtype, device=q[0].device)
     elif tuple(out.shape) != (rows, cols) or out.dtype not in _DT or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"mx_dequantize: out must be a contiguous 16-byte aligned bf16 or fp32 [{rows}, {cols}] tensor")
+    else:
+        _apart("mx_dequantize", ((out.data_ptr(), rows * cols * out.element_size()),),
+               _mx_spans(codes, scales, f, rows, cols))
     if rows:
         _call_on(dev, "fg_mx_dequantize", codes, scales, f, rows, cols, out.data_ptr(), dtype_code(out), cols)
     return out
@@ -832,8 +852,8 @@ def mx_dequantize(q, dtype=torch.bfloat16, *, out=None):
 def rmsnorm_mx(x, weight, eps, *, delta=None, sum_out=None, out=None) -> MX:
     """``rmsnorm`` with an 8-bit output (``fg_rmsnorm_mx``): MX e4m3 of RMSNorm(x [+ delta]) * weight over the last
     dimension of x [rows, H], H a multiple of 32 up to 8192. With delta the sum, rounded to x's dtype, is written to
-    ``sum_out`` (x itself when not given). x, delta, weight and sum_out contiguous, one dtype (bf16 or fp32). The
-    norm is not rounded between its steps: the codes are those of the formula in 64 bits."""
+    ``sum_out`` (x itself when not given; x, delta, or apart from both). x, delta, weight and sum_out contiguous, one
+    dtype (bf16 or fp32). The norm is not rounded between its steps: the codes are those of the formula in 64 bits."""
     dev = x.get_device()
     _same_device("rmsnorm_mx", dev, weight, delta, sum_out)
     dt = dtype_code(x)
@@ -854,14 +874,26 @@ def rmsnorm_mx(x, weight, eps, *, delta=None, sum_out=None, out=None) -> MX:
         rest = (x, delta)
     else:
         rest = (x, delta, sum_out)
+    at = []
     for t in rest:
-        if not t.is_contiguous() or t.data_ptr() % 16 or (t is not x and (t.shape != shape or t.dtype is not dtype)):
+        p = t.data_ptr()
+        if not t.is_contiguous() or p % 16 or (t is not x and (t.shape != shape or t.dtype is not dtype)):
             raise ValueError("rmsnorm_mx: x, delta and sum_out must be contiguous, 16-byte aligned and of one shape and "
                              "dtype")
-    q = _mx_out(out, rows, H, 0, x.device, "rmsnorm_mx")
+        at.append(p)
+    row = H * (2 if dt else 4)
+    size, w, total = rows * row, weight.data_ptr(), None
+    if delta is not None:
+        total = at[0] if sum_out is x else at[2]
+        for p in at:
+            if -size < p - total < size and p != total:
+                raise ValueError("rmsnorm_mx: sum_out overlaps x or delta without being it")
+        if w < total + size and total < w + row:
+            raise ValueError("rmsnorm_mx: sum_out overlaps the weight")
+    q = _mx_out(out, rows, H, 0, x.device, "rmsnorm_mx", () if out is None else ((w, row), *((p, size) for p in at)))
     if rows:
-        _call_on(dev, "fg_rmsnorm_mx", x.data_ptr(), _ptr(delta), weight.data_ptr(), _ptr(sum_out), dt, rows, H,
-                 float(eps), q[0].data_ptr(), q[1].data_ptr())
+        _call_on(dev, "fg_rmsnorm_mx", at[0], None if delta is None else at[1], w, total, dt, rows, H, float(eps),
+                 q[0].data_ptr(), q[1].data_ptr())
     return q
 
 
@@ -883,7 +915,10 @@ def residual_rmsnorm_mx_parts(parts, x, weight, eps, *, out=None) -> MX:
         raise ValueError("residual_rmsnorm_mx_parts: rows must be apart and start 16-byte aligned")
     if weight.dtype is not _BF16 or weight.numel() != H or not weight.is_contiguous() or weight.data_ptr() % 16:
         raise ValueError("residual_rmsnorm_mx_parts: weight must be a contiguous 16-byte aligned bf16 [H] tensor")
-    q = _mx_out(out, rows, H, 0, x.device, "residual_rmsnorm_mx_parts")
+    into = (x.data_ptr(), ((rows - 1) * ldx + H) * 2)
+    read = (parts.data_ptr(), S * rows * H * 4), (weight.data_ptr(), H * 2)
+    _apart("residual_rmsnorm_mx_parts", (into,), read)
+    q = _mx_out(out, rows, H, 0, x.device, "residual_rmsnorm_mx_parts", (into, *read))
     if rows:
         _call_on(dev, "fg_residual_rmsnorm_mx_parts", parts.data_ptr(), S, rows, H, x.data_ptr(), ldx, weight.data_ptr(),
                  float(eps), q[0].data_ptr(), q[1].data_ptr())
@@ -923,13 +958,15 @@ def mx_linear(x, w, *, bias=None, residual=None, out=None):
     """bf16 [rows, N] = x . w^T (+ bias) (+ residual) of MX rows x [rows, K] (e4m3 or e2m1) and a 4-bit MX weight w
     [N, K] (``fg_mx_linear``), summed in fp32 and rounded once (of e4m3 rows' products, the bits below 2^-13 of the
     largest of eight neighbours are lost: 1e-5 of the sum of magnitudes). bias bf16 [N]; residual bf16 [rows, N] with unit
-    column stride; ``out`` bf16 with unit column stride, which may be the residual (an update in place)."""
+    column stride; ``out`` bf16 with unit column stride, which may be the residual (an update in place) and must not overlap
+    an operand otherwise."""
     operands, rows, N, k, dev = _mx_operands(x, w, "mx_linear")
     _same_device("mx_linear", dev, bias, residual, out)
     if bias is not None and (bias.dtype is not _BF16 or bias.numel() != N or not bias.is_contiguous()):
         raise ValueError(f"mx_linear: bias must be a contiguous bf16 [{N}] tensor")
     device = w[0].device
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(rows, N, dtype=_BF16, device=device)
         ldo = N
     else:
@@ -937,6 +974,13 @@ def mx_linear(x, w, *, bias=None, residual=None, out=None):
     ldr = N if residual is None else _mx_rows(residual, rows, N, "residual")
     if rows == 0 or N == 0:
         return out
+    if given:
+        xc, xs, f, wc, ws = operands
+        _apart("mx_linear", ((out.data_ptr(), 2 * ((rows - 1) * ldo + N)),),
+               (*_mx_spans(xc, xs, f, rows, k), *_mx_spans(wc, ws, 1, N, k),
+                (0, 0) if bias is None else (bias.data_ptr(), 2 * N)))
+        if residual is not None and _rows_meet(out.data_ptr() // 2, ldo, residual.data_ptr() // 2, ldr, rows, N):
+            raise ValueError("mx_linear: out overlaps the residual without being it")
     ws, ws_ptr, ws_bytes = _mx_workspace("fg_mx_linear_workspace", rows, N, k, operands[2], device)
     _call_on(dev, "fg_mx_linear", *operands, rows, N, k, _ptr(bias), _ptr(residual), ldr, out.data_ptr(), ldo, ws_ptr,
              ws_bytes)
@@ -954,6 +998,14 @@ def _mx_rows(t, rows, n, what):
     return t.stride(0)
 
 
+def _rows_meet(a, lda, b, ldb, rows, n) -> bool:
+    """Whether rows x n elements at a (row stride lda >= n) and at b (ldb) share any without being the same."""
+    if a == b and lda == ldb or a + (rows - 1) * lda + n <= b or b + (rows - 1) * ldb + n <= a:
+        return False
+    d = (b - a) % lda
+    return lda != ldb or not n <= d <= lda - n  # of one buffer's columns beside each other, none
+
+
 def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
     """MX e4m3 [rows, I] of SiLU(x . w[:I]^T) * (x . w[I:]^T) (``fg_mx_gate_up_swiglu``): MX rows x [rows, K] (e4m3
     or e2m1), a 4-bit MX weight w [2I, K] (gate rows, then up rows), I a multiple of 32. Sums (of whole products, where
@@ -963,7 +1015,9 @@ def mx_gate_up_swiglu(x, w, *, out=None) -> MX:
         raise ValueError("mx_gate_up_swiglu: the weight must have 2 I rows, I a multiple of 32")
     device = w[0].device
     inter = n2 // 2
-    q = _mx_out(out, rows, inter, 0, device, "mx_gate_up_swiglu")
+    xc, xs, f, wc, ws = operands
+    q = _mx_out(out, rows, inter, 0, device, "mx_gate_up_swiglu", () if out is None else
+                (*_mx_spans(xc, xs, f, rows, k), *_mx_spans(wc, ws, 1, n2, k)))
     if rows:
         ws, ws_ptr, ws_bytes = _mx_workspace("fg_mx_gate_up_swiglu_workspace", rows, inter, k, operands[2], device)
         _call_on(dev, "fg_mx_gate_up_swiglu", *operands, rows, inter, k, q[0].data_ptr(), q[1].data_ptr(), ws_ptr,
