@@ -235,7 +235,8 @@ int fg_linear_rope_kv_write(const void* x, int64_t ldx, const void* w_pairs, int
  * fg_mx_quantize: x [rows, cols] (row stride ldx, a multiple of 8; dtype fp32 or bf16) to codes and scales. A block's
  * scale is the smallest power of two >= 2^-126 that holds its largest magnitude without saturation (448 for e4m3, 6
  * for e2m1), codes are rounded to nearest, ties to even; a block with an infinity or a NaN becomes NaN.
- * fg_mx_dequantize: the values, in fp32 or bf16 (row stride ldo, a multiple of 8). */
+ * fg_mx_dequantize: the values, in fp32 or bf16 (row stride ldo, a multiple of 8). Both: less than 2^24 pieces of 16
+ * rows x 512 columns (2^37 elements where the rows fill them). */
 int fg_mx_quantize(const void* x, int dtype, int64_t ldx, int rows, int cols, int format, void* codes, void* scales,
                    void* stream);
 int fg_mx_dequantize(const void* codes, const void* scales, int format, int rows, int cols, void* out, int dtype,
@@ -243,7 +244,8 @@ int fg_mx_dequantize(const void* codes, const void* scales, int format, int rows
 
 /* fg_rmsnorm with an MX e4m3 output: s = x (+ delta, rounded to the row dtype and written to sum, which may be x),
  * MX of s * rsqrt(mean(s^2) + eps) * weight, not rounded in between. x, delta, sum [rows, hidden] and weight contiguous,
- * in one dtype; delta NULL: sum is not written. hidden a multiple of 32, at most 8192. */
+ * in one dtype; sum may also be delta; delta NULL: sum is not written. hidden a multiple of 32, at most 8192; less than
+ * 2^23 rows. */
 int fg_rmsnorm_mx(const void* x, const void* delta, const void* weight, void* sum, int dtype, int rows, int hidden,
                   float eps, void* codes, void* scales, void* stream);
 
@@ -256,10 +258,11 @@ int fg_residual_rmsnorm_mx_parts(const float* part, int splits, int rows, int hi
 /* out = bf16(x . w^T (+ bias) (+ residual)): MX rows x [rows, hidden] (x_format 0 or 1) times an MX e2m1 weight w
  * [cols, hidden], fp32 sums rounded once (with e4m3 rows the matrix instruction cuts the products of eight neighbouring
  * elements to multiples of 2^-13 of the largest power of two that two factors' exponents add up to); bias [cols], residual
- * [rows, cols] (row stride ldr) and out (row stride ldo) bf16; out may be the residual. hidden a multiple of 32; rows
- * and cols at most 2^22, the weight's codes and either operand's scales under 2 GiB. Long reductions over few output
- * tiles are split over workgroups, whose fp32 sums need workspace >= fg_mx_linear_workspace(...) bytes (0 when no split
- * is used; a null or smaller workspace runs unsplit), 16-byte aligned and one call's at a time. */
+ * [rows, cols] (row stride ldr) and out (row stride ldo) bf16; out may be the residual. hidden a multiple of 32, at
+ * most 2^20; rows and cols at most 2^22, ceil(rows / 64) * ceil(cols / 128) less than 2^23, the weight's codes and either
+ * operand's scales under 2 GiB. Long reductions over few output tiles are split over workgroups, whose fp32 sums need
+ * workspace >= fg_mx_linear_workspace(...) bytes (0 when no split is used; a null or smaller workspace runs unsplit),
+ * 16-byte aligned and one call's at a time. */
 size_t fg_mx_linear_workspace(int rows, int cols, int hidden, int x_format);
 int fg_mx_linear(const void* x_codes, const void* x_scales, int x_format, const void* w_codes, const void* w_scales,
                  int rows, int cols, int hidden, const void* bias, const void* residual, int64_t ldr, void* out,

@@ -123,15 +123,18 @@ FG_DEVICE double wave_sum(double v) {
 // workgroup per row, eight columns per thread and chunk; the row stays in registers between the two passes. An 8-bit
 // code has a rounding border every 1/8 of a value, and with plain 32-bit arithmetic one value in a million falls on
 // another side of it than the definition's. So the squares are summed in 64 bits (bf16's are exact there, and so is
-// their sum to 2^-50), and where a product is so near a tie that its two roundings decide (by the 19 bits at its end:
-// one wave in 400), it is taken again with the rounding errors of both multiplications, which fused multiply-adds
-// give exactly. For 1856 rows of 3584 with an addend, 46.6 MB: 12.5 us (3.7 TB/s; 5.0 for 8192 x 4096); with every
-// product in 64 bits and the sums shuffled through LDS 15.4.
+// their sum to 2^-50), and where a product is so near a tie that its two roundings decide (by the 19 bits at its end, 5
+// of whose 2^19 values are: one wave in 205 per chunk of its 512 products, so one in 100 over 2048 columns), it is taken
+// again with the rounding errors of both multiplications, which fused multiply-adds give exactly. For 1856 rows of 3584
+// with an addend, 46.8 MB: 12.7 us (3.7 TB/s; 5.3 for 8192 x 4096); with every product in 64 bits and the sums shuffled
+// through LDS 15.4. Without an addend bf16 rows move half the bytes under the same conversions and 64-bit multiply-adds,
+// which bound them then: 8.2 us for 1856 x 3584 (2.5 TB/s), 14.7 for 4096 x 4096 (3.5), 104 for 37,888 x 3584 (4.0).
+// fp32 rows: 42.5 us for 8192 x 5120 (5.0).
 //
 // PARTS: delta is a projection's split-K parts, fp32 [splits][rows][H], added in split order and rounded to bf16.
 template <int DT, int CHUNKS, bool PARTS>
-__global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, int64_t ldx, const void* __restrict__ delta,
-                                                         int splits, const void* __restrict__ w, void* sum, int rows,
+__global__ void __launch_bounds__(512) rmsnorm_mx_kernel(const void* x, int64_t ldx, const void* delta, int splits,
+                                                         const void* __restrict__ w, void* sum, int rows,
                                                          int H, double inv_h, float eps, uint8_t* __restrict__ codes,
                                                          uint32_t* __restrict__ scales) {
   const int64_t row = blockIdx.x;
