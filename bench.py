@@ -746,9 +746,10 @@ def main():
     ap.add_argument("--cpu-rounds", type=int, default=None,
                     help="verify rounds the CPU oracle runs (default: 32 for the tiny config, 1 otherwise)")
     ap.add_argument("--seed", type=int, default=0)
-    ap.add_argument("--decoder-gemms", default="table", choices=("table", "hand", "library"),
+    ap.add_argument("--decoder-gemms", default="table", choices=("table", "hand", "library", "mx"),
                     help="decoder projections: as the measured path tables choose (default), all on the "
-                         "hand-written split-K / fused MLP kernels, or all on hipBLASLt")
+                         "hand-written split-K / fused MLP kernels, all on hipBLASLt, or as the tables choose "
+                         "with every MLP on 4-bit weights and 8-bit rows (TargetModel.quantize_mlp)")
     ap.add_argument("--roofline-kernel", default="fg_tree_attention",
                     help="C-ABI entry point whose launches are event-timed in the timed rounds")
     ap.add_argument("--roofline-every", type=int, default=7,
@@ -808,7 +809,9 @@ def main():
     elem = 4 if dtype == torch.float32 else 2
     log = lambda msg: print(f"bench: {msg}", file=sys.stderr, flush=True)
     cfg, model, heads, dec = build(work, dtype, seed=args.seed)
-    if args.decoder_gemms != "table":
+    if args.decoder_gemms == "mx":
+        model.quantize_mlp()
+    elif args.decoder_gemms != "table":
         hand = args.decoder_gemms == "hand"
         model.split_k_linear = hand  # QKV, O, down: fg_linear_parts + its finishing kernels, or the library
         model.fused_mlp = hand       # gate/up: fg_gate_up_swiglu, or the library projection + fg_swiglu
@@ -993,7 +996,8 @@ def main():
         "higher_is_better": True,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": "bf16" if dtype == torch.bfloat16 else "fp32",
+        "dtype": ("bf16, MLPs e4m3 x e2m1" if args.decoder_gemms == "mx" else
+                  "bf16" if dtype == torch.bfloat16 else "fp32"),
         "data": "synthetic (uniform-random prefix tokens, seeded random-init weights and Medusa heads, counter noise)",
         "config": {"workload": work["name"], "sequences": len(r.active), "prefix": work["prefix"],
                    "tree_nodes": rounds[-1]["num_nodes"], "internal_nodes": rounds[-1]["internal"],
