@@ -22,9 +22,9 @@
 // the first in registers 4g .. 4g + 3. The weights are the first operand, so that a lane ends with four consecutive
 // output columns of one row.
 //
-// Tiling: a workgroup of 4 or 8 waves (1 for the smallest) per output tile of BM rows x BN weight rows. K advances 128 elements (one dword of
-// scales per row) per step through an NS-stage ring in LDS that direct HBM->LDS loads fill: x rows of 128 (or 64)
-// bytes, weight rows of 64, and the step's scale dwords of both, which lie side by side in memory. Chunks of 16
+// Tiling: a workgroup of 4 or 8 waves (1 for the smallest) per output tile of BM rows x BN weight rows. K advances 128
+// elements (one dword of scales per row) per step through an NS-stage ring in LDS that direct HBM->LDS loads fill: x rows
+// of 128 (or 64) bytes, weight rows of 64, and the step's scale dwords of both, which lie side by side in memory. Chunks of 16
 // bytes are XOR-swizzled by row so that the fragment reads of neighbouring rows hit distinct banks. A step is two
 // sub-steps of 64 elements; a sub-step's fragment reads stand between the matrix instructions of the one before,
 // and the loads of step t + NS between those of step t's second sub-step, after the step's one barrier.
@@ -814,7 +814,7 @@ struct TileCost {
     step = t.step_us * (!e4m3 ? t.e2m1 : gate_up ? t.parts : 1.0f);
     const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
     flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.44e9f));
-    in = ((float)wrows * steps * 68 + (float)rows * steps * 132) / kReadRate;
+    in = ((float)wrows * steps * 68 + (float)rows * steps * (e4m3 ? 132 : 68)) / kReadRate;
     out = (float)rows * wrows * (gate_up ? 0.5f : 2.0f) / kReadRate;
     sums = (float)rows * wrows * 4 * 2;
   }
@@ -988,7 +988,8 @@ void run(MxArgs p, int x_format, void* workspace, size_t workspace_bytes, hipStr
     run_format<fg::kE2M1, EPI>(p, plan, s);
 }
 
-// Row counts whose grids (up to 512 threads for each 128 x 256 tile, 256 for each 64 x 128, 64 for each 32 x 64) stay under 2^32 threads.
+// Row counts whose grids (up to 512 threads for each 128 x 256 tile, 256 for each 64 x 128, 64 for each 32 x 64) stay under
+// 2^32 threads.
 bool sizes_ok(int rows, int64_t wrows, int hidden) {
   return rows > 0 && rows <= (1 << 22) && wrows > 0 && wrows <= (1 << 22) && hidden > 0 && hidden <= (1 << 20) &&
          (int64_t)((rows + 63) / 64) * ((wrows + 127) / 128) < (1 << 23);
