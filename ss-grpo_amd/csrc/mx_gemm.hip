@@ -24,8 +24,8 @@
 //
 // Tiling: a workgroup of 4 or 8 waves (1 for the smallest) per output tile of BM rows x BN weight rows. K advances 128
 // elements (one dword of scales per row) per step through an NS-stage ring in LDS that direct HBM->LDS loads fill: x rows
-// of 128 (or 64) bytes, weight rows of 64, and the step's scale dwords of both, which lie side by side in memory. Chunks of 16
-// bytes are XOR-swizzled by row so that the fragment reads of neighbouring rows hit distinct banks. A step is two
+// of 128 (or 64) bytes, weight rows of 64, and the step's scale dwords of both, which lie side by side in memory. Chunks
+// of 16 bytes are XOR-swizzled by row so that the fragment reads of neighbouring rows hit distinct banks. A step is two
 // sub-steps of 64 elements; a sub-step's fragment reads stand between the matrix instructions of the one before,
 // and the loads of step t + NS between those of step t's second sub-step, after the step's one barrier.
 #include "fg_mx.h"
@@ -763,30 +763,35 @@ __global__ void __launch_bounds__(256) mx_finish_gate_up_kernel(MxArgs p) {
 }
 
 // ------------------------------------------------------------------ which kernel
-struct Tile {
-  int bm, bn, wave_rows, stages;  // rows and weight rows of a workgroup, rows of a wave, steps in the ring
-  float step_us;   // one step of one workgroup, a CU to itself, with e4m3 rows
-  float e2m1;      // what a step takes of that with e2m1 rows
-  float parts;     // and with e4m3 rows in two parts (gate_up)
+struct Cost {
+  float step_us;   // one step of one workgroup, a CU to itself
   float tile_us;   // what a workgroup takes beside its steps: filling the ring, the epilogue
   float pflops;    // what the whole card sustains with it: power bounds it, and smaller tiles move more bytes per product
   float pair;      // where two workgroups or more fit a CU: what each of many takes of a lone one's time (0: one fits)
   float least;     // and what more than 256 of them take at least, in lone ones' times
 };
+struct Tile {
+  int bm, bn, wave_rows, stages;  // rows and weight rows of a workgroup, rows of a wave, steps in the ring
+  float e2m1;  // what a step takes of `once` with e2m1 rows
+  Cost once;   // with e4m3 rows
+  Cost parts;  // with e4m3 rows in two parts (gate_up)
+};
 // Fitted to times of every tile and many splits with rows of both formats over some 1900 sizes, 1 .. 8192 rows x 64 ..
 // 152000 columns x 160 .. 19000. Over 860 others what the estimates pick is 1.3 % behind the fastest in the geometric
-// mean, 35 % at worst. `parts` alone was fitted to 3600 sizes of the gate/up in two parts; over 1950 others 1 % and 66 %.
+// mean, 35 % at worst. `parts` was fitted to 3600 sizes of the gate/up and the four model sizes that this repository names
+// with 1 .. 4096 rows (0.4 % behind, 8 % at worst); over 1950 others 0.6 % and 32 %.
 constexpr Tile kTiles[] = {
-    {64, 128, 32, 4, 0.329f, 1.02f, 1.74f, 2.42f, 1.63f, 0.762f, 2.95f},
-    {128, 128, 64, 3, 0.424f, 0.922f, 2.06f, 4.49f, 2.08f, 0.906f, 2.47f},
-    {128, 256, 64, 4, 0.68f, 0.881f, 2.1f, 4.36f, 2.73f, 0, 0},
-    {192, 256, 96, 3, 0.787f, 0.946f, 2.35f, 5.48f, 2.8f, 0, 0},
-    {256, 256, 64, 3, 1.08f, 0.725f, 1.74f, 5.61f, 2.77f, 0, 0},
+    {64, 128, 32, 4, 1.02f, {0.329f, 2.42f, 1.63f, 0.762f, 2.95f}, {0.588f, 3.07f, 1.61f, 0.832f, 1.4f}},
+    {128, 128, 64, 3, 0.922f, {0.424f, 4.49f, 2.08f, 0.906f, 2.47f}, {0.909f, 5.39f, 2.08f, 0.906f, 2.49f}},
+    {128, 256, 64, 4, 0.881f, {0.68f, 4.36f, 2.73f, 0, 0}, {1.4f, 3.49f, 2.75f, 0, 0}},
+    {192, 256, 96, 3, 0.946f, {0.787f, 5.48f, 2.8f, 0, 0}, {2.11f, 4.76f, 2.81f, 0, 0}},
+    {256, 256, 64, 3, 0.725f, {1.08f, 5.61f, 2.77f, 0, 0}, {2.03f, 7.99f, 2.74f, 0, 0}},
     // up to 32 rows by more columns than the first tile has a CU for: the weights' loads spread over all of them (37888 x
-    // 3584, 32 rows: 22.0 us, the first tile 25.0 and the last 26.0; 28672 x 4096, 224 of the first tile: both 17.4)
-    {32, 64, 32, 4, 0.434f, 0.962f, 1.55f, 1.85f, 0.703f, 0.627f, 1.08f},
-    {128, 256, 64, 2, 1.02f, 1.2f, 1.24f, 3.06f, 2.06f, 0.749f, 2.21f},
-    {64, 128, 32, 2, 0.328f, 1.03f, 1.37f, 1.97f, 0.96f, 0.381f, 1.89f},
+    // 3584, 32 rows: 22.0 us, the first tile 25.0 and the last 26.0, in two parts 22.4, 25.9 and 33; 28672 x 4096, 224 of the
+    // first tile: both 17.4)
+    {32, 64, 32, 4, 0.962f, {0.434f, 1.85f, 0.703f, 0.627f, 1.08f}, {0.709f, 1.98f, 0.701f, 0.372f, 1.09f}},
+    {128, 256, 64, 2, 1.2f, {1.02f, 3.06f, 2.06f, 0.749f, 2.21f}, {1.16f, 3.27f, 1.84f, 0.735f, 1.95f}},
+    {64, 128, 32, 2, 1.03f, {0.328f, 1.97f, 0.96f, 0.381f, 1.89f}, {0.46f, 1.93f, 1.17f, 0.389f, 1.84f}},
 };
 constexpr int kTileCount = 8, kUnsplit = 5, kMaxSplits = 16;  // from kUnsplit on: never split
 
@@ -803,17 +808,19 @@ constexpr float kReadRate = 5.5e6f;  // bytes per us that the weights are read a
 // meanwhile. A split product writes and reads its fp32 sums instead and takes a second launch. (A call of few rows waits for
 // these lines on the host, so what does not depend on the split is computed once per tile.)
 struct TileCost {
-  const Tile& t;
+  const Cost& t;
   int steps;
   int64_t tiles;
   float step, flops, in, out, sums;
-  TileCost(const Tile& tile, bool gate_up, int fmt, int rows, int wrows, int ksteps) : t(tile), steps(ksteps) {
-    const int tiles_n = (wrows + t.bn - 1) / t.bn;
-    tiles = (int64_t)((rows + t.bm - 1) / t.bm) * tiles_n;
+  TileCost(const Tile& tile, bool gate_up, int fmt, int rows, int wrows, int ksteps)
+      : t(gate_up && fmt == fg::kE4M3 ? tile.parts : tile.once), steps(ksteps) {
+    const int tiles_n = (wrows + tile.bn - 1) / tile.bn;
+    tiles = (int64_t)((rows + tile.bm - 1) / tile.bm) * tiles_n;
     const bool e4m3 = fmt == fg::kE4M3;
-    step = t.step_us * (!e4m3 ? t.e2m1 : gate_up ? t.parts : 1.0f);
-    const float active = (float)((rows + t.wave_rows - 1) / t.wave_rows) * t.wave_rows;  // the others multiply nothing
-    flops = 2.0f * active * tiles_n * t.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.44e9f));
+    step = t.step_us * (e4m3 ? 1.0f : tile.e2m1);
+    // waves without a row multiply nothing
+    const float active = (float)((rows + tile.wave_rows - 1) / tile.wave_rows) * tile.wave_rows;
+    flops = 2.0f * active * tiles_n * tile.bn * steps * kStep / (t.pflops * (e4m3 ? 1e9f : 1.44e9f));
     in = ((float)wrows * steps * 68 + (float)rows * steps * (e4m3 ? 132 : 68)) / kReadRate;
     out = (float)rows * wrows * (gate_up ? 0.5f : 2.0f) / kReadRate;
     sums = (float)rows * wrows * 4 * 2;
@@ -857,8 +864,9 @@ Plan make_plan(bool gate_up, int fmt, int rows, int wrows, int steps, bool may_s
     if (c == kTileCount - 1 && steps > 8 && cost.tiles <= 256) continue;
     // No splits of less than three steps, of the last tiles (two stages keep too little in flight, and few columns leave the
     // smallest nothing to spread) or of what fills the card four times.
-    // The third tile is never taken whole with rows in two parts: of 5500 sizes it was the fastest at none.
-    const int fewest = c == 2 && gate_up && fmt == fg::kE4M3 ? 2 : 1;
+    // With rows in two parts the second and third tiles are taken in splits only: whole, the second was the fastest at 3 of
+    // 5500 sizes, by 6 % at most, and the third at none.
+    const int fewest = (c == 1 || c == 2) && gate_up && fmt == fg::kE4M3 ? 2 : 1;
     const int most = !may_split || c >= kUnsplit || cost.tiles > 1024 ? 1 : std::max(1, std::min(kMaxSplits, steps / 3));
     for (int s = fewest; s <= most; ++s) {
       const int per = (steps + s - 1) / s;
@@ -901,11 +909,14 @@ void launch_one(const MxArgs& p, int splits, hipStream_t s) {
 
 template <int FMT, int EPI, int PARTS>
 void launch_tile(const MxArgs& p, const Plan& plan, hipStream_t s) {
+  constexpr bool kWhole = EPI != kGateUp || PARTS == 1;  // (make_plan: those two in splits only)
   switch (plan.tile) {
     case 0: launch_one<0, 2, 2, FMT, EPI, PARTS>(p, plan.splits, s); break;
-    case 1: launch_one<1, 2, 2, FMT, EPI, PARTS>(p, plan.splits, s); break;
-    case 2:  // (make_plan)
-      if constexpr (EPI != kGateUp || PARTS == 1) launch_one<2, 2, 4, FMT, EPI, PARTS>(p, plan.splits, s);
+    case 1:
+      if constexpr (kWhole) launch_one<1, 2, 2, FMT, EPI, PARTS>(p, plan.splits, s);
+      break;
+    case 2:
+      if constexpr (kWhole) launch_one<2, 2, 4, FMT, EPI, PARTS>(p, plan.splits, s);
       break;
     case 3: launch_one<3, 2, 4, FMT, EPI, PARTS>(p, plan.splits, s); break;
     case 4: launch_one<4, 4, 2, FMT, EPI, PARTS>(p, plan.splits, s); break;

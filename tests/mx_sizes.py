@@ -23,10 +23,12 @@ STREAM = [((16, 16, 12), 1, 3584, 18944), ((16, 16, 12), 1, 4096, 14336), ((16, 
           ((64, 16, 8), 64, 3584, 3584)]
 STREAM_OF = {"e4m3": [], "e2m1": [((16, 16, 12), 16, 3584, 18944), ((32, 16, 12), 17, 1496, 12928), ((64, 16, 12), 37, 3472, 14080)]}
 
-# The gate/up product: tile, rows, intermediate size, reduction. (The third tile is only taken in splits with e4m3 rows.)
-GATE_UP = [(0, 66, 96, 1056), (1, 2171, 928, 2848), (3, 2811, 2080, 544), (4, 2033, 3488, 416), (6, 1237, 8800, 64), (7, 65, 96, 160)]
-GATE_UP_SPLIT = [(0, 81, 96, 1824), (1, 555, 608, 6944), (2, 897, 704, 9920), (3, 547, 3360, 8160), (4, 1055, 1952, 9792)]
-GATE_UP_OF = {"e4m3": [(5, 17, 16416, 32)], "e2m1": [(2, 2062, 1888, 672), (5, 29, 18944, 3584)]}
+# The gate/up product: tile, rows, intermediate size, reduction. (The second and third tiles are only taken in splits with
+# e4m3 rows.)
+GATE_UP = [(0, 66, 96, 1248), (3, 1317, 4544, 1312), (4, 3361, 1824, 1568), (6, 1237, 8800, 64), (7, 65, 96, 160)]
+GATE_UP_SPLIT = [(0, 81, 96, 1824), (1, 853, 736, 7072), (2, 1062, 608, 9568), (3, 554, 2336, 14752), (4, 385, 2848, 11968)]
+GATE_UP_OF = {"e4m3": [(5, 23, 32, 1056), (5, 29, 18944, 3584)],
+              "e2m1": [(1, 1271, 800, 416), (2, 2062, 1888, 672), (5, 29, 18944, 3584)]}
 GATE_UP_STREAM = [(8, 1, 480, 1536), (8, 16, 8960, 1536), (3, 5, 96, 288)]  # waves, rows, intermediate size, reduction
 
 
@@ -38,7 +40,7 @@ def linear(fmt):
 
 
 def gate_up(fmt):
-    return ([(TILES[t], False, *size) for t, *size in GATE_UP + [s for s in GATE_UP_OF[fmt]]]
+    return ([(TILES[t], False, *size) for t, *size in GATE_UP + GATE_UP_OF[fmt]]
             + [(TILES[t], True, *size) for t, *size in GATE_UP_SPLIT]
             + [((16, 64, 0), waves, *size) for waves, *size in GATE_UP_STREAM])
 
