@@ -1039,6 +1039,8 @@ def mx_plan(rows, cols, k, *, fmt="e4m3", gate_up=False) -> MXPlan:
     (``fg_mx_plan``); for profiles and tests. Needs no GPU."""
     if fmt not in MX_FORMATS:
         raise ValueError(f"mx_plan: fmt must be one of {tuple(MX_FORMATS)}")
+    if max(rows, cols, k) >> 31:
+        _too_large("mx_plan")
     p = (C.c_int * 4)()
     _lib.call("fg_mx_plan", int(gate_up), rows, cols, k, MX_FORMATS[fmt], p)
     return MXPlan(*p)

@@ -88,3 +88,47 @@ def test_nan_blocks_of_gate_up_reach_their_own_blocks_only(fmt, shape, detail, r
     keep = ~np.repeat(nan, 32, 1)
     assert np.array_equal(got_c[keep], clean[0][keep])
     assert np.array_equal(by_block[~nan], clean[1].transpose(1, 0, 2).reshape(rows, -1)[:, :inter // 32][~nan])
+
+
+SPLIT = [case for case in S.every(S.gate_up) if case[1][2] and case[2]]
+
+
+@pytest.mark.parametrize("fmt,shape,detail,rows,inter,k", SPLIT)
+def test_gate_up_without_workspace_and_in_two_graphs(fmt, shape, detail, rows, inter, k):
+    """A split gate/up without its workspace, or with less, runs unsplit; two captured ones replayed in turn with eager calls
+    between share nothing."""
+    from flashgrpo_amd import _lib
+
+    lib, kk = _lib.load(), K()
+    (x, xv), (w, wv) = device_pair(rows, k, fmt, rows, spread=0.5), device_pair(2 * inter, k, "e2m1", k, k ** -0.5, 0.5)
+    other = device_pair(rows, k, fmt, rows + 1, spread=0.5)[0]
+    need = lib.fg_mx_gate_up_swiglu_workspace(rows, inter, k, kk.MX_FORMATS[fmt])
+    assert need >= 2 * rows * 2 * inter * 4
+    want = kk.mx_gate_up_swiglu(x, w)
+    y = xv.double() @ wv.double().t()
+    want_c = O.quantize(O.silu_mul(y[:, :inter].cpu().numpy(), y[:, inter:].cpu().numpy()), "e4m3")[0]
+    d = 2 * (k / 32 + 8) * 2.0 ** -24
+    for given in (0, need - 16, need):
+        ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)
+        q = kk.MX(torch.zeros(rows, inter, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn), torch.zeros_like(want.scales))
+        rc = lib.fg_mx_gate_up_swiglu(x.codes.data_ptr(), x.scales.data_ptr(), kk.MX_FORMATS[fmt], w.codes.data_ptr(),
+                                      w.scales.data_ptr(), rows, inter, k, q.codes.data_ptr(), q.scales.data_ptr(),
+                                      ws.data_ptr() if given else None, given, kk._stream())
+        assert rc == 0, lib.fg_last_error()
+        assert (held(q)[0] != want_c).mean() <= 2 * d / 2.0 ** -4 + 1 / want_c.size
+        assert (ws[need:] == 255).all() and ((ws == 255).all() or given == need)
+    assert torch.equal(q.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(q.scales, want.scales)
+    wanted, graphs = [want, kk.mx_gate_up_swiglu(other, w)], []
+    for rows_in in (x, other):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = kk.mx_gate_up_swiglu(rows_in, w)
+        graphs.append((g, out))
+    for _ in range(3):
+        for (g, out), ref in zip(graphs, wanted):
+            out.codes.view(torch.uint8).zero_()
+            g.replay()
+            kk.mx_gate_up_swiglu(x, w)
+        torch.cuda.synchronize()
+        for (_, out), ref in zip(graphs, wanted):
+            assert torch.equal(out.codes.view(torch.uint8), ref.codes.view(torch.uint8)) and torch.equal(out.scales, ref.scales)

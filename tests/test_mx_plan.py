@@ -48,6 +48,6 @@ def test_plans_agree_with_workspaces_and_refuse():
         plan = K.mx_plan(rows, cols, k, fmt=fmt)
         assert need == (plan.splits_or_waves * rows * ((cols + 3) // 4 * 4) * 4 if plan.stages and plan.splits_or_waves > 1 else 0)
     for bad in (dict(rows=0), dict(cols=0), dict(k=48), dict(k=0), dict(rows=(1 << 22) + 1), dict(fmt="e5m2"),
-                dict(cols=1 << 30, gate_up=True)):
+                dict(rows=2 ** 32 + 4), dict(cols=2 ** 32 + 64), dict(k=2 ** 32 + 64), dict(cols=1 << 30, gate_up=True)):
         with pytest.raises(ValueError):
             K.mx_plan(**{**dict(rows=4, cols=64, k=64), **bad})
