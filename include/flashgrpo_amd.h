@@ -281,6 +281,75 @@ int fg_mx_gate_up_swiglu(const void* x_codes, const void* x_scales, int x_format
  * weights are streamed past few rows, 0 in place of the steps and then the waves that share the reduction. */
 int fg_mx_plan(int gate_up, int rows, int cols, int hidden, int x_format, int plan[4]);
 
+/* K and V in pages: token t of a cache row lies in page table[row * table_stride + t / page_size], slot t % page_size; an
+ * entry outside [0, pages) is no page. A page holds, for one layer, [kv_heads][page_size][head_dim] rows of K and of V,
+ * `page_stride` elements behind the page before (so that a pool may hold every layer of a page side by side). format 0: MX
+ * e4m3, codes of 8 bits (no NaN codes; a NaN block is told by its scale), with scales [kv_heads][page_size][head_dim / 32], bytes,
+ * `scale_stride` bytes behind those of the page before (fg_mx_quantize's blocks, a row's scales side by side); 1: bf16. head_dim
+ * 64 or 128, page_size a power of two from 16 on, table_width * page_size less than 2^31 - 65536 tokens per row. Pages 16-byte
+ * and scales 4-byte aligned. A host struct of device addresses, read during the call. No counterpart in the reference, whose
+ * cache is DynamicCache. */
+typedef struct fg_kv_pages {
+  void* k;
+  void* v;
+  void* k_scales;
+  void* v_scales;
+  const int32_t* table;
+  int64_t page_stride;
+  int64_t scale_stride;
+  int64_t table_stride;
+  int32_t format;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t table_rows;
+  int32_t table_width;
+} fg_kv_pages;
+
+/* fg_rope_kv_write and fg_rope_kv_write_parts into pages (bf16 rows and q_out): token n of sequence b is written to slot
+ * seq_len[b] + n of cache row row_map[b] (NULL: b). new_len (NULL: num_nodes): the tokens of sequence b from new_len[b] on
+ * are left out, their q_out rows and slots as they were. A slot without a page is not written and sets err_flag bit 8 (so does
+ * a cache row outside the table; q_out is written). bf16 pages and q get fg_rope_kv_write's values, bit for bit. e4m3 pages:
+ * q is rotated in fp32 by angles taken in 64 bits and rounded once; K is rotated in 64 bits, and K and V are quantised from there
+ * as fg_mx_quantize does it. num_nodes at most 8192, rows 8-byte aligned with a stride ld_qkv that is a multiple of 4.
+ * Two tokens of one call must not have one slot (cache rows that share a page must not both write to it). */
+int fg_rope_kv_write_paged(const void* qkv, int64_t ld_qkv, int batch, int num_nodes, int q_heads,
+                           const fg_kv_pages* pages, const int32_t* seq_len, const int32_t* pos_offset,
+                           int64_t pos_batch_stride, const float* inv_freq, const int32_t* new_len,
+                           const int32_t* row_map, void* q_out, int32_t* err_flag, void* stream);
+int fg_rope_kv_write_paged_parts(const float* part, int splits, const void* bias, int batch, int num_nodes, int q_heads,
+                                 const fg_kv_pages* pages, const int32_t* seq_len, const int32_t* pos_offset,
+                                 int64_t pos_batch_stride, const float* inv_freq, const int32_t* new_len,
+                                 const int32_t* row_map, void* q_out, int32_t* err_flag, void* stream);
+
+/* The values of tokens start[b] .. start[b] + count - 1 (start NULL: 0) of cache row row_map[b]: k_out and v_out
+ * [batch, kv_heads, count, head_dim] contiguous, fp32 or bf16 (dtype). Tokens without a page are 0. */
+int fg_kv_read_paged(const fg_kv_pages* pages, int batch, const int32_t* start, int count, const int32_t* row_map,
+                     void* k_out, void* v_out, int dtype, void* stream);
+
+/* fg_tree_attention over pages (bf16 q and out [batch, num_nodes, q_heads, head_dim]): node n of sequence b attends to tokens
+ * [0, seq_len[b]) of cache row row_map[b] and to new tokens seq_len[b] + m for every bit m of anc[b * anc_batch_stride + n]
+ * (num_nodes <= 64), or, anc NULL, to new tokens 0..n (num_nodes <= 8192). new_len as in fg_rope_kv_write_paged: rows from
+ * new_len[b] on are not written, and no row sees their tokens. Tokens without a page are not seen; a row that sees nothing is
+ * 0. Infinities and NaN of tokens that a row does not see do not reach it. Scores, softmax sums and O in fp32, the weights
+ * rounded to bf16 before they meet V. Where few rows meet many tokens, a sequence's tokens are split over
+ * workgroups whose parts are merged by a second launch; that needs workspace >= fg_paged_attention_workspace(...) bytes (capacity:
+ * table_width * page_size; 0 when nothing is split), 16-byte aligned and one call's at a time; a null or smaller one runs unsplit. */
+size_t fg_paged_attention_workspace(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int capacity);
+int fg_paged_attention(const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes, int q_heads,
+                       const int32_t* seq_len, const int32_t* new_len, const int32_t* row_map, const uint64_t* anc,
+                       int64_t anc_batch_stride, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* fg_kv_path_gather over pages, for `layers` layers in one launch: `pages` describes the first, the others lie layer_stride
+ * elements (scale_layer_stride bytes) behind each other. Moves tokens seq_len[b] + acc_nodes[b, j] to seq_len[b] + j for
+ * j < acc_len[b], codes and scales as they are; all sources are read before any destination is written. acc_stride at most
+ * 32. err_flag bit 1: a node outside [0, tree_nodes), a path longer than the tree, or a token without a page (that row, or its
+ * column, is skipped). */
+int fg_kv_path_gather_paged(const fg_kv_pages* pages, int layers, int64_t layer_stride, int64_t scale_layer_stride,
+                            int batch, const int32_t* seq_len, const int32_t* row_map, const int32_t* acc_nodes,
+                            int acc_stride, const int32_t* acc_len, int tree_nodes, int32_t* err_flag, void* stream);
+
 /* dst[i] = src[i] (bytes[i] bytes, a positive multiple of 4, 4-byte aligned device addresses, no
  * overlaps) for i < count <= 8, in one launch; src, dst and bytes are host arrays. No counterpart in the
  * reference: it brings a captured verify forward's inputs into the graph's static buffers. */

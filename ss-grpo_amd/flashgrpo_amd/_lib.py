@@ -20,6 +20,14 @@ _F = C.c_float
 _U32 = C.c_uint32
 _U64 = C.c_uint64
 
+
+class KvPages(C.Structure):
+    """struct fg_kv_pages."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scales", _P), ("v_scales", _P), ("table", _P), ("page_stride", _I64),
+                ("scale_stride", _I64), ("table_stride", _I64)] + [
+        (n, C.c_int32) for n in ("format", "pages", "page_size", "kv_heads", "head_dim", "table_rows", "table_width")]
+
+
 # name -> (restype, argtypes); mirrors include/flashgrpo_amd.h
 SIGNATURES = {
     "fg_last_error": (C.c_char_p, []),
@@ -64,6 +72,12 @@ SIGNATURES = {
     "fg_mx_gate_up_swiglu_workspace": (_SZ, [_I, _I, _I, _I]),
     "fg_mx_gate_up_swiglu": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _SZ, _P]),
     "fg_mx_plan": (_I, [_I, _I, _I, _I, _I, _P]),
+    "fg_rope_kv_write_paged": (_I, [_P, _I64, _I, _I, _I, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P]),
+    "fg_rope_kv_write_paged_parts": (_I, [_P, _I, _P, _I, _I, _I, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P]),
+    "fg_kv_read_paged": (_I, [_P, _I, _P, _I, _P, _P, _P, _I, _P]),
+    "fg_paged_attention_workspace": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "fg_paged_attention": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I64, _F, _P, _SZ, _P]),
+    "fg_kv_path_gather_paged": (_I, [_P, _I, _I64, _I64, _I, _P, _P, _P, _I, _P, _I, _P, _P]),
     "fg_sample_workspace": (_SZ, [_I]),
     "fg_sample_tokens": (_I, [_P, _I, _I64, _I, _I, _P, _P, _P, _I, _I, _U64, _U64, _P, _I, _F, _I, _I, _U32, _P,
                               _P, _SZ, _P]),

@@ -1046,6 +1046,251 @@ def mx_plan(rows, cols, k, *, fmt="e4m3", gate_up=False) -> MXPlan:
     return MXPlan(*p)
 
 
+# ------------------------------------------------------------------ a KV cache in pages
+PAGE_FORMATS = {torch.float8_e4m3fn: 0, torch.bfloat16: 1}  # struct fg_kv_pages' format
+
+
+class KVPages:
+    """One layer's K and V in pages (struct ``fg_kv_pages``), checked once: token t of cache row r lies in page
+    ``table[r, t // page_size]``, slot ``t % page_size`` (a page number outside [0, pages): no page).
+
+    ``k``, ``v``: bf16 or float8_e4m3fn [pages, kv_heads, page_size, head_dim] views of the same strides, each page
+    contiguous and 16-byte aligned (a pool may hold a page's layers side by side), head_dim 64 or 128, page_size a power of
+    two from 16 on. float8_e4m3fn pages hold MX rows: ``k_scales``, ``v_scales`` uint8 [pages, kv_heads, page_size, head_dim /
+    32], as ``mx_quantize`` makes them but a row's scales side by side (codes 0x7f and 0xff must not occur; a scale of 255
+    makes its block NaN). ``table``: int32 [rows, width]. The tensors are kept and their contents may change."""
+
+    __slots__ = ("k", "v", "k_scales", "v_scales", "table", "format", "pages", "page_size", "kv_heads", "head_dim", "rows",
+                 "width", "device", "address", "_c")
+
+    def __init__(self, k, v, k_scales, v_scales, table):
+        fmt = PAGE_FORMATS.get(k.dtype)
+        if fmt is None or v.dtype is not k.dtype:
+            raise TypeError("KVPages: k and v must be bfloat16 or float8_e4m3fn")
+        if table.dtype is not torch.int32 or table.dim() != 2 or 0 in table.shape:
+            raise ValueError("KVPages: table must be a non-empty int32 [rows, width] tensor")
+        dev = k.get_device()
+        _same_device("KVPages", dev, v, table, k_scales, v_scales)
+        stride, scale_stride = _page_stride(k, "k"), 0
+        n, heads, size, d = k.shape
+        if v.shape != k.shape or _page_stride(v, "v") != stride:
+            raise ValueError("KVPages: k and v must have one shape and one page stride")
+        if d not in (64, 128) or size < 16 or size & (size - 1):
+            raise ValueError("KVPages: head_dim must be 64 or 128 and page_size a power of two from 16 on")
+        if (fmt == 0) != (k_scales is not None) or (k_scales is None) != (v_scales is None):
+            raise ValueError("KVPages: float8_e4m3fn pages need scales, bfloat16 pages have none")
+        if fmt == 0:
+            shape = (n, heads, size, d // MX_BLOCK)
+            if k_scales.shape != shape or v_scales.shape != shape or k_scales.dtype is not _U8 or v_scales.dtype is not _U8:
+                raise ValueError(f"KVPages: scales must be uint8 {list(shape)}")
+            scale_stride = _page_stride(k_scales, "k_scales")
+            if _page_stride(v_scales, "v_scales") != scale_stride:
+                raise ValueError("KVPages: k_scales and v_scales must have one page stride")
+        rows, width = table.shape
+        if (width > 1 and table.stride(1) != 1) or (rows > 1 and table.stride(0) < width):
+            raise ValueError("KVPages: table rows must have unit stride and be apart")
+        if width * size >= (1 << 31) - 65536 or heads * size * d * 2 >= 1 << 31 or n >> 31 or rows >> 31:
+            raise ValueError("KVPages: rows must hold less than 2^31 - 65536 tokens and pages less than 2 GiB")
+        at = [None if t is None else t.data_ptr() for t in (k, v, k_scales, v_scales, table)]
+        if at[0] % 16 or at[1] % 16 or stride * (2 if fmt else 1) % 16 or (fmt == 0 and (at[2] % 4 or at[3] % 4 or scale_stride % 4)):
+            raise ValueError("KVPages: pages must start 16-byte aligned and scales 4-byte aligned")
+        self.k, self.v, self.k_scales, self.v_scales, self.table = k, v, k_scales, v_scales, table
+        self.format, self.pages, self.page_size, self.kv_heads, self.head_dim = fmt, n, size, heads, d
+        self.rows, self.width, self.device = rows, width, dev
+        self._c = _lib.KvPages(*at, stride, scale_stride, table.stride(0) if rows > 1 else width, fmt, n, size, heads, d, rows, width)
+        self.address = C.addressof(self._c)
+
+    @property
+    def capacity(self) -> int:
+        """Tokens that a cache row's table has entries for."""
+        return self.width * self.page_size
+
+
+def _page_stride(t, what):
+    """Elements between pages of a [pages, heads, size, n] view whose pages are contiguous."""
+    if t.dim() != 4 or 0 in t.shape:
+        raise ValueError(f"KVPages: {what} must be a non-empty [pages, kv_heads, page_size, n] tensor")
+    n, heads, size, d = t.shape
+    a, b, c, e = t.stride()
+    if e != 1 or c != d or (heads > 1 and b != size * d) or (n > 1 and a < heads * size * d):
+        raise ValueError(f"KVPages: {what} must have contiguous pages that are apart")
+    return a if n > 1 else heads * size * d
+
+
+def _index(what, dev, rows, *named):
+    """Raises unless each given (name, tensor) is a contiguous int32 tensor of at least ``rows`` entries on GPU ``dev``."""
+    for name, t in named:
+        if t is not None and (t.dtype is not torch.int32 or t.numel() < rows or not t.is_contiguous() or t.get_device() != dev):
+            raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of {rows} entries on the pages' device")
+
+
+def _paged_sizes(what, pages, kv_heads, head_dim):
+    if not isinstance(pages, KVPages):
+        raise TypeError(f"{what}: pages must be KVPages")
+    if pages.device < 0:
+        raise ValueError("flashgrpo_amd kernels take device tensors (got a CPU tensor)")
+    if kv_heads != pages.kv_heads or head_dim != pages.head_dim:
+        raise ValueError(f"{what}: the pages hold {pages.kv_heads} kv heads of {pages.head_dim}")
+
+
+def _write_paged(name, lead, pages, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out, new_len,
+                 row_map, err_flag, read):
+    what, dev = name[3:], pages.device
+    _index(what, dev, batch, ("seq_len", seq_len), ("new_len", new_len), ("row_map", row_map))
+    _index(what, dev, num_nodes, ("pos_offset", pos_offset))
+    _index(what, dev, 1, ("err_flag", err_flag))
+    pos_stride = _pos_stride(pos_offset, batch, num_nodes, what)
+    if inv_freq.dtype is not torch.float32 or inv_freq.numel() < head_dim // 2 or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
+        raise ValueError(f"{what}: inv_freq must be a contiguous fp32 tensor of {head_dim // 2} entries on the pages' device")
+    size = batch * num_nodes * q_heads * head_dim
+    at = q_out.data_ptr()
+    if q_out.dtype is not _BF16 or q_out.numel() != size or not q_out.is_contiguous() or q_out.get_device() != dev or at % 8:
+        raise ValueError(f"{what}: q_out must be a contiguous bf16 [batch * num_nodes, q_heads, d] tensor")
+    _apart(what, ((at, 2 * size),), read)
+    if size:
+        _call_on(dev, name, *lead, batch, num_nodes, q_heads, pages.address, seq_len.data_ptr(), pos_offset.data_ptr(), pos_stride,
+                 inv_freq.data_ptr(), _ptr(new_len), _ptr(row_map), at, _ptr(err_flag))
+
+
+def rope_kv_write_paged(qkv, pages, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out,
+                        new_len=None, row_map=None, err_flag=None):
+    """``rope_kv_write`` into pages (``fg_rope_kv_write_paged``): bf16 qkv rows; K and V go to slots seq_len[b] + n of cache
+    row row_map[b], in the pages' format. e4m3 pages: q is rotated in fp32 and rounded once, K and V are quantised from what the
+    formula gives, angles and K in 64 bits; bf16 pages and their q: ``rope_kv_write``'s values. ``new_len`` int32 [batch]:
+    tokens from new_len[b] on are left out (their q_out rows and slots stay as they were). A slot without a page sets
+    err_flag bit 8. Cache rows that share a page must not both write to it."""
+    what = "rope_kv_write_paged"
+    _paged_sizes(what, pages, kv_heads, head_dim)
+    width, rows = (q_heads + 2 * kv_heads) * head_dim, batch * num_nodes
+    if qkv.dtype is not _BF16 or qkv.dim() < 2 or qkv.stride(-1) != 1 or qkv.shape[-1] < width or qkv.numel() != rows * qkv.shape[-1] \
+            or qkv.get_device() != pages.device or (qkv.dim() > 2 and not qkv.is_contiguous()):
+        raise ValueError(f"{what}: qkv must hold {rows} rows of >= {width} unit-stride bf16 values on the pages' device")
+    ld = qkv.stride(-2) if rows > 1 and qkv.dim() == 2 else qkv.shape[-1]
+    at = qkv.data_ptr()
+    if at % 8 or ld % 4 or ld < width:
+        raise ValueError(f"{what}: qkv rows must be apart and start 8-byte aligned")
+    _write_paged("fg_rope_kv_write_paged", (at, ld), pages, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset,
+                 inv_freq, q_out, new_len, row_map, err_flag, ((at, 2 * ((rows - 1) * ld + width)),))
+
+
+def rope_kv_write_paged_parts(parts, bias, pages, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq,
+                              q_out, new_len=None, row_map=None, err_flag=None):
+    """``rope_kv_write_parts`` into pages (``fg_rope_kv_write_paged_parts``): the qkv rows are bf16(parts.sum(0) + bias), parts fp32
+    [S, batch * num_nodes, (q_heads + 2 kv_heads) * head_dim], then written as ``rope_kv_write_paged`` does."""
+    what = "rope_kv_write_paged_parts"
+    _paged_sizes(what, pages, kv_heads, head_dim)
+    width, rows = (q_heads + 2 * kv_heads) * head_dim, batch * num_nodes
+    if parts.dtype is not torch.float32 or parts.dim() != 3 or tuple(parts.shape[1:]) != (rows, width) or not parts.is_contiguous() \
+            or parts.shape[0] == 0 or parts.data_ptr() % 16 or parts.get_device() != pages.device:
+        raise ValueError(f"{what}: parts must be contiguous 16-byte aligned fp32 [S, {rows}, {width}] on the pages' device")
+    read = [(parts.data_ptr(), parts.numel() * 4)]
+    if bias is not None:
+        if bias.dtype is not _BF16 or bias.numel() != width or not bias.is_contiguous() or bias.data_ptr() % 8 \
+                or bias.get_device() != pages.device:
+            raise ValueError(f"{what}: bias must be a contiguous 8-byte aligned bf16 [{width}] tensor")
+        read.append((bias.data_ptr(), 2 * width))
+    _write_paged("fg_rope_kv_write_paged_parts", (parts.data_ptr(), parts.shape[0], _ptr(bias)), pages, batch, num_nodes, q_heads,
+                 kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out, new_len, row_map, err_flag, read)
+
+
+def kv_read_paged(pages, *, count, start=None, row_map=None, batch=None, dtype=torch.bfloat16):
+    """(k, v), each [batch, kv_heads, count, head_dim] in bf16 (exact but under 2^-126) or fp32: the values of tokens start[b] ..
+    start[b] + count - 1 (start None: 0) of cache row row_map[b] (None: b); tokens without a page are 0 (``fg_kv_read_paged``).
+    batch: that of start or row_map, or every row of the table."""
+    what = "kv_read_paged"
+    if not isinstance(pages, KVPages):
+        raise TypeError(f"{what}: pages must be KVPages")
+    dev = pages.device
+    _same_device(what, dev)
+    if batch is None:
+        batch = start.numel() if start is not None else row_map.numel() if row_map is not None else pages.rows
+    if dtype not in _DT:
+        raise TypeError(f"{what}: dtype must be bfloat16 or float32")
+    if batch < 0 or count < 0:
+        raise ValueError(f"{what}: batch and count must not be negative")
+    _index(what, dev, batch, ("start", start), ("row_map", row_map))
+    out = torch.empty(2, batch, pages.kv_heads, count, pages.head_dim, dtype=dtype, device=pages.k.device)
+    k, v = out.unbind(0)
+    if batch and count:
+        _call_on(dev, "fg_kv_read_paged", pages.address, batch, _ptr(start), count, _ptr(row_map), k.data_ptr(), v.data_ptr(),
+                 _DT[dtype])
+    return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace_bytes(batch, num_nodes, q_heads, kv_heads, head_dim, capacity):
+    return _lib.load().fg_paged_attention_workspace(batch, num_nodes, q_heads, kv_heads, head_dim, capacity)
+
+
+def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, head_dim, out=None, new_len=None, row_map=None, scale=None):
+    """``tree_attention`` over pages (``fg_paged_attention``): q bf16 [B, N, Hq, d] contiguous; anc int64 [B, N] or [N] (bits of
+    the new tokens that a node sees), or None for a causal chain. ``new_len`` int32 [B]: the rows of nodes from new_len[b] on
+    stay as they were in ``out`` (bf16, q's shape, apart from q), and nobody sees their tokens. A row that sees no token is 0, and
+    infinities and NaN of tokens that it does not see do not reach it."""
+    what = "paged_attention"
+    _paged_sizes(what, pages, kv_heads, head_dim)
+    dev, shape = pages.device, q.shape
+    if q.dtype is not _BF16 or len(shape) != 4 or shape[1:] != (num_nodes, q_heads, head_dim) or not q.is_contiguous() \
+            or q.get_device() != dev:
+        raise ValueError(f"{what}: q must be contiguous bf16 [B, {num_nodes}, {q_heads}, {head_dim}] on the pages' device")
+    B = shape[0]
+    _index(what, dev, B, ("seq_len", seq_len), ("new_len", new_len), ("row_map", row_map))
+    anc_stride = 0
+    if anc is not None:
+        if anc.dtype is not torch.int64:
+            raise TypeError("anc must be int64 (bit pattern of the uint64 masks)")
+        two = anc.dim() == 2
+        if anc.get_device() != dev or anc.shape != ((B, num_nodes) if two else (num_nodes,)) or (num_nodes > 1 and anc.stride(-1) != 1):
+            raise ValueError(f"{what}: anc must be [{B}, {num_nodes}] or [{num_nodes}] with unit stride on the pages' device")
+        anc_stride = anc.stride(0) if two else 0
+    at = q.data_ptr()
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        if out.dtype is not _BF16 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
+            raise ValueError(f"{what}: out must be a contiguous bf16 tensor of q's shape")
+        _apart(what, ((out.data_ptr(), 2 * q.numel()),), ((at, 2 * q.numel()),))
+    if at % 16 or out.data_ptr() % 8:
+        raise ValueError(f"{what}: q must start 16-byte aligned and out 8-byte aligned")
+    if q.numel() == 0:
+        return out
+    n = _paged_workspace_bytes(B, num_nodes, q_heads, kv_heads, head_dim, pages.width * pages.page_size)
+    ws = torch.empty(n, dtype=_U8, device=q.device) if n else None  # the call's own, as in _mx_workspace
+    _call_on(dev, "fg_paged_attention", at, out.data_ptr(), pages.address, B, num_nodes, q_heads, seq_len.data_ptr(), _ptr(new_len),
+             _ptr(row_map), _ptr(anc), anc_stride, 1.0 / math.sqrt(head_dim) if scale is None else float(scale), _ptr(ws), n)
+    return out
+
+
+def kv_path_gather_paged(pages, *, seq_len, acc_nodes, acc_len, tree_nodes, layers=1, layer_stride=0, scale_layer_stride=0,
+                         row_map=None, err_flag=None):
+    """``kv_path_gather`` over pages (``fg_kv_path_gather_paged``): tokens seq_len[b] + acc_nodes[b, j] move to seq_len[b] + j for
+    j < acc_len[b], in ``layers`` layers whose pages lie ``layer_stride`` elements (their scales ``scale_layer_stride`` bytes)
+    behind each other in the same pool. acc_nodes int32 [B, up to 32] contiguous."""
+    what = "kv_path_gather_paged"
+    if not isinstance(pages, KVPages):
+        raise TypeError(f"{what}: pages must be KVPages")
+    dev = pages.device
+    _same_device(what, dev)
+    B = seq_len.numel()
+    _index(what, dev, B, ("seq_len", seq_len), ("acc_len", acc_len), ("acc_nodes", acc_nodes), ("row_map", row_map))
+    _index(what, dev, 1, ("err_flag", err_flag))
+    if acc_nodes.dim() != 2 or acc_nodes.shape[0] != B or not 1 <= acc_nodes.shape[1] <= 32:
+        raise ValueError(f"{what}: acc_nodes must be [{B}, 1 to 32]")
+    if layers < 1 or not 1 <= tree_nodes <= pages.capacity:
+        raise ValueError(f"{what}: layers must be positive and the tree fit a cache row")
+    if layers > 1:
+        for t, s in ((pages.k, layer_stride), (pages.v, layer_stride), (pages.k_scales, scale_layer_stride),
+                     (pages.v_scales, scale_layer_stride)):
+            if t is not None:
+                size = t.shape[1] * t.shape[2] * t.shape[3]
+                last = t.storage_offset() + (pages.pages - 1) * t.stride(0) + (layers - 1) * s + size
+                if s < size or last * t.element_size() > t.untyped_storage().nbytes():
+                    raise ValueError(f"{what}: {layers} layers that far apart reach behind the pool")
+    if B:
+        _call_on(dev, "fg_kv_path_gather_paged", pages.address, layers, layer_stride, scale_layer_stride, B, seq_len.data_ptr(),
+                 _ptr(row_map), acc_nodes.data_ptr(), acc_nodes.shape[1], acc_len.data_ptr(), tree_nodes, _ptr(err_flag))
+
+
 # ------------------------------------------------------------------ sampling / acceptance
 def sample_workspace(rows, device):
     """Scratch that lets draws of long rows run split over several workgroups per row."""
