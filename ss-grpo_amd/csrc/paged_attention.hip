@@ -20,6 +20,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef __attribute__((address_space(4))) int32_t const_i32;  // read by the scalar unit
 
 struct PagedAttn {
   Pages pages;
@@ -113,44 +114,74 @@ FG_DEVICE float v_element(const Pages& pg, int page, int r, int d) {
   return x[0] * fg::mx_scale(pg.vs[page * pg.scale_bytes + (int64_t)r * (D / fg::kMxBlock) + d / fg::kMxBlock]);
 }
 
-// A workgroup of RW x KW waves takes 32 RW query rows of one (sequence, kv head, part of the keys), row r being head r % G of
-// node r / G. Tiles of KB KW keys go through LDS as bf16: every thread fetches 16-byte pieces of K and V rows, expands codes
-// (exactly) and stores them. Wave (rw, kw) multiplies rows 32 rw .. with keys KB kw .. of each tile; S^T = K Q^T puts a query
-// into a lane, so that the softmax needs one exchange with the other half-wave, and P^T goes from the accumulators straight
-// into O^T += V^T P^T. The KW waves of a row tile merge their (m, l, O) at the end through LDS; parts are merged by a second
-// kernel.
+// Where the non-finite elements of V's row `row` are visible to this lane's query they are added to O as they are: p > 0 times
+// an infinity or a NaN is that. (Loads one by one: the path is rare, and 64 of them in flight would cost the loop registers.)
+template <int FMT, int D>
+FG_DEVICE void add_unusual(const Pages& pg, int page, int row, int lane, bool sees, floatx16 (&o)[D / 32]) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = v_element<FMT, D>(pg, page, row, db * 32 + c_row32(i, lane));
+      o[db][i] += sees && !(fabsf(x) < INFINITY) ? x : 0.0f;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+template <int RW>
+FG_DEVICE void tile_barrier() {  // over the waves that share a tile
+  if constexpr (RW > 1) {
+    __syncthreads();
+  } else {  // one wave: its LDS operations are done in order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// A workgroup takes 32 RW query rows of one (sequence, kv head, part of the keys), row r being head r % G of node r / G, in KW
+// groups of RW waves. Tiles of KB keys go to the groups in turn. A group's threads fetch a tile's K and V rows into registers,
+// 16 bytes each, while the tile before is multiplied; every load of a wave is a consecutive 1 KB of at most 16 tokens, which lie
+// in one page, so that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their way to LDS. S^T = K Q^T
+// puts a query into a lane: the softmax needs one exchange with the other half-wave, and P^T goes from the accumulators
+// straight into O^T += V^T P^T. The groups merge their (m, l, O) at the end through LDS, the parts by a second kernel.
+//
+// RW = 1 (up to 32 rows: single tokens): a wave has its tiles and its piece of LDS for itself, no barrier; what bounds it is
+// the stream of pages, so P goes to V in two bf16 parts (hi + lo, which is p to 16 bits) at no cost. RW > 1: two LDS
+// stages, one barrier per tile; P is rounded to bf16 once (2^-9 of each weight, the error of the bf16 output again), and the sum
+// is that of the rounded weights.
 template <int FMT, int D, int RW, int KW, int KB>
 __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a, int m_tiles) {
-  constexpr int T = RW * KW * 64, KT = KB * KW, ROWS = RW * 32;
+  constexpr int T = RW * 64, ROWS = RW * 32, NBUF = RW > 1 ? 2 : 1;
+  constexpr bool TWO = RW == 1;                           // P in two parts
   constexpr int CPK = D * fg::page_elem_bytes<FMT> / 16;  // 16-byte pieces of a K or V row
-  constexpr int PIECES = KT * CPK, NP = 2 * PIECES / T;   // pieces of a tile's K (and of its V), of both per thread
+  constexpr int PIECES = KB * CPK, NP = 2 * PIECES / T;   // of a tile's K (and of its V); of both per thread
   constexpr int CHUNKS = FMT == kPageBF16 ? 1 : 2;        // 16-byte chunks that a piece is as bf16
   constexpr int KROW = D * 2 + 16, VROW = D * 2;
   constexpr int NB = KB / 32, ND = D / 32, NS = D / 16;
-  static_assert(2 * PIECES % T == 0 && NP >= 1 && NP <= 32 && PIECES % 64 == 0, "pieces");
-  constexpr int TILE = KT * (KROW + VROW);
+  static_assert(2 * PIECES % T == 0 && NP >= 1 && NP <= 32 && PIECES % 64 == 0 && 64 / CPK <= 16 && KB <= 64, "pieces");
+  constexpr int TILE = KB * (KROW + VROW);
   constexpr int MERGE = KW > 1 ? RW * KW * 32 * ((D + 4) * 4 + 8) : 0;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[TILE > MERGE ? TILE : MERGE];
-  __shared__ uint64_t odd_keys[2][(KT + 63) / 64], no_page[2][(KT + 63) / 64];
-  unsigned char* const kt = lds;
-  unsigned char* const vt = lds + KT * KROW;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[KW * NBUF * TILE > MERGE ? KW * NBUF * TILE : MERGE];
+  __shared__ uint64_t odd_keys[3][KW], no_page[3][KW];  // RW > 1: of a tile's keys
 
   const Pages& pg = a.pages;
   const int unit = blockIdx.x / m_tiles, mt = blockIdx.x % m_tiles;
   const int sp = unit % a.splits, hkv = unit / a.splits % pg.kv_heads, b = unit / (a.splits * pg.kv_heads);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   const int rw = wave % RW, kw = wave / RW;
   const int G = a.Hq / pg.kv_heads;
   const Span seq = span_of(a, b);
   const int M = G * seq.fresh;
   if (mt * ROWS >= M) return;  // rows behind the sequence's new tokens stay as they are
   const int keys = keys_of(a, seq);
-  const int part = part_keys(keys, a.splits, KT);
+  const int part = part_keys(keys, a.splits, KB);
   const int last = a.anc ? seq.fresh : (min((mt + 1) * ROWS, M) - 1) / G + 1;  // a chain's rows see no later token
   const int begin = min(sp * part, keys);
   const int end = max(begin, min(min(begin + part, keys), seq.committed + last));
   const int s0 = seq.committed;
-  const int32_t* trow = pg.table + (int64_t)max(seq.row, 0) * pg.table_stride;
+  const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
+  unsigned char* const group = lds + kw * NBUF * TILE;
 
   const int row0 = mt * ROWS + rw * 32, r = row0 + l32;
   const bool row_ok = r < M;
@@ -173,9 +204,10 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   const float sl2 = a.scale * 1.44269504088896341f;
   const bf16x2 ones2 = __builtin_bit_cast(bf16x2, 0x3f803f80u);
 
-  const uint32_t k_lane = (uint32_t)((kw * KB + l32) * KROW + g * 16);
-  // V^T fragments by transposed reads, as laid out in v_chunk below: lane 16 gq + i addresses key 4 (gq / 2) + i / 4 and d
-  // 32 db + 16 (gq % 2) + 4 (i % 4), and receives keys 4 (lane / 32) + j (and 8 + ..) of d = 32 db + lane % 32.
+  const uint32_t k_lane = (uint32_t)(l32 * KROW + g * 16);
+  // V^T fragments by transposed reads: lane 16 gq + i addresses key 4 (gq / 2) + i / 4 and d 32 db + 16 (gq % 2) + 4 (i % 4),
+  // and receives keys 4 (lane / 32) + j (and 8 + ..) of d = 32 db + lane % 32. V's 16-byte chunks are swizzled by their key,
+  // so that the 4 keys of a 16-lane read meet different banks.
   auto v_swizzle = [](int key) { return D == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); };
   uint32_t v_lane[ND];
   {
@@ -183,46 +215,56 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     const int low = 2 * (gq & 1) + ((i & 3) >> 1);
 #pragma unroll
     for (int db = 0; db < ND; ++db)
-      v_lane[db] = (uint32_t)((kw * KB + key) * VROW + (((4 * db + low) ^ v_swizzle(key)) * 16) + 8 * (i & 1));
+      v_lane[db] = (uint32_t)(KB * KROW + key * VROW + (((4 * db + low) ^ v_swizzle(key)) * 16) + 8 * (i & 1));
   }
 
-  if (tid < 2 * ((KT + 63) / 64)) (&odd_keys[0][0])[tid] = 0, (&no_page[0][0])[tid] = 0;
   uint4 piece[NP];
-  uint32_t scale[NP], held = 0;  // held: bit u, piece u's token is in the part and has a page
+  uint32_t scale[NP], paged = 0;  // paged: bit u, piece u's tokens have a page (the wave's)
   auto fetch = [&](int key0) __attribute__((always_inline)) {
-    held = 0;
+    paged = 0;
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
-      const int i = u * T + tid;
+      const int i = u * T + rw * 64;  // the wave's first piece
       const bool is_v = i >= PIECES;
-      const int j = (is_v ? i - PIECES : i) / CPK, c = i % CPK;
-      const int key = min(key0 + j, end - 1), page = pg.page(trow, key);  // loads are unconditional, from a place that exists
-      held |= (uint32_t)(key0 + j < end && page >= 0) << u;
-      const int64_t p = max(page, 0), row = pg.row_in_page(hkv, key);
-      piece[u] = *(const uint4*)((is_v ? pg.v : pg.k) + p * pg.page_bytes + row * (CPK * 16) + c * 16);
-      if constexpr (FMT == kPageE4M3) scale[u] = (is_v ? pg.vs : pg.ks)[p * pg.scale_bytes + row * (D / 32) + c / 2];
+      const int key = min(key0 + (is_v ? i - PIECES : i) / CPK, end - 1), found = trow[key >> pg.log2_page];
+      const bool ok = (unsigned)found < (unsigned)pg.pages;
+      paged |= (uint32_t)ok << u;
+      // the 16 tokens from a multiple of 16 on lie in one page: loads behind the part's end read rows that exist
+      const int64_t p = ok ? found : 0;
+      const int row = pg.row_in_page(hkv, key & -(64 / CPK));
+      piece[u] = *(const uint4*)((is_v ? pg.v : pg.k) + p * pg.page_bytes + (int64_t)row * (CPK * 16) + lane * 16);
+      if constexpr (FMT == kPageE4M3)
+        scale[u] = ((is_v ? pg.vs : pg.ks) + p * pg.scale_bytes + (int64_t)row * (D / 32))[lane / CPK * (D / 32) + lane % CPK / 2];
     }
   };
-  // Rows behind the part's end are 0; so is V where it is not finite (its products with p = 0 must stay 0), which the tile's
-  // odd_keys bits tell, and keys that have no page (no_page bits).
-  auto put = [&](int key0, int slot) __attribute__((always_inline)) {
+  uint64_t odd = 0, gone = 0;  // keys of the tile whose V is not finite somewhere; that have no page
+  // Rows behind the part's end are 0; so is V where it is not finite (its products with p = 0 must stay 0), and keys without a
+  // page.
+  auto put = [&](int key0, int buf, int slot) __attribute__((always_inline)) {
+    unsigned char* const at = group + buf * TILE;
+    uint64_t odd_here = 0, gone_here = 0;
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
-      const int i = u * T + tid;
-      const bool is_v = i >= PIECES, ok = (held >> u) & 1u;
-      const int j = (is_v ? i - PIECES : i) / CPK, c = i % CPK;
+      const int i = u * T + rw * 64;
+      const bool is_v = i >= PIECES, there = (paged >> u) & 1u;
+      const int j0 = (is_v ? i - PIECES : i) / CPK, j = j0 + lane / CPK, c = lane % CPK;
+      const bool ok = there && key0 + j < end;
       uint4 w = piece[u];
       bool bad = false;
       if constexpr (FMT == kPageE4M3) bad = scale[u] == 255u;
       if (is_v) {
         bad |= unusual<FMT>(w);
-        if (ok && bad) atomicOr((unsigned long long*)&odd_keys[slot][j >> 6], 1ull << (j & 63));
+        uint64_t lanes = __ballot(ok && bad);
+        while (lanes) {  // wave-uniform, rare
+          odd_here |= 1ull << (j0 + __builtin_ctzll(lanes) / CPK);
+          lanes &= lanes - 1;
+        }
         if (bad) w = make_uint4(0, 0, 0, 0);
-      } else if (!ok && c == 0 && key0 + j < end) {
-        atomicOr((unsigned long long*)&no_page[slot][j >> 6], 1ull << (j & 63));
+      } else if (!there) {
+        gone_here |= low_bits(64 / CPK) << j0;
       }
       if (!ok) w = make_uint4(0, 0, 0, 0);
-      unsigned char* dst = is_v ? vt + j * VROW : kt + j * KROW;
+      unsigned char* dst = is_v ? at + KB * KROW + j * VROW : at + j * KROW;
       const int c0 = is_v ? (c * CHUNKS) ^ v_swizzle(j) : c * CHUNKS;
       if constexpr (FMT == kPageE4M3) {
         uint4 lo, hi;
@@ -234,15 +276,24 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
         *(uint4*)(dst + c0 * 16) = w;
       }
     }
+    if constexpr (RW == 1) {
+      odd = odd_here;
+      gone = gone_here;
+    } else if (odd_here | gone_here) {
+      if (lane == 0) {
+        atomicOr((unsigned long long*)&odd_keys[slot][kw], odd_here);
+        atomicOr((unsigned long long*)&no_page[slot][kw], gone_here);
+      }
+    }
   };
 
-  auto compute = [&](int key0, int slot) __attribute__((always_inline)) {
-    const int first = key0 + kw * KB;  // this wave's keys
-    bf16x8 kf[NB * NS];
+  auto compute = [&](int first, int buf, int slot) __attribute__((always_inline)) {
+    const unsigned char* const at = group + buf * TILE;
+    bf16x8 fr[NB * NS];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int s = 0; s < NS; ++s) kf[kb * NS + s] = *(const bf16x8*)(kt + k_lane + kb * 32 * KROW + s * 32);
+      for (int s = 0; s < NS; ++s) fr[kb * NS + s] = *(const bf16x8*)(at + k_lane + kb * 32 * KROW + s * 32);
     floatx16 sc[NB];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
@@ -250,12 +301,11 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
-        sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb * NS + s], qf[s], sc[kb], 0, 0, 0);
+        sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[kb * NS + s], qf[s], sc[kb], 0, 0, 0);
     }
-    uint64_t odd = odd_keys[slot][kw * KB / 64], gone = no_page[slot][kw * KB / 64];
-    if (KB < 64) {
-      odd = (odd >> (kw * KB % 64)) & low_bits(KB);
-      gone = (gone >> (kw * KB % 64)) & low_bits(KB);
+    if constexpr (RW > 1) {
+      odd = odd_keys[slot][kw];
+      gone = no_page[slot][kw];
     }
     const uint64_t sees = a.anc ? seen_mask(s0 - first, bits) : low_bits(s0 + qn + 1 - first);
     const uint64_t allowed = sees & low_bits(end - first) & ~gone;
@@ -288,21 +338,27 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     }
     const float m_sub = m_run == -INFINITY ? 0.0f : m_run;
     float psum = l_run;
-    bf16x8 pf[NB][2];
+    bf16x8 pf[NB][2], lo[TWO ? NB : 1][2];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        uint32_t packed[4];
+        uint32_t packed[4], rest[4];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j], sl2, -m_sub));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j + 1], sl2, -m_sub));
           packed[j / 2] = fg::pack_bf16x2(p0, p1);
-          // the sum is that of the rounded p, the ones that multiply V
-          psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
+          if constexpr (TWO) {
+            psum += p0 + p1;
+            rest[j / 2] = fg::pack_bf16x2(p0 - __uint_as_float(packed[j / 2] << 16),
+                                          p1 - __uint_as_float(packed[j / 2] & 0xffff0000u));
+          } else {
+            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
+          }
         }
         pf[kb][ks] = __builtin_bit_cast(bf16x8, make_uint4(packed[0], packed[1], packed[2], packed[3]));
+        if constexpr (TWO) lo[kb][ks] = __builtin_bit_cast(bf16x8, make_uint4(rest[0], rest[1], rest[2], rest[3]));
       }
     l_run = psum;
 #pragma unroll
@@ -311,38 +367,53 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const unsigned char* p0 = vt + v_lane[db] + (kb * 2 + ks) * 16 * VROW;
-          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
-          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
-          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          const unsigned char* p0 = at + v_lane[db] + (kb * 2 + ks) * 16 * VROW;
+          const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
+          const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
           o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[kb][ks], o[db], 0, 0, 0);
+          if constexpr (TWO) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo[kb][ks], o[db], 0, 0, 0);
         }
     // Infinities and NaN of V reach only the rows that see their key.
     while (odd) {
-      const int j = __builtin_ctzll(odd);
+      const int j = __builtin_ctzll(odd), key = first + j;
       odd &= odd - 1;
-      if (!((allowed >> j) & 1ull)) continue;
-      const int page = pg.page(trow, first + j), row = pg.row_in_page(hkv, first + j);
-#pragma unroll
-      for (int db = 0; db < ND; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = v_element<FMT, D>(pg, page, row, db * 32 + c_row32(i, lane));
-          if (!(fabsf(x) < INFINITY)) o[db][i] += x;
-        }
+      add_unusual<FMT, D>(pg, trow[key >> pg.log2_page], pg.row_in_page(hkv, key), lane, (allowed >> j) & 1ull, o);
     }
   };
 
-  __syncthreads();
-  const int ntiles = (end - begin + KT - 1) / KT;
-  for (int t = 0; t < ntiles; ++t) {
-    const int key0 = begin + t * KT, slot = t & 1;
-    fetch(key0);
-    __syncthreads();  // every wave is done with the tile before
-    put(key0, slot);
-    if (tid < (KT + 63) / 64) odd_keys[slot ^ 1][tid] = 0, no_page[slot ^ 1][tid] = 0;
+  const int tiles = (end - begin + KB - 1) / KB;  // group kw takes tiles kw, kw + KW, ..
+  const int mine = (tiles - kw + KW - 1) / KW;
+  auto key_of = [&](int t) { return begin + (t * KW + kw) * KB; };
+  if constexpr (RW == 1) {
+    if (mine > 0) fetch(key_of(0));
+    for (int t = 0; t < mine; ++t) {
+      put(key_of(t), 0, 0);
+      if (t + 1 < mine) fetch(key_of(t + 1));
+      tile_barrier<RW>();
+      compute(key_of(t), 0, 0);
+      tile_barrier<RW>();
+    }
+  } else {
+    const int turns = (tiles + KW - 1) / KW;  // the same for every wave: the barriers are the workgroup's
+    if (tid < 3 * KW) (&odd_keys[0][0])[tid] = 0, (&no_page[0][0])[tid] = 0;
+    if (mine > 0) fetch(key_of(0));
     __syncthreads();
-    if (row0 < M) compute(key0, slot);
+    if (mine > 0) put(key_of(0), 0, 0);
+    if (mine > 1) fetch(key_of(1));
+    __syncthreads();
+    int slot = 0;
+    for (int t = 0; t < turns; ++t) {
+      const int next = slot == 2 ? 0 : slot + 1;
+      if (t + 1 < mine) put(key_of(t + 1), (t + 1) & 1, next);
+      if (t + 2 < mine) fetch(key_of(t + 2));
+      if (t < mine && row0 < M) compute(key_of(t), t & 1, slot);
+      // the bits of tile t - 1 become those of tile t + 2, which are written behind the next barrier
+      const int old = next == 2 ? 0 : next + 1;
+      if (tid < KW) odd_keys[old][tid] = 0, no_page[old][tid] = 0;
+      __syncthreads();
+      slot = next;
+    }
   }
 
   float l = xor32_sum(l_run);
@@ -443,13 +514,14 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int til
 struct Plan {
   int rw, kw, kb, splits;
   int rows() const { return rw * 32; }
-  int tile() const { return kw * kb; }
+  int tile() const { return kb; }
 };
 
 Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int64_t capacity) {
   const int64_t m = (int64_t)(q_heads / kv_heads) * num_nodes;
   Plan p;
   if (m <= 32) p = {1, 4, 32, 1};
+  else if (m <= 64) p = {2, 2, 32, 1};
   else if (m <= 128) p = {4, 1, 64, 1};
   else p = {8, 1, 64, 1};
   const int64_t base = (int64_t)batch * kv_heads * ((m + p.rows() - 1) / p.rows());
@@ -473,6 +545,8 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)a.batch * a.pages.kv_heads * a.splits * m_tiles)), block(p.rw * p.kw * 64);
   if (p.rw == 1)
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1, 4, 32>), grid, block, 0, s, a, m_tiles);
+  else if (p.rw == 2)
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 2, 32>), grid, block, 0, s, a, m_tiles);
   else if (p.rw == 4)
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 1, 64>), grid, block, 0, s, a, m_tiles);
   else
