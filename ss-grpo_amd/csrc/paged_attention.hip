@@ -40,6 +40,7 @@ struct PagedAttn {
 
 constexpr float kRescaleSlack = 8.0f;  // log2 units
 constexpr int kMinPartKeys = 256;      // a part of a sequence's keys is at least so long
+constexpr int kMaxParts = 64;
 
 FG_DEVICE int c_row32(int i, int lane) { return (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3); }
 
@@ -483,32 +484,61 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   }
 }
 
-// The parts of a row, in order: D / 4 lanes per row, 4 dims each. Parts that saw no key (m = -inf) weigh nothing.
-template <int D>
+// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims. A row has SLOTS groups of
+// D / 4 lanes, each with every SLOTS-th part, and a workgroup 256 / (SLOTS D / 4) rows. A lane p < parts of each wave reads part
+// p's (m, l) in one round trip and the loads of O do not wait for each other: 64 parts of 64 rows take 5 us, in one
+// loop over the parts 26.
+template <int D, int SLOTS>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int tile) {
-  constexpr int LANES = D / 4;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = D / 4, PER = 256 / (LANES * SLOTS);
+  __shared__ float4 sums[SLOTS > 1 ? 256 : 1];
+  const int slot = threadIdx.x / LANES % SLOTS, lane = threadIdx.x & 63, d0 = threadIdx.x % LANES * 4;
   const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
-  if (row >= rows) return;
-  const int n = (int)(row / a.Hq % a.N), b = (int)(row / a.Hq / a.N), d0 = threadIdx.x % LANES * 4;
+  const int64_t row = min((int64_t)blockIdx.x * PER + threadIdx.x / (LANES * SLOTS), rows - 1);  // (a row past the last: again)
+  const int n = (int)(row / a.Hq % a.N), b = (int)(row / a.Hq / a.N);
   const Span seq = span_of(a, b);
-  if (n >= seq.fresh) return;
   const int keys = keys_of(a, seq), part = part_keys(keys, a.splits, tile);
-  const int parts = part > 0 ? min(a.splits, (keys + part - 1) / part) : 0;
-  float mx = -INFINITY;
-  for (int p = 0; p < parts; ++p) mx = fmaxf(mx, a.ml_part[p * rows + row].x);
-  float den = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.ml_part[p * rows + row];
-    if (ml.y == 0.0f) continue;
-    const float w = __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
-    const float4 x = *(const float4*)(a.o_part + (p * rows + row) * D + d0);
-    den += w * ml.y;
-    o[0] += w * x.x; o[1] += w * x.y; o[2] += w * x.z; o[3] += w * x.w;
+  const int parts = part > 0 && n < seq.fresh ? min(a.splits, (keys + part - 1) / part) : 0;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float den = 0.0f;
+  if constexpr (SLOTS > 1) {  // a wave has one row
+    const float2 ml = lane < parts ? a.ml_part[lane * rows + row] : make_float2(-INFINITY, 0.0f);
+    const float mx = fg::wave_max(ml.x);
+    const float w = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
+    den = fg::wave_sum(w * ml.y);
+    static_assert(kMaxParts <= 64 && kMaxParts % SLOTS == 0, "a lane per part");
+#pragma unroll 4
+    for (int p0 = 0; p0 < parts; p0 += SLOTS) {  // all lanes stay: the weights come from other lanes
+      const int p = p0 + slot;
+      const float f = __shfl(w, p, 64);
+      const float4 x = *(const float4*)(a.o_part + (min(p, parts - 1) * rows + row) * D + d0);
+      if (f != 0.0f) o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+    }
+    sums[threadIdx.x] = o;
+    __syncthreads();
+    if (slot) return;
+#pragma unroll
+    for (int s = 1; s < SLOTS; ++s) {
+      const float4 x = sums[threadIdx.x + s * LANES];
+      o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    }
+  } else {
+    float mx = -INFINITY;
+    for (int p = 0; p < parts; ++p) mx = fmaxf(mx, a.ml_part[p * rows + row].x);
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const float2 ml = a.ml_part[p * rows + row];
+      const float4 x = *(const float4*)(a.o_part + (p * rows + row) * D + d0);
+      if (ml.y == 0.0f) continue;
+      const float f = __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
+      den += f * ml.y;
+      o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+    }
   }
+  if (n >= seq.fresh) return;
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   *(uint2*)((uint16_t*)a.out + row * D + d0) =
-      make_uint2(fg::pack_bf16x2(o[0] * inv, o[1] * inv), fg::pack_bf16x2(o[2] * inv, o[3] * inv));
+      make_uint2(fg::pack_bf16x2(o.x * inv, o.y * inv), fg::pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 struct Plan {
@@ -528,7 +558,7 @@ Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int64_t capaci
   const int64_t target = 256 * (8 / (p.rw * p.kw));
   if (base < target) {
     const int64_t most = std::max<int64_t>(1, capacity / kMinPartKeys);
-    p.splits = (int)std::min<int64_t>(std::min<int64_t>((target + base - 1) / base, most), 64);
+    p.splits = (int)std::min<int64_t>(std::min<int64_t>((target + base - 1) / base, most), kMaxParts);
   }
   return p;
 }
@@ -553,8 +583,11 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 8, 1, 64>), grid, block, 0, s, a, m_tiles);
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
-    const int per = 256 / (D / 4);
-    hipLaunchKernelGGL(paged_combine_kernel<D>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a, p.tile());
+    constexpr int SLOTS = 1024 / D;  // a workgroup's row
+    if (a.splits > 8)
+      hipLaunchKernelGGL((paged_combine_kernel<D, SLOTS>), dim3((unsigned)rows), dim3(256), 0, s, a, p.tile());
+    else
+      hipLaunchKernelGGL((paged_combine_kernel<D, 1>), dim3((unsigned)((rows + SLOTS - 1) / SLOTS)), dim3(256), 0, s, a, p.tile());
   }
 }
 
