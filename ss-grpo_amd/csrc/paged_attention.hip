@@ -484,6 +484,289 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   }
 }
 
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+FG_DEVICE float quad_max(float x) {  // over the four lanes of a query: lane, + 16, + 32, + 48
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return xor32_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+FG_DEVICE float quad_sum(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return xor32_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Few rows (single tokens; at most 16 NQ rows of a kv head): the pages are streamed past them. A workgroup of four waves takes one
+// (sequence, kv head, part of the keys), its waves 32-key tiles in turn, each with registers and LDS of its own, no
+// barrier in the loop. S^T = K Q^T on 16 x 16 x 32 MFMAs: lane 16 gq + i holds key i of 16 and, of every 64 bytes of its
+// row, the 16 at 16 gq; which d a k index stands for is free as long as Q follows, so K's rows go from memory through the
+// expansion into the MFMA's registers and never see LDS. V is expanded into a tile of LDS and read transposed. P goes to V in two
+// bf16 parts (hi + lo, p to 16 bits): what bounds the kernel is the stream.
+template <int FMT, int D, int NQ>
+struct StreamTile {  // a tile's loads: 32 keys
+  static constexpr int kLoads = D * fg::page_elem_bytes<FMT> / 64;  // 16-byte loads of a lane per 16 keys
+  uint4 k[2][kLoads], v[2 * kLoads];
+  uint32_t ks[2], vs[2 * kLoads];  // scales: of K's key all four, of a piece of V its own
+  int there;                       // bit h: keys 16 h .. have a page
+};
+
+template <int FMT, int D, int NQ>
+__global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(PagedAttn a) {
+  constexpr int ES = fg::page_elem_bytes<FMT>, CPK = D * ES / 16, VROW = D * 2;
+  constexpr int NL = StreamTile<FMT, D, NQ>::kLoads, NS = D / 32, ND = D / 16, BLOCKS = D / fg::kMxBlock;
+  constexpr int VTILE = 32 * VROW, OROW = D + 4;
+  constexpr int MERGE = 4 * NQ * 16 * (OROW * 4 + 8);
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * VTILE > MERGE ? 4 * VTILE : MERGE];
+  const Pages& pg = a.pages;
+  const int unit = blockIdx.x;
+  const int sp = unit % a.splits, hkv = unit / a.splits % pg.kv_heads, b = unit / (a.splits * pg.kv_heads);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gq = lane >> 4, i16 = lane & 15;
+  const int G = a.Hq / pg.kv_heads;
+  const Span seq = span_of(a, b);
+  const int M = G * seq.fresh;
+  if (M == 0) return;
+  const int keys = keys_of(a, seq), part = part_keys(keys, a.splits, 32), s0 = seq.committed;
+  const int begin = min(sp * part, keys), end = min(begin + part, keys);
+  const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
+  unsigned char* const vt = lds + wave * VTILE;
+  typedef StreamTile<FMT, D, NQ> Tile;
+
+  auto fetch = [&](int key0, Tile& t) __attribute__((always_inline)) {
+    t.there = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = min(key0 + 16 * h, end - 1), found = trow[key >> pg.log2_page];
+      const bool ok = (unsigned)found < (unsigned)pg.pages;
+      t.there |= (int)ok << h;
+      const int64_t p = ok ? found : 0;  // behind the part's end, and without a page, rows that exist are read and not used
+      const int row = pg.row_in_page(hkv, key & -16);
+      const uint8_t* kr = pg.k + p * pg.page_bytes + (int64_t)row * (D * ES);
+      const uint8_t* vr = pg.v + p * pg.page_bytes + (int64_t)row * (D * ES);
+#pragma unroll
+      for (int s = 0; s < NL; ++s) t.k[h][s] = *(const uint4*)(kr + i16 * (D * ES) + s * 64 + gq * 16);
+#pragma unroll
+      for (int s = 0; s < NL; ++s) t.v[h * NL + s] = *(const uint4*)(vr + s * 1024 + lane * 16);
+      if constexpr (FMT == kPageE4M3) {
+        const uint8_t* ks = pg.ks + p * pg.scale_bytes + (int64_t)row * BLOCKS;
+        const uint8_t* vs = pg.vs + p * pg.scale_bytes + (int64_t)row * BLOCKS;
+        t.ks[h] = BLOCKS == 4 ? *(const uint32_t*)(ks + i16 * 4) : *(const uint16_t*)(ks + i16 * 2);
+#pragma unroll
+        for (int s = 0; s < NL; ++s) t.vs[h * NL + s] = vs[s * (1024 / 32) + lane / 2];
+      }
+    }
+  };
+  const int tiles = (end - begin + 31) / 32, mine = (tiles - wave + 3) / 4;
+  auto key_of = [&](int t) { return begin + (t * 4 + wave) * 32; };
+  Tile cur;
+  if (mine > 0) fetch(key_of(0), cur);
+
+  int qn[NQ], qh[NQ];
+  bool row_ok[NQ];
+  uint64_t bits[NQ];
+  bf16x8 qf[NQ][NS];
+#pragma unroll
+  for (int c = 0; c < NQ; ++c) {
+    const int r = c * 16 + i16;
+    row_ok[c] = r < M;
+    qn[c] = row_ok[c] ? r / G : 0;
+    qh[c] = hkv * G + (row_ok[c] ? r % G : 0);
+    bits[c] = row_ok[c] && a.anc ? a.anc[(int64_t)b * a.anc_stride + qn[c]] & low_bits(seq.fresh) : 0ull;
+    const uint16_t* qrow = (const uint16_t*)a.q + (((int64_t)b * a.N + qn[c]) * a.Hq + qh[c]) * D;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      // the d of k-step s: e4m3: 8 of the 16 codes of load s / 2, bf16: the 8 elements of load s
+      const int d = FMT == kPageE4M3 ? s / 2 * 64 + gq * 16 + s % 2 * 8 : s * 32 + gq * 8;
+      qf[c][s] = __builtin_bit_cast(bf16x8, row_ok[c] ? *(const uint4*)(qrow + d) : make_uint4(0, 0, 0, 0));
+    }
+  }
+  floatx4 o[NQ][ND];
+  float m_run[NQ], l_run[NQ];
+#pragma unroll
+  for (int c = 0; c < NQ; ++c) {
+    m_run[c] = -INFINITY;
+    l_run[c] = 0.0f;
+#pragma unroll
+    for (int db = 0; db < ND; ++db) o[c][db] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const float sl2 = a.scale * 1.44269504088896341f;
+  // V^T fragments (16 d x 32 keys): lane 16 gq + i addresses key 4 gq + i / 4 (+ 16) and d 16 db + 4 (i % 4), and receives keys
+  // 4 gq + j (and 16 + ..) of d = 16 db + i: the keys of S^T's accumulators. Chunks of 16 bytes are swizzled by their key, so that
+  // the four keys of a 16-lane read meet different banks.
+  auto v_swizzle = [](int key) { return D == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); };
+  const int v_key = 4 * gq + (i16 >> 2);
+  const uint32_t v_at = (uint32_t)(v_key * VROW + 8 * (i16 & 1)), v_x = (uint32_t)v_swizzle(v_key), v_low = (i16 & 3) >> 1;
+
+  for (int t = 0; t < mine; ++t) {
+    const int first = key_of(t);
+    // ---------------- V to LDS
+    uint64_t odd = 0;  // keys whose V is not finite somewhere; there it is 0, and so it is behind the end and without a page
+    const bool whole = first + 32 <= end && cur.there == 3;
+#pragma unroll
+    for (int s = 0; s < 2 * NL; ++s) {
+      const int j = s * (64 / CPK) + lane / CPK, c = lane % CPK;
+      uint4 w = cur.v[s];
+      bool bad = unusual<FMT>(w);
+      uint32_t e = 127u;
+      if constexpr (FMT == kPageE4M3) e = cur.vs[s], bad |= e == 255u;
+      const bool ok = whole || (first + j < end && ((cur.there >> (j >> 4)) & 1));
+      if (__any(bad || !ok)) {
+        uint64_t lanes = __ballot(bad && ok);
+        while (lanes) {
+          odd |= 1ull << (s * (64 / CPK) + __builtin_ctzll(lanes) / CPK);
+          lanes &= lanes - 1;
+        }
+        if (bad || !ok) w = make_uint4(0, 0, 0, 0), e = 127u;
+      }
+      if constexpr (FMT == kPageE4M3) {
+        uint4 lo, hi;
+        expand16(w, e, lo, hi);
+        unsigned char* dst = vt + j * VROW + ((2 * c) ^ v_swizzle(j)) * 16;
+        *(uint4*)dst = lo;
+        *(uint4*)(dst + 16) = hi;
+      } else {
+        *(uint4*)(vt + j * VROW + (c ^ v_swizzle(j)) * 16) = w;
+      }
+    }
+    // ---------------- S^T
+    floatx4 sc[NQ][2];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) sc[c][0] = sc[c][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < NL; ++s) {
+        uint4 part[2];
+        if constexpr (FMT == kPageE4M3) {
+          uint32_t e = (cur.ks[h] >> (8 * (2 * s + (gq >> 1)))) & 255u;
+          uint4 w = cur.k[h][s];
+          if (__any(e == 255u) && e == 255u) w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), e = 127u;  // NaN
+          expand16(w, e, part[0], part[1]);
+#pragma unroll
+          for (int c = 0; c < NQ; ++c)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              sc[c][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, part[x]), qf[c][2 * s + x], sc[c][h], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int c = 0; c < NQ; ++c)
+            sc[c][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, cur.k[h][s]), qf[c][s], sc[c][h], 0, 0, 0);
+        }
+      }
+    const uint64_t gone = (cur.there & 1 ? 0ull : 0xffffull) | (cur.there & 2 ? 0ull : 0xffff0000ull);
+    if (t + 1 < mine) fetch(key_of(t + 1), cur);
+    // ---------------- softmax
+    const bool masked = first + 32 > s0 || first + 32 > end || gone;
+    uint64_t allowed[NQ];
+    bf16x8 hi[NQ], lo[NQ];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+      allowed[c] = (a.anc ? seen_mask(s0 - first, bits[c]) : low_bits(s0 + qn[c] + 1 - first)) & low_bits(end - first) & ~gone;
+      if (masked) {
+        const uint64_t at = allowed[c] >> (4 * gq);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[c][h][i] = (at >> (16 * h + i)) & 1ull ? sc[c][h][i] : -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[c][h][i]);
+      const float m_new = fmaxf(m_run[c], quad_max(top) * sl2);
+      if (__any(m_new > m_run[c] + kRescaleSlack)) {
+        const float alpha = __builtin_amdgcn_exp2f(m_run[c] - (m_new == -INFINITY ? 0.0f : m_new));
+        l_run[c] *= alpha;
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[c][db][i] *= alpha;
+        m_run[c] = m_new;
+      }
+      const float sub = m_run[c] == -INFINITY ? 0.0f : m_run[c];
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[c][x >> 1][2 * (x & 1)], sl2, -sub));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[c][x >> 1][2 * (x & 1) + 1], sl2, -sub));
+        l_run[c] += p0 + p1;
+        ph[x] = fg::pack_bf16x2(p0, p1);
+        pl[x] = fg::pack_bf16x2(p0 - __uint_as_float(ph[x] << 16), p1 - __uint_as_float(ph[x] & 0xffff0000u));
+      }
+      hi[c] = __builtin_bit_cast(bf16x8, make_uint4(ph[0], ph[1], ph[2], ph[3]));
+      lo[c] = __builtin_bit_cast(bf16x8, make_uint4(pl[0], pl[1], pl[2], pl[3]));
+    }
+    // ---------------- O^T += V^T P^T
+    tile_barrier<1>();
+#pragma unroll
+    for (int db = 0; db < ND; ++db) {
+      const unsigned char* at = vt + v_at + (((2 * db + v_low) ^ v_x) * 16);
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+      const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 16 * VROW));
+      const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int c = 0; c < NQ; ++c) {
+        o[c][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi[c], o[c][db], 0, 0, 0);
+        o[c][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[c], o[c][db], 0, 0, 0);
+      }
+    }
+    while (odd) {  // infinities and NaN of V reach only the rows that see their key
+      const int j = __builtin_ctzll(odd), key = first + j;
+      odd &= odd - 1;
+      const int page = trow[key >> pg.log2_page], row = pg.row_in_page(hkv, key);
+#pragma unroll
+      for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = v_element<FMT, D>(pg, page, row, 16 * db + 4 * gq + i);
+            o[c][db][i] += ((allowed[c] >> j) & 1ull) && !(fabsf(x) < INFINITY) ? x : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+    }
+    tile_barrier<1>();
+  }
+
+  // ---------------- merge the waves
+  float* om = (float*)lds;
+  float2* ml = (float2*)(lds + 4 * NQ * 16 * OROW * 4);
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < NQ; ++c) {
+    const int at = (wave * NQ + c) * 16 + i16;
+#pragma unroll
+    for (int db = 0; db < ND; ++db) *(floatx4*)(om + at * OROW + 16 * db + 4 * gq) = o[c][db];
+    const float l = quad_sum(l_run[c]);
+    if (gq == 0) ml[at] = make_float2(m_run[c], l);
+  }
+  __syncthreads();
+  for (int e = tid; e < M * (D / 4); e += 256) {
+    const int r = e / (D / 4), d0 = e % (D / 4) * 4;
+    float mx = -INFINITY, den = 0.0f, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w * NQ * 16 + r].x);
+    const float sub = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int at = w * NQ * 16 + r;
+      const float f = __builtin_amdgcn_exp2f(ml[at].x - sub);
+      const float4 x = *(const float4*)(om + at * OROW + d0);
+      den += f * ml[at].y;
+      s[0] += f * x.x; s[1] += f * x.y; s[2] += f * x.z; s[3] += f * x.w;
+    }
+    const int64_t orow = ((int64_t)b * a.N + r / G) * a.Hq + hkv * G + r % G;
+    if (a.splits > 1) {
+      const int64_t prow = (int64_t)sp * a.batch * a.N * a.Hq + orow;
+      *(float4*)(a.o_part + prow * D + d0) = make_float4(s[0], s[1], s[2], s[3]);
+      if (d0 == 0) a.ml_part[prow] = make_float2(mx, den);
+    } else {
+      const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+      *(uint2*)((uint16_t*)a.out + orow * D + d0) =
+          make_uint2(fg::pack_bf16x2(s[0] * inv, s[1] * inv), fg::pack_bf16x2(s[2] * inv, s[3] * inv));
+    }
+  }
+}
+
 // The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims. A row has SLOTS groups of
 // D / 4 lanes, each with every SLOTS-th part, and a workgroup 256 / (SLOTS D / 4) rows. A lane p < parts of each wave reads part
 // p's (m, l) in one round trip and the loads of O do not wait for each other: 64 parts of 64 rows take 5 us, in one
@@ -573,8 +856,10 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   const int64_t m = (int64_t)(a.Hq / a.pages.kv_heads) * a.N;
   const int m_tiles = (int)((m + p.rows() - 1) / p.rows());
   const dim3 grid((unsigned)((int64_t)a.batch * a.pages.kv_heads * a.splits * m_tiles)), block(p.rw * p.kw * 64);
-  if (p.rw == 1)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1, 4, 32>), grid, block, 0, s, a, m_tiles);
+  if (m <= 16)
+    hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 1>), grid, block, 0, s, a);
+  else if (m <= 32)
+    hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 2>), grid, block, 0, s, a);
   else if (p.rw == 2)
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 2, 32>), grid, block, 0, s, a, m_tiles);
   else if (p.rw == 4)
