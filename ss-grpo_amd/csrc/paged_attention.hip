@@ -40,7 +40,8 @@ struct PagedAttn {
 
 constexpr float kRescaleSlack = 8.0f;  // log2 units
 constexpr int kMinPartKeys = 256;      // a part of a sequence's keys is at least so long
-constexpr int kMaxParts = 64;
+constexpr int kMaxParts = 256;
+constexpr int kStreamWaves = 8;          // of a workgroup of the stream kernel
 
 FG_DEVICE int c_row32(int i, int lane) { return (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3); }
 
@@ -98,12 +99,18 @@ FG_DEVICE void expand16(uint4 w, uint32_t s, uint4& lo, uint4& hi) {
   hi = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
-// Whether 16 bytes hold a value that is not finite: e4m3 code 0x7f (or 0xff), bf16 with all exponent bits set.
-template <int FMT>
-FG_DEVICE bool unusual(uint4 w) {
-  const uint32_t keep = FMT == kPageE4M3 ? 0x7f7f7f7fu : 0x7f807f80u, one = FMT == kPageE4M3 ? 0x01010101u : 0x00800080u,
-                 top = FMT == kPageE4M3 ? 0x80808080u : 0x80008000u;
-  return (((w.x & keep) + one) | ((w.y & keep) + one) | ((w.z & keep) + one) | ((w.w & keep) + one)) & top;
+// bf16 values that are not finite have all exponent bits: as 15-bit numbers they are 0x7f80 or more.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+FG_DEVICE uint32_t max_u16x2(uint32_t x, uint32_t y) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
+}
+FG_DEVICE uint32_t largest_u16(uint4 w) {  // by halves
+  constexpr uint32_t m = 0x7fff7fffu;
+  return max_u16x2(max_u16x2(w.x & m, w.y & m), max_u16x2(w.z & m, w.w & m));
+}
+FG_DEVICE bool not_finite(uint4 w) {
+  const uint32_t x = largest_u16(w);
+  return (x & 0xffffu) >= 0x7f80u || x >= 0x7f800000u;
 }
 
 // One element of V as a float.
@@ -115,56 +122,51 @@ FG_DEVICE float v_element(const Pages& pg, int page, int r, int d) {
   return x[0] * fg::mx_scale(pg.vs[page * pg.scale_bytes + (int64_t)r * (D / fg::kMxBlock) + d / fg::kMxBlock]);
 }
 
-// Where the non-finite elements of V's row `row` are visible to this lane's query they are added to O as they are: p > 0 times
-// an infinity or a NaN is that. (Loads one by one: the path is rare, and 64 of them in flight would cost the loop registers.)
-template <int FMT, int D>
-FG_DEVICE void add_unusual(const Pages& pg, int page, int row, int lane, bool sees, floatx16 (&o)[D / 32]) {
+// Infinities and NaN of V at tokens that only some rows see (the new tokens' tiles). The loops keep them at 0 there, since p = 0
+// times them would be NaN, and here, once, they are added for the rows that see them: p > 0 times an infinity or a NaN is
+// that. `add(page, row, token)` is called for each such token in [from, end).
+template <int FMT, int D, typename F>
+FG_DEVICE void each_unusual(const Pages& pg, const const_i32* trow, int hkv, int lane, int from, int end, F add) {
+  constexpr int PER = D / 64;  // elements of a lane
+  for (int key = from; key < end; ++key) {
+    const int page = trow[key >> pg.log2_page];
+    if ((unsigned)page >= (unsigned)pg.pages) continue;
+    const int row = pg.row_in_page(hkv, key);
+    bool bad = false;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float x = v_element<FMT, D>(pg, page, row, db * 32 + c_row32(i, lane));
-      o[db][i] += sees && !(fabsf(x) < INFINITY) ? x : 0.0f;
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int i = 0; i < PER; ++i) bad |= !(fabsf(v_element<FMT, D>(pg, page, row, lane * PER + i)) < INFINITY);
+    if (__any(bad)) add(page, row, key);
+  }
 }
 
-template <int RW>
-FG_DEVICE void tile_barrier() {  // over the waves that share a tile
-  if constexpr (RW > 1) {
-    __syncthreads();
-  } else {  // one wave: its LDS operations are done in order
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
+FG_DEVICE void wave_barrier() {  // a wave's LDS operations are done in order; this keeps the compiler's in theirs
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // A workgroup takes 32 RW query rows of one (sequence, kv head, part of the keys), row r being head r % G of node r / G, in KW
 // groups of RW waves. Tiles of KB keys go to the groups in turn. A group's threads fetch a tile's K and V rows into registers,
-// 16 bytes each, while the tile before is multiplied; every load of a wave is a consecutive 1 KB of at most 16 tokens, which lie
-// in one page, so that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their way to LDS. S^T = K Q^T
-// puts a query into a lane: the softmax needs one exchange with the other half-wave, and P^T goes from the accumulators
-// straight into O^T += V^T P^T. The groups merge their (m, l, O) at the end through LDS, the parts by a second kernel.
-//
-// RW = 1 (up to 32 rows: single tokens): a wave has its tiles and its piece of LDS for itself, no barrier; what bounds it is
-// the stream of pages, so P goes to V in two bf16 parts (hi + lo, which is p to 16 bits) at no cost. RW > 1: two LDS
-// stages, one barrier per tile; P is rounded to bf16 once (2^-9 of each weight, the error of the bf16 output again), and the sum
-// is that of the rounded weights.
+// 16 bytes each, two tiles ahead; every load of a wave is a consecutive 1 KB of at most 16 tokens, which lie in one page, so
+// that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their way to one of two LDS stages, while
+// the tile in the other is multiplied; one barrier per tile. S^T = K Q^T puts a query into a lane: the softmax needs one
+// exchange with the other half-wave, and P^T goes from the accumulators straight into O^T += V^T P^T, rounded to bf16 once (2^-9
+// of each weight in the mean, the error of the bf16 output again); the sum is that of the rounded weights. The groups merge
+// their (m, l, O) at the end through LDS, the parts by a second kernel.
 template <int FMT, int D, int RW, int KW, int KB>
 __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a, int m_tiles) {
-  constexpr int T = RW * 64, ROWS = RW * 32, NBUF = RW > 1 ? 2 : 1;
-  constexpr bool TWO = RW == 1;                           // P in two parts
+  constexpr int T = RW * 64, ROWS = RW * 32;
   constexpr int CPK = D * fg::page_elem_bytes<FMT> / 16;  // 16-byte pieces of a K or V row
-  constexpr int PIECES = KB * CPK, NP = 2 * PIECES / T;   // of a tile's K (and of its V); of both per thread
+  constexpr int NU = KB * CPK / T, KPW = 64 / CPK;        // pieces of a tile's K (and of its V) per thread; keys of a load
   constexpr int CHUNKS = FMT == kPageBF16 ? 1 : 2;        // 16-byte chunks that a piece is as bf16
-  constexpr int KROW = D * 2 + 16, VROW = D * 2;
+  constexpr int KROW = D * 2 + 16, VROW = D * 2, BLOCKS = D / fg::kMxBlock;
   constexpr int NB = KB / 32, ND = D / 32, NS = D / 16;
-  static_assert(2 * PIECES % T == 0 && NP >= 1 && NP <= 32 && PIECES % 64 == 0 && 64 / CPK <= 16 && KB <= 64, "pieces");
+  static_assert(KB * CPK % T == 0 && NU >= 1 && NU <= 32 && KPW <= 16 && KB <= 64, "pieces");
   constexpr int TILE = KB * (KROW + VROW);
   constexpr int MERGE = KW > 1 ? RW * KW * 32 * ((D + 4) * 4 + 8) : 0;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[KW * NBUF * TILE > MERGE ? KW * NBUF * TILE : MERGE];
-  __shared__ uint64_t odd_keys[3][KW], no_page[3][KW];  // RW > 1: of a tile's keys
+  __shared__ __attribute__((aligned(16))) unsigned char lds[KW * 2 * TILE > MERGE ? KW * 2 * TILE : MERGE];
+  __shared__ uint64_t no_page[3][KW];  // a tile's keys without a page
+  __shared__ int gone_any[3][KW], odd_any;  // whether there are any; whether V was kept at 0 where it is not finite
 
   const Pages& pg = a.pages;
   const int unit = blockIdx.x / m_tiles, mt = blockIdx.x % m_tiles;
@@ -180,9 +182,37 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   const int last = a.anc ? seq.fresh : (min((mt + 1) * ROWS, M) - 1) / G + 1;  // a chain's rows see no later token
   const int begin = min(sp * part, keys);
   const int end = max(begin, min(min(begin + part, keys), seq.committed + last));
-  const int s0 = seq.committed;
+  const int s0 = seq.committed, clear = a.anc ? s0 : s0 + mt * ROWS / G + 1;  // every row sees the keys before `clear`
   const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
-  unsigned char* const group = lds + kw * NBUF * TILE;
+  unsigned char* const group = lds + kw * 2 * TILE;
+
+  uint4 kp[NU], vp[NU];
+  uint32_t ksc[NU], vsc[NU], paged = 0;  // paged: bit u, the tokens of load u have a page
+  const uint32_t head_row = (uint32_t)hkv << pg.log2_page, slot_mask = (1u << pg.log2_page) - 1u;
+  const uint32_t sc_lane = (uint32_t)(lane / CPK * BLOCKS + lane % CPK / 2);
+  auto fetch = [&](int key0) __attribute__((always_inline)) {
+    paged = 0;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      // Behind the part's end, and without a page, rows that exist are read and not used.
+      const int key = min(key0 + (u * RW + rw) * KPW, end - 1), found = trow[key >> pg.log2_page];
+      const bool ok = (unsigned)found < (unsigned)pg.pages;
+      paged |= (uint32_t)ok << u;
+      const uint32_t row = head_row + ((uint32_t)key & slot_mask & ~(uint32_t)(KPW - 1));
+      const int64_t at = (ok ? found : 0) * pg.page_bytes + (int64_t)row * (CPK * 16);
+      kp[u] = *(const uint4*)(pg.k + at + (uint32_t)lane * 16);
+      vp[u] = *(const uint4*)(pg.v + at + (uint32_t)lane * 16);
+      if constexpr (FMT == kPageE4M3) {
+        const int64_t sat = (ok ? found : 0) * pg.scale_bytes + (int64_t)row * BLOCKS;
+        ksc[u] = (pg.ks + sat)[sc_lane];
+        vsc[u] = (pg.vs + sat)[sc_lane];
+      }
+    }
+  };
+  const int tiles = (end - begin + KB - 1) / KB;  // group kw takes tiles kw, kw + KW, ..
+  const int turns = (tiles + KW - 1) / KW, mine = (tiles - kw + KW - 1) / KW;  // (the barriers are the workgroup's)
+  auto key_of = [&](int t) { return begin + (t * KW + kw) * KB; };
+  if (tiles) fetch(key_of(0));
 
   const int row0 = mt * ROWS + rw * 32, r = row0 + l32;
   const bool row_ok = r < M;
@@ -219,78 +249,70 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       v_lane[db] = (uint32_t)(KB * KROW + key * VROW + (((4 * db + low) ^ v_swizzle(key)) * 16) + 8 * (i & 1));
   }
 
-  uint4 piece[NP];
-  uint32_t scale[NP], paged = 0;  // paged: bit u, piece u's tokens have a page (the wave's)
-  auto fetch = [&](int key0) __attribute__((always_inline)) {
-    paged = 0;
+  // V is 0 behind the part's end and without a page and, in the tiles that reach the new tokens, where it is not finite; K's rows
+  // there may be anything, their scores are masked.
+  uint32_t k_put[NU], v_put[NU];  // where this thread's pieces go
 #pragma unroll
-    for (int u = 0; u < NP; ++u) {
-      const int i = u * T + rw * 64;  // the wave's first piece
-      const bool is_v = i >= PIECES;
-      const int key = min(key0 + (is_v ? i - PIECES : i) / CPK, end - 1), found = trow[key >> pg.log2_page];
-      const bool ok = (unsigned)found < (unsigned)pg.pages;
-      paged |= (uint32_t)ok << u;
-      // the 16 tokens from a multiple of 16 on lie in one page: loads behind the part's end read rows that exist
-      const int64_t p = ok ? found : 0;
-      const int row = pg.row_in_page(hkv, key & -(64 / CPK));
-      piece[u] = *(const uint4*)((is_v ? pg.v : pg.k) + p * pg.page_bytes + (int64_t)row * (CPK * 16) + lane * 16);
-      if constexpr (FMT == kPageE4M3)
-        scale[u] = ((is_v ? pg.vs : pg.ks) + p * pg.scale_bytes + (int64_t)row * (D / 32))[lane / CPK * (D / 32) + lane % CPK / 2];
-    }
-  };
-  uint64_t odd = 0, gone = 0;  // keys of the tile whose V is not finite somewhere; that have no page
-  // Rows behind the part's end are 0; so is V where it is not finite (its products with p = 0 must stay 0), and keys without a
-  // page.
+  for (int u = 0; u < NU; ++u) {
+    const int j = (u * RW + rw) * KPW + lane / CPK, c = lane % CPK;
+    k_put[u] = (uint32_t)(j * KROW + c * CHUNKS * 16);
+    v_put[u] = (uint32_t)(KB * KROW + j * VROW + ((c * CHUNKS) ^ v_swizzle(j)) * 16);
+  }
   auto put = [&](int key0, int buf, int slot) __attribute__((always_inline)) {
     unsigned char* const at = group + buf * TILE;
-    uint64_t odd_here = 0, gone_here = 0;
+    if (key0 + KB > clear || key0 + KB > end || paged != (1u << NU) - 1u) {  // the last tiles, and the rare ones
+      uint64_t gone = 0;
+      bool odd = false;
 #pragma unroll
-    for (int u = 0; u < NP; ++u) {
-      const int i = u * T + rw * 64;
-      const bool is_v = i >= PIECES, there = (paged >> u) & 1u;
-      const int j0 = (is_v ? i - PIECES : i) / CPK, j = j0 + lane / CPK, c = lane % CPK;
-      const bool ok = there && key0 + j < end;
-      uint4 w = piece[u];
-      bool bad = false;
-      if constexpr (FMT == kPageE4M3) bad = scale[u] == 255u;
-      if (is_v) {
-        bad |= unusual<FMT>(w);
-        uint64_t lanes = __ballot(ok && bad);
-        while (lanes) {  // wave-uniform, rare
-          odd_here |= 1ull << (j0 + __builtin_ctzll(lanes) / CPK);
-          lanes &= lanes - 1;
-        }
-        if (bad) w = make_uint4(0, 0, 0, 0);
-      } else if (!there) {
-        gone_here |= low_bits(64 / CPK) << j0;
+      for (int u = 0; u < NU; ++u) {
+        const int j0 = (u * RW + rw) * KPW;
+        const bool ok = ((paged >> u) & 1u) && key0 + j0 + lane / CPK < end;
+        const bool bad = ok && key0 + KB > clear && (FMT == kPageE4M3 ? vsc[u] == 255u : not_finite(vp[u]));
+        odd |= bad;
+        if (!((paged >> u) & 1u)) gone |= low_bits(KPW) << j0;
+        if (bad || !ok) vp[u] = make_uint4(0, 0, 0, 0);
+        if (FMT == kPageE4M3 && (bad || !ok)) vsc[u] = 127u;
       }
-      if (!ok) w = make_uint4(0, 0, 0, 0);
-      unsigned char* dst = is_v ? at + KB * KROW + j * VROW : at + j * KROW;
-      const int c0 = is_v ? (c * CHUNKS) ^ v_swizzle(j) : c * CHUNKS;
-      if constexpr (FMT == kPageE4M3) {
-        uint4 lo, hi;
-        expand16(w, bad || !ok ? 127u : scale[u], lo, hi);
-        if (!is_v && ok && bad) lo = hi = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-        *(uint4*)(dst + c0 * 16) = lo;
-        *(uint4*)(dst + c0 * 16 + 16) = hi;
-      } else {
-        *(uint4*)(dst + c0 * 16) = w;
+      if (__any(odd) && lane == 0) odd_any = 1;
+      if (gone && lane == 0) {
+        atomicOr((unsigned long long*)&no_page[slot][kw], gone);
+        gone_any[slot][kw] = 1;
       }
     }
-    if constexpr (RW == 1) {
-      odd = odd_here;
-      gone = gone_here;
-    } else if (odd_here | gone_here) {
-      if (lane == 0) {
-        atomicOr((unsigned long long*)&odd_keys[slot][kw], odd_here);
-        atomicOr((unsigned long long*)&no_page[slot][kw], gone_here);
+    if constexpr (FMT == kPageE4M3) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) most = max(most, max(ksc[u], vsc[u]));
+      if (__any(most == 255u)) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {  // NaN blocks
+          if (ksc[u] == 255u) kp[u] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), ksc[u] = 127u;
+          if (vsc[u] == 255u) vp[u] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), vsc[u] = 127u;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      if constexpr (FMT == kPageE4M3) {
+        uint4 lo, hi;
+        expand16(kp[u], ksc[u], lo, hi);
+        *(uint4*)(at + k_put[u]) = lo;
+        *(uint4*)(at + k_put[u] + 16) = hi;
+        expand16(vp[u], vsc[u], lo, hi);
+        *(uint4*)(at + v_put[u]) = lo;
+        *(uint4*)(at + v_put[u] + 16) = hi;
+      } else {
+        *(uint4*)(at + k_put[u]) = kp[u];
+        *(uint4*)(at + v_put[u]) = vp[u];
       }
     }
   };
 
   auto compute = [&](int first, int buf, int slot) __attribute__((always_inline)) {
     const unsigned char* const at = group + buf * TILE;
+    const int is_gone = __builtin_amdgcn_readfirstlane(gone_any[slot][kw]);
     bf16x8 fr[NB * NS];
+    // all K fragments before the first MFMA (one LDS latency)
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -304,14 +326,10 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       for (int s = 0; s < NS; ++s)
         sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[kb * NS + s], qf[s], sc[kb], 0, 0, 0);
     }
-    if constexpr (RW > 1) {
-      odd = odd_keys[slot][kw];
-      gone = no_page[slot][kw];
-    }
-    const uint64_t sees = a.anc ? seen_mask(s0 - first, bits) : low_bits(s0 + qn + 1 - first);
-    const uint64_t allowed = sees & low_bits(end - first) & ~gone;
-    if (first + KB > s0 || first + KB > end || gone) {
-      const uint64_t mine = allowed >> (g * 4);
+    if (first + KB > clear || first + KB > end || is_gone) {
+      uint64_t sees = (a.anc ? seen_mask(s0 - first, bits) : low_bits(s0 + qn + 1 - first)) & low_bits(end - first);
+      if (is_gone) sees &= ~no_page[slot][kw];
+      const uint64_t mine = sees >> (g * 4);
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -339,83 +357,66 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     }
     const float m_sub = m_run == -INFINITY ? 0.0f : m_run;
     float psum = l_run;
-    bf16x8 pf[NB][2], lo[TWO ? NB : 1][2];
+    bf16x8 pf[NB][2];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        uint32_t packed[4], rest[4];
+        uint32_t packed[4];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j], sl2, -m_sub));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j + 1], sl2, -m_sub));
           packed[j / 2] = fg::pack_bf16x2(p0, p1);
-          if constexpr (TWO) {
-            psum += p0 + p1;
-            rest[j / 2] = fg::pack_bf16x2(p0 - __uint_as_float(packed[j / 2] << 16),
-                                          p1 - __uint_as_float(packed[j / 2] & 0xffff0000u));
-          } else {
-            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
-          }
+          psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
         }
         pf[kb][ks] = __builtin_bit_cast(bf16x8, make_uint4(packed[0], packed[1], packed[2], packed[3]));
-        if constexpr (TWO) lo[kb][ks] = __builtin_bit_cast(bf16x8, make_uint4(rest[0], rest[1], rest[2], rest[3]));
       }
     l_run = psum;
 #pragma unroll
     for (int db = 0; db < ND; ++db)
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const unsigned char* p0 = at + v_lane[db] + (kb * 2 + ks) * 16 * VROW;
-          const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
-          const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
-          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[kb][ks], o[db], 0, 0, 0);
-          if constexpr (TWO) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo[kb][ks], o[db], 0, 0, 0);
-        }
-    // Infinities and NaN of V reach only the rows that see their key.
-    while (odd) {
-      const int j = __builtin_ctzll(odd), key = first + j;
-      odd &= odd - 1;
-      add_unusual<FMT, D>(pg, trow[key >> pg.log2_page], pg.row_in_page(hkv, key), lane, (allowed >> j) & 1ull, o);
-    }
+      for (int ks = 0; ks < 2 * NB; ++ks) {
+        const unsigned char* p0 = at + v_lane[db] + ks * 16 * VROW;
+        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
+        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[ks >> 1][ks & 1], o[db], 0, 0, 0);
+      }
   };
 
-  const int tiles = (end - begin + KB - 1) / KB;  // group kw takes tiles kw, kw + KW, ..
-  const int mine = (tiles - kw + KW - 1) / KW;
-  auto key_of = [&](int t) { return begin + (t * KW + kw) * KB; };
-  if constexpr (RW == 1) {
-    if (mine > 0) fetch(key_of(0));
-    for (int t = 0; t < mine; ++t) {
-      put(key_of(t), 0, 0);
-      if (t + 1 < mine) fetch(key_of(t + 1));
-      tile_barrier<RW>();
-      compute(key_of(t), 0, 0);
-      tile_barrier<RW>();
-    }
-  } else {
-    const int turns = (tiles + KW - 1) / KW;  // the same for every wave: the barriers are the workgroup's
-    if (tid < 3 * KW) (&odd_keys[0][0])[tid] = 0, (&no_page[0][0])[tid] = 0;
-    if (mine > 0) fetch(key_of(0));
-    __syncthreads();
+  if (tid < 3 * KW) (&no_page[0][0])[tid] = 0, (&gone_any[0][0])[tid] = 0;
+  if (tid == 0) odd_any = 0;
+  __syncthreads();
+  if (tiles) {
     if (mine > 0) put(key_of(0), 0, 0);
-    if (mine > 1) fetch(key_of(1));
-    __syncthreads();
-    int slot = 0;
-    for (int t = 0; t < turns; ++t) {
-      const int next = slot == 2 ? 0 : slot + 1;
-      if (t + 1 < mine) put(key_of(t + 1), (t + 1) & 1, next);
-      if (t + 2 < mine) fetch(key_of(t + 2));
-      if (t < mine && row0 < M) compute(key_of(t), t & 1, slot);
-      // the bits of tile t - 1 become those of tile t + 2, which are written behind the next barrier
-      const int old = next == 2 ? 0 : next + 1;
-      if (tid < KW) odd_keys[old][tid] = 0, no_page[old][tid] = 0;
-      __syncthreads();
-      slot = next;
-    }
+    fetch(key_of(1));
   }
+  __syncthreads();
+  int slot = 0;
+  for (int t = 0; t < turns; ++t) {
+    const int next = slot == 2 ? 0 : slot + 1;
+    if (t + 1 < mine) put(key_of(t + 1), (t + 1) & 1, next);
+    fetch(key_of(t + 2));
+    if (t < mine && row0 < M) compute(key_of(t), t & 1, slot);
+    // the bits of tile t - 1 become those of tile t + 2, which are written behind the next barrier
+    const int old = next == 2 ? 0 : next + 1;
+    if (tid < KW) no_page[old][tid] = 0, gone_any[old][tid] = 0;
+    __syncthreads();
+    slot = next;
+  }
+  if (odd_any && row0 < M)
+    each_unusual<FMT, D>(pg, trow, hkv, lane, max(begin, clear - KB), end, [&](int page, int row, int key) {
+      if ((key - begin) / KB % KW != kw) return;  // (the group that met the key: the others' m may be -inf)
+      const bool sees = key < s0 || (a.anc ? (bits >> (key - s0)) & 1ull : key - s0 <= qn);
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = v_element<FMT, D>(pg, page, row, db * 32 + c_row32(i, lane));
+          if (sees && !(fabsf(x) < INFINITY)) o[db][i] += x;
+        }
+    });
 
   float l = xor32_sum(l_run);
   if constexpr (KW > 1) {
@@ -501,7 +502,7 @@ FG_DEVICE float quad_sum(float x) {
 // row, the 16 at 16 gq; which d a k index stands for is free as long as Q follows, so K's rows go from memory through the
 // expansion into the MFMA's registers and never see LDS. V is expanded into a tile of LDS and read transposed. P goes to V in two
 // bf16 parts (hi + lo, p to 16 bits): what bounds the kernel is the stream.
-template <int FMT, int D, int NQ>
+template <int FMT, int D>
 struct StreamTile {  // a tile's loads: 32 keys
   static constexpr int kLoads = D * fg::page_elem_bytes<FMT> / 64;  // 16-byte loads of a lane per 16 keys
   uint4 k[2][kLoads], v[2 * kLoads];
@@ -510,12 +511,13 @@ struct StreamTile {  // a tile's loads: 32 keys
 };
 
 template <int FMT, int D, int NQ>
-__global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(PagedAttn a) {
+__global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(PagedAttn a) {
+  constexpr int W = kStreamWaves;
   constexpr int ES = fg::page_elem_bytes<FMT>, CPK = D * ES / 16, VROW = D * 2;
-  constexpr int NL = StreamTile<FMT, D, NQ>::kLoads, NS = D / 32, ND = D / 16, BLOCKS = D / fg::kMxBlock;
+  constexpr int NL = StreamTile<FMT, D>::kLoads, NS = D / 32, ND = D / 16, BLOCKS = D / fg::kMxBlock;
   constexpr int VTILE = 32 * VROW, OROW = D + 4;
-  constexpr int MERGE = 4 * NQ * 16 * (OROW * 4 + 8);
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4 * VTILE > MERGE ? 4 * VTILE : MERGE];
+  constexpr int MERGE = W * NQ * 16 * (OROW * 4 + 8);
+  __shared__ __attribute__((aligned(16))) unsigned char lds[W * VTILE > MERGE ? W * VTILE : MERGE];
   const Pages& pg = a.pages;
   const int unit = blockIdx.x;
   const int sp = unit % a.splits, hkv = unit / a.splits % pg.kv_heads, b = unit / (a.splits * pg.kv_heads);
@@ -528,34 +530,41 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
   const int begin = min(sp * part, keys), end = min(begin + part, keys);
   const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
   unsigned char* const vt = lds + wave * VTILE;
-  typedef StreamTile<FMT, D, NQ> Tile;
+  typedef StreamTile<FMT, D> Tile;
 
+  // A head's rows within a page, and those of its scales.
+  const uint32_t head_row = (uint32_t)hkv << pg.log2_page, slot_mask = (1u << pg.log2_page) - 1u;
+  const uint32_t k_lane = (uint32_t)(i16 * (D * ES) + gq * 16);
   auto fetch = [&](int key0, Tile& t) __attribute__((always_inline)) {
+    // Behind the part's end, and without a page, rows that exist are read and not used.
+    int found = trow[min(key0, end - 1) >> pg.log2_page];
     t.there = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = min(key0 + 16 * h, end - 1), found = trow[key >> pg.log2_page];
+      const int key = min(key0 + 16 * h, end - 1);
+      if (h && pg.log2_page == 4) found = trow[key >> 4];  // (tiles start at multiples of 32)
       const bool ok = (unsigned)found < (unsigned)pg.pages;
       t.there |= (int)ok << h;
-      const int64_t p = ok ? found : 0;  // behind the part's end, and without a page, rows that exist are read and not used
-      const int row = pg.row_in_page(hkv, key & -16);
-      const uint8_t* kr = pg.k + p * pg.page_bytes + (int64_t)row * (D * ES);
-      const uint8_t* vr = pg.v + p * pg.page_bytes + (int64_t)row * (D * ES);
+      const uint32_t row = head_row + ((uint32_t)key & slot_mask & ~15u);
+      const int64_t at = (ok ? found : 0) * pg.page_bytes + (int64_t)row * (D * ES);
+      const uint8_t* kr = pg.k + at;
+      const uint8_t* vr = pg.v + at;
 #pragma unroll
-      for (int s = 0; s < NL; ++s) t.k[h][s] = *(const uint4*)(kr + i16 * (D * ES) + s * 64 + gq * 16);
+      for (int s = 0; s < NL; ++s) t.k[h][s] = *(const uint4*)(kr + k_lane + s * 64);
 #pragma unroll
-      for (int s = 0; s < NL; ++s) t.v[h * NL + s] = *(const uint4*)(vr + s * 1024 + lane * 16);
+      for (int s = 0; s < NL; ++s) t.v[h * NL + s] = *(const uint4*)(vr + (uint32_t)lane * 16 + s * 1024);
       if constexpr (FMT == kPageE4M3) {
-        const uint8_t* ks = pg.ks + p * pg.scale_bytes + (int64_t)row * BLOCKS;
-        const uint8_t* vs = pg.vs + p * pg.scale_bytes + (int64_t)row * BLOCKS;
+        const int64_t sat = (ok ? found : 0) * pg.scale_bytes + (int64_t)row * BLOCKS;
+        const uint8_t* ks = pg.ks + sat;
+        const uint8_t* vs = pg.vs + sat;
         t.ks[h] = BLOCKS == 4 ? *(const uint32_t*)(ks + i16 * 4) : *(const uint16_t*)(ks + i16 * 2);
 #pragma unroll
         for (int s = 0; s < NL; ++s) t.vs[h * NL + s] = vs[s * (1024 / 32) + lane / 2];
       }
     }
   };
-  const int tiles = (end - begin + 31) / 32, mine = (tiles - wave + 3) / 4;
-  auto key_of = [&](int t) { return begin + (t * 4 + wave) * 32; };
+  const int tiles = (end - begin + 31) / 32, mine = (tiles - wave + W - 1) / W;
+  auto key_of = [&](int t) { return begin + (t * W + wave) * 32; };
   Tile cur;
   if (mine > 0) fetch(key_of(0), cur);
 
@@ -595,35 +604,55 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
   const int v_key = 4 * gq + (i16 >> 2);
   const uint32_t v_at = (uint32_t)(v_key * VROW + 8 * (i16 & 1)), v_x = (uint32_t)v_swizzle(v_key), v_low = (i16 & 3) >> 1;
 
+  int odd_from = end, odd_to = 0;  // the tokens among which V was kept at 0 where it is not finite
   for (int t = 0; t < mine; ++t) {
     const int first = key_of(t);
     // ---------------- V to LDS
-    uint64_t odd = 0;  // keys whose V is not finite somewhere; there it is 0, and so it is behind the end and without a page
-    const bool whole = first + 32 <= end && cur.there == 3;
+    // As in put() above, but that V in bf16 is looked at in every tile: P's lower part is 0 or negative too, which would make
+    // NaN of infinities.
+    bool look = first + 32 > end || cur.there != 3;
+    if constexpr (FMT == kPageE4M3) {
+      look |= first + 32 > s0;
+    } else {
+      uint32_t most = 0;
+#pragma unroll
+      for (int s = 0; s < 2 * NL; ++s) most = max_u16x2(most, largest_u16(cur.v[s]));
+      look |= __any((most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u);
+    }
+    if (look) {
+      bool odd = false;
+#pragma unroll
+      for (int s = 0; s < 2 * NL; ++s) {
+        const int j = s * (64 / CPK) + lane / CPK;
+        const bool ok = first + j < end && ((cur.there >> (j >> 4)) & 1);
+        const bool bad = ok && (FMT == kPageE4M3 ? first + 32 > s0 && cur.vs[s] == 255u : not_finite(cur.v[s]));
+        odd |= bad;
+        if (bad || !ok) cur.v[s] = make_uint4(0, 0, 0, 0);
+        if (FMT == kPageE4M3 && (bad || !ok)) cur.vs[s] = 127u;
+      }
+      if (__any(odd)) odd_from = min(odd_from, first), odd_to = min(first + 32, end);
+    }
+    if constexpr (FMT == kPageE4M3) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int s = 0; s < 2 * NL; ++s) most = max(most, cur.vs[s]);
+      if (__any(most == 255u)) {
+#pragma unroll
+        for (int s = 0; s < 2 * NL; ++s)  // NaN blocks
+          if (cur.vs[s] == 255u) cur.v[s] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), cur.vs[s] = 127u;
+      }
+    }
 #pragma unroll
     for (int s = 0; s < 2 * NL; ++s) {
       const int j = s * (64 / CPK) + lane / CPK, c = lane % CPK;
-      uint4 w = cur.v[s];
-      bool bad = unusual<FMT>(w);
-      uint32_t e = 127u;
-      if constexpr (FMT == kPageE4M3) e = cur.vs[s], bad |= e == 255u;
-      const bool ok = whole || (first + j < end && ((cur.there >> (j >> 4)) & 1));
-      if (__any(bad || !ok)) {
-        uint64_t lanes = __ballot(bad && ok);
-        while (lanes) {
-          odd |= 1ull << (s * (64 / CPK) + __builtin_ctzll(lanes) / CPK);
-          lanes &= lanes - 1;
-        }
-        if (bad || !ok) w = make_uint4(0, 0, 0, 0), e = 127u;
-      }
       if constexpr (FMT == kPageE4M3) {
         uint4 lo, hi;
-        expand16(w, e, lo, hi);
+        expand16(cur.v[s], cur.vs[s], lo, hi);
         unsigned char* dst = vt + j * VROW + ((2 * c) ^ v_swizzle(j)) * 16;
         *(uint4*)dst = lo;
         *(uint4*)(dst + 16) = hi;
       } else {
-        *(uint4*)(vt + j * VROW + (c ^ v_swizzle(j)) * 16) = w;
+        *(uint4*)(vt + j * VROW + (c ^ v_swizzle(j)) * 16) = cur.v[s];
       }
     }
     // ---------------- S^T
@@ -636,10 +665,13 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
       for (int s = 0; s < NL; ++s) {
         uint4 part[2];
         if constexpr (FMT == kPageE4M3) {
-          uint32_t e = (cur.ks[h] >> (8 * (2 * s + (gq >> 1)))) & 255u;
-          uint4 w = cur.k[h][s];
-          if (__any(e == 255u) && e == 255u) w = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), e = 127u;  // NaN
-          expand16(w, e, part[0], part[1]);
+          const uint32_t e = __builtin_amdgcn_ubfe(cur.ks[h], (uint32_t)(16 * s + 8 * (gq >> 1)), 8u);
+          expand16(cur.k[h][s], e, part[0], part[1]);
+          if (__any(e == 255u)) {  // a NaN block
+            const uint32_t nan = e == 255u ? 0x7fc07fc0u : 0u;
+            part[0] = make_uint4(part[0].x | nan, part[0].y | nan, part[0].z | nan, part[0].w | nan);
+            part[1] = make_uint4(part[1].x | nan, part[1].y | nan, part[1].z | nan, part[1].w | nan);
+          }
 #pragma unroll
           for (int c = 0; c < NQ; ++c)
 #pragma unroll
@@ -652,16 +684,15 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
         }
       }
     const uint64_t gone = (cur.there & 1 ? 0ull : 0xffffull) | (cur.there & 2 ? 0ull : 0xffff0000ull);
-    if (t + 1 < mine) fetch(key_of(t + 1), cur);
+    fetch(key_of(t + 1), cur);  // (past the last tile: rows that exist, not used)
     // ---------------- softmax
     const bool masked = first + 32 > s0 || first + 32 > end || gone;
-    uint64_t allowed[NQ];
     bf16x8 hi[NQ], lo[NQ];
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-      allowed[c] = (a.anc ? seen_mask(s0 - first, bits[c]) : low_bits(s0 + qn[c] + 1 - first)) & low_bits(end - first) & ~gone;
       if (masked) {
-        const uint64_t at = allowed[c] >> (4 * gq);
+        const uint64_t sees = (a.anc ? seen_mask(s0 - first, bits[c]) : low_bits(s0 + qn[c] + 1 - first)) & low_bits(end - first) & ~gone;
+        const uint64_t at = sees >> (4 * gq);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -696,7 +727,7 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
       lo[c] = __builtin_bit_cast(bf16x8, make_uint4(pl[0], pl[1], pl[2], pl[3]));
     }
     // ---------------- O^T += V^T P^T
-    tile_barrier<1>();
+    wave_barrier();
 #pragma unroll
     for (int db = 0; db < ND; ++db) {
       const unsigned char* at = vt + v_at + (((2 * db + v_low) ^ v_x) * 16);
@@ -709,27 +740,27 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
         o[c][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[c], o[c][db], 0, 0, 0);
       }
     }
-    while (odd) {  // infinities and NaN of V reach only the rows that see their key
-      const int j = __builtin_ctzll(odd), key = first + j;
-      odd &= odd - 1;
-      const int page = trow[key >> pg.log2_page], row = pg.row_in_page(hkv, key);
+    wave_barrier();
+  }
+  if (odd_from < odd_to)
+    each_unusual<FMT, D>(pg, trow, hkv, lane, odd_from, odd_to, [&](int page, int row, int key) {
+      if ((key - begin) / 32 % W != wave) return;  // (the wave that met the key: the others' m may be -inf)
 #pragma unroll
-      for (int c = 0; c < NQ; ++c)
+      for (int c = 0; c < NQ; ++c) {
+        const bool sees = key < s0 || (a.anc ? (bits[c] >> (key - s0)) & 1ull : key - s0 <= qn[c]);
 #pragma unroll
         for (int db = 0; db < ND; ++db)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = v_element<FMT, D>(pg, page, row, 16 * db + 4 * gq + i);
-            o[c][db][i] += ((allowed[c] >> j) & 1ull) && !(fabsf(x) < INFINITY) ? x : 0.0f;
-            __builtin_amdgcn_sched_barrier(0);
+            if (sees && !(fabsf(x) < INFINITY)) o[c][db][i] += x;
           }
-    }
-    tile_barrier<1>();
-  }
+      }
+    });
 
   // ---------------- merge the waves
   float* om = (float*)lds;
-  float2* ml = (float2*)(lds + 4 * NQ * 16 * OROW * 4);
+  float2* ml = (float2*)(lds + W * NQ * 16 * OROW * 4);
   __syncthreads();
 #pragma unroll
   for (int c = 0; c < NQ; ++c) {
@@ -740,14 +771,14 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
     if (gq == 0) ml[at] = make_float2(m_run[c], l);
   }
   __syncthreads();
-  for (int e = tid; e < M * (D / 4); e += 256) {
+  for (int e = tid; e < M * (D / 4); e += W * 64) {
     const int r = e / (D / 4), d0 = e % (D / 4) * 4;
     float mx = -INFINITY, den = 0.0f, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w * NQ * 16 + r].x);
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, ml[w * NQ * 16 + r].x);
     const float sub = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const int at = w * NQ * 16 + r;
       const float f = __builtin_amdgcn_exp2f(ml[at].x - sub);
       const float4 x = *(const float4*)(om + at * OROW + d0);
@@ -767,36 +798,60 @@ __global__ void __launch_bounds__(256, NQ == 1 ? 3 : 2) paged_stream_kernel(Page
   }
 }
 
-// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims. A row has SLOTS groups of
-// D / 4 lanes, each with every SLOTS-th part, and a workgroup 256 / (SLOTS D / 4) rows. A lane p < parts of each wave reads part
-// p's (m, l) in one round trip and the loads of O do not wait for each other: 64 parts of 64 rows take 5 us, in one
-// loop over the parts 26.
-template <int D, int SLOTS>
+// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims of a part. Up to 8 parts: D / 4
+// threads a row. More (WIDE): a workgroup a row, 1024 / D parts side by side. A thread reads a part's (m, l), so that all
+// of them take one round trip, and no load of O waits for another.
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int tile) {
-  constexpr int LANES = D / 4, PER = 256 / (LANES * SLOTS);
-  __shared__ float4 sums[SLOTS > 1 ? 256 : 1];
-  const int slot = threadIdx.x / LANES % SLOTS, lane = threadIdx.x & 63, d0 = threadIdx.x % LANES * 4;
+  constexpr int LANES = D / 4, SLOTS = WIDE ? 256 / LANES : 1, PER = 256 / (LANES * SLOTS), MOST = WIDE ? kMaxParts : 8;
+  __shared__ float weight[PER][MOST], wave_at[8];
+  __shared__ float4 sums[WIDE ? 256 : 1];
+  const int ti = threadIdx.x % (LANES * SLOTS), in = threadIdx.x / (LANES * SLOTS), slot = ti / LANES, d0 = ti % LANES * 4;
   const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
-  const int64_t row = min((int64_t)blockIdx.x * PER + threadIdx.x / (LANES * SLOTS), rows - 1);  // (a row past the last: again)
+  const int64_t row = min((int64_t)blockIdx.x * PER + in, rows - 1);  // (behind the last row: it once more)
   const int n = (int)(row / a.Hq % a.N), b = (int)(row / a.Hq / a.N);
   const Span seq = span_of(a, b);
   const int keys = keys_of(a, seq), part = part_keys(keys, a.splits, tile);
   const int parts = part > 0 && n < seq.fresh ? min(a.splits, (keys + part - 1) / part) : 0;
+  const float2 ml = ti < parts ? a.ml_part[ti * rows + row] : make_float2(-INFINITY, 0.0f);
+  float mx = ml.x, den;
+  if constexpr (WIDE) {
+    static_assert(kMaxParts <= 256, "a thread per part");
+    mx = fg::wave_max(mx);
+    if ((threadIdx.x & 63) == 0) wave_at[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(wave_at[0], wave_at[1]), fmaxf(wave_at[2], wave_at[3]));
+  } else {
+#pragma unroll
+    for (int x = 4; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+    mx = __shfl(mx, (threadIdx.x & 63) / LANES * LANES, 64);
+  }
+  const float w = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
+  den = w * ml.y;
+  if (ti < MOST) weight[in][ti] = w;
+  if constexpr (WIDE) {
+    den = fg::wave_sum(den);
+    if ((threadIdx.x & 63) == 0) wave_at[4 + (threadIdx.x >> 6)] = den;
+    __syncthreads();
+    den = wave_at[4] + wave_at[5] + wave_at[6] + wave_at[7];
+  } else {
+#pragma unroll
+    for (int x = 4; x; x >>= 1) den += __shfl_xor(den, x, 64);
+    den = __shfl(den, (threadIdx.x & 63) / LANES * LANES, 64);
+    __syncthreads();
+  }
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float den = 0.0f;
-  if constexpr (SLOTS > 1) {  // a wave has one row
-    const float2 ml = lane < parts ? a.ml_part[lane * rows + row] : make_float2(-INFINITY, 0.0f);
-    const float mx = fg::wave_max(ml.x);
-    const float w = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
-    den = fg::wave_sum(w * ml.y);
-    static_assert(kMaxParts <= 64 && kMaxParts % SLOTS == 0, "a lane per part");
-#pragma unroll 4
-    for (int p0 = 0; p0 < parts; p0 += SLOTS) {  // all lanes stay: the weights come from other lanes
-      const int p = p0 + slot;
-      const float f = __shfl(w, p, 64);
-      const float4 x = *(const float4*)(a.o_part + (min(p, parts - 1) * rows + row) * D + d0);
-      if (f != 0.0f) o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+  for (int p0 = slot; p0 < parts; p0 += 4 * SLOTS) {
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = *(const float4*)(a.o_part + (min(p0 + u * SLOTS, parts - 1) * rows + row) * D + d0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = p0 + u * SLOTS < parts ? weight[in][p0 + u * SLOTS] : 0.0f;
+      if (f != 0.0f) o.x += f * x[u].x, o.y += f * x[u].y, o.z += f * x[u].z, o.w += f * x[u].w;
     }
+  }
+  if constexpr (WIDE) {
     sums[threadIdx.x] = o;
     __syncthreads();
     if (slot) return;
@@ -804,18 +859,6 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int til
     for (int s = 1; s < SLOTS; ++s) {
       const float4 x = sums[threadIdx.x + s * LANES];
       o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-    }
-  } else {
-    float mx = -INFINITY;
-    for (int p = 0; p < parts; ++p) mx = fmaxf(mx, a.ml_part[p * rows + row].x);
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      const float2 ml = a.ml_part[p * rows + row];
-      const float4 x = *(const float4*)(a.o_part + (p * rows + row) * D + d0);
-      if (ml.y == 0.0f) continue;
-      const float f = __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
-      den += f * ml.y;
-      o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
     }
   }
   if (n >= seq.fresh) return;
@@ -830,15 +873,15 @@ struct Plan {
   int tile() const { return kb; }
 };
 
-Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int64_t capacity) {
+Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int64_t capacity) {
   const int64_t m = (int64_t)(q_heads / kv_heads) * num_nodes;
   Plan p;
-  if (m <= 32) p = {1, 4, 32, 1};
+  if (m <= 32) p = {1, kStreamWaves, 32, 1};
   else if (m <= 64) p = {2, 2, 32, 1};
-  else if (m <= 128) p = {4, 1, 64, 1};
+  else if (m <= 128 || head_dim == 64) p = {4, 1, 64, 1};
   else p = {8, 1, 64, 1};
   const int64_t base = (int64_t)batch * kv_heads * ((m + p.rows() - 1) / p.rows());
-  const int64_t target = 256 * (8 / (p.rw * p.kw));
+  const int64_t target = p.rw * p.kw == 4 ? 512 : 256;
   if (base < target) {
     const int64_t most = std::max<int64_t>(1, capacity / kMinPartKeys);
     p.splits = (int)std::min<int64_t>(std::min<int64_t>((target + base - 1) / base, most), kMaxParts);
@@ -862,17 +905,17 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 2>), grid, block, 0, s, a);
   else if (p.rw == 2)
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 2, 32>), grid, block, 0, s, a, m_tiles);
-  else if (p.rw == 4)
+  else if (D == 64 || p.rw == 4)
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 1, 64>), grid, block, 0, s, a, m_tiles);
   else
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 8, 1, 64>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64>), grid, block, 0, s, a, m_tiles);
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
-    constexpr int SLOTS = 1024 / D;  // a workgroup's row
     if (a.splits > 8)
-      hipLaunchKernelGGL((paged_combine_kernel<D, SLOTS>), dim3((unsigned)rows), dim3(256), 0, s, a, p.tile());
+      hipLaunchKernelGGL((paged_combine_kernel<D, true>), dim3((unsigned)rows), dim3(256), 0, s, a, p.tile());
     else
-      hipLaunchKernelGGL((paged_combine_kernel<D, 1>), dim3((unsigned)((rows + SLOTS - 1) / SLOTS)), dim3(256), 0, s, a, p.tile());
+      hipLaunchKernelGGL((paged_combine_kernel<D, false>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, s, a,
+                         p.tile());
   }
 }
 
@@ -886,7 +929,7 @@ bool sizes_ok(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim)
 extern "C" size_t fg_paged_attention_workspace(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim,
                                                int capacity) {
   if (!sizes_ok(batch, num_nodes, q_heads, kv_heads, head_dim) || capacity <= 0) return 0;
-  return (size_t)workspace_of(plan_of(batch, num_nodes, q_heads, kv_heads, capacity), batch, num_nodes, q_heads, head_dim);
+  return (size_t)workspace_of(plan_of(batch, num_nodes, q_heads, kv_heads, head_dim, capacity), batch, num_nodes, q_heads, head_dim);
 }
 
 extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes,
@@ -910,7 +953,7 @@ extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* p
   a.N = num_nodes;
   a.Hq = q_heads;
   a.scale = scale;
-  Plan p = plan_of(batch, num_nodes, q_heads, pages->kv_heads, (int64_t)pages->table_width * pages->page_size);
+  Plan p = plan_of(batch, num_nodes, q_heads, pages->kv_heads, pages->head_dim, (int64_t)pages->table_width * pages->page_size);
   const int64_t need = workspace_of(p, batch, num_nodes, q_heads, pages->head_dim);
   if (need && (!workspace || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 15))) p.splits = 1;
   const int64_t m = (int64_t)(q_heads / pages->kv_heads) * num_nodes;
