@@ -19,6 +19,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef __attribute__((address_space(4))) int32_t const_i32;  // read by the scalar unit
 
@@ -86,17 +87,15 @@ FG_DEVICE int part_keys(int keys, int splits, int tile) {
 }
 
 // 16 e4m3 codes times 2^(s - 127) as bf16 (exact).
-FG_DEVICE void expand16(uint4 w, uint32_t s, uint4& lo, uint4& hi) {
+FG_DEVICE void expand16(u32x4 w, uint32_t s, u32x4& lo, u32x4& hi) {
   const float f = __uint_as_float(s << 23);
-  uint32_t r[8];
-  const uint32_t c[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], f, false));
-    r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], f, true));
+  for (int i = 0; i < 2; ++i) {
+    lo[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], f, false));
+    lo[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], f, true));
+    hi[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 + i], f, false));
+    hi[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 + i], f, true));
   }
-  lo = make_uint4(r[0], r[1], r[2], r[3]);
-  hi = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
 // bf16 values that are not finite have all exponent bits: as 15-bit numbers they are 0x7f80 or more.
@@ -104,11 +103,11 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 FG_DEVICE uint32_t max_u16x2(uint32_t x, uint32_t y) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
 }
-FG_DEVICE uint32_t largest_u16(uint4 w) {  // by halves
+FG_DEVICE uint32_t largest_u16(u32x4 w) {  // by halves
   constexpr uint32_t m = 0x7fff7fffu;
-  return max_u16x2(max_u16x2(w.x & m, w.y & m), max_u16x2(w.z & m, w.w & m));
+  return max_u16x2(max_u16x2(w[0] & m, w[1] & m), max_u16x2(w[2] & m, w[3] & m));
 }
-FG_DEVICE bool not_finite(uint4 w) {
+FG_DEVICE bool not_finite(u32x4 w) {
   const uint32_t x = largest_u16(w);
   return (x & 0xffffu) >= 0x7f80u || x >= 0x7f800000u;
 }
@@ -186,33 +185,51 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
   unsigned char* const group = lds + kw * 2 * TILE;
 
-  uint4 kp[NU], vp[NU];
-  uint32_t ksc[NU], vsc[NU], paged = 0;  // paged: bit u, the tokens of load u have a page
+  struct Loads {
+    u32x4 kp[NU], vp[NU];
+    uint32_t ksc[NU], vsc[NU], paged;  // paged: bit u, the tokens of load u have a page
+  };
+  constexpr int DEPTH = 2;  // tiles in flight
+  Loads ring[DEPTH];
   const uint32_t head_row = (uint32_t)hkv << pg.log2_page, slot_mask = (1u << pg.log2_page) - 1u;
   const uint32_t sc_lane = (uint32_t)(lane / CPK * BLOCKS + lane % CPK / 2);
-  auto fetch = [&](int key0) __attribute__((always_inline)) {
-    paged = 0;
+  // Page numbers are looked up a turn before they are needed, in front of its barrier: scalar loads come back in any order, so
+  // that a wait for LDS reads waits for one that is under way as well.
+  int page_of[NU];
+  auto lookup = [&](int key0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) page_of[u] = trow[min(key0 + (u * RW + rw) * KPW, end - 1) >> pg.log2_page];
+  };
+  auto fetch = [&](int key0, Loads& x) __attribute__((always_inline)) {
+    x.paged = 0;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       // Behind the part's end, and without a page, rows that exist are read and not used.
-      const int key = min(key0 + (u * RW + rw) * KPW, end - 1), found = trow[key >> pg.log2_page];
+      const int key = min(key0 + (u * RW + rw) * KPW, end - 1), found = page_of[u];
       const bool ok = (unsigned)found < (unsigned)pg.pages;
-      paged |= (uint32_t)ok << u;
+      x.paged |= (uint32_t)ok << u;
       const uint32_t row = head_row + ((uint32_t)key & slot_mask & ~(uint32_t)(KPW - 1));
       const int64_t at = (ok ? found : 0) * pg.page_bytes + (int64_t)row * (CPK * 16);
-      kp[u] = *(const uint4*)(pg.k + at + (uint32_t)lane * 16);
-      vp[u] = *(const uint4*)(pg.v + at + (uint32_t)lane * 16);
+      x.kp[u] = *(const u32x4*)(pg.k + at + (uint32_t)lane * 16);
+      x.vp[u] = *(const u32x4*)(pg.v + at + (uint32_t)lane * 16);
       if constexpr (FMT == kPageE4M3) {
         const int64_t sat = (ok ? found : 0) * pg.scale_bytes + (int64_t)row * BLOCKS;
-        ksc[u] = (pg.ks + sat)[sc_lane];
-        vsc[u] = (pg.vs + sat)[sc_lane];
+        x.ksc[u] = (pg.ks + sat)[sc_lane];
+        x.vsc[u] = (pg.vs + sat)[sc_lane];
       }
     }
   };
   const int tiles = (end - begin + KB - 1) / KB;  // group kw takes tiles kw, kw + KW, ..
   const int turns = (tiles + KW - 1) / KW, mine = (tiles - kw + KW - 1) / KW;  // (the barriers are the workgroup's)
   auto key_of = [&](int t) { return begin + (t * KW + kw) * KB; };
-  if (tiles) fetch(key_of(0));
+  if (tiles) {
+#pragma unroll
+    for (int x = 0; x < DEPTH; ++x) {
+      lookup(key_of(x));
+      fetch(key_of(x), ring[x]);
+    }
+    lookup(key_of(DEPTH));
+  }
 
   const int row0 = mt * ROWS + rw * 32, r = row0 + l32;
   const bool row_ok = r < M;
@@ -224,7 +241,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     const uint16_t* qrow = (const uint16_t*)a.q + (((int64_t)b * a.N + qn) * a.Hq + qh) * D;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
-      qf[s] = __builtin_bit_cast(bf16x8, row_ok ? *(const uint4*)(qrow + s * 16 + g * 8) : make_uint4(0, 0, 0, 0));
+      qf[s] = __builtin_bit_cast(bf16x8, row_ok ? *(const u32x4*)(qrow + s * 16 + g * 8) : u32x4(0));
   }
   floatx16 o[ND];
 #pragma unroll
@@ -258,20 +275,20 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     k_put[u] = (uint32_t)(j * KROW + c * CHUNKS * 16);
     v_put[u] = (uint32_t)(KB * KROW + j * VROW + ((c * CHUNKS) ^ v_swizzle(j)) * 16);
   }
-  auto put = [&](int key0, int buf, int slot) __attribute__((always_inline)) {
+  auto put = [&](int key0, int buf, int slot, Loads& x) __attribute__((always_inline)) {
     unsigned char* const at = group + buf * TILE;
-    if (key0 + KB > clear || key0 + KB > end || paged != (1u << NU) - 1u) {  // the last tiles, and the rare ones
+    if (key0 + KB > clear || key0 + KB > end || x.paged != (1u << NU) - 1u) {  // the last tiles, and the rare ones
       uint64_t gone = 0;
       bool odd = false;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const int j0 = (u * RW + rw) * KPW;
-        const bool ok = ((paged >> u) & 1u) && key0 + j0 + lane / CPK < end;
-        const bool bad = ok && key0 + KB > clear && (FMT == kPageE4M3 ? vsc[u] == 255u : not_finite(vp[u]));
+        const bool ok = ((x.paged >> u) & 1u) && key0 + j0 + lane / CPK < end;
+        const bool bad = ok && key0 + KB > clear && (FMT == kPageE4M3 ? x.vsc[u] == 255u : not_finite(x.vp[u]));
         odd |= bad;
-        if (!((paged >> u) & 1u)) gone |= low_bits(KPW) << j0;
-        if (bad || !ok) vp[u] = make_uint4(0, 0, 0, 0);
-        if (FMT == kPageE4M3 && (bad || !ok)) vsc[u] = 127u;
+        if (!((x.paged >> u) & 1u)) gone |= low_bits(KPW) << j0;
+        if (bad || !ok) x.vp[u] = u32x4(0);
+        if (FMT == kPageE4M3 && (bad || !ok)) x.vsc[u] = 127u;
       }
       if (__any(odd) && lane == 0) odd_any = 1;
       if (gone && lane == 0) {
@@ -282,28 +299,28 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     if constexpr (FMT == kPageE4M3) {
       uint32_t most = 0;
 #pragma unroll
-      for (int u = 0; u < NU; ++u) most = max(most, max(ksc[u], vsc[u]));
+      for (int u = 0; u < NU; ++u) most = max(most, max(x.ksc[u], x.vsc[u]));
       if (__any(most == 255u)) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {  // NaN blocks
-          if (ksc[u] == 255u) kp[u] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), ksc[u] = 127u;
-          if (vsc[u] == 255u) vp[u] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), vsc[u] = 127u;
+          if (x.ksc[u] == 255u) x.kp[u] = u32x4(0x7f7f7f7fu), x.ksc[u] = 127u;
+          if (x.vsc[u] == 255u) x.vp[u] = u32x4(0x7f7f7f7fu), x.vsc[u] = 127u;
         }
       }
     }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       if constexpr (FMT == kPageE4M3) {
-        uint4 lo, hi;
-        expand16(kp[u], ksc[u], lo, hi);
-        *(uint4*)(at + k_put[u]) = lo;
-        *(uint4*)(at + k_put[u] + 16) = hi;
-        expand16(vp[u], vsc[u], lo, hi);
-        *(uint4*)(at + v_put[u]) = lo;
-        *(uint4*)(at + v_put[u] + 16) = hi;
+        u32x4 lo, hi;
+        expand16(x.kp[u], x.ksc[u], lo, hi);
+        *(u32x4*)(at + k_put[u]) = lo;
+        *(u32x4*)(at + k_put[u] + 16) = hi;
+        expand16(x.vp[u], x.vsc[u], lo, hi);
+        *(u32x4*)(at + v_put[u]) = lo;
+        *(u32x4*)(at + v_put[u] + 16) = hi;
       } else {
-        *(uint4*)(at + k_put[u]) = kp[u];
-        *(uint4*)(at + v_put[u]) = vp[u];
+        *(u32x4*)(at + k_put[u]) = x.kp[u];
+        *(u32x4*)(at + v_put[u]) = x.vp[u];
       }
     }
   };
@@ -370,13 +387,13 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
           packed[j / 2] = fg::pack_bf16x2(p0, p1);
           psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
         }
-        pf[kb][ks] = __builtin_bit_cast(bf16x8, make_uint4(packed[0], packed[1], packed[2], packed[3]));
+        pf[kb][ks] = __builtin_bit_cast(bf16x8, u32x4{packed[0], packed[1], packed[2], packed[3]});
       }
     l_run = psum;
 #pragma unroll
-    for (int db = 0; db < ND; ++db)
+    for (int ks = 0; ks < 2 * NB; ++ks)
 #pragma unroll
-      for (int ks = 0; ks < 2 * NB; ++ks) {
+      for (int db = 0; db < ND; ++db) {
         const unsigned char* p0 = at + v_lane[db] + ks * 16 * VROW;
         const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
         const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
@@ -389,21 +406,28 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   if (tid == 0) odd_any = 0;
   __syncthreads();
   if (tiles) {
-    if (mine > 0) put(key_of(0), 0, 0);
-    fetch(key_of(1));
+    if (mine > 0) put(key_of(0), 0, 0, ring[0]);
+    fetch(key_of(DEPTH), ring[0]);
+    lookup(key_of(DEPTH + 1));
   }
   __syncthreads();
   int slot = 0;
-  for (int t = 0; t < turns; ++t) {
+  auto turn = [&](int t, Loads& x) __attribute__((always_inline)) {
     const int next = slot == 2 ? 0 : slot + 1;
-    if (t + 1 < mine) put(key_of(t + 1), (t + 1) & 1, next);
-    fetch(key_of(t + 2));
+    if (t + 1 < mine) put(key_of(t + 1), (t + 1) & 1, next, x);
+    fetch(key_of(t + 1 + DEPTH), x);
     if (t < mine && row0 < M) compute(key_of(t), t & 1, slot);
     // the bits of tile t - 1 become those of tile t + 2, which are written behind the next barrier
     const int old = next == 2 ? 0 : next + 1;
     if (tid < KW) no_page[old][tid] = 0, gone_any[old][tid] = 0;
+    lookup(key_of(t + 2 + DEPTH));
     __syncthreads();
     slot = next;
+  };
+  for (int t = 0; t < turns;) {
+    turn(t++, ring[1]);
+    if (t == turns) break;
+    turn(t++, ring[0]);
   }
   if (odd_any && row0 < M)
     each_unusual<FMT, D>(pg, trow, hkv, lane, max(begin, clear - KB), end, [&](int page, int row, int key) {
@@ -505,7 +529,7 @@ FG_DEVICE float quad_sum(float x) {
 template <int FMT, int D>
 struct StreamTile {  // a tile's loads: 32 keys
   static constexpr int kLoads = D * fg::page_elem_bytes<FMT> / 64;  // 16-byte loads of a lane per 16 keys
-  uint4 k[2][kLoads], v[2 * kLoads];
+  u32x4 k[2][kLoads], v[2 * kLoads];
   uint32_t ks[2], vs[2 * kLoads];  // scales: of K's key all four, of a piece of V its own
   int there;                       // bit h: keys 16 h .. have a page
 };
@@ -535,14 +559,17 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   // A head's rows within a page, and those of its scales.
   const uint32_t head_row = (uint32_t)hkv << pg.log2_page, slot_mask = (1u << pg.log2_page) - 1u;
   const uint32_t k_lane = (uint32_t)(i16 * (D * ES) + gq * 16);
+  int page_of[2];  // of the next tile's two times 16 tokens: looked up a turn ahead
+  auto lookup = [&](int key0) __attribute__((always_inline)) {
+    page_of[0] = trow[min(key0, end - 1) >> pg.log2_page];
+    page_of[1] = trow[min(key0 + 16, end - 1) >> pg.log2_page];
+  };
   auto fetch = [&](int key0, Tile& t) __attribute__((always_inline)) {
     // Behind the part's end, and without a page, rows that exist are read and not used.
-    int found = trow[min(key0, end - 1) >> pg.log2_page];
     t.there = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = min(key0 + 16 * h, end - 1);
-      if (h && pg.log2_page == 4) found = trow[key >> 4];  // (tiles start at multiples of 32)
+      const int key = min(key0 + 16 * h, end - 1), found = page_of[h];
       const bool ok = (unsigned)found < (unsigned)pg.pages;
       t.there |= (int)ok << h;
       const uint32_t row = head_row + ((uint32_t)key & slot_mask & ~15u);
@@ -550,9 +577,9 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
       const uint8_t* kr = pg.k + at;
       const uint8_t* vr = pg.v + at;
 #pragma unroll
-      for (int s = 0; s < NL; ++s) t.k[h][s] = *(const uint4*)(kr + k_lane + s * 64);
+      for (int s = 0; s < NL; ++s) t.k[h][s] = *(const u32x4*)(kr + k_lane + s * 64);
 #pragma unroll
-      for (int s = 0; s < NL; ++s) t.v[h * NL + s] = *(const uint4*)(vr + (uint32_t)lane * 16 + s * 1024);
+      for (int s = 0; s < NL; ++s) t.v[h * NL + s] = *(const u32x4*)(vr + (uint32_t)lane * 16 + s * 1024);
       if constexpr (FMT == kPageE4M3) {
         const int64_t sat = (ok ? found : 0) * pg.scale_bytes + (int64_t)row * BLOCKS;
         const uint8_t* ks = pg.ks + sat;
@@ -566,7 +593,11 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   const int tiles = (end - begin + 31) / 32, mine = (tiles - wave + W - 1) / W;
   auto key_of = [&](int t) { return begin + (t * W + wave) * 32; };
   Tile cur;
-  if (mine > 0) fetch(key_of(0), cur);
+  if (mine > 0) {
+    lookup(key_of(0));
+    fetch(key_of(0), cur);
+    lookup(key_of(1));
+  }
 
   int qn[NQ], qh[NQ];
   bool row_ok[NQ];
@@ -584,7 +615,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
     for (int s = 0; s < NS; ++s) {
       // the d of k-step s: e4m3: 8 of the 16 codes of load s / 2, bf16: the 8 elements of load s
       const int d = FMT == kPageE4M3 ? s / 2 * 64 + gq * 16 + s % 2 * 8 : s * 32 + gq * 8;
-      qf[c][s] = __builtin_bit_cast(bf16x8, row_ok[c] ? *(const uint4*)(qrow + d) : make_uint4(0, 0, 0, 0));
+      qf[c][s] = __builtin_bit_cast(bf16x8, row_ok[c] ? *(const u32x4*)(qrow + d) : u32x4(0));
     }
   }
   floatx4 o[NQ][ND];
@@ -627,7 +658,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
         const bool ok = first + j < end && ((cur.there >> (j >> 4)) & 1);
         const bool bad = ok && (FMT == kPageE4M3 ? first + 32 > s0 && cur.vs[s] == 255u : not_finite(cur.v[s]));
         odd |= bad;
-        if (bad || !ok) cur.v[s] = make_uint4(0, 0, 0, 0);
+        if (bad || !ok) cur.v[s] = u32x4(0);
         if (FMT == kPageE4M3 && (bad || !ok)) cur.vs[s] = 127u;
       }
       if (__any(odd)) odd_from = min(odd_from, first), odd_to = min(first + 32, end);
@@ -639,20 +670,20 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
       if (__any(most == 255u)) {
 #pragma unroll
         for (int s = 0; s < 2 * NL; ++s)  // NaN blocks
-          if (cur.vs[s] == 255u) cur.v[s] = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu), cur.vs[s] = 127u;
+          if (cur.vs[s] == 255u) cur.v[s] = u32x4(0x7f7f7f7fu), cur.vs[s] = 127u;
       }
     }
 #pragma unroll
     for (int s = 0; s < 2 * NL; ++s) {
       const int j = s * (64 / CPK) + lane / CPK, c = lane % CPK;
       if constexpr (FMT == kPageE4M3) {
-        uint4 lo, hi;
+        u32x4 lo, hi;
         expand16(cur.v[s], cur.vs[s], lo, hi);
         unsigned char* dst = vt + j * VROW + ((2 * c) ^ v_swizzle(j)) * 16;
-        *(uint4*)dst = lo;
-        *(uint4*)(dst + 16) = hi;
+        *(u32x4*)dst = lo;
+        *(u32x4*)(dst + 16) = hi;
       } else {
-        *(uint4*)(vt + j * VROW + (c ^ v_swizzle(j)) * 16) = cur.v[s];
+        *(u32x4*)(vt + j * VROW + (c ^ v_swizzle(j)) * 16) = cur.v[s];
       }
     }
     // ---------------- S^T
@@ -663,14 +694,14 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int s = 0; s < NL; ++s) {
-        uint4 part[2];
+        u32x4 part[2];
         if constexpr (FMT == kPageE4M3) {
           const uint32_t e = __builtin_amdgcn_ubfe(cur.ks[h], (uint32_t)(16 * s + 8 * (gq >> 1)), 8u);
           expand16(cur.k[h][s], e, part[0], part[1]);
           if (__any(e == 255u)) {  // a NaN block
             const uint32_t nan = e == 255u ? 0x7fc07fc0u : 0u;
-            part[0] = make_uint4(part[0].x | nan, part[0].y | nan, part[0].z | nan, part[0].w | nan);
-            part[1] = make_uint4(part[1].x | nan, part[1].y | nan, part[1].z | nan, part[1].w | nan);
+            part[0] |= u32x4(nan);
+            part[1] |= u32x4(nan);
           }
 #pragma unroll
           for (int c = 0; c < NQ; ++c)
@@ -685,6 +716,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
       }
     const uint64_t gone = (cur.there & 1 ? 0ull : 0xffffull) | (cur.there & 2 ? 0ull : 0xffff0000ull);
     fetch(key_of(t + 1), cur);  // (past the last tile: rows that exist, not used)
+    lookup(key_of(t + 2));
     // ---------------- softmax
     const bool masked = first + 32 > s0 || first + 32 > end || gone;
     bf16x8 hi[NQ], lo[NQ];
@@ -723,8 +755,8 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
         ph[x] = fg::pack_bf16x2(p0, p1);
         pl[x] = fg::pack_bf16x2(p0 - __uint_as_float(ph[x] << 16), p1 - __uint_as_float(ph[x] & 0xffff0000u));
       }
-      hi[c] = __builtin_bit_cast(bf16x8, make_uint4(ph[0], ph[1], ph[2], ph[3]));
-      lo[c] = __builtin_bit_cast(bf16x8, make_uint4(pl[0], pl[1], pl[2], pl[3]));
+      hi[c] = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
+      lo[c] = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
     }
     // ---------------- O^T += V^T P^T
     wave_barrier();
