@@ -907,16 +907,16 @@ struct Plan {
 
 Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int64_t capacity) {
   const int64_t m = (int64_t)(q_heads / kv_heads) * num_nodes;
+  // Eight waves, one workgroup per CU: row tiles side by side as far as there are rows, the rest of the waves on other keys.
   Plan p;
   if (m <= 32) p = {1, kStreamWaves, 32, 1};
-  else if (m <= 64) p = {2, 2, 32, 1};
-  else if (m <= 128 || head_dim == 64) p = {4, 1, 64, 1};
+  else if (m <= 64) p = {2, 4, 32, 1};
+  else if (m <= 128 || head_dim == 64) p = {4, 2, 64, 1};
   else p = {8, 1, 64, 1};
   const int64_t base = (int64_t)batch * kv_heads * ((m + p.rows() - 1) / p.rows());
-  const int64_t target = p.rw * p.kw == 4 ? 512 : 256;
-  if (base < target) {
+  if (base < 256) {
     const int64_t most = std::max<int64_t>(1, capacity / kMinPartKeys);
-    p.splits = (int)std::min<int64_t>(std::min<int64_t>((target + base - 1) / base, most), kMaxParts);
+    p.splits = (int)std::min<int64_t>(std::min<int64_t>((255 + base) / base, most), kMaxParts);
   }
   return p;
 }
@@ -936,9 +936,9 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   else if (m <= 32)
     hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 2>), grid, block, 0, s, a);
   else if (p.rw == 2)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 2, 32>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 4, 32>), grid, block, 0, s, a, m_tiles);
   else if (D == 64 || p.rw == 4)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 1, 64>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 2, 64>), grid, block, 0, s, a, m_tiles);
   else
     hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64>), grid, block, 0, s, a, m_tiles);
   if (a.splits > 1) {

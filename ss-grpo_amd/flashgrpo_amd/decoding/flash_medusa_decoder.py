@@ -140,6 +140,11 @@ class FlashMedusaConfig:
     # Replay the verify forward as one HIP graph per (batch, tree width) once that shape
     # repeats; identical results, one launch instead of ~9 per layer.
     graph_verify_forward: bool = True
+    # The rollout's KV cache: "contiguous"; "paged": bf16 pages, a prompt's shared by its repeats; "paged_e4m3": 8-bit pages,
+    # quantised as they are written (bf16 models with heads of 64 or 128; the rollout then samples from the model with that
+    # cache, exactly).
+    kv_cache: str = "contiguous"
+    kv_page_size: int = 64
     # tree_layout="sparse_asymmetric" (flashgrpo_b200/decoding/flash_medusa_decoder.py:65-73);
     # the head-3 quality calibrator and its exploration rounds are not built: every
     # row keeps head 3 (build_batch_trees accepts an explicit per-row gate).
@@ -178,6 +183,8 @@ class FlashMedusaDecoder:
         self._ar_cache = {}   # (n, device) -> arange(n), read-only
         if config.acceptance != "exact_target":
             raise NotImplementedError("Only exact_target acceptance is implemented in the main FlashGRPO path")
+        if config.kv_cache not in {"contiguous", "paged", "paged_e4m3"}:
+            raise ValueError(f"Unsupported kv_cache={config.kv_cache}")
         if config.cache_update_mode not in {"extract_path", "recompute_accepted"}:
             raise ValueError(f"Unsupported cache_update_mode={config.cache_update_mode}")
         if config.proposal_mode not in {"medusa", "chain"}:
@@ -448,7 +455,14 @@ class FlashMedusaDecoder:
             packed[b, :lens[b]] = ids_h[b][mask_h[b]].to(torch.int32)
         B = B0 * repeats
         capacity = max(int(max_length), pmax + 1) + 80
-        r.cache = model.new_cache(B, capacity)
+        if cfg.kv_cache == "contiguous":
+            r.cache = model.new_cache(B, capacity)
+        else:
+            # the pages that a prompt fills once, whatever else a row may come to hold for each row
+            filled = lens // int(cfg.kv_page_size)
+            pages = int(filled.sum() + repeats * (-(-capacity // int(cfg.kv_page_size)) - filled).sum())
+            r.cache = model.new_cache(B, capacity, kv_format="e4m3" if cfg.kv_cache == "paged_e4m3" else "bf16",
+                                      page_size=int(cfg.kv_page_size), pages=pages)
         first_rows = torch.arange(B0, dtype=torch.int32, device=dev) * repeats
         r.sync()
         t0 = time.time()
@@ -465,6 +479,7 @@ class FlashMedusaDecoder:
             r.logits = first_logits.repeat_interleave(repeats, dim=0).contiguous()
         else:
             r.hidden, r.logits = last_hidden, first_logits
+        r.cache.reserve(capacity, first=np.repeat(lens, repeats))
         r.active = list(range(B))
         r.row_map = torch.arange(B, dtype=torch.int32, device=dev)
         r.seq = r.cache.seq_len.clone()

@@ -1069,8 +1069,9 @@ class KVPages:
             raise TypeError("KVPages: k and v must be bfloat16 or float8_e4m3fn")
         if table.dtype is not torch.int32 or table.dim() != 2 or 0 in table.shape:
             raise ValueError("KVPages: table must be a non-empty int32 [rows, width] tensor")
-        dev = k.get_device()
-        _same_device("KVPages", dev, v, table, k_scales, v_scales)
+        dev = k.get_device()  # (-1: on the host, which no call takes)
+        if any(t is not None and t.get_device() != dev for t in (v, table, k_scales, v_scales)):
+            raise ValueError("KVPages: tensors on different devices")
         stride, scale_stride = _page_stride(k, "k"), 0
         n, heads, size, d = k.shape
         if v.shape != k.shape or _page_stride(v, "v") != stride:

@@ -90,12 +90,7 @@ def clone_cache(cache, causal_lm=None, *, clone_tensors: bool = False):
     c = _need_cache(cache)
     if not clone_tensors:
         return c.container_copy()
-    out = c.container_copy()
-    out.kv = c.kv.clone()
-    out.seq_len = c.seq_len.clone()
-    out.tensor_ptrs = torch.tensor([out.kv[l, j].data_ptr() for l in range(c.cfg.num_layers) for j in range(2)],
-                                   dtype=torch.int64, device=c.device)
-    return out
+    return c.deep_copy()
 
 
 def select_cache_batch(cache, indices: torch.Tensor, causal_lm=None):
@@ -128,10 +123,12 @@ def _check_prefix(mask2d: torch.Tensor, seq_len: torch.Tensor, what: str):
         raise ValueError(f"{what}: the mask's valid prefix columns must equal each row's committed cache length")
 
 
-def prefill(causal_lm, input_ids: torch.Tensor, attention_mask: torch.Tensor, *, capacity: int | None = None):
+def prefill(causal_lm, input_ids: torch.Tensor, attention_mask: torch.Tensor, *, capacity: int | None = None,
+            kv_format: str | None = None):
     """``qwen_flashgrpo_wrapper.py:189-199``: causal forward of (left-padded) prompts into
     a new cache. Returns ``{"hidden_states": [B, T, H] (the caller's layout, 0 on
-    padding), "logits": None, "past_key_values": KVCache}``."""
+    padding), "logits": None, "past_key_values": KVCache}`` (``kv_format``: as in
+    ``TargetModel.new_cache``)."""
     model = as_target_model(causal_lm)
     ids_h = input_ids.detach().cpu()
     mask_h = attention_mask.detach().cpu().bool()
@@ -145,7 +142,7 @@ def prefill(causal_lm, input_ids: torch.Tensor, attention_mask: torch.Tensor, *,
     cap = int(capacity) if capacity is not None else T + PREFILL_HEADROOM
     if cap < int(lens.max()):
         raise ValueError(f"prefill: capacity {cap} below the longest prompt {int(lens.max())}")
-    cache = model.new_cache(B, cap)
+    cache = model.new_cache(B, cap, kv_format=kv_format)
     every = model.prefill(packed.to(model.device), cache, lengths=lens, return_all=True)
     hidden = torch.zeros((B, T, model.cfg.hidden), dtype=model.dtype, device=model.device)
     cols = torch.from_numpy(np.nonzero(mask_h.numpy())[1]).to(model.device)
@@ -182,6 +179,7 @@ def forward_tokens(causal_lm, input_ids: torch.Tensor, full_attention_mask: torc
     if int((seq + n).max()) > cache.capacity:
         raise ValueError(f"forward_tokens: {n} tokens after {int(seq.max())} exceed the cache capacity "
                          f"{cache.capacity}")
+    cache.reserve((seq + n).numpy(), first=seq.numpy())
     dev = model.device
     offset = (position_ids.to(torch.int64).cpu() - seq[:, None]).to(torch.int32)
     err = torch.zeros(1, dtype=torch.int32, device=dev)

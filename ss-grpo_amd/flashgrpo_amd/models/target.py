@@ -157,6 +157,17 @@ class KVCache:
         t = self.kv[0, 0]
         return t.stride(0), t.stride(1), t.stride(2)
 
+    def reserve(self, lengths, *, rows=None, first=None) -> None:
+        """Makes room for the first ``lengths`` tokens of the given cache rows; here every row has its room from the start."""
+
+    def deep_copy(self) -> "KVCache":
+        """A cache with copies of the tensors."""
+        out = self.container_copy()
+        out.kv = self.kv.clone()
+        out.tensor_ptrs = torch.tensor([out.kv[l, j].data_ptr() for l in range(self.cfg.num_layers) for j in range(2)],
+                                       dtype=torch.int64, device=self.device)
+        return out
+
     def gather_path(self, seq_len, acc_nodes, acc_len, tree_nodes, *, row_map=None, err_flag=None):
         K.kv_path_gather(self.tensor_ptrs, batch=seq_len.numel(), kv_heads=self.cfg.kv_heads,
                          head_dim=self.cfg.head_dim, elem_bytes=self.kv.element_size(), strides=self.strides,
@@ -177,7 +188,7 @@ class KVCache:
         (the reference's clone_cache(clone_tensors=False)). Committed rows are shared
         read-only; the slots past a row's committed length are shared scratch, so two
         containers that append past the same length overwrite each other there."""
-        c = KVCache.__new__(KVCache)
+        c = type(self).__new__(type(self))
         c.__dict__.update(self.__dict__)
         c.seq_len = self.seq_len.clone()
         return c
@@ -191,6 +202,196 @@ class KVCache:
         for src, dst in zip(self.kv, out.kv):  # one layer's gathered rows at a time
             dst[..., :keep, :].copy_(src.index_select(1, rows)[..., :keep, :])
         out.seq_len.copy_(self.seq_len.index_select(0, rows).clamp_max(cap))
+        return out
+
+
+class PagedKVCache(KVCache):
+    """A KV cache in pages of ``page_size`` tokens: bf16, or quantised to 8 bits as it is written (``kv_format`` "e4m3": MX
+    rows, 33/64 of the bytes). Cache rows take pages from one pool as they need them (``reserve``), and rows that are repeated
+    share the pages that their prompt fills.
+
+    ``codes`` [pages, L, 2, Hkv, page_size, d] (and ``scales`` [.., d / 32]) is the pool, a page's layers side by side;
+    ``table`` [batch, width] int32 the page of every ``page_size`` tokens of a row, -1 where it has none. ``seq_len`` as in
+    ``KVCache``. The page numbers are kept on the host too; ``reserve``, ``release`` and ``repeat_rows`` change them there and
+    copy the table to the device, in order with the current stream. ``pages``: how many the pool has (None: enough for every
+    row to fill ``capacity``)."""
+
+    def __init__(self, cfg: TargetConfig, batch: int, capacity: int, *, device, kv_format: str = "e4m3", page_size: int = 64,
+                 pages: int | None = None):
+        if kv_format not in ("bf16", "e4m3"):
+            raise ValueError("PagedKVCache: kv_format must be 'bf16' or 'e4m3'")
+        self.cfg = cfg
+        self.batch = int(batch)
+        self.capacity = int(capacity)
+        self.dtype = torch.bfloat16
+        self.kv_format = kv_format
+        self.page_size = P = int(page_size)
+        self.device = torch.device(device)
+        width = max(1, -(-self.capacity // P))
+        n = max(1, self.batch * width if pages is None else int(pages))
+        shape = (n, cfg.num_layers, 2, cfg.kv_heads, P, cfg.head_dim)
+        quantised = kv_format == "e4m3"
+        self.codes = torch.zeros(shape, dtype=torch.uint8 if quantised else torch.bfloat16, device=device)
+        if quantised:
+            self.codes = self.codes.view(torch.float8_e4m3fn)
+        self.scales = torch.ones(*shape[:-1], cfg.head_dim // K.MX_BLOCK, dtype=torch.uint8, device=device) if quantised else None
+        self.table = torch.full((self.batch, width), -1, dtype=torch.int32, device=device)
+        self.seq_len = torch.zeros(self.batch, dtype=torch.int32, device=device)
+        self._rows = np.full((self.batch, width), -1, np.int32)  # the table, on the host
+        self._uses = np.zeros(n, np.int64)                        # rows that hold a page
+        self._free = list(range(n - 1, -1, -1))
+        self._make_views()
+
+    def _make_views(self):
+        c, s = self.codes, self.scales
+        part = lambda l, i: None if s is None else s[:, l, i]
+        self._layers = [K.KVPages(c[:, l, 0], c[:, l, 1], part(l, 0), part(l, 1), self.table) for l in range(self.cfg.num_layers)]
+
+    @property
+    def kv(self) -> torch.Tensor:
+        return self.codes
+
+    def pages(self, layer: int) -> K.KVPages:
+        """One layer's pages, as the kernels take them."""
+        return self._layers[layer]
+
+    def k(self, layer: int) -> torch.Tensor:
+        """The values of K, [batch, Hkv, capacity, d] bf16: a copy, 0 where a row has no page."""
+        return K.kv_read_paged(self._layers[layer], count=self.capacity)[0]
+
+    def v(self, layer: int) -> torch.Tensor:
+        return K.kv_read_paged(self._layers[layer], count=self.capacity)[1]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self) -> int:
+        if not self._free:
+            raise RuntimeError(f"PagedKVCache: all {self._uses.size} pages are in use")
+        p = self._free.pop()
+        self._uses[p] = 1
+        return p
+
+    def _drop(self, p: int) -> None:
+        self._uses[p] -= 1
+        if self._uses[p] == 0:
+            self._free.append(int(p))
+
+    def _copy_pages(self, pairs) -> None:
+        """Contents of pages, all layers: (from, to) pairs whose targets are not among the sources."""
+        if pairs:
+            src, dst = (torch.tensor(x, dtype=torch.long, device=self.device) for x in zip(*pairs))
+            for t in (self.codes, self.scales):
+                if t is not None:
+                    t = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+                    t.index_copy_(0, dst, t.index_select(0, src))
+
+    def _upload(self) -> None:
+        self.table.copy_(torch.from_numpy(self._rows))
+
+    def reserve(self, lengths, *, rows=None, first=None) -> None:
+        """Gives the cache rows ``rows`` (None: all) pages for their first ``lengths`` tokens. Of the tokens from ``first`` on
+        (None: the tokens that get new pages), which the caller is about to write, a page that other rows share is replaced
+        by a copy of it. Raises RuntimeError, with nothing changed, when the pool has too few pages."""
+        rows = np.arange(self.batch) if rows is None else np.asarray(rows, np.int64)
+        lengths = np.broadcast_to(np.asarray(lengths, np.int64), rows.shape)
+        first = None if first is None else np.broadcast_to(np.asarray(first, np.int64), rows.shape)
+        if (lengths > self.capacity).any():
+            raise ValueError(f"PagedKVCache: {int(lengths.max())} tokens exceed the cache capacity {self.capacity}")
+        need, P = [], self.page_size
+        uses = self._uses.copy()
+        for i, (r, n) in enumerate(zip(rows, lengths)):
+            held = self._rows[r]
+            for slot in range(0 if first is None else int(first[i]) // P, -(-int(n) // P)):
+                p = held[slot]
+                if p < 0:
+                    need.append((r, slot, -1))
+                elif first is not None and uses[p] > 1:
+                    need.append((r, slot, int(p)))
+                    uses[p] -= 1  # the last row that asks keeps the page itself
+            if first is not None:  # tokens before it
+                need += [(r, slot, -1) for slot in range(min(int(first[i]) // P, -(-int(n) // P))) if held[slot] < 0]
+        if not need:
+            return
+        if len(need) > len(self._free):
+            raise RuntimeError(f"PagedKVCache: {len(need)} more pages needed, {len(self._free)} of {self._uses.size} free")
+        copies = []
+        for r, slot, shared in need:
+            p = self._take()
+            self._rows[r, slot] = p
+            if shared >= 0:
+                copies.append((shared, p))
+                self._drop(shared)
+        self._copy_pages(copies)
+        self._upload()
+
+    def release(self, rows) -> None:
+        """Gives the pages of the given cache rows back (their committed lengths become 0)."""
+        for r in np.asarray(rows, np.int64).reshape(-1):
+            for p in self._rows[r][self._rows[r] >= 0]:
+                self._drop(int(p))
+            self._rows[r] = -1
+            self.seq_len[int(r)] = 0
+        self._upload()
+
+    def gather_path(self, seq_len, acc_nodes, acc_len, tree_nodes, *, row_map=None, err_flag=None):
+        K.kv_path_gather_paged(self._layers[0], seq_len=seq_len, acc_nodes=acc_nodes, acc_len=acc_len, tree_nodes=tree_nodes,
+                               layers=self.cfg.num_layers, layer_stride=self.codes.stride(1),
+                               scale_layer_stride=0 if self.scales is None else self.scales.stride(1), row_map=row_map,
+                               err_flag=err_flag)
+
+    def repeat_rows(self, src_rows: torch.Tensor, dst_rows: torch.Tensor) -> None:
+        """Cache rows dst become repeats of rows src: they share the pages that src's committed tokens fill and get a copy of
+        the one that they end in. Pages that dst held go back to the pool first."""
+        src, dst = (np.asarray(t.cpu() if isinstance(t, torch.Tensor) else t, np.int64).reshape(-1) for t in (src_rows, dst_rows))
+        if src.shape != dst.shape or len(set(dst.tolist())) < dst.size or set(src.tolist()) & set(dst.tolist()):
+            raise ValueError("PagedKVCache.repeat_rows: one row src for each of distinct rows dst, none of which is a src")
+        lens = self.seq_len.cpu().numpy()
+        for r in dst:
+            for p in self._rows[r][self._rows[r] >= 0]:
+                self._drop(int(p))
+            self._rows[r] = -1
+        copies = []
+        for s, r in zip(src, dst):
+            whole, rest = divmod(int(lens[s]), self.page_size)
+            self._rows[r, :whole] = self._rows[s, :whole]
+            self._uses[self._rows[s, :whole]] += 1
+            if rest:
+                self._rows[r, whole] = self._take()
+                copies.append((int(self._rows[s, whole]), int(self._rows[r, whole])))
+        self._copy_pages(copies)
+        self._upload()
+        self.seq_len.index_copy_(0, torch.as_tensor(dst, device=self.device),
+                                 self.seq_len.index_select(0, torch.as_tensor(src, device=self.device)))
+
+    def select_rows(self, rows: torch.Tensor, capacity: int | None = None) -> "PagedKVCache":
+        """A new cache, with a pool of its own, holding copies of the given rows' committed tokens (in that order)."""
+        rows = torch.as_tensor(rows).to(dtype=torch.long, device="cpu").numpy()
+        cap = self.capacity if capacity is None else int(capacity)
+        out = PagedKVCache(self.cfg, rows.size, cap, device=self.device, kv_format=self.kv_format, page_size=self.page_size)
+        lens = np.minimum(self.seq_len.cpu().numpy()[rows], cap)
+        out.reserve(lens)
+        pairs = [(int(self._rows[r, i]), int(out._rows[j, i])) for j, r in enumerate(rows)
+                 for i in range(-(-int(lens[j]) // self.page_size))]
+        if pairs:
+            src, dst = (torch.tensor(x, dtype=torch.long, device=self.device) for x in zip(*pairs))
+            for a, b in ((self.codes, out.codes), (self.scales, out.scales)):
+                if a is not None:
+                    a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
+                    for l in range(self.cfg.num_layers):  # one layer's pages at a time
+                        b[:, l].index_copy_(0, dst, a[:, l].index_select(0, src))
+        out.seq_len.copy_(torch.from_numpy(lens.astype(np.int32)))
+        return out
+
+    def deep_copy(self) -> "PagedKVCache":
+        out = self.container_copy()
+        out.codes = (self.codes.view(torch.uint8).clone().view(torch.float8_e4m3fn) if self.kv_format == "e4m3"
+                     else self.codes.clone())
+        out.scales = None if self.scales is None else self.scales.clone()
+        out.table = self.table.clone()
+        out._rows, out._uses, out._free = self._rows.copy(), self._uses.copy(), list(self._free)
+        out._make_views()
         return out
 
 
@@ -632,8 +833,15 @@ class TargetModel:
         return K.MX(self._buf(name, (rows, cols), torch.float8_e4m3fn),
                     self._buf(name + "_scales", (-(-cols // 128), rows, 4), torch.uint8))
 
-    def new_cache(self, batch: int, capacity: int) -> KVCache:
-        return KVCache(self.cfg, batch, capacity, dtype=self.dtype, device=self.device)
+    def new_cache(self, batch: int, capacity: int, *, kv_format: str | None = None, page_size: int = 64,
+                  pages: int | None = None) -> KVCache:
+        """A cache of ``batch`` rows of up to ``capacity`` tokens: contiguous, or, with ``kv_format`` "bf16" or "e4m3" (8 bits),
+        in pages (``PagedKVCache``; bf16 models with heads of 64 or 128)."""
+        if kv_format is None:
+            return KVCache(self.cfg, batch, capacity, dtype=self.dtype, device=self.device)
+        if self.dtype != torch.bfloat16 or self.cfg.head_dim not in (64, 128):
+            raise ValueError("new_cache: a paged cache needs a bf16 model with heads of 64 or 128")
+        return PagedKVCache(self.cfg, batch, capacity, device=self.device, kv_format=kv_format, page_size=page_size, pages=pages)
 
     # -------------------------------------------------------------- forward
     def _buf(self, name, shape, dtype=None):
@@ -663,14 +871,17 @@ class TargetModel:
 
     def forward(self, tokens: torch.Tensor, cache: KVCache, *, pos_offset: torch.Tensor, anc: torch.Tensor,
                 seq_len: torch.Tensor | None = None, row_map: torch.Tensor | None = None,
-                err_flag: torch.Tensor | None = None, graph: bool = False) -> torch.Tensor:
+                err_flag: torch.Tensor | None = None, graph: bool = False,
+                new_len: torch.Tensor | None = None) -> torch.Tensor:
         """Forward N new tokens per row after each row's committed prefix.
 
         tokens [B, N] int (device); pos_offset int32 [N] (shared) or [B, N]: position =
         seq_len[b] + pos_offset[(b,) n]; anc: int64 bit masks [N] (shared) or [B, N], or None for a causal
         chain (node n sees new tokens 0..n; up to MAX_CHAIN_TOKENS); node n's K/V land in cache slot
         seq_len[b] + n of cache row row_map[b]. Returns final-normed hidden [B, N, H].
-        ``seq_len`` defaults to ``cache.seq_len`` and is not advanced here.
+        ``seq_len`` defaults to ``cache.seq_len`` and is not advanced here. A paged cache has to have pages for the new
+        tokens (``cache.reserve``); it also takes ``new_len`` int32 [B], of how many of a row's N tokens count: the others are
+        not written, nobody sees them, and their hidden states are of no account.
 
         ``graph=True`` replays a HIP graph of the whole forward (captured on the second
         call with the same shapes, cache and error word): one launch instead of ~9 per
@@ -679,7 +890,9 @@ class TargetModel:
         eagerly so every launch stays visible to it.
         """
         seq_len = cache.seq_len if seq_len is None else seq_len
-        if graph and anc is not None and timing.idle() and not torch.cuda.is_current_stream_capturing():
+        if new_len is not None and not isinstance(cache, PagedKVCache):
+            raise ValueError("forward: new_len needs a paged cache")
+        if graph and anc is not None and new_len is None and timing.idle() and not torch.cuda.is_current_stream_capturing():
             key = (tuple(tokens.shape), tokens.dtype, tuple(pos_offset.shape), tuple(anc.shape), cache.kv.data_ptr(),
                    tuple(cache.kv.shape), tuple(seq_len.shape), None if row_map is None else tuple(row_map.shape),
                    None if err_flag is None else err_flag.data_ptr())
@@ -693,11 +906,14 @@ class TargetModel:
             if g:
                 return g.run(tokens, pos_offset, anc, seq_len, row_map)
         return self._forward_eager(tokens, cache, pos_offset=pos_offset, anc=anc, seq_len=seq_len, row_map=row_map,
-                                   err_flag=err_flag)
+                                   err_flag=err_flag, new_len=new_len)
 
-    def _forward_eager(self, tokens, cache, *, pos_offset, anc, seq_len, row_map, err_flag):
+    def _forward_eager(self, tokens, cache, *, pos_offset, anc, seq_len, row_map, err_flag, new_len=None):
         st = self._forward_begin(tokens, cache, pos_offset=pos_offset, anc=anc, seq_len=seq_len, row_map=row_map,
                                  err_flag=err_flag)
+        if new_len is not None:
+            st["new_len"] = new_len
+            st["attn"].zero_()  # the rows that do not count
         self._forward_layers(st, 0, self.cfg.num_layers)
         return self._forward_end(st)
 
@@ -734,8 +950,17 @@ class TargetModel:
             h = st.pop("h", None)
             if h is None:
                 h = K.rmsnorm(x, lw["input_norm"], cfg.rms_eps, out=self._buf("h", (T, H)))
-            plan = self._linear_plan("qkv", h, lw["qkv_w"])
-            if plan and len(plan) == 5:  # the projection with the rotary + cache write in its epilogue
+            paged = isinstance(cache, PagedKVCache)
+            plan = self._linear_plan("qkv", h, lw["qkv_w"], rope=not paged)
+            if paged:
+                kw = dict(batch=B, num_nodes=N, q_heads=cfg.q_heads, kv_heads=cfg.kv_heads, head_dim=d, seq_len=seq_len,
+                          pos_offset=pos_offset, inv_freq=self.inv_freq, q_out=q, new_len=st.get("new_len"), row_map=row_map,
+                          err_flag=err_flag)
+                if plan:
+                    K.rope_kv_write_paged_parts(self._linear_parts(h, lw["qkv_w"], plan), lw["qkv_b"], cache.pages(l), **kw)
+                else:
+                    K.rope_kv_write_paged(F.linear(h, lw["qkv_w"], lw["qkv_b"]), cache.pages(l), **kw)
+            elif plan and len(plan) == 5:  # the projection with the rotary + cache write in its epilogue
                 wp, bp = self._rope_pairs(l)
                 cs = st.get("rope_cs")
                 if cs is None:  # the rows' rotary table, once per forward
@@ -757,8 +982,12 @@ class TargetModel:
                 K.rope_kv_write(qkv, batch=B, num_nodes=N, q_heads=cfg.q_heads, kv_heads=cfg.kv_heads, head_dim=d,
                                 seq_len=seq_len, pos_offset=pos_offset, inv_freq=self.inv_freq, q_out=q,
                                 k_cache=cache.k(l), v_cache=cache.v(l), row_map=row_map, err_flag=err_flag)
-            K.tree_attention(q, cache.k(l), cache.v(l), seq_len=seq_len, anc=anc, num_nodes=N, q_heads=cfg.q_heads,
-                             kv_heads=cfg.kv_heads, head_dim=d, out=attn, row_map=row_map)
+            if paged:
+                K.paged_attention(q, cache.pages(l), seq_len=seq_len, anc=anc, num_nodes=N, q_heads=cfg.q_heads,
+                                  kv_heads=cfg.kv_heads, head_dim=d, out=attn, new_len=st.get("new_len"), row_map=row_map)
+            else:
+                K.tree_attention(q, cache.k(l), cache.v(l), seq_len=seq_len, anc=anc, num_nodes=N, q_heads=cfg.q_heads,
+                                 kv_heads=cfg.kv_heads, head_dim=d, out=attn, row_map=row_map)
             a2 = attn.view(T, cfg.q_heads * d)
             plan = self._linear_plan("o", a2, lw["o_w"])
             if self.mlp_mx is not None:  # from the post-attention norm to the residual stream on MX rows
@@ -804,10 +1033,11 @@ class TargetModel:
             else:
                 x.addmm_(act, lw["down_w"].t())
 
-    def _linear_plan(self, kind: str, x: torch.Tensor, w: torch.Tensor):
+    def _linear_plan(self, kind: str, x: torch.Tensor, w: torch.Tensor, rope: bool = True):
         """(tile_m, tile_n, splits, stages) when projection ``kind`` of x by w runs split-K, else None;
         for QKV, (tile_m, tile_n, 1, stages, "rope") when the projection runs with the rotary + cache
-        write in its epilogue (``fg_linear_rope_kv_write``), the measured table's fastest path."""
+        write in its epilogue (``fg_linear_rope_kv_write``), the measured table's fastest path (``rope``
+        False: that path aside)."""
         if self.split_k_linear is False or not K.linear_ok(x, w):
             return None
         rows, hidden = x.shape
@@ -816,7 +1046,7 @@ class TargetModel:
         if self.split_k_linear:  # forced: the best measured split-K plan of the shape, else the default
             plan = (linear_table_split_plan(kind, rows, cols, hidden)
                     or default_linear_plan(rows, cols, hidden, _cu_count(x.device)))
-        if kind == "qkv" and x.dtype == torch.bfloat16 and self.cfg.head_dim % 8 == 0:
+        if rope and kind == "qkv" and x.dtype == torch.bfloat16 and self.cfg.head_dim % 8 == 0:
             rope = linear_table_times("qkv_rope", rows, cols, hidden)
             base = linear_table_times("qkv", rows, cols, hidden)
             if rope is not None and base is not None:
@@ -971,14 +1201,18 @@ class TargetModel:
         last = torch.empty(B, self.cfg.hidden, dtype=self.dtype, device=self.device)
         every = torch.zeros(B, P, self.cfg.hidden, dtype=self.dtype, device=self.device) if return_all else None
         chunk = max(1, min(int(chunk), MAX_CHAIN_TOKENS))
+        paged = isinstance(cache, PagedKVCache)
+        if paged:
+            cache.reserve(lens, rows=None if row_map is None else row_map.cpu().numpy(), first=0)
         offs_full = torch.arange(chunk, dtype=torch.int32, device=self.device)
         for start in range(0, int(lens.max()), chunk):
             n = min(chunk, P - start)
             tok = ids[:, start:start + n].contiguous()
-            hid = self.forward(tok, cache, pos_offset=offs_full[:n], anc=None, seq_len=seq, row_map=row_map)
+            adv = np.clip(lens - start, 0, n)
+            hid = self.forward(tok, cache, pos_offset=offs_full[:n], anc=None, seq_len=seq, row_map=row_map,
+                               new_len=torch.from_numpy(adv.astype(np.int32)).to(self.device) if paged else None)
             if every is not None:
                 every[:, start:start + n].copy_(hid)
-            adv = np.clip(lens - start, 0, n)
             ends = np.nonzero((lens > start) & (lens <= start + n))[0]
             if ends.size:
                 e = torch.from_numpy(ends).to(self.device)
@@ -1046,6 +1280,8 @@ def forward_tree(causal_lm: TargetModel, ids: torch.Tensor, mask4d: torch.Tensor
     if int(seq.max()) + N > pkv.capacity:
         raise ValueError(f"forward_tree: {N} tree nodes after {int(seq.max())} committed tokens exceed the "
                          f"cache capacity {pkv.capacity}")
+    committed = pkv.seq_len.cpu().numpy()
+    pkv.reserve(committed + N, first=committed)
     anc, offset = native_tree_inputs(mask4d, pos, pkv.seq_len)
     tree_cache = pkv.container_copy() if clone_past else pkv
     err = torch.zeros(1, dtype=torch.int32, device=dev)
