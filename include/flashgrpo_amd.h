@@ -286,8 +286,8 @@ int fg_mx_plan(int gate_up, int rows, int cols, int hidden, int x_format, int pl
  * `page_stride` elements behind the page before (so that a pool may hold every layer of a page side by side). format 0: MX
  * e4m3, codes of 8 bits (no NaN codes; a NaN block is told by its scale), with scales [kv_heads][page_size][head_dim / 32], bytes,
  * `scale_stride` bytes behind those of the page before (fg_mx_quantize's blocks, a row's scales side by side); 1: bf16. head_dim
- * 64 or 128, page_size a power of two from 16 on, table_width * page_size less than 2^31 - 65536 tokens per row. Pages 16-byte
- * and scales 4-byte aligned. A host struct of device addresses, read during the call. No counterpart in the reference, whose
+ * 64 or 128, page_size a power of two from 16 to 2^20, table_width * page_size less than 2^31 - 65536 tokens per row, a page (one
+ * layer's K) less than 2^30 elements, page_stride less than 2^31. Pages 16-byte and scales 4-byte aligned. A host struct of device addresses, read during the call. No counterpart in the reference, whose
  * cache is DynamicCache. */
 typedef struct fg_kv_pages {
   void* k;

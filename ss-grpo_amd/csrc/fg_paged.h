@@ -47,7 +47,9 @@ inline int pages_of(const fg_kv_pages* p, const char* what, Pages& out) {
              w + ": page_size must be a power of two in [16, 2^20]");
   FG_REQUIRE(p->pages > 0 && p->kv_heads > 0 && p->table_rows > 0 && p->table_width > 0, w + ": bad sizes");
   FG_REQUIRE((int64_t)p->table_width * p->page_size < (1ll << 31) - 65536, w + ": a row must hold less than 2^31 tokens");
-  FG_REQUIRE((int64_t)p->kv_heads * p->page_size * p->head_dim * 2 < (1ll << 31), w + ": a page must be smaller than 2 GiB");
+  FG_REQUIRE((int64_t)p->kv_heads * p->page_size * p->head_dim < (1ll << 30) && p->page_stride < (1ll << 31) &&
+                 p->scale_stride < (1ll << 32),
+             w + ": a page must have less than 2^30 elements, pages lie less than 2^31 elements (scales 4 GiB) apart");
   const int es = p->format == kPageBF16 ? 2 : 1;
   FG_REQUIRE(p->page_stride >= (int64_t)p->kv_heads * p->page_size * p->head_dim && p->table_stride >= p->table_width,
              w + ": pages and table rows must not overlap");

@@ -693,7 +693,7 @@ def linear_rope_kv_write(x, w_pairs, bias_pairs, *, tile=(64, 64), stages=0, bat
 # ------------------------------------------------------------------ microscaled (MX) rows
 MX_BLOCK = 32                         # elements per scale
 MX_FORMATS = {"e4m3": 0, "e2m1": 1}   # fg_mx_quantize's format codes
-_U8, _FP8, _BF16 = torch.uint8, torch.float8_e4m3fn, torch.bfloat16
+_U8, _FP8, _BF16, _I32 = torch.uint8, torch.float8_e4m3fn, torch.bfloat16, torch.int32
 
 
 class MX(NamedTuple):
@@ -1065,11 +1065,50 @@ class KVPages:
 
     def __init__(self, k, v, k_scales, v_scales, table):
         fmt = PAGE_FORMATS.get(k.dtype)
+        shape, stride, dev = k.shape, k.stride(), k.get_device()  # (-1: on the host, which no call takes)
+        if fmt is None or v.dtype is not k.dtype or table.dtype is not _I32 or len(shape) != 4 or table.dim() != 2:
+            self._refuse(k, v, k_scales, v_scales, table)
+        n, heads, size, d = shape
+        (rows, width), (row, unit) = table.shape, table.stride()
+        at, at_v, page = k.data_ptr(), v.data_ptr(), heads * size * d
+        first = stride[0] if n > 1 else page
+        ok = (v.shape == shape and (d == 64 or d == 128) and size >= 16 and not size & (size - 1) and n and heads and rows and width
+              and stride[3] == 1 and stride[2] == d and (heads == 1 or stride[1] == size * d) and first >= page
+              and v.stride() == stride and (width == 1 or unit == 1) and (rows == 1 or row >= width)
+              and width * size < (1 << 31) - 65536 and page < 1 << 30 and not (n | rows) >> 31
+              and first < 1 << 31 and not (at | at_v | first * (1 + fmt)) & 15 and v.get_device() == dev == table.get_device())
+        at_ks = at_vs = scale_first = None
+        if ok and fmt == 0:
+            ok = k_scales is not None and v_scales is not None
+            if ok:
+                blocks = d >> 5
+                page >>= 5
+                s = k_scales.stride()
+                scale_first = s[0] if n > 1 else page
+                at_ks, at_vs = k_scales.data_ptr(), v_scales.data_ptr()
+                ok = (k_scales.shape == (n, heads, size, blocks) == v_scales.shape and k_scales.dtype is _U8 is v_scales.dtype
+                      and s[3] == 1 and s[2] == blocks and (heads == 1 or s[1] == size * blocks) and scale_first >= page
+                      and v_scales.stride() == s and scale_first < 1 << 32 and not (at_ks | at_vs | scale_first) & 3
+                      and k_scales.get_device() == dev == v_scales.get_device())
+        elif ok:
+            ok = k_scales is None is v_scales
+        if not ok:
+            self._refuse(k, v, k_scales, v_scales, table)
+        self.k, self.v, self.k_scales, self.v_scales, self.table = k, v, k_scales, v_scales, table
+        self.format, self.pages, self.page_size, self.kv_heads, self.head_dim = fmt, n, size, heads, d
+        self.rows, self.width, self.device = rows, width, dev
+        self._c = _lib.KvPages(at, at_v, at_ks, at_vs, table.data_ptr(), first, scale_first or 0, row if rows > 1 else width, fmt, n, size,
+                               heads, d, rows, width)
+        self.address = C.addressof(self._c)
+
+    @staticmethod
+    def _refuse(k, v, k_scales, v_scales, table):
+        fmt = PAGE_FORMATS.get(k.dtype)
         if fmt is None or v.dtype is not k.dtype:
             raise TypeError("KVPages: k and v must be bfloat16 or float8_e4m3fn")
-        if table.dtype is not torch.int32 or table.dim() != 2 or 0 in table.shape:
+        if table.dtype is not _I32 or table.dim() != 2 or 0 in table.shape:
             raise ValueError("KVPages: table must be a non-empty int32 [rows, width] tensor")
-        dev = k.get_device()  # (-1: on the host, which no call takes)
+        dev = k.get_device()
         if any(t is not None and t.get_device() != dev for t in (v, table, k_scales, v_scales)):
             raise ValueError("KVPages: tensors on different devices")
         stride, scale_stride = _page_stride(k, "k"), 0
@@ -1090,16 +1129,10 @@ class KVPages:
         rows, width = table.shape
         if (width > 1 and table.stride(1) != 1) or (rows > 1 and table.stride(0) < width):
             raise ValueError("KVPages: table rows must have unit stride and be apart")
-        if width * size >= (1 << 31) - 65536 or heads * size * d * 2 >= 1 << 31 or n >> 31 or rows >> 31:
-            raise ValueError("KVPages: rows must hold less than 2^31 - 65536 tokens and pages less than 2 GiB")
-        at = [None if t is None else t.data_ptr() for t in (k, v, k_scales, v_scales, table)]
-        if at[0] % 16 or at[1] % 16 or stride * (2 if fmt else 1) % 16 or (fmt == 0 and (at[2] % 4 or at[3] % 4 or scale_stride % 4)):
-            raise ValueError("KVPages: pages must start 16-byte aligned and scales 4-byte aligned")
-        self.k, self.v, self.k_scales, self.v_scales, self.table = k, v, k_scales, v_scales, table
-        self.format, self.pages, self.page_size, self.kv_heads, self.head_dim = fmt, n, size, heads, d
-        self.rows, self.width, self.device = rows, width, dev
-        self._c = _lib.KvPages(*at, stride, scale_stride, table.stride(0) if rows > 1 else width, fmt, n, size, heads, d, rows, width)
-        self.address = C.addressof(self._c)
+        if width * size >= (1 << 31) - 65536 or heads * size * d >= 1 << 30 or (n | rows) >> 31 or stride >> 31 or scale_stride >> 32:
+            raise ValueError("KVPages: rows must hold less than 2^31 - 65536 tokens, pages less than 2^30 elements and lie less than "
+                             "2^31 elements apart")
+        raise ValueError("KVPages: pages must start 16-byte aligned and scales 4-byte aligned")
 
     @property
     def capacity(self) -> int:
@@ -1118,15 +1151,19 @@ def _page_stride(t, what):
     return a if n > 1 else heads * size * d
 
 
+def _held(t, dev, rows) -> bool:
+    """Whether t is a contiguous int32 tensor of at least ``rows`` entries on GPU ``dev``."""
+    return t.dtype is _I32 and t.numel() >= rows and t.is_contiguous() and t.get_device() == dev
+
+
 def _index(what, dev, rows, *named):
-    """Raises unless each given (name, tensor) is a contiguous int32 tensor of at least ``rows`` entries on GPU ``dev``."""
     for name, t in named:
-        if t is not None and (t.dtype is not torch.int32 or t.numel() < rows or not t.is_contiguous() or t.get_device() != dev):
+        if t is not None and not _held(t, dev, rows):
             raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of {rows} entries on the pages' device")
 
 
 def _paged_sizes(what, pages, kv_heads, head_dim):
-    if not isinstance(pages, KVPages):
+    if type(pages) is not KVPages:
         raise TypeError(f"{what}: pages must be KVPages")
     if pages.device < 0:
         raise ValueError("flashgrpo_amd kernels take device tensors (got a CPU tensor)")
@@ -1134,23 +1171,31 @@ def _paged_sizes(what, pages, kv_heads, head_dim):
         raise ValueError(f"{what}: the pages hold {pages.kv_heads} kv heads of {pages.head_dim}")
 
 
-def _write_paged(name, lead, pages, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out, new_len,
-                 row_map, err_flag, read):
-    what, dev = name[3:], pages.device
-    _index(what, dev, batch, ("seq_len", seq_len), ("new_len", new_len), ("row_map", row_map))
-    _index(what, dev, num_nodes, ("pos_offset", pos_offset))
-    _index(what, dev, 1, ("err_flag", err_flag))
-    pos_stride = _pos_stride(pos_offset, batch, num_nodes, what)
-    if inv_freq.dtype is not torch.float32 or inv_freq.numel() < head_dim // 2 or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
-        raise ValueError(f"{what}: inv_freq must be a contiguous fp32 tensor of {head_dim // 2} entries on the pages' device")
-    size = batch * num_nodes * q_heads * head_dim
-    at = q_out.data_ptr()
-    if q_out.dtype is not _BF16 or q_out.numel() != size or not q_out.is_contiguous() or q_out.get_device() != dev or at % 8:
-        raise ValueError(f"{what}: q_out must be a contiguous bf16 [batch * num_nodes, q_heads, d] tensor")
-    _apart(what, ((at, 2 * size),), read)
+def _write_paged(name, lead, pages, batch, num_nodes, q_heads, head_dim, seq_len, pos_offset, inv_freq, q_out, new_len, row_map, err_flag,
+                 read):
+    dev, size, at = pages.device, batch * num_nodes * q_heads * head_dim, q_out.data_ptr()
+    pos_stride = num_nodes if pos_offset.dim() == 2 else 0
+    if not (_held(seq_len, dev, batch) and _held(pos_offset, dev, num_nodes)
+            and (pos_stride == 0 or pos_offset.shape == (batch, num_nodes)) and inv_freq.dtype is torch.float32
+            and inv_freq.numel() >= head_dim >> 1 and inv_freq.is_contiguous() and inv_freq.get_device() == dev
+            and q_out.dtype is _BF16 and q_out.numel() == size and q_out.is_contiguous() and q_out.get_device() == dev and not at & 7
+            and (new_len is None or _held(new_len, dev, batch)) and (row_map is None or _held(row_map, dev, batch))
+            and (err_flag is None or _held(err_flag, dev, 1))):
+        what = name[3:]
+        _index(what, dev, batch, ("seq_len", seq_len), ("new_len", new_len), ("row_map", row_map))
+        _index(what, dev, num_nodes, ("pos_offset", pos_offset))
+        _index(what, dev, 1, ("err_flag", err_flag))
+        _pos_stride(pos_offset, batch, num_nodes, what)
+        if inv_freq.dtype is not torch.float32 or inv_freq.numel() < head_dim >> 1 or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
+            raise ValueError(f"{what}: inv_freq must be a contiguous fp32 tensor of {head_dim // 2} entries on the pages' device")
+        raise ValueError(f"{what}: q_out must be a contiguous 8-byte aligned bf16 [batch * num_nodes, q_heads, d] tensor on the pages' device")
     if size:
+        for a, n in read:
+            if a < at + 2 * size and at < a + n:
+                raise ValueError(f"{name[3:]}: q_out overlaps an operand")
         _call_on(dev, name, *lead, batch, num_nodes, q_heads, pages.address, seq_len.data_ptr(), pos_offset.data_ptr(), pos_stride,
-                 inv_freq.data_ptr(), _ptr(new_len), _ptr(row_map), at, _ptr(err_flag))
+                 inv_freq.data_ptr(), None if new_len is None else new_len.data_ptr(), None if row_map is None else row_map.data_ptr(),
+                 at, None if err_flag is None else err_flag.data_ptr())
 
 
 def rope_kv_write_paged(qkv, pages, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out,
@@ -1160,18 +1205,15 @@ def rope_kv_write_paged(qkv, pages, *, batch, num_nodes, q_heads, kv_heads, head
     formula gives, angles and K in 64 bits; bf16 pages and their q: ``rope_kv_write``'s values. ``new_len`` int32 [batch]:
     tokens from new_len[b] on are left out (their q_out rows and slots stay as they were). A slot without a page sets
     err_flag bit 8. Cache rows that share a page must not both write to it."""
-    what = "rope_kv_write_paged"
-    _paged_sizes(what, pages, kv_heads, head_dim)
-    width, rows = (q_heads + 2 * kv_heads) * head_dim, batch * num_nodes
-    if qkv.dtype is not _BF16 or qkv.dim() < 2 or qkv.stride(-1) != 1 or qkv.shape[-1] < width or qkv.numel() != rows * qkv.shape[-1] \
-            or qkv.get_device() != pages.device or (qkv.dim() > 2 and not qkv.is_contiguous()):
-        raise ValueError(f"{what}: qkv must hold {rows} rows of >= {width} unit-stride bf16 values on the pages' device")
-    ld = qkv.stride(-2) if rows > 1 and qkv.dim() == 2 else qkv.shape[-1]
-    at = qkv.data_ptr()
-    if at % 8 or ld % 4 or ld < width:
-        raise ValueError(f"{what}: qkv rows must be apart and start 8-byte aligned")
-    _write_paged("fg_rope_kv_write_paged", (at, ld), pages, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset,
-                 inv_freq, q_out, new_len, row_map, err_flag, ((at, 2 * ((rows - 1) * ld + width)),))
+    _paged_sizes("rope_kv_write_paged", pages, kv_heads, head_dim)
+    width, rows, shape, at = (q_heads + 2 * kv_heads) * head_dim, batch * num_nodes, qkv.shape, qkv.data_ptr()
+    last, ld = shape[-1], qkv.stride(0) if len(shape) == 2 and rows > 1 else shape[-1]
+    if qkv.dtype is not _BF16 or len(shape) < 2 or last < width or qkv.numel() != rows * last or qkv.get_device() != pages.device \
+            or not (qkv.is_contiguous() or len(shape) == 2 and qkv.stride(1) == 1) or at & 7 or ld & 3 or ld < width:
+        raise ValueError(f"rope_kv_write_paged: qkv must hold {rows} rows of >= {width} unit-stride bf16 values on the pages' device, apart "
+                         "and 8-byte aligned")
+    _write_paged("fg_rope_kv_write_paged", (at, ld), pages, batch, num_nodes, q_heads, head_dim, seq_len, pos_offset, inv_freq, q_out,
+                 new_len, row_map, err_flag, ((at, 2 * ((rows - 1) * ld + width)),))
 
 
 def rope_kv_write_paged_parts(parts, bias, pages, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq,
@@ -1191,30 +1233,31 @@ def rope_kv_write_paged_parts(parts, bias, pages, *, batch, num_nodes, q_heads, 
             raise ValueError(f"{what}: bias must be a contiguous 8-byte aligned bf16 [{width}] tensor")
         read.append((bias.data_ptr(), 2 * width))
     _write_paged("fg_rope_kv_write_paged_parts", (parts.data_ptr(), parts.shape[0], _ptr(bias)), pages, batch, num_nodes, q_heads,
-                 kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out, new_len, row_map, err_flag, read)
+                 head_dim, seq_len, pos_offset, inv_freq, q_out, new_len, row_map, err_flag, read)
 
 
 def kv_read_paged(pages, *, count, start=None, row_map=None, batch=None, dtype=torch.bfloat16):
     """(k, v), each [batch, kv_heads, count, head_dim] in bf16 (exact but under 2^-126) or fp32: the values of tokens start[b] ..
     start[b] + count - 1 (start None: 0) of cache row row_map[b] (None: b); tokens without a page are 0 (``fg_kv_read_paged``).
     batch: that of start or row_map, or every row of the table."""
-    what = "kv_read_paged"
-    if not isinstance(pages, KVPages):
-        raise TypeError(f"{what}: pages must be KVPages")
+    if type(pages) is not KVPages:
+        raise TypeError("kv_read_paged: pages must be KVPages")
     dev = pages.device
-    _same_device(what, dev)
     if batch is None:
         batch = start.numel() if start is not None else row_map.numel() if row_map is not None else pages.rows
+    if dev < 0:
+        _same_device("kv_read_paged", dev)
     if dtype not in _DT:
-        raise TypeError(f"{what}: dtype must be bfloat16 or float32")
+        raise TypeError("kv_read_paged: dtype must be bfloat16 or float32")
     if batch < 0 or count < 0:
-        raise ValueError(f"{what}: batch and count must not be negative")
-    _index(what, dev, batch, ("start", start), ("row_map", row_map))
-    out = torch.empty(2, batch, pages.kv_heads, count, pages.head_dim, dtype=dtype, device=pages.k.device)
-    k, v = out.unbind(0)
+        raise ValueError("kv_read_paged: batch and count must not be negative")
+    if not ((start is None or _held(start, dev, batch)) and (row_map is None or _held(row_map, dev, batch))):
+        _index("kv_read_paged", dev, batch, ("start", start), ("row_map", row_map))
+    k = torch.empty((batch, pages.kv_heads, count, pages.head_dim), dtype=dtype, device=pages.k.device)
+    v = torch.empty_like(k)
     if batch and count:
-        _call_on(dev, "fg_kv_read_paged", pages.address, batch, _ptr(start), count, _ptr(row_map), k.data_ptr(), v.data_ptr(),
-                 _DT[dtype])
+        _call_on(dev, "fg_kv_read_paged", pages.address, batch, None if start is None else start.data_ptr(), count,
+                 None if row_map is None else row_map.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[dtype])
     return k, v
 
 
@@ -1228,37 +1271,41 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
     the new tokens that a node sees), or None for a causal chain. ``new_len`` int32 [B]: the rows of nodes from new_len[b] on
     stay as they were in ``out`` (bf16, q's shape, apart from q), and nobody sees their tokens. A row that sees no token is 0, and
     infinities and NaN of tokens that it does not see do not reach it."""
-    what = "paged_attention"
-    _paged_sizes(what, pages, kv_heads, head_dim)
-    dev, shape = pages.device, q.shape
-    if q.dtype is not _BF16 or len(shape) != 4 or shape[1:] != (num_nodes, q_heads, head_dim) or not q.is_contiguous() \
-            or q.get_device() != dev:
-        raise ValueError(f"{what}: q must be contiguous bf16 [B, {num_nodes}, {q_heads}, {head_dim}] on the pages' device")
+    _paged_sizes("paged_attention", pages, kv_heads, head_dim)
+    dev, shape, at = pages.device, q.shape, q.data_ptr()
+    given = out is not None
+    if len(shape) != 4:
+        raise ValueError(f"paged_attention: q must be contiguous bf16 [B, {num_nodes}, {q_heads}, {head_dim}]")
     B = shape[0]
-    _index(what, dev, B, ("seq_len", seq_len), ("new_len", new_len), ("row_map", row_map))
-    anc_stride = 0
-    if anc is not None:
+    if not given:
+        out = torch.empty_like(q)
+    into, anc_stride, size = out.data_ptr(), 0, B * num_nodes * q_heads * head_dim
+    ok = (q.dtype is _BF16 is out.dtype and shape == (B, num_nodes, q_heads, head_dim) == out.shape and q.is_contiguous()
+          and out.is_contiguous() and q.get_device() == dev == out.get_device() and not at & 15 and not into & 7
+          and _held(seq_len, dev, B) and (new_len is None or _held(new_len, dev, B)) and (row_map is None or _held(row_map, dev, B))
+          and not (given and at < into + 2 * size and into < at + 2 * size and size))
+    if ok and anc is not None:
         if anc.dtype is not torch.int64:
             raise TypeError("anc must be int64 (bit pattern of the uint64 masks)")
         two = anc.dim() == 2
-        if anc.get_device() != dev or anc.shape != ((B, num_nodes) if two else (num_nodes,)) or (num_nodes > 1 and anc.stride(-1) != 1):
-            raise ValueError(f"{what}: anc must be [{B}, {num_nodes}] or [{num_nodes}] with unit stride on the pages' device")
+        ok = anc.shape == ((B, num_nodes) if two else (num_nodes,)) and (num_nodes == 1 or anc.stride(-1) == 1) and anc.get_device() == dev
         anc_stride = anc.stride(0) if two else 0
-    at = q.data_ptr()
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        if out.dtype is not _BF16 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
-            raise ValueError(f"{what}: out must be a contiguous bf16 tensor of q's shape")
-        _apart(what, ((out.data_ptr(), 2 * q.numel()),), ((at, 2 * q.numel()),))
-    if at % 16 or out.data_ptr() % 8:
-        raise ValueError(f"{what}: q must start 16-byte aligned and out 8-byte aligned")
-    if q.numel() == 0:
+    if not ok:
+        what = "paged_attention"
+        _index(what, dev, B, ("seq_len", seq_len), ("new_len", new_len), ("row_map", row_map))
+        if anc is not None and (anc.get_device() != dev or tuple(anc.shape) not in ((B, num_nodes), (num_nodes,)) or (num_nodes > 1 and anc.stride(-1) != 1)):
+            raise ValueError(f"{what}: anc must be [{B}, {num_nodes}] or [{num_nodes}] with unit stride on the pages' device")
+        if q.dtype is not _BF16 or shape != (B, num_nodes, q_heads, head_dim) or not q.is_contiguous() or at & 15 or q.get_device() != dev:
+            raise ValueError(f"{what}: q must be contiguous 16-byte aligned bf16 [B, {num_nodes}, {q_heads}, {head_dim}] on the pages' device")
+        raise ValueError(f"{what}: out must be a contiguous 8-byte aligned bf16 tensor of q's shape, apart from it")
+    if size == 0:
         return out
     n = _paged_workspace_bytes(B, num_nodes, q_heads, kv_heads, head_dim, pages.width * pages.page_size)
     ws = torch.empty(n, dtype=_U8, device=q.device) if n else None  # the call's own, as in _mx_workspace
-    _call_on(dev, "fg_paged_attention", at, out.data_ptr(), pages.address, B, num_nodes, q_heads, seq_len.data_ptr(), _ptr(new_len),
-             _ptr(row_map), _ptr(anc), anc_stride, 1.0 / math.sqrt(head_dim) if scale is None else float(scale), _ptr(ws), n)
+    _call_on(dev, "fg_paged_attention", at, into, pages.address, B, num_nodes, q_heads, seq_len.data_ptr(),
+             None if new_len is None else new_len.data_ptr(), None if row_map is None else row_map.data_ptr(),
+             None if anc is None else anc.data_ptr(), anc_stride, head_dim ** -0.5 if scale is None else scale,
+             None if ws is None else ws.data_ptr(), n)
     return out
 
 
@@ -1270,11 +1317,13 @@ def kv_path_gather_paged(pages, *, seq_len, acc_nodes, acc_len, tree_nodes, laye
     what = "kv_path_gather_paged"
     if not isinstance(pages, KVPages):
         raise TypeError(f"{what}: pages must be KVPages")
-    dev = pages.device
-    _same_device(what, dev)
-    B = seq_len.numel()
-    _index(what, dev, B, ("seq_len", seq_len), ("acc_len", acc_len), ("acc_nodes", acc_nodes), ("row_map", row_map))
-    _index(what, dev, 1, ("err_flag", err_flag))
+    dev, B = pages.device, seq_len.numel()
+    if dev < 0:
+        _same_device(what, dev)
+    if not (_held(seq_len, dev, B) and _held(acc_len, dev, B) and _held(acc_nodes, dev, B) and (row_map is None or _held(row_map, dev, B))
+            and (err_flag is None or _held(err_flag, dev, 1))):
+        _index(what, dev, B, ("seq_len", seq_len), ("acc_len", acc_len), ("acc_nodes", acc_nodes), ("row_map", row_map))
+        _index(what, dev, 1, ("err_flag", err_flag))
     if acc_nodes.dim() != 2 or acc_nodes.shape[0] != B or not 1 <= acc_nodes.shape[1] <= 32:
         raise ValueError(f"{what}: acc_nodes must be [{B}, 1 to 32]")
     if layers < 1 or not 1 <= tree_nodes <= pages.capacity:

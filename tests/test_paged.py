@@ -238,7 +238,8 @@ def struct(**changed):
     (dict(kv_heads=-1), b"bad sizes"), (dict(table_width=0), b"bad sizes"), (dict(table_rows=0), b"bad sizes"),
     (dict(table_width=2 ** 27, table_stride=2 ** 27), b"2^31 tokens"), (dict(page_stride=4095), b"overlap"), (dict(table_stride=2), b"overlap"),
     (dict(k=4100), b"16-byte"), (dict(page_stride=4104), b"16-byte"), (dict(k_scales=66), b"4-byte"), (dict(scale_stride=126), b"4-byte"),
-    (dict(scale_stride=64), b"overlap"), (dict(page_size=2 ** 20, kv_heads=8, page_stride=2 ** 40, scale_stride=2 ** 40), b"2 GiB"),
+    (dict(scale_stride=64), b"overlap"), (dict(page_size=2 ** 20, kv_heads=8, page_stride=2 ** 30, scale_stride=2 ** 25, table_width=1), b"2^30 elements"),
+    (dict(page_stride=2 ** 31), b"2^31 elements"),
 ])
 def test_descriptions_of_pages_that_every_entry_point_refuses(changed, message):
     _, lib = library()
