@@ -19,7 +19,8 @@ struct Pages {
   uint8_t* ks;  // scales (e4m3)
   uint8_t* vs;
   const int32_t* table;
-  int64_t page_bytes, scale_bytes, table_stride;
+  uint32_t page_bytes, scale_bytes;  // from page to page
+  int64_t table_stride;
   int pages, table_rows, table_width, log2_page, kv_heads;
 
   FG_DEVICE int capacity() const { return table_width << log2_page; }
@@ -28,6 +29,9 @@ struct Pages {
     const int p = row[t >> log2_page];
     return (unsigned)p < (unsigned)pages ? p : -1;
   }
+  // Bytes from page 0 to page p (p >= 0), and from its scales.
+  FG_DEVICE uint64_t at(int p) const { return (uint64_t)(uint32_t)p * page_bytes; }
+  FG_DEVICE uint64_t scales_at(int p) const { return (uint64_t)(uint32_t)p * scale_bytes; }
   // The row of kv head h and token t within its page.
   FG_DEVICE int row_in_page(int h, int t) const { return (h << log2_page) + (t & ((1 << log2_page) - 1)); }
 };
@@ -64,8 +68,8 @@ inline int pages_of(const fg_kv_pages* p, const char* what, Pages& out) {
   out.ks = (uint8_t*)p->k_scales;
   out.vs = (uint8_t*)p->v_scales;
   out.table = p->table;
-  out.page_bytes = p->page_stride * es;
-  out.scale_bytes = p->scale_stride;
+  out.page_bytes = (uint32_t)(p->page_stride * es);
+  out.scale_bytes = (uint32_t)p->scale_stride;
   out.table_stride = p->table_stride;
   out.pages = p->pages;
   out.table_rows = p->table_rows;

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(WriteArgs a, Rows
     const int r = pg.row_in_page(h - Hq, slot);
     if constexpr (FMT == kPageBF16) {
       if (page < 0) continue;
-      uint16_t* dst = (uint16_t*)(pg.k + page * pg.page_bytes) + (int64_t)r * D;
+      uint16_t* dst = (uint16_t*)(pg.k + pg.at(page)) + (int64_t)r * D;
       store4(dst, i0, y1);
       store4(dst, i0 + HALF, y2);
     } else {
@@ -170,11 +170,11 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(WriteArgs a, Rows
       const uint32_t c1 = quantize4(y1, group8_max(amax4(y1)), s1);
       const uint32_t c2 = quantize4(y2, group8_max(amax4(y2)), s2);
       if (page < 0) continue;
-      uint8_t* dst = pg.k + page * pg.page_bytes + (int64_t)r * D;
+      uint8_t* dst = pg.k + pg.at(page) + (int64_t)r * D;
       *(uint32_t*)(dst + i0) = c1;
       *(uint32_t*)(dst + i0 + HALF) = c2;
       if (i0 % fg::kMxBlock == 0) {
-        uint8_t* sc = pg.ks + page * pg.scale_bytes + (int64_t)r * BLOCKS;
+        uint8_t* sc = pg.ks + pg.scales_at(page) + (int64_t)r * BLOCKS;
         sc[i0 / fg::kMxBlock] = (uint8_t)s1;
         sc[(i0 + HALF) / fg::kMxBlock] = (uint8_t)s2;
       }
@@ -186,13 +186,13 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(WriteArgs a, Rows
     in.get4(row, (Hq + Hkv + h) * D + i0, x);
     const int r = pg.row_in_page(h, slot);
     if constexpr (FMT == kPageBF16) {
-      if (page >= 0) store4(pg.v + page * pg.page_bytes, (int64_t)r * D + i0, x);
+      if (page >= 0) store4(pg.v + pg.at(page), (int64_t)r * D + i0, x);
     } else {
       uint32_t s1;
       const uint32_t c = quantize4(x, group8_max(amax4(x)), s1);
       if (page < 0) continue;
-      *(uint32_t*)(pg.v + page * pg.page_bytes + (int64_t)r * D + i0) = c;
-      if (i0 % fg::kMxBlock == 0) pg.vs[page * pg.scale_bytes + (int64_t)r * BLOCKS + i0 / fg::kMxBlock] = (uint8_t)s1;
+      *(uint32_t*)(pg.v + pg.at(page) + (int64_t)r * D + i0) = c;
+      if (i0 % fg::kMxBlock == 0) pg.vs[pg.scales_at(page) + (int64_t)r * BLOCKS + i0 / fg::kMxBlock] = (uint8_t)s1;
     }
   }
 }
@@ -217,12 +217,12 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(Pages pg, int batc
   float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   if (page >= 0) {
     const int row = pg.row_in_page(h, (int)t);
-    const uint8_t* base = (is_v ? pg.v : pg.k) + page * pg.page_bytes;
+    const uint8_t* base = (is_v ? pg.v : pg.k) + pg.at(page);
     if constexpr (FMT == kPageBF16) {
       fg::load8<fg::kBF16>(base, (int64_t)row * D + c, x);
     } else {
       const uint2 w = *(const uint2*)(base + (int64_t)row * D + c);
-      const uint8_t* sc = (is_v ? pg.vs : pg.ks) + page * pg.scale_bytes;
+      const uint8_t* sc = (is_v ? pg.vs : pg.ks) + pg.scales_at(page);
       const float f = fg::mx_scale(sc[(int64_t)row * (D / fg::kMxBlock) + c / fg::kMxBlock]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -300,21 +300,21 @@ __global__ void __launch_bounds__(kThreads) paged_path_gather_kernel(GatherArgs 
     typedef typename std::conditional<BLOCKS == 4, uint32_t, uint16_t>::type S;
 #pragma unroll
     for (int j = 0; j < MAXACC; ++j)
-      v[j] = nd[j] != j ? *(const S*)(base + from[j] * pg.scale_bytes + pg.row_in_page(h, s0 + nd[j]) * BLOCKS) : 0u;
+      v[j] = nd[j] != j ? *(const S*)(base + pg.scales_at(from[j]) + pg.row_in_page(h, s0 + nd[j]) * BLOCKS) : 0u;
 #pragma unroll
     for (int j = 0; j < MAXACC; ++j)
-      if (nd[j] != j) *(S*)(base + to[j] * pg.scale_bytes + pg.row_in_page(h, s0 + j) * BLOCKS) = (S)v[j];
+      if (nd[j] != j) *(S*)(base + pg.scales_at(to[j]) + pg.row_in_page(h, s0 + j) * BLOCKS) = (S)v[j];
     return;
   }
   uint8_t* base = (is_v ? pg.v : pg.k) + (int64_t)(t >> 1) * a.layer_bytes + col * 16;
   uint4 v[MAXACC];
 #pragma unroll
   for (int j = 0; j < MAXACC; ++j)
-    v[j] = nd[j] != j ? *(const uint4*)(base + from[j] * pg.page_bytes + (int64_t)pg.row_in_page(h, s0 + nd[j]) * ROW)
+    v[j] = nd[j] != j ? *(const uint4*)(base + pg.at(from[j]) + (int64_t)pg.row_in_page(h, s0 + nd[j]) * ROW)
                       : make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int j = 0; j < MAXACC; ++j)
-    if (nd[j] != j) *(uint4*)(base + to[j] * pg.page_bytes + (int64_t)pg.row_in_page(h, s0 + j) * ROW) = v[j];
+    if (nd[j] != j) *(uint4*)(base + pg.at(to[j]) + (int64_t)pg.row_in_page(h, s0 + j) * ROW) = v[j];
 }
 
 template <bool PARTS>

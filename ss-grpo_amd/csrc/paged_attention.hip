@@ -86,7 +86,8 @@ FG_DEVICE int part_keys(int keys, int splits, int tile) {
   return ((keys + n - 1) / n + tile - 1) / tile * tile;
 }
 
-// 16 e4m3 codes times 2^(s - 127) as bf16 (exact).
+// 16 e4m3 codes times 2^(s - 127) as bf16: exact, and NaN for s = 255 (a float scale of infinity makes the conversion answer NaN
+// for every code, zero included).
 FG_DEVICE void expand16(u32x4 w, uint32_t s, u32x4& lo, u32x4& hi) {
   const float f = __uint_as_float(s << 23);
 #pragma unroll
@@ -115,10 +116,10 @@ FG_DEVICE bool not_finite(u32x4 w) {
 // One element of V as a float.
 template <int FMT, int D>
 FG_DEVICE float v_element(const Pages& pg, int page, int r, int d) {
-  const uint8_t* base = pg.v + page * pg.page_bytes;
+  const uint8_t* base = pg.v + pg.at(page);
   if constexpr (FMT == kPageBF16) return fg::bf16_to_f32(((const uint16_t*)base)[(int64_t)r * D + d]);
   const auto x = __builtin_amdgcn_cvt_pk_f32_fp8((int)base[(int64_t)r * D + d], false);
-  return x[0] * fg::mx_scale(pg.vs[page * pg.scale_bytes + (int64_t)r * (D / fg::kMxBlock) + d / fg::kMxBlock]);
+  return x[0] * fg::mx_scale(pg.vs[pg.scales_at(page) + (int64_t)r * (D / fg::kMxBlock) + d / fg::kMxBlock]);
 }
 
 // Infinities and NaN of V at tokens that only some rows see (the new tokens' tiles). The loops keep them at 0 there, since p = 0
@@ -209,11 +210,11 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       const bool ok = (unsigned)found < (unsigned)pg.pages;
       x.paged |= (uint32_t)ok << u;
       const uint32_t row = head_row + ((uint32_t)key & slot_mask & ~(uint32_t)(KPW - 1));
-      const int64_t at = (ok ? found : 0) * pg.page_bytes + (int64_t)row * (CPK * 16);
+      const uint64_t at = pg.at(ok ? found : 0) + row * (CPK * 16);
       x.kp[u] = *(const u32x4*)(pg.k + at + (uint32_t)lane * 16);
       x.vp[u] = *(const u32x4*)(pg.v + at + (uint32_t)lane * 16);
       if constexpr (FMT == kPageE4M3) {
-        const int64_t sat = (ok ? found : 0) * pg.scale_bytes + (int64_t)row * BLOCKS;
+        const uint64_t sat = pg.scales_at(ok ? found : 0) + row * BLOCKS;
         x.ksc[u] = (pg.ks + sat)[sc_lane];
         x.vsc[u] = (pg.vs + sat)[sc_lane];
       }
@@ -294,18 +295,6 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       if (gone && lane == 0) {
         atomicOr((unsigned long long*)&no_page[slot][kw], gone);
         gone_any[slot][kw] = 1;
-      }
-    }
-    if constexpr (FMT == kPageE4M3) {
-      uint32_t most = 0;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) most = max(most, max(x.ksc[u], x.vsc[u]));
-      if (__any(most == 255u)) {
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {  // NaN blocks
-          if (x.ksc[u] == 255u) x.kp[u] = u32x4(0x7f7f7f7fu), x.ksc[u] = 127u;
-          if (x.vsc[u] == 255u) x.vp[u] = u32x4(0x7f7f7f7fu), x.vsc[u] = 127u;
-        }
       }
     }
 #pragma unroll
@@ -573,7 +562,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
       const bool ok = (unsigned)found < (unsigned)pg.pages;
       t.there |= (int)ok << h;
       const uint32_t row = head_row + ((uint32_t)key & slot_mask & ~15u);
-      const int64_t at = (ok ? found : 0) * pg.page_bytes + (int64_t)row * (D * ES);
+      const uint64_t at = pg.at(ok ? found : 0) + row * (D * ES);
       const uint8_t* kr = pg.k + at;
       const uint8_t* vr = pg.v + at;
 #pragma unroll
@@ -581,7 +570,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
 #pragma unroll
       for (int s = 0; s < NL; ++s) t.v[h * NL + s] = *(const u32x4*)(vr + (uint32_t)lane * 16 + s * 1024);
       if constexpr (FMT == kPageE4M3) {
-        const int64_t sat = (ok ? found : 0) * pg.scale_bytes + (int64_t)row * BLOCKS;
+        const uint64_t sat = pg.scales_at(ok ? found : 0) + row * BLOCKS;
         const uint8_t* ks = pg.ks + sat;
         const uint8_t* vs = pg.vs + sat;
         t.ks[h] = BLOCKS == 4 ? *(const uint32_t*)(ks + i16 * 4) : *(const uint16_t*)(ks + i16 * 2);
@@ -663,16 +652,6 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
       }
       if (__any(odd)) odd_from = min(odd_from, first), odd_to = min(first + 32, end);
     }
-    if constexpr (FMT == kPageE4M3) {
-      uint32_t most = 0;
-#pragma unroll
-      for (int s = 0; s < 2 * NL; ++s) most = max(most, cur.vs[s]);
-      if (__any(most == 255u)) {
-#pragma unroll
-        for (int s = 0; s < 2 * NL; ++s)  // NaN blocks
-          if (cur.vs[s] == 255u) cur.v[s] = u32x4(0x7f7f7f7fu), cur.vs[s] = 127u;
-      }
-    }
 #pragma unroll
     for (int s = 0; s < 2 * NL; ++s) {
       const int j = s * (64 / CPK) + lane / CPK, c = lane % CPK;
@@ -698,11 +677,6 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
         if constexpr (FMT == kPageE4M3) {
           const uint32_t e = __builtin_amdgcn_ubfe(cur.ks[h], (uint32_t)(16 * s + 8 * (gq >> 1)), 8u);
           expand16(cur.k[h][s], e, part[0], part[1]);
-          if (__any(e == 255u)) {  // a NaN block
-            const uint32_t nan = e == 255u ? 0x7fc07fc0u : 0u;
-            part[0] |= u32x4(nan);
-            part[1] |= u32x4(nan);
-          }
 #pragma unroll
           for (int c = 0; c < NQ; ++c)
 #pragma unroll
