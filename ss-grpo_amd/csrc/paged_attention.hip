@@ -34,16 +34,21 @@ struct PagedAttn {
   int64_t anc_stride;
   int batch, N, Hq;
   float scale;
-  int splits;  // parts that a sequence's keys may be cut into
-  float* o_part;
-  float2* ml_part;
+  int slots;   // parts that the sequences' keys may be cut into together (a kv head's, of a row tile); 0: none is cut
+  int most;    // parts of one sequence at most
+  float* o_part;    // [slots][N, Hq, D]
+  float2* ml_part;  // [slots][N, Hq]
+  int2* shares;     // [B] a sequence's first slot and its parts
 };
 
 constexpr float kRescaleSlack = 8.0f;  // log2 units
 constexpr int kMinPartKeys = 256;      // a part of a sequence's keys is at least so long
-constexpr int kMaxParts = 256;
-constexpr int kStreamWaves = 8;          // of a workgroup of the stream kernel
+constexpr int kCUs = 256;
+constexpr int kMaxRanked = 512;        // sequences that are put in order: a thread each
+constexpr int kMaxCut = 64;            // sequences that are cut: a lane each
+constexpr int kStreamWaves = 8;        // of a workgroup of the stream kernel
 
+FG_DEVICE int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 FG_DEVICE int c_row32(int i, int lane) { return (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3); }
 
 // Bits j < n of a 64-bit mask.
@@ -80,10 +85,105 @@ FG_DEVICE Span span_of(const PagedAttn& a, int b) {
 FG_DEVICE int keys_of(const PagedAttn& a, const Span& s) {
   return s.row < 0 ? 0 : min(s.committed + s.fresh, a.pages.capacity());
 }
-// Parts of a sequence's keys, and a part's length (a multiple of `tile`).
-FG_DEVICE int part_keys(int keys, int splits, int tile) {
-  const int n = min(splits, max(1, (keys + kMinPartKeys - 1) / kMinPartKeys));
-  return ((keys + n - 1) / n + tile - 1) / tile * tile;
+// What a workgroup does: a sequence's keys [begin, end), and the slot of its partial result. b < 0: nothing.
+struct Work {
+  Span seq;
+  int b, begin, end, slot;
+};
+
+// Sums over the lanes up to each: row shifts, then the last lane of each row and of the lower half to those behind.
+template <typename T>
+FG_DEVICE T scan_add(T x) {
+#define FG_ADD(ctrl, rows) x += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, false))
+  FG_ADD(0x111, 0xf);
+  FG_ADD(0x112, 0xf);
+  FG_ADD(0x114, 0xf);
+  FG_ADD(0x118, 0xf);
+  FG_ADD(0x142, 0xa);
+  FG_ADD(0x143, 0xc);
+#undef FG_ADD
+  return x;
+}
+
+// Which part of which sequence is slot idx, from lengths that only the device knows. A sequence of k keys gets 1 + floor((k - 1) f)
+// parts of equal length, f the same for all: as large as the slots allow (all of them over all keys, else five steps of bisection
+// down to slots - batch, with which the parts always fit). Every wave works that out for itself, a lane a sequence; the first
+// workgroup leaves the shares for the kernel that joins the parts. (A token over 65536 keys beside seven over 1000, at 8B: 44 us, with the same number of parts for each sequence
+// 102; 3 verify rounds of 29 over 1096 to 4096 at 14B: 31 and 40. What it costs: 0.3 us of 9.6 for a few tokens over short lengths.)
+template <int TILE>
+FG_DEVICE Work cut_work(const PagedAttn& a, int idx) {
+  const int lane = threadIdx.x & 63;
+  const Span s = span_of(a, min(lane, a.batch - 1));
+  const int keys = lane < a.batch && s.fresh ? keys_of(a, s) : 0;
+  const float sum = fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan_add((float)keys)), 63)), 1.0f);
+  int n, upto;  // a lane's parts, and the parts up to it
+  auto fits = [&](float f) __attribute__((always_inline)) {
+    n = keys ? min(1 + (int)((float)(keys - 1) * f), a.most) : 0;
+    upto = scan_add(n);
+    return __builtin_amdgcn_readlane(upto, 63) <= a.slots;
+  };
+  float high = fminf((float)a.slots / sum, 1.0f / kMinPartKeys), low = fminf((float)(a.slots - a.batch) / sum, high);
+  if (!fits(high)) {
+    for (int step = 0; step < 5; ++step) {
+      const float f = 0.5f * (low + high);
+      const bool ok = fits(f);
+      high = ok ? high : f;
+      low = ok ? f : low;
+    }
+    if (!fits(low)) fits(low * (1.0f - 1e-4f));  // (one part more by rounding)
+  }
+  if (blockIdx.x == 0 && threadIdx.x < 64 && lane < a.batch) a.shares[lane] = make_int2(upto - n, n);
+  const uint64_t it = __ballot((unsigned)(idx - (upto - n)) < (unsigned)n);
+  if (!it) return {{0, 0, -1}, -1, 0, 0, 0};
+  const int b = __builtin_ctzll(it);
+  auto of = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, b); };
+  const int all = of(keys), parts = of(n), p = idx - of(upto - n);
+  const int part = ((all + parts - 1) / parts + TILE - 1) & ~(TILE - 1);
+  const int begin = (int)min((int64_t)p * part, (int64_t)all);
+  return {{of(s.committed), of(s.fresh), of(s.row)}, b, begin, (int)min((int64_t)begin + part, (int64_t)all), idx};
+}
+
+// The sequence with the idx-th most keys: more workgroups than CUs go longest first, so that no long one begins when the others
+// end (64 tokens over 1096 to 4096 keys at 8B 71.5 -> 65.4 us, 128 verify rounds of 29 over 548 to 2048 at 7B 128 -> 111; with
+// equal lengths the count costs 0.5 us for 64 and 2.4 us for 128 sequences, of 67 and 56). A sequence's rank is how many go
+// before it, counted by as many threads as there are for each.
+FG_DEVICE Work ranked_work(const PagedAttn& a, int idx, unsigned char* scratch, int* pick) {
+  const int i = threadIdx.x;
+  int* const keys = (int*)scratch;
+  int4* const spans = (int4*)(scratch + kMaxRanked * 4);
+  int k = -1;
+  if (i < a.batch) {
+    const Span s = span_of(a, i);
+    k = s.fresh ? keys_of(a, s) : 0;
+    spans[i] = make_int4(s.committed, s.fresh, s.row, i);
+  }
+  keys[i] = k;
+  __syncthreads();
+  int each = 0;  // log2 of the threads that count for a sequence
+  while (each < 6 && (a.batch << (each + 1)) <= kMaxRanked) ++each;
+  const int j = i >> each;
+  k = keys[j];
+  int r = 0;
+  for (int c = (i - (j << each)) * 4; c < a.batch; c += 4 << each) {
+    const int4 x = *(const int4*)(keys + c);
+    r += (x.x > k - (c < j)) + (x.y > k - (c + 1 < j)) + (x.z > k - (c + 2 < j)) + (x.w > k - (c + 3 < j));
+  }
+  for (int x = 1; x < 1 << each; x <<= 1) r += __shfl_xor(r, x, 64);
+  if (i == j << each && j < a.batch && r == idx) *(int4*)pick = spans[j];
+  __syncthreads();  // (after it the tiles may lie where these lay)
+  const int4 x = *(const int4*)pick;
+  const Span s = {x.x, x.y, x.z};
+  return {s, x.w, 0, keys_of(a, s), 0};
+}
+
+// The work of workgroup idx of a kv head and row tile (the same in all its threads: scalars); A workgroup has
+// kMaxRanked threads and at least 20 bytes of scratch for each.
+template <int TILE>
+FG_DEVICE Work work_of(const PagedAttn& a, int idx, unsigned char* scratch, int* pick) {
+  if (a.slots) return cut_work<TILE>(a, idx);
+  if (gridDim.x > kCUs && a.batch <= kMaxRanked) return ranked_work(a, idx, scratch, pick);
+  const Span s = span_of(a, idx);
+  return {s, idx, 0, keys_of(a, s), 0};
 }
 
 // 16 e4m3 codes times 2^(s - 127) as bf16: exact, and NaN for s = 255 (a float scale of infinity makes the conversion answer NaN
@@ -169,19 +269,28 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   __shared__ int gone_any[3][KW], odd_any;  // whether there are any; whether V was kept at 0 where it is not finite
 
   const Pages& pg = a.pages;
-  const int unit = blockIdx.x / m_tiles, mt = blockIdx.x % m_tiles;
-  const int sp = unit % a.splits, hkv = unit / a.splits % pg.kv_heads, b = unit / (a.splits * pg.kv_heads);
+  static_assert(KW * T == kMaxRanked && sizeof(lds) >= 20 * kMaxRanked, "threads and LDS of work_of");
+  __shared__ __attribute__((aligned(16))) int pick[4];
+  int unit = blockIdx.x / m_tiles, mt = blockIdx.x % m_tiles;
+  if (gridDim.x > kCUs) {
+    // The row tiles of a unit on one XCD (workgroups go to the eight in turn), those with the most keys first: 4 x 1024 tokens
+    // 110.5 -> 105 us, on bf16 pages 136 -> 129.5, 8 x 512 at 7B's heads 225 -> 214.
+    const int whole = gridDim.x / m_tiles & ~7u, turn = blockIdx.x / 8;
+    if ((int)(blockIdx.x / m_tiles) < whole) unit = turn / m_tiles * 8 + blockIdx.x % 8, mt = turn % m_tiles;
+    mt = m_tiles - 1 - mt;
+  }
+  const int hkv = unit % pg.kv_heads;
+  const Work work = work_of<KB>(a, unit / pg.kv_heads, lds, pick);
+  const int b = scalar(work.b);
+  if (b < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   const int rw = wave % RW, kw = wave / RW;
   const int G = a.Hq / pg.kv_heads;
-  const Span seq = span_of(a, b);
+  const Span seq = {scalar(work.seq.committed), scalar(work.seq.fresh), scalar(work.seq.row)};
   const int M = G * seq.fresh;
   if (mt * ROWS >= M) return;  // rows behind the sequence's new tokens stay as they are
-  const int keys = keys_of(a, seq);
-  const int part = part_keys(keys, a.splits, KB);
   const int last = a.anc ? seq.fresh : (min((mt + 1) * ROWS, M) - 1) / G + 1;  // a chain's rows see no later token
-  const int begin = min(sp * part, keys);
-  const int end = max(begin, min(min(begin + part, keys), seq.committed + last));
+  const int begin = scalar(work.begin), end = max(begin, min(scalar(work.end), seq.committed + last));
   const int s0 = seq.committed, clear = a.anc ? s0 : s0 + mt * ROWS / G + 1;  // every row sees the keys before `clear`
   const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
   unsigned char* const group = lds + kw * 2 * TILE;
@@ -463,8 +572,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
         s[0] += f * x.x; s[1] += f * x.y; s[2] += f * x.z; s[3] += f * x.w;
       }
       const int64_t orow = ((int64_t)b * a.N + gr / G) * a.Hq + hkv * G + gr % G;
-      if (a.splits > 1) {
-        const int64_t prow = (int64_t)sp * a.batch * a.N * a.Hq + orow;
+      if (a.slots) {
+        const int64_t prow = orow + (int64_t)(scalar(work.slot) - b) * a.N * a.Hq;
         *(float4*)(a.o_part + prow * D + d0) = make_float4(s[0], s[1], s[2], s[3]);
         if (d0 == 0) a.ml_part[prow] = make_float2(mx, den);
       } else {
@@ -476,8 +585,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   } else {
     if (!row_ok) return;
     const int64_t orow = ((int64_t)b * a.N + qn) * a.Hq + qh;
-    if (a.splits > 1) {
-      const int64_t prow = (int64_t)sp * a.batch * a.N * a.Hq + orow;
+    if (a.slots) {
+      const int64_t prow = orow + (int64_t)(scalar(work.slot) - b) * a.N * a.Hq;
 #pragma unroll
       for (int db = 0; db < ND; ++db)
 #pragma unroll
@@ -532,15 +641,18 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   constexpr int MERGE = W * NQ * 16 * (OROW * 4 + 8);
   __shared__ __attribute__((aligned(16))) unsigned char lds[W * VTILE > MERGE ? W * VTILE : MERGE];
   const Pages& pg = a.pages;
-  const int unit = blockIdx.x;
-  const int sp = unit % a.splits, hkv = unit / a.splits % pg.kv_heads, b = unit / (a.splits * pg.kv_heads);
+  static_assert(W * 64 == kMaxRanked && sizeof(lds) >= 20 * kMaxRanked, "threads and LDS of work_of");
+  __shared__ __attribute__((aligned(16))) int pick[4];
+  const int hkv = blockIdx.x % pg.kv_heads;
+  const Work work = work_of<32>(a, blockIdx.x / pg.kv_heads, lds, pick);
+  const int b = scalar(work.b);
+  if (b < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gq = lane >> 4, i16 = lane & 15;
   const int G = a.Hq / pg.kv_heads;
-  const Span seq = span_of(a, b);
+  const Span seq = {scalar(work.seq.committed), scalar(work.seq.fresh), scalar(work.seq.row)};
   const int M = G * seq.fresh;
   if (M == 0) return;
-  const int keys = keys_of(a, seq), part = part_keys(keys, a.splits, 32), s0 = seq.committed;
-  const int begin = min(sp * part, keys), end = min(begin + part, keys);
+  const int begin = scalar(work.begin), end = scalar(work.end), s0 = seq.committed;
   const const_i32* trow = (const const_i32*)(uintptr_t)(pg.table + (int64_t)max(seq.row, 0) * pg.table_stride);
   unsigned char* const vt = lds + wave * VTILE;
   typedef StreamTile<FMT, D> Tile;
@@ -792,8 +904,8 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
       s[0] += f * x.x; s[1] += f * x.y; s[2] += f * x.z; s[3] += f * x.w;
     }
     const int64_t orow = ((int64_t)b * a.N + r / G) * a.Hq + hkv * G + r % G;
-    if (a.splits > 1) {
-      const int64_t prow = (int64_t)sp * a.batch * a.N * a.Hq + orow;
+    if (a.slots) {
+      const int64_t prow = orow + (int64_t)(scalar(work.slot) - b) * a.N * a.Hq;
       *(float4*)(a.o_part + prow * D + d0) = make_float4(s[0], s[1], s[2], s[3]);
       if (d0 == 0) a.ml_part[prow] = make_float2(mx, den);
     } else {
@@ -804,37 +916,36 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   }
 }
 
-// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims of a part. Up to 8 parts: D / 4
-// threads a row. More (WIDE): a workgroup a row, 1024 / D parts side by side. A thread reads a part's (m, l), so that all
+// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims of a part. Up to D / 4 parts:
+// D / 4 threads a row. More (WIDE): a workgroup a row, 1024 / D parts side by side. A thread reads a part's (m, l), so that all
 // of them take one round trip, and no load of O waits for another.
 template <int D, bool WIDE>
-__global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int tile) {
-  constexpr int LANES = D / 4, SLOTS = WIDE ? 256 / LANES : 1, PER = 256 / (LANES * SLOTS), MOST = WIDE ? kMaxParts : 8;
+__global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a) {
+  constexpr int LANES = D / 4, SLOTS = WIDE ? 256 / LANES : 1, PER = 256 / (LANES * SLOTS), MOST = LANES * SLOTS;
   __shared__ float weight[PER][MOST], wave_at[8];
   __shared__ float4 sums[WIDE ? 256 : 1];
   const int ti = threadIdx.x % (LANES * SLOTS), in = threadIdx.x / (LANES * SLOTS), slot = ti / LANES, d0 = ti % LANES * 4;
-  const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
+  const int64_t rows = (int64_t)a.batch * a.N * a.Hq, step = (int64_t)a.N * a.Hq;
   const int64_t row = min((int64_t)blockIdx.x * PER + in, rows - 1);  // (behind the last row: it once more)
-  const int n = (int)(row / a.Hq % a.N), b = (int)(row / a.Hq / a.N);
-  const Span seq = span_of(a, b);
-  const int keys = keys_of(a, seq), part = part_keys(keys, a.splits, tile);
-  const int parts = part > 0 && n < seq.fresh ? min(a.splits, (keys + part - 1) / part) : 0;
-  const float2 ml = ti < parts ? a.ml_part[ti * rows + row] : make_float2(-INFINITY, 0.0f);
+  const int n = (int)(row / a.Hq % a.N), b = (int)(row / step);
+  const bool asked = n < (a.new_len ? min(max(a.new_len[b], 0), a.N) : a.N);
+  const int2 share = a.shares[b];
+  const int parts = asked ? share.y : 0;
+  const int64_t first = share.x * step + row % step;
+  const float2 ml = ti < parts ? a.ml_part[ti * step + first] : make_float2(-INFINITY, 0.0f);
   float mx = ml.x, den;
   if constexpr (WIDE) {
-    static_assert(kMaxParts <= 256, "a thread per part");
     mx = fg::wave_max(mx);
     if ((threadIdx.x & 63) == 0) wave_at[threadIdx.x >> 6] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(wave_at[0], wave_at[1]), fmaxf(wave_at[2], wave_at[3]));
   } else {
 #pragma unroll
-    for (int x = 4; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
-    mx = __shfl(mx, (threadIdx.x & 63) / LANES * LANES, 64);
+    for (int x = LANES / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
   }
   const float w = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx));
   den = w * ml.y;
-  if (ti < MOST) weight[in][ti] = w;
+  weight[in][ti] = w;
   if constexpr (WIDE) {
     den = fg::wave_sum(den);
     if ((threadIdx.x & 63) == 0) wave_at[4 + (threadIdx.x >> 6)] = den;
@@ -842,15 +953,14 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int til
     den = wave_at[4] + wave_at[5] + wave_at[6] + wave_at[7];
   } else {
 #pragma unroll
-    for (int x = 4; x; x >>= 1) den += __shfl_xor(den, x, 64);
-    den = __shfl(den, (threadIdx.x & 63) / LANES * LANES, 64);
+    for (int x = LANES / 2; x; x >>= 1) den += __shfl_xor(den, x, 64);
     __syncthreads();
   }
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int p0 = slot; p0 < parts; p0 += 4 * SLOTS) {
     float4 x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = *(const float4*)(a.o_part + (min(p0 + u * SLOTS, parts - 1) * rows + row) * D + d0);
+    for (int u = 0; u < 4; ++u) x[u] = *(const float4*)(a.o_part + (min(p0 + u * SLOTS, parts - 1) * step + first) * D + d0);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const float f = p0 + u * SLOTS < parts ? weight[in][p0 + u * SLOTS] : 0.0f;
@@ -867,44 +977,47 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a, int til
       o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
     }
   }
-  if (n >= seq.fresh) return;
+  if (!asked) return;
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   *(uint2*)((uint16_t*)a.out + row * D + d0) =
       make_uint2(fg::pack_bf16x2(o.x * inv, o.y * inv), fg::pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 struct Plan {
-  int rw, kw, kb, splits;
+  int rw, kw, kb, slots;
   int rows() const { return rw * 32; }
-  int tile() const { return kb; }
+  // Narrow rows of the kernel that joins the parts, or a workgroup for each.
+  bool wide(int batch) const { return slots > 8 * batch; }
 };
 
 Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int64_t capacity) {
   const int64_t m = (int64_t)(q_heads / kv_heads) * num_nodes;
   // Eight waves, one workgroup per CU: row tiles side by side as far as there are rows, the rest of the waves on other keys.
   Plan p;
-  if (m <= 32) p = {1, kStreamWaves, 32, 1};
-  else if (m <= 64) p = {2, 4, 32, 1};
-  else if (m <= 128 || head_dim == 64) p = {4, 2, 64, 1};
-  else p = {8, 1, 64, 1};
-  const int64_t base = (int64_t)batch * kv_heads * ((m + p.rows() - 1) / p.rows());
-  if (base < 256) {
+  if (m <= 32) p = {1, kStreamWaves, 32, 0};
+  else if (m <= 64) p = {2, 4, 32, 0};
+  else if (m <= 128 || head_dim == 64) p = {4, 2, 64, 0};
+  else p = {8, 1, 64, 0};
+  const int64_t each = kv_heads * ((m + p.rows() - 1) / p.rows());  // workgroups of a sequence that is not cut
+  // Parts where every sequence gets two at least (20 tokens over 2048 keys at 8B, 160 workgroups: whole 19.5 us, in 320 parts 28),
+  // and no more workgroups than CUs, which would take two rounds (3 over 8192: 264 workgroups 22.5 us, 256 17.6).
+  if (batch <= kMaxCut && 2 * batch * each <= kCUs) {
     const int64_t most = std::max<int64_t>(1, capacity / kMinPartKeys);
-    p.splits = (int)std::min<int64_t>(std::min<int64_t>((255 + base) / base, most), kMaxParts);
+    p.slots = (int)std::min<int64_t>(kCUs / each, batch * most);
+    if (p.slots < 2 * batch) p.slots = 0;
   }
   return p;
 }
 
 int64_t workspace_of(const Plan& p, int batch, int num_nodes, int q_heads, int head_dim) {
-  if (p.splits <= 1) return 0;
-  return (int64_t)p.splits * batch * num_nodes * q_heads * (head_dim * 4 + 8);
+  return p.slots ? (int64_t)p.slots * num_nodes * q_heads * (head_dim * 4 + 8) + batch * 8ll : 0;
 }
 
 template <int FMT, int D>
 void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   const int64_t m = (int64_t)(a.Hq / a.pages.kv_heads) * a.N;
   const int m_tiles = (int)((m + p.rows() - 1) / p.rows());
-  const dim3 grid((unsigned)((int64_t)a.batch * a.pages.kv_heads * a.splits * m_tiles)), block(p.rw * p.kw * 64);
+  const dim3 grid((unsigned)((int64_t)(a.slots ? a.slots : a.batch) * a.pages.kv_heads * m_tiles)), block(p.rw * p.kw * 64);
   if (m <= 16)
     hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 1>), grid, block, 0, s, a);
   else if (m <= 32)
@@ -915,13 +1028,12 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 2, 64>), grid, block, 0, s, a, m_tiles);
   else
     hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64>), grid, block, 0, s, a, m_tiles);
-  if (a.splits > 1) {
+  if (a.slots) {
     const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
-    if (a.splits > 8)
-      hipLaunchKernelGGL((paged_combine_kernel<D, true>), dim3((unsigned)rows), dim3(256), 0, s, a, p.tile());
+    if (p.wide(a.batch))
+      hipLaunchKernelGGL((paged_combine_kernel<D, true>), dim3((unsigned)rows), dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((paged_combine_kernel<D, false>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, s, a,
-                         p.tile());
+      hipLaunchKernelGGL((paged_combine_kernel<D, false>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, s, a);
   }
 }
 
@@ -961,13 +1073,15 @@ extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* p
   a.scale = scale;
   Plan p = plan_of(batch, num_nodes, q_heads, pages->kv_heads, pages->head_dim, (int64_t)pages->table_width * pages->page_size);
   const int64_t need = workspace_of(p, batch, num_nodes, q_heads, pages->head_dim);
-  if (need && (!workspace || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 15))) p.splits = 1;
+  if (need && (!workspace || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 15))) p.slots = 0;
   const int64_t m = (int64_t)(q_heads / pages->kv_heads) * num_nodes;
-  FG_REQUIRE((int64_t)batch * pages->kv_heads * p.splits * ((m + p.rows() - 1) / p.rows()) < (1ll << 31),
+  FG_REQUIRE((int64_t)batch * pages->kv_heads * ((m + p.rows() - 1) / p.rows()) < (1ll << 31),
              "fg_paged_attention: bad shape (too many workgroups)");
-  a.splits = p.splits;
+  a.slots = p.slots;
+  a.most = p.wide(batch) ? 256 : pages->head_dim / 4;
   a.o_part = (float*)workspace;
-  a.ml_part = (float2*)((char*)workspace + (int64_t)p.splits * batch * num_nodes * q_heads * pages->head_dim * 4);
+  a.ml_part = (float2*)(a.o_part + (int64_t)p.slots * num_nodes * q_heads * pages->head_dim);
+  a.shares = (int2*)(a.ml_part + (int64_t)p.slots * num_nodes * q_heads);
   hipStream_t s = (hipStream_t)stream;
   if (pages->format == kPageE4M3)
     pages->head_dim == 128 ? launch<kPageE4M3, 128>(a, p, s) : launch<kPageE4M3, 64>(a, p, s);

@@ -303,5 +303,5 @@ def test_workspace_only_where_parts_are_made():
     assert w(64, 29, 28, 4, 128, 4096) == 0 and w(64, 1, 32, 8, 128, 131072) == 0    # a workgroup per CU without it
     assert w(1, 1, 12, 2, 128, 256) == 0                                              # too short to cut
     few = w(2, 1, 32, 8, 128, 131072)
-    assert few > 0 and few % (2 * 32 * (128 * 4 + 8)) == 0                            # (O, m, l) of every row and part
+    assert few == 256 // 8 * 32 * (128 * 4 + 8) + 2 * 8                              # (O, m, l) of a row in 32 parts, each sequence's share
     assert w(0, 1, 32, 8, 128, 4096) == 0 and w(1, 1, 32, 8, 96, 4096) == 0 and w(1, 1, 5, 2, 128, 4096) == 0
