@@ -8,6 +8,7 @@
 #include "fg_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -253,17 +254,22 @@ FG_DEVICE void wave_barrier() {  // a wave's LDS operations are done in order; t
 // exchange with the other half-wave, and P^T goes from the accumulators straight into O^T += V^T P^T, rounded to bf16 once (2^-9
 // of each weight in the mean, the error of the bf16 output again); the sum is that of the rounded weights. The groups merge
 // their (m, l, O) at the end through LDS, the parts by a second kernel.
-template <int FMT, int D, int RW, int KW, int KB>
+//
+// SHARED, for five or six 32-row blocks: waves w and w + 4 sit on one SIMD, so that a fifth block doubles the time of a tile. Two waves
+// take 32 keys each of every tile for such a block instead, and join their results at the end (32 verify rounds of 29 over 3096 to
+// 4096 keys at 14B, 145 rows: 124 -> 114 us, on bf16 pages 130 -> 124). Steps of 32 keys cost rows that are not shared 2 to 5 %
+// (203 rows 77.3 -> 79.3, 4 x 1024 tokens 101 -> 106).
+template <int FMT, int D, int RW, int KW, int KB, bool SHARED>
 __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a, int m_tiles) {
   constexpr int T = RW * 64, ROWS = RW * 32;
   constexpr int CPK = D * fg::page_elem_bytes<FMT> / 16;  // 16-byte pieces of a K or V row
   constexpr int NU = KB * CPK / T, KPW = 64 / CPK;        // pieces of a tile's K (and of its V) per thread; keys of a load
   constexpr int CHUNKS = FMT == kPageBF16 ? 1 : 2;        // 16-byte chunks that a piece is as bf16
   constexpr int KROW = D * 2 + 16, VROW = D * 2, BLOCKS = D / fg::kMxBlock;
-  constexpr int NB = KB / 32, ND = D / 32, NS = D / 16;
-  static_assert(KB * CPK % T == 0 && NU >= 1 && NU <= 32 && KPW <= 16 && KB <= 64, "pieces");
+  constexpr int ND = D / 32, NS = D / 16;
+  static_assert(KB * CPK % T == 0 && NU >= 1 && NU <= 32 && KPW <= 16 && KB <= 64 && (!SHARED || (RW == 8 && KB == 64)), "pieces");
   constexpr int TILE = KB * (KROW + VROW);
-  constexpr int MERGE = KW > 1 ? RW * KW * 32 * ((D + 4) * 4 + 8) : 0;
+  constexpr int MERGE = KW > 1 ? RW * KW * 32 * ((D + 4) * 4 + 8) : SHARED ? RW * 32 * (D * 4 + 16) : 0;
   __shared__ __attribute__((aligned(16))) unsigned char lds[KW * 2 * TILE > MERGE ? KW * 2 * TILE : MERGE];
   __shared__ uint64_t no_page[3][KW];  // a tile's keys without a page
   __shared__ int gone_any[3][KW], odd_any;  // whether there are any; whether V was kept at 0 where it is not finite
@@ -341,7 +347,13 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     lookup(key_of(DEPTH));
   }
 
-  const int row0 = mt * ROWS + rw * 32, r = row0 + l32;
+  // A wave's 32-row block, and which of its sharers this is.
+  int block = rw, share = 0, sharers = 1;
+  if constexpr (SHARED) {
+    const int half = rw >> 2, in = rw & 3, blocks = min(max((M - mt * ROWS + 31) / 32 - 4 * half, 0), 4);
+    if (blocks == 1 || blocks == 2) share = in / blocks, sharers = 2, block = share < 2 ? 4 * half + in % blocks : RW;
+  }
+  const int row0 = block < RW ? mt * ROWS + block * 32 : M, r = row0 + l32;
   const bool row_ok = r < M;
   const int qn = row_ok ? r / G : 0, qh = hkv * G + (row_ok ? r % G : 0);
   const uint64_t anc = (row_ok && a.anc) ? a.anc[(int64_t)b * a.anc_stride + qn] : 0ull;
@@ -423,8 +435,11 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     }
   };
 
-  auto compute = [&](int first, int buf, int slot) __attribute__((always_inline)) {
-    const unsigned char* const at = group + buf * TILE;
+  // Keys first .. first + 32 nb - 1, which lie `from` keys into the tile.
+  auto compute = [&](auto nb, int first, int from, int buf, int slot) __attribute__((always_inline)) {
+    constexpr int NB = decltype(nb)::value, KEYS = 32 * NB;
+    const unsigned char* const at = group + buf * TILE + from * KROW;
+    const unsigned char* const v_base = group + buf * TILE + from * VROW;
     const int is_gone = __builtin_amdgcn_readfirstlane(gone_any[slot][kw]);
     bf16x8 fr[NB * NS];
     // all K fragments before the first MFMA (one LDS latency)
@@ -441,9 +456,9 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       for (int s = 0; s < NS; ++s)
         sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[kb * NS + s], qf[s], sc[kb], 0, 0, 0);
     }
-    if (first + KB > clear || first + KB > end || is_gone) {
+    if (first + KEYS > clear || first + KEYS > end || is_gone) {
       uint64_t sees = (a.anc ? seen_mask(s0 - first, bits) : low_bits(s0 + qn + 1 - first)) & low_bits(end - first);
-      if (is_gone) sees &= ~no_page[slot][kw];
+      if (is_gone) sees &= ~(no_page[slot][kw] >> from);
       const uint64_t mine = sees >> (g * 4);
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
@@ -492,7 +507,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     for (int ks = 0; ks < 2 * NB; ++ks)
 #pragma unroll
       for (int db = 0; db < ND; ++db) {
-        const unsigned char* p0 = at + v_lane[db] + ks * 16 * VROW;
+        const unsigned char* p0 = v_base + v_lane[db] + ks * 16 * VROW;
         const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
         const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
         const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -514,7 +529,14 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     const int next = slot == 2 ? 0 : slot + 1;
     if (t + 1 < mine) put(key_of(t + 1), (t + 1) & 1, next, x);
     fetch(key_of(t + 1 + DEPTH), x);
-    if (t < mine && row0 < M) compute(key_of(t), t & 1, slot);
+    if (t < mine && row0 < M) {
+      if constexpr (!SHARED) {
+        compute(std::integral_constant<int, KB / 32>(), key_of(t), 0, t & 1, slot);
+      } else {
+        if (share == 0) compute(std::integral_constant<int, 1>(), key_of(t), 0, t & 1, slot);
+        if (sharers == 1 || share) compute(std::integral_constant<int, 1>(), key_of(t) + 32, 32, t & 1, slot);
+      }
+    }
     // the bits of tile t - 1 become those of tile t + 2, which are written behind the next barrier
     const int old = next == 2 ? 0 : next + 1;
     if (tid < KW) no_page[old][tid] = 0, gone_any[old][tid] = 0;
@@ -529,7 +551,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   }
   if (odd_any && row0 < M)
     each_unusual<FMT, D>(pg, trow, hkv, lane, max(begin, clear - KB), end, [&](int page, int row, int key) {
-      if ((key - begin) / KB % KW != kw) return;  // (the group that met the key: the others' m may be -inf)
+      // (the waves that met the key: the others' m may be -inf)
+      if (KW > 1 ? (key - begin) / KB % KW != kw : (key - begin) % KB * sharers / KB != share) return;
       const bool sees = key < s0 || (a.anc ? (bits >> (key - s0)) & 1ull : key - s0 <= qn);
 #pragma unroll
       for (int db = 0; db < ND; ++db)
@@ -540,6 +563,39 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
         }
     });
 
+  if constexpr (SHARED) {
+    // a shared block's waves to its first one: lanes hold the same rows and dims
+    float* const om = (float*)lds + wave * 64 * (D / 2) + lane * 4;
+    float2* const ml = (float2*)(lds + RW * 64 * (D / 2) * 4);
+    if (share) {
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *(float4*)(om + (db * 4 + i / 4) * 256) = make_float4(o[db][i], o[db][i + 1], o[db][i + 2], o[db][i + 3]);
+      ml[tid] = make_float2(m_run, l_run);
+    }
+    __syncthreads();
+    if (share || row0 >= M) return;
+    if (sharers == 2) {
+      const int there = min((M - mt * ROWS + 31) / 32 - 4 * (rw >> 2), 2);  // waves on
+      const float2 its = ml[tid + there * 64];
+      const float m_new = fmaxf(m_run, its.x), m_sub = m_new == -INFINITY ? 0.0f : m_new;
+      const float mine = __builtin_amdgcn_exp2f(m_run - m_sub), other = __builtin_amdgcn_exp2f(its.x - m_sub);
+      m_run = m_new;
+      l_run = l_run * mine + its.y * other;
+#pragma unroll
+      for (int db = 0; db < ND; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 v = *(const float4*)(om + there * 64 * (D / 2) + (db * 4 + i / 4) * 256);
+          o[db][i] = o[db][i] * mine + v.x * other;
+          o[db][i + 1] = o[db][i + 1] * mine + v.y * other;
+          o[db][i + 2] = o[db][i + 2] * mine + v.z * other;
+          o[db][i + 3] = o[db][i + 3] * mine + v.w * other;
+        }
+    }
+  }
   float l = xor32_sum(l_run);
   if constexpr (KW > 1) {
     // merge the key waves' results: O and (m, l) of 32 rows each
@@ -1023,11 +1079,13 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   else if (m <= 32)
     hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 2>), grid, block, 0, s, a);
   else if (p.rw == 2)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 4, 32>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 4, 32, false>), grid, block, 0, s, a, m_tiles);
   else if (D == 64 || p.rw == 4)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 2, 64>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 2, 64, false>), grid, block, 0, s, a, m_tiles);
+  else if (m <= 192)
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, true>), grid, block, 0, s, a, m_tiles);
   else
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, false>), grid, block, 0, s, a, m_tiles);
   if (a.slots) {
     const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
     if (p.wide(a.batch))

@@ -81,3 +81,39 @@ def test_row_tiles_in_order(b, hkv, hq, n):
     committed = lengths("any", b, 100, np.random.default_rng(hkv))
     fresh = None if b == 1 else [n - 30 * i for i in range(b)]
     check(Held(b, -(-(n + 100) // 64), 64, hkv, 64, "e4m3", seed=1), n, hq, committed, fresh=fresh)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+@pytest.mark.parametrize("hq", [4, 5, 6, 7, 9])
+def test_pages_that_are_missing_whatever_the_rows(fmt, hq):
+    n, committed = 29, [300, 127, 140]
+    held = Held(3, 11, 32, 1, 128, fmt, seed=hq)
+    held.table[0, 3], held.table[0, 0], held.table[1, 4] = -1, held.pages_n, 2 ** 31 - 1
+    held.table[2] = -5
+    held.upload()
+    check(held, n, hq, committed, trees=True, seed=hq)
+    check(held, n, hq, committed, seed=hq)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+@pytest.mark.parametrize("hq", [4, 5, 6, 7, 9])
+@pytest.mark.parametrize("committed", [3, 40, 64, 95])
+def test_values_that_are_not_finite_whatever_the_rows(fmt, hq, committed):
+    """V of node 3, and of the slot behind the nodes, is NaN or infinite: who sees node 3 shows it, nobody else does."""
+    n, d = 29, 128
+    held = Held(1, 4, 32, 1, d, fmt, seed=hq)
+    held.set_rows(1, 0, [committed + 3], float("inf"))
+    if committed + n < 128:
+        held.set_rows(1, 0, [committed + n], float("nan"))
+    held.upload()
+    words = [tree_words(n, committed)]
+    q = queries(1, n, hq, d, 1)
+    out = kernels().paged_attention(q.to(DEV), held.pages(), seq_len=i32([committed]), anc=masks(words), num_nodes=n, q_heads=hq,
+                                    kv_heads=1, head_dim=d)
+    sees = np.array([w >> 3 & 1 for w in words[0]], bool)
+    assert sees.any() and not sees.all()
+    x = out[0].double().cpu().numpy()
+    assert (np.isnan(x[sees]) if fmt == "e4m3" else x[sees] == np.inf).all()
+    keep = [i for i in range(n) if not sees[i]]
+    want = attention_oracle(held, q, [committed], [n], words, d ** -0.5, None)
+    close(out[:, keep], [(want[0][0][keep], want[0][1][keep])], [len(keep)])
