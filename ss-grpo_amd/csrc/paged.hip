@@ -94,6 +94,8 @@ FG_DEVICE uint32_t amax4(const float (&v)[4]) {
 // projected row and the codes: q is rotated in fp32 and rounded once; the angles are taken in 64 bits (of an angle of
 // 10^5 radians fp32 keeps 2 decimals), and so is K's rotation (512 elements a token, hidden behind the row's loads), because
 // a code next to a tie follows the last bit.
+// Memory bounds it: 2944 tokens at 8B (66 MB) 16 us, 4.2 TB/s of the 4.9 that a large copy reaches; 64 x 29 at 7B (32 MB) 8.8 us;
+// one token 2.7 us, its length, its page and its row one after the other.
 template <int FMT, int D, bool PARTS>
 __global__ void __launch_bounds__(kThreads) paged_write_kernel(WriteArgs a, Rows<PARTS> in) {
   constexpr int HALF = D / 2, QUADS = HALF / 4, BLOCKS = D / fg::kMxBlock;
@@ -197,7 +199,8 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(WriteArgs a, Rows
   }
 }
 
-// The values of 8 elements of a row; tokens without a page are 0.
+// The values of 8 elements of a row; tokens without a page are 0. (4 x 1024 tokens at 8B, 25 MB: 9.2 us; a few tokens 2 us,
+// the latency of the page and the row.)
 template <int FMT, int D, int DT>
 __global__ void __launch_bounds__(kThreads) paged_read_kernel(Pages pg, int batch, const int32_t* start, int count,
                                                               const int32_t* row_map, void* k_out, void* v_out) {
@@ -240,7 +243,8 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(Pages pg, int batc
 }
 
 // As kv_path_gather_kernel: a thread owns one column (16 bytes of codes, or the row's scales) of one (layer, K or V, sequence,
-// kv head) and reads all its accepted rows before it writes any, so moves may overlap.
+// kv head) and reads all its accepted rows before it writes any, so moves may overlap. Three dependent reads bound it, the path and
+// lengths, the pages, the rows: 6.0 us for 64 rounds at 7B, 5.2 for 32 at 1.5B.
 struct GatherArgs {
   Pages pages;
   int layers, batch, cols;  // cols: 16-byte columns of a row, and one more for its scales (e4m3)

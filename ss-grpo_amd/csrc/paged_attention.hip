@@ -95,28 +95,31 @@ struct Work {
 // Sums over the lanes up to each: row shifts, then the last lane of each row and of the lower half to those behind.
 template <typename T>
 FG_DEVICE T scan_add(T x) {
-#define FG_ADD(ctrl, rows) x += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, false))
-  FG_ADD(0x111, 0xf);
-  FG_ADD(0x112, 0xf);
-  FG_ADD(0x114, 0xf);
-  FG_ADD(0x118, 0xf);
-  FG_ADD(0x142, 0xa);
-  FG_ADD(0x143, 0xc);
-#undef FG_ADD
+#define FG_MOVED(ctrl, rows) \
+  __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, rows, 0xf, false))
+  x += FG_MOVED(0x111, 0xf);
+  x += FG_MOVED(0x112, 0xf);
+  x += FG_MOVED(0x114, 0xf);
+  x += FG_MOVED(0x118, 0xf);
+  x += FG_MOVED(0x142, 0xa);
+  x += FG_MOVED(0x143, 0xc);
+#undef FG_MOVED
   return x;
 }
 
-// Which part of which sequence is slot idx, from lengths that only the device knows. A sequence of k keys gets 1 + floor((k - 1) f)
-// parts of equal length, f the same for all: as large as the slots allow (all of them over all keys, else five steps of bisection
-// down to slots - batch, with which the parts always fit). Every wave works that out for itself, a lane a sequence; the first
-// workgroup leaves the shares for the kernel that joins the parts. (A token over 65536 keys beside seven over 1000, at 8B: 44 us, with the same number of parts for each sequence
-// 102; 3 verify rounds of 29 over 1096 to 4096 at 14B: 31 and 40. What it costs: 0.3 us of 9.6 for a few tokens over short lengths.)
+// Which part of which sequence is slot idx, from lengths that only the device knows. A sequence of k keys gets
+// 1 + floor((k - 1) f) parts of equal length, f the same for all: as large as the slots allow (all of them over all keys, else
+// five steps of bisection down to slots - batch, with which the parts always fit). Every wave works that out for itself, a lane a sequence;
+// the first workgroup leaves the shares for the kernel that joins the parts. (A token over 65536 keys beside seven over 1000,
+// at 8B: 44 us, with the same number of parts for each sequence 102; 3 verify rounds of 29 over 1096 to 4096 at 14B: 31 and 40.
+// What it costs: 0.3 us of 9.6 for a few tokens over short lengths.)
 template <int TILE>
 FG_DEVICE Work cut_work(const PagedAttn& a, int idx) {
   const int lane = threadIdx.x & 63;
   const Span s = span_of(a, min(lane, a.batch - 1));
   const int keys = lane < a.batch && s.fresh ? keys_of(a, s) : 0;
-  const float sum = fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan_add((float)keys)), 63)), 1.0f);
+  const float sums = scan_add((float)keys);
+  const float sum = fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sums), 63)), 1.0f);
   int n, upto;  // a lane's parts, and the parts up to it
   auto fits = [&](float f) __attribute__((always_inline)) {
     n = keys ? min(1 + (int)((float)(keys - 1) * f), a.most) : 0;
@@ -177,8 +180,8 @@ FG_DEVICE Work ranked_work(const PagedAttn& a, int idx, unsigned char* scratch, 
   return {s, x.w, 0, keys_of(a, s), 0};
 }
 
-// The work of workgroup idx of a kv head and row tile (the same in all its threads: scalars); A workgroup has
-// kMaxRanked threads and at least 20 bytes of scratch for each.
+// The work of workgroup idx of a kv head and row tile (the same in all its threads). A workgroup has kMaxRanked
+// threads and at least 20 bytes of scratch for each.
 template <int TILE>
 FG_DEVICE Work work_of(const PagedAttn& a, int idx, unsigned char* scratch, int* pick) {
   if (a.slots) return cut_work<TILE>(a, idx);
@@ -187,8 +190,8 @@ FG_DEVICE Work work_of(const PagedAttn& a, int idx, unsigned char* scratch, int*
   return {s, idx, 0, keys_of(a, s), 0};
 }
 
-// 16 e4m3 codes times 2^(s - 127) as bf16: exact, and NaN for s = 255 (a float scale of infinity makes the conversion answer NaN
-// for every code, zero included).
+// 16 e4m3 codes times 2^(s - 127) as bf16: exact, and NaN for s = 255 (a float scale of infinity makes the conversion answer
+// NaN for every code, zero included).
 FG_DEVICE void expand16(u32x4 w, uint32_t s, u32x4& lo, u32x4& hi) {
   const float f = __uint_as_float(s << 23);
 #pragma unroll
@@ -246,19 +249,25 @@ FG_DEVICE void wave_barrier() {  // a wave's LDS operations are done in order; t
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A workgroup takes 32 RW query rows of one (sequence, kv head, part of the keys), row r being head r % G of node r / G, in KW
-// groups of RW waves. Tiles of KB keys go to the groups in turn. A group's threads fetch a tile's K and V rows into registers,
-// 16 bytes each, two tiles ahead; every load of a wave is a consecutive 1 KB of at most 16 tokens, which lie in one page, so
-// that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their way to one of two LDS stages, while
-// the tile in the other is multiplied; one barrier per tile. S^T = K Q^T puts a query into a lane: the softmax needs one
-// exchange with the other half-wave, and P^T goes from the accumulators straight into O^T += V^T P^T, rounded to bf16 once (2^-9
-// of each weight in the mean, the error of the bf16 output again); the sum is that of the rounded weights. The groups merge
-// their (m, l, O) at the end through LDS, the parts by a second kernel.
+// More than 32 rows of a kv head. A workgroup takes 32 RW query rows of one (sequence, kv head, part of the keys), row r being
+// head r % G of node r / G, in KW groups of RW waves. Tiles of KB keys go to the groups in turn. A group's threads fetch a
+// tile's K and V rows into registers, 16 bytes each, two tiles ahead; every load of a wave is a consecutive 1 KB of at most 16
+// tokens, which lie in one page, so that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their
+// way to one of two LDS stages, while the tile in the other is multiplied; one barrier per tile. S^T = K Q^T puts a query into
+// a lane: the softmax needs one exchange with the other half-wave, and P^T goes from the accumulators straight into O^T += V^T
+// P^T, rounded to bf16 once (2^-9 of each weight in the mean, the error of the bf16 output again); the sum is that of the
+// rounded weights. The groups merge their (m, l, O) at the end through LDS, the parts by a second kernel.
 //
-// SHARED, for five or six 32-row blocks: waves w and w + 4 sit on one SIMD, so that a fifth block doubles the time of a tile. Two waves
-// take 32 keys each of every tile for such a block instead, and join their results at the end (32 verify rounds of 29 over 3096 to
-// 4096 keys at 14B, 145 rows: 124 -> 114 us, on bf16 pages 130 -> 124). Steps of 32 keys cost rows that are not shared 2 to 5 %
-// (203 rows 77.3 -> 79.3, 4 x 1024 tokens 101 -> 106).
+// What bounds it: the matrix units and what stands in their way. 64 rounds of 29 nodes over 2048 keys at 7B (203 of 256 rows)
+// take 76 us, 720 TFLOP/s; the padded rows alone would take 57 at the 1215 TFLOP/s of a large product. Without fetching and
+// expanding it takes 67, without the barrier too 63, without reading the fragments 57. 4 x 1024 tokens at 8B: 100 us, 655 TFLOP/s.
+// Slower: two workgroups of four waves per CU (85 us), halves of the waves a phase apart (83), 32-key steps with the next
+// fragments read ahead (81), tiles of 128 keys (87); 3 or 4 tiles in flight took the same.
+//
+// SHARED, for five or six 32-row blocks: waves w and w + 4 sit on one SIMD, so that a fifth block doubles the time of a tile.
+// Two waves take 32 keys each of every tile for such a block instead, and join their results at the end (32 verify rounds of 29
+// over 3096 to 4096 keys at 14B, 145 rows: 124 -> 114 us, on bf16 pages 130 -> 124). Steps of 32 keys cost rows that are not
+// shared 2 to 5 % (203 rows 77.3 -> 79.3, 4 x 1024 tokens 101 -> 106).
 template <int FMT, int D, int RW, int KW, int KB, bool SHARED>
 __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a, int m_tiles) {
   constexpr int T = RW * 64, ROWS = RW * 32;
@@ -674,12 +683,14 @@ FG_DEVICE float quad_sum(float x) {
   return xor32_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// Few rows (single tokens; at most 16 NQ rows of a kv head): the pages are streamed past them. A workgroup of four waves takes one
-// (sequence, kv head, part of the keys), its waves 32-key tiles in turn, each with registers and LDS of its own, no
-// barrier in the loop. S^T = K Q^T on 16 x 16 x 32 MFMAs: lane 16 gq + i holds key i of 16 and, of every 64 bytes of its
-// row, the 16 at 16 gq; which d a k index stands for is free as long as Q follows, so K's rows go from memory through the
-// expansion into the MFMA's registers and never see LDS. V is expanded into a tile of LDS and read transposed. P goes to V in two
-// bf16 parts (hi + lo, p to 16 bits): what bounds the kernel is the stream.
+// Few rows (single tokens; at most 16 NQ rows of a kv head): the pages are streamed past them. A workgroup of eight waves takes
+// one (sequence, kv head, part of the keys), its waves 32-key tiles in turn, each with registers and LDS of its own, no barrier
+// in the loop. S^T = K Q^T on 16 x 16 x 32 MFMAs: lane 16 gq + i holds key i of 16 and, of every 64 bytes of its row, the 16 at
+// 16 gq; which d a k index stands for is free as long as Q follows, so K's rows go from memory through the expansion into the
+// MFMA's registers and never see LDS. V is expanded into a tile of LDS and read transposed. P goes to V in two bf16 parts (hi +
+// lo, p to 16 bits), which costs nothing: what bounds the kernel is the stream of codes. 64 tokens over 1096 to 4096 keys at
+// 8B: 62 us, 5.5 TB/s; 2 over 131072 and 101071: 96 us, 5.4 TB/s (a large sum reads 6.0). The other kernel, which takes K
+// through LDS too, took 98 us for the first. Four or twelve waves, and two tiles in flight, were no faster.
 template <int FMT, int D>
 struct StreamTile {  // a tile's loads: 32 keys
   static constexpr int kLoads = D * fg::page_elem_bytes<FMT> / 64;  // 16-byte loads of a lane per 16 keys
@@ -972,9 +983,10 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   }
 }
 
-// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims of a part. Up to D / 4 parts:
-// D / 4 threads a row. More (WIDE): a workgroup a row, 1024 / D parts side by side. A thread reads a part's (m, l), so that all
-// of them take one round trip, and no load of O waits for another.
+// The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims of a part. Up to D / 4
+// parts: D / 4 threads a row. More (WIDE): a workgroup a row, 1024 / D parts side by side. A thread reads a part's (m, l), so
+// that all of them take one round trip, and no load of O waits for another: 64 rows of 16 parts 4.8 us (one part after the
+// other 26), 2496 rows of 2 parts 4.1 us.
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a) {
   constexpr int LANES = D / 4, SLOTS = WIDE ? 256 / LANES : 1, PER = 256 / (LANES * SLOTS), MOST = LANES * SLOTS;
@@ -1048,7 +1060,8 @@ struct Plan {
 
 Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int64_t capacity) {
   const int64_t m = (int64_t)(q_heads / kv_heads) * num_nodes;
-  // Eight waves, one workgroup per CU: row tiles side by side as far as there are rows, the rest of the waves on other keys.
+  // Eight waves, one workgroup per CU: row tiles side by side as far as there are rows, the rest of the waves on other keys (32
+  // rounds of 29 at 8B, 116 rows: 55 us; a wave per 32 rows and no more, 61).
   Plan p;
   if (m <= 32) p = {1, kStreamWaves, 32, 0};
   else if (m <= 64) p = {2, 4, 32, 0};
