@@ -689,7 +689,7 @@ FG_DEVICE float quad_sum(float x) {
 // 16 gq; which d a k index stands for is free as long as Q follows, so K's rows go from memory through the expansion into the
 // MFMA's registers and never see LDS. V is expanded into a tile of LDS and read transposed. P goes to V in two bf16 parts (hi +
 // lo, p to 16 bits), which costs nothing: what bounds the kernel is the stream of codes. 64 tokens over 1096 to 4096 keys at
-// 8B: 62 us, 5.5 TB/s; 2 over 131072 and 101071: 96 us, 5.4 TB/s (a large sum reads 6.0). The other kernel, which takes K
+// 8B: 62 us, 5.5 TB/s; 2 over 131072 and 123140: 96 us, 5.6 TB/s (a large sum reads 6.0). The other kernel, which takes K
 // through LDS too, took 98 us for the first. Four or twelve waves, and two tiles in flight, were no faster.
 template <int FMT, int D>
 struct StreamTile {  // a tile's loads: 32 keys
@@ -986,7 +986,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
 // The parts of a row: sum_p 2^(m_p - M) (O_p, l_p) over the parts that saw a key, a lane for 4 dims of a part. Up to D / 4
 // parts: D / 4 threads a row. More (WIDE): a workgroup a row, 1024 / D parts side by side. A thread reads a part's (m, l), so
 // that all of them take one round trip, and no load of O waits for another: 64 rows of 16 parts 4.8 us (one part after the
-// other 26), 2496 rows of 2 parts 4.1 us.
+// other 26), 4992 rows of 2 parts 4.1 us.
 template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a) {
   constexpr int LANES = D / 4, SLOTS = WIDE ? 256 / LANES : 1, PER = 256 / (LANES * SLOTS), MOST = LANES * SLOTS;
