@@ -185,6 +185,8 @@ class FlashMedusaDecoder:
             raise NotImplementedError("Only exact_target acceptance is implemented in the main FlashGRPO path")
         if config.kv_cache not in {"contiguous", "paged", "paged_e4m3"}:
             raise ValueError(f"Unsupported kv_cache={config.kv_cache}")
+        if config.kv_cache != "contiguous" and (int(config.kv_page_size) < 16 or int(config.kv_page_size) & (int(config.kv_page_size) - 1)):
+            raise ValueError("kv_page_size must be a power of two from 16 on")
         if config.cache_update_mode not in {"extract_path", "recompute_accepted"}:
             raise ValueError(f"Unsupported cache_update_mode={config.cache_update_mode}")
         if config.proposal_mode not in {"medusa", "chain"}:

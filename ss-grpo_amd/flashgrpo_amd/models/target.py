@@ -157,6 +157,10 @@ class KVCache:
         t = self.kv[0, 0]
         return t.stride(0), t.stride(1), t.stride(2)
 
+    def buffers(self) -> tuple:
+        """Where a captured forward finds the cache: it holds for a cache of the same ``buffers`` only."""
+        return ((self.kv.data_ptr(), tuple(self.kv.shape)),)
+
     def reserve(self, lengths, *, rows=None, first=None) -> None:
         """Makes room for the first ``lengths`` tokens of the given cache rows; here every row has its room from the start."""
 
@@ -226,6 +230,8 @@ class PagedKVCache(KVCache):
         self.dtype = torch.bfloat16
         self.kv_format = kv_format
         self.page_size = P = int(page_size)
+        if P < 16 or P & (P - 1):
+            raise ValueError("PagedKVCache: page_size must be a power of two from 16 on")
         self.device = torch.device(device)
         width = max(1, -(-self.capacity // P))
         n = max(1, self.batch * width if pages is None else int(pages))
@@ -251,6 +257,9 @@ class PagedKVCache(KVCache):
     def kv(self) -> torch.Tensor:
         return self.codes
 
+    def buffers(self) -> tuple:
+        return tuple((t.data_ptr(), tuple(t.shape)) for t in (self.codes, self.scales, self.table) if t is not None)
+
     def pages(self, layer: int) -> K.KVPages:
         """One layer's pages, as the kernels take them."""
         return self._layers[layer]
@@ -265,6 +274,21 @@ class PagedKVCache(KVCache):
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def _checked(self, rows, distinct=False) -> np.ndarray:
+        rows = np.asarray(rows, np.int64).reshape(-1)
+        if ((rows < 0) | (rows >= self.batch)).any() or (distinct and np.unique(rows).size < rows.size):
+            raise ValueError(f"PagedKVCache: rows must be {'distinct and ' if distinct else ''}among the cache's {self.batch}")
+        return rows
+
+    def _committed(self, rows) -> np.ndarray:
+        """The committed lengths of rows, all of whose tokens have pages."""
+        lens = self.seq_len.cpu().numpy()
+        for r in rows:
+            n = int(lens[r])
+            if n < 0 or n > self.capacity or (self._rows[r, :-(-n // self.page_size)] < 0).any():
+                raise ValueError(f"PagedKVCache: some of the {n} committed tokens of row {r} have no page")
+        return lens
 
     def _take(self) -> int:
         if not self._free:
@@ -294,9 +318,11 @@ class PagedKVCache(KVCache):
         """Gives the cache rows ``rows`` (None: all) pages for their first ``lengths`` tokens. Of the tokens from ``first`` on
         (None: the tokens that get new pages), which the caller is about to write, a page that other rows share is replaced
         by a copy of it. Raises RuntimeError, with nothing changed, when the pool has too few pages."""
-        rows = np.arange(self.batch) if rows is None else np.asarray(rows, np.int64)
+        rows = np.arange(self.batch) if rows is None else self._checked(rows, distinct=True)
         lengths = np.broadcast_to(np.asarray(lengths, np.int64), rows.shape)
         first = None if first is None else np.broadcast_to(np.asarray(first, np.int64), rows.shape)
+        if (lengths < 0).any() or (first is not None and (first < 0).any()):
+            raise ValueError("PagedKVCache: lengths and first must not be negative")
         if (lengths > self.capacity).any():
             raise ValueError(f"PagedKVCache: {int(lengths.max())} tokens exceed the cache capacity {self.capacity}")
         need, P = [], self.page_size
@@ -328,7 +354,7 @@ class PagedKVCache(KVCache):
 
     def release(self, rows) -> None:
         """Gives the pages of the given cache rows back (their committed lengths become 0)."""
-        for r in np.asarray(rows, np.int64).reshape(-1):
+        for r in self._checked(rows):
             for p in self._rows[r][self._rows[r] >= 0]:
                 self._drop(int(p))
             self._rows[r] = -1
@@ -343,11 +369,18 @@ class PagedKVCache(KVCache):
 
     def repeat_rows(self, src_rows: torch.Tensor, dst_rows: torch.Tensor) -> None:
         """Cache rows dst become repeats of rows src: they share the pages that src's committed tokens fill and get a copy of
-        the one that they end in. Pages that dst held go back to the pool first."""
+        the one that they end in. Pages that dst held go back to the pool first. Raises, with nothing changed, where the pool has
+        too few pages or a committed token none."""
         src, dst = (np.asarray(t.cpu() if isinstance(t, torch.Tensor) else t, np.int64).reshape(-1) for t in (src_rows, dst_rows))
         if src.shape != dst.shape or len(set(dst.tolist())) < dst.size or set(src.tolist()) & set(dst.tolist()):
             raise ValueError("PagedKVCache.repeat_rows: one row src for each of distinct rows dst, none of which is a src")
-        lens = self.seq_len.cpu().numpy()
+        src, dst = self._checked(src), self._checked(dst)
+        lens = self._committed(src)
+        back, times = np.unique(self._rows[dst], return_counts=True)
+        free = len(self._free) + int((self._uses[back] == times)[back >= 0].sum())
+        need = int((lens[src] % self.page_size > 0).sum())
+        if need > free:
+            raise RuntimeError(f"PagedKVCache: {need} more pages needed, {free} of {self._uses.size} free")
         for r in dst:
             for p in self._rows[r][self._rows[r] >= 0]:
                 self._drop(int(p))
@@ -367,10 +400,11 @@ class PagedKVCache(KVCache):
 
     def select_rows(self, rows: torch.Tensor, capacity: int | None = None) -> "PagedKVCache":
         """A new cache, with a pool of its own, holding copies of the given rows' committed tokens (in that order)."""
-        rows = torch.as_tensor(rows).to(dtype=torch.long, device="cpu").numpy()
+        rows = self._checked(torch.as_tensor(rows).cpu().numpy())
+        committed = self._committed(rows)
         cap = self.capacity if capacity is None else int(capacity)
         out = PagedKVCache(self.cfg, rows.size, cap, device=self.device, kv_format=self.kv_format, page_size=self.page_size)
-        lens = np.minimum(self.seq_len.cpu().numpy()[rows], cap)
+        lens = np.minimum(committed[rows], cap)
         out.reserve(lens)
         pairs = [(int(self._rows[r, i]), int(out._rows[j, i])) for j, r in enumerate(rows)
                  for i in range(-(-int(lens[j]) // self.page_size))]
@@ -894,7 +928,7 @@ class TargetModel:
             raise ValueError("forward: new_len needs a paged cache")
         if graph and anc is not None and new_len is None and timing.idle() and not torch.cuda.is_current_stream_capturing():
             key = (tuple(tokens.shape), tokens.dtype, tuple(pos_offset.shape), tuple(anc.shape), cache.kv.data_ptr(),
-                   tuple(cache.kv.shape), tuple(seq_len.shape), None if row_map is None else tuple(row_map.shape),
+                   cache.buffers(), tuple(seq_len.shape), None if row_map is None else tuple(row_map.shape),
                    None if err_flag is None else err_flag.data_ptr())
             g = self._graphs.get(key, False)
             if g is False:

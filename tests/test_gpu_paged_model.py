@@ -198,3 +198,25 @@ def test_wrapper_functions(model, fmt):
     got = extract_accepted_path_kv(cache, tree_cache, [[0, 1, 3], [0]]).past_key_values
     assert got.seq_len.tolist() == [15, 16] and cache.seq_len.tolist() == [12, 15]
     assert all(torch.equal(got.k(1)[0, :, 12 + j], w) for j, w in enumerate(want))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_captured_forward_belongs_to_one_table(model, fmt):
+    """A second cache over the same pool, with a table (and scales) of its own, does not replay the first one's graph."""
+    ids, lens = prompts(2, 40), [40, 23]
+    first = model.new_cache(2, 80, kv_format=fmt, page_size=16, pages=20)
+    model.prefill(ids, first, lengths=lens)
+    first.reserve(np.array(lens) + 8, first=lens)
+    anc, pos = tree(8)
+    tok = prompts(2, 8, 9).to(DEV, torch.int32)
+    want = model.forward(tok, first, pos_offset=pos, anc=anc).clone()
+    for _ in range(3):
+        assert torch.equal(model.forward(tok, first, pos_offset=pos, anc=anc, graph=True), want)
+    second = first.container_copy()  # its rows in the other order
+    second.table = first.table.flip(0).contiguous()
+    second.scales = None if first.scales is None else first.scales.clone()
+    second.seq_len = first.seq_len.flip(0).contiguous()
+    second._make_views()
+    for _ in range(3):
+        assert torch.equal(model.forward(tok.flip(0), second, pos_offset=pos, anc=anc, graph=True), want.flip(0))
+    model.drop_graphs(first)

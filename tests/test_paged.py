@@ -126,6 +126,43 @@ def test_repeats_share_whole_pages_and_copy_the_last(fmt):
     consistent(c)
 
 
+def test_rows_that_are_refused():
+    """Rows that are not there, or twice, tokens before the first, lengths without pages: refused, with nothing changed."""
+    c = PagedKVCache(CFG, 3, 64, device="cpu", page_size=16, pages=7)
+    c.reserve([40, 16, 0])
+    c.seq_len.copy_(torch.tensor([40, 16, 0]))
+    before, free = c._rows.copy(), c.free_pages
+    for call in (lambda: c.reserve(64, rows=[2, 2]), lambda: c.reserve(16, rows=[-1]), lambda: c.reserve(16, rows=[3]),
+                 lambda: c.reserve([1, 2], rows=[0, 1, 2]), lambda: c.reserve(-1), lambda: c.reserve(16, first=-1),
+                 lambda: c.release([3]), lambda: c.release([-1]), lambda: c.repeat_rows(torch.tensor([0]), torch.tensor([3])),
+                 lambda: c.repeat_rows(torch.tensor([-3]), torch.tensor([1])), lambda: c.select_rows(torch.tensor([3])),
+                 lambda: c.select_rows(torch.tensor([-1]))):
+        with pytest.raises(ValueError):
+            call()
+        assert (c._rows == before).all() and c.free_pages == free
+    c.seq_len[2] = 20  # committed tokens that were never written
+    with pytest.raises(ValueError, match="no page"):
+        c.repeat_rows(torch.tensor([2]), torch.tensor([1]))
+    with pytest.raises(ValueError, match="no page"):
+        c.select_rows(torch.tensor([2]))
+    assert (c._rows == before).all() and c.free_pages == free
+    consistent(c)
+
+
+def test_repeat_rows_without_room_changes_nothing():
+    c = PagedKVCache(CFG, 4, 64, device="cpu", page_size=16, pages=5)
+    c.reserve([40, 0, 0, 16])
+    c.seq_len.copy_(torch.tensor([40, 0, 0, 16]))
+    before, lens = c._rows.copy(), c.seq_len.clone()
+    with pytest.raises(RuntimeError, match="3 more pages needed, 2 of 5 free"):  # (row 3's page comes back)
+        c.repeat_rows(torch.tensor([0, 0, 0]), torch.tensor([1, 2, 3]))
+    assert (c._rows == before).all() and c.free_pages == 1 and torch.equal(c.seq_len, lens)
+    consistent(c)
+    c.repeat_rows(torch.tensor([0, 0]), torch.tensor([1, 3]))
+    assert c.free_pages == 0
+    consistent(c)
+
+
 def test_repeat_rows_refusals():
     c = PagedKVCache(CFG, 3, 32, device="cpu", page_size=16)
     for src, dst in (([0, 1], [1, 2]), ([0, 0], [1, 1]), ([0], [1, 2])):
@@ -162,6 +199,9 @@ def test_formats():
         PagedKVCache(TargetConfig(1, 64, 2, 2, 32, 128, 100), 1, 16, device="cpu")
     with pytest.raises(ValueError, match="page_size"):
         PagedKVCache(CFG, 1, 16, device="cpu", page_size=24)
+    for size in (0, -16, 8):
+        with pytest.raises(ValueError):
+            PagedKVCache(CFG, 1, 16, device="cpu", page_size=size)
 
 
 # ------------------------------------------------------------------ refusals
