@@ -1069,8 +1069,10 @@ Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, 
   else p = {8, 1, 64, 0};
   const int64_t each = kv_heads * ((m + p.rows() - 1) / p.rows());  // workgroups of a sequence that is not cut
   // Parts where every sequence gets two at least (20 tokens over 2048 keys at 8B, 160 workgroups: whole 19.5 us, in 320 parts 28),
-  // and no more workgroups than CUs, which would take two rounds (3 over 8192: 264 workgroups 22.5 us, 256 17.6).
-  if (batch <= kMaxCut && 2 * batch * each <= kCUs) {
+  // and no more workgroups than CUs, which would take two rounds (3 over 8192: 264 workgroups 22.5 us, 256 17.6). Few rows stay
+  // whole in short caches, where the second launch costs more (one over 600 keys at 8B: 8.2 us whole, 10.5 in parts; 4 over 1000
+  // at most: 11.4 and 10.3).
+  if (batch <= kMaxCut && 2 * batch * each <= kCUs && (m > 32 || capacity >= 1024)) {
     const int64_t most = std::max<int64_t>(1, capacity / kMinPartKeys);
     p.slots = (int)std::min<int64_t>(kCUs / each, batch * most);
     if (p.slots < 2 * batch) p.slots = 0;

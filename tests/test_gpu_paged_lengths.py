@@ -52,7 +52,7 @@ def held_rows(b, width, hkv, d):
 @pytest.mark.parametrize("b,n,hq,d", [(b, *s) for b in (1, 7, 64, 65) for s in ((1, 2, 128), (9, 4, 64), (29, 7, 128)) if b < 64 or s[0] < 29])
 @pytest.mark.parametrize("kind", ["one long", "last long", "none", "equal", "any"])
 def test_parts(b, n, hq, d, kind):
-    most = 2500 if b <= 7 else 600
+    most = 2500 if b <= 7 else 1100
     committed = lengths(kind, b, most, np.random.default_rng([b, n]))
     check(held_rows(b, -(-(most + n) // 32), 1, d), n, hq, committed, trees=n > 1, seed=b)
 
