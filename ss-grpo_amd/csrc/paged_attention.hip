@@ -1054,8 +1054,9 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttn a) {
 struct Plan {
   int rw, kw, kb, slots;
   int rows() const { return rw * 32; }
-  // Narrow rows of the kernel that joins the parts, or a workgroup for each.
-  bool wide(int batch) const { return slots > 8 * batch; }
+  // Whether the kernel that joins the parts takes a workgroup for each row: where there are many parts (3 tokens of 10 parts 17.6
+  // us, narrow 18.7), and few rows or too many parts for narrow ones (3 verify rounds of 10 parts, 3480 rows: 30.5 us, narrow 28.9).
+  bool wide(int batch, int64_t rows) const { return slots > 8 * batch && (rows < 1024 || slots > 16 * batch); }
 };
 
 Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int64_t capacity) {
@@ -1103,7 +1104,7 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, false>), grid, block, 0, s, a, m_tiles);
   if (a.slots) {
     const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
-    if (p.wide(a.batch))
+    if (p.wide(a.batch, rows))
       hipLaunchKernelGGL((paged_combine_kernel<D, true>), dim3((unsigned)rows), dim3(256), 0, s, a);
     else
       hipLaunchKernelGGL((paged_combine_kernel<D, false>), dim3((unsigned)((rows + 1024 / D - 1) / (1024 / D))), dim3(256), 0, s, a);
@@ -1151,7 +1152,7 @@ extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* p
   FG_REQUIRE((int64_t)batch * pages->kv_heads * ((m + p.rows() - 1) / p.rows()) < (1ll << 31),
              "fg_paged_attention: bad shape (too many workgroups)");
   a.slots = p.slots;
-  a.most = p.wide(batch) ? 256 : pages->head_dim / 4;
+  a.most = p.wide(batch, (int64_t)batch * num_nodes * q_heads) ? 256 : pages->head_dim / 4;
   a.o_part = (float*)workspace;
   a.ml_part = (float2*)(a.o_part + (int64_t)p.slots * num_nodes * q_heads * pages->head_dim);
   a.shares = (int2*)(a.ml_part + (int64_t)p.slots * num_nodes * q_heads);
