@@ -45,7 +45,7 @@ struct PagedAttn {
 constexpr float kRescaleSlack = 8.0f;  // log2 units
 constexpr int kMinPartKeys = 256;      // a part of a sequence's keys is at least so long
 constexpr int kCUs = 256;
-constexpr int kMaxRanked = 512;        // sequences that are put in order: a thread each
+constexpr int kThreads = 512;          // of a workgroup of the attention kernels; sequences that are put in order
 constexpr int kMaxCut = 64;            // sequences that are cut: a lane each
 constexpr int kStreamWaves = 8;        // of a workgroup of the stream kernel
 
@@ -147,45 +147,70 @@ FG_DEVICE Work cut_work(const PagedAttn& a, int idx) {
   return {{of(s.committed), of(s.fresh), of(s.row)}, b, begin, (int)min((int64_t)begin + part, (int64_t)all), idx};
 }
 
-// The sequence with the idx-th most keys: more workgroups than CUs go longest first, so that no long one begins when the others
-// end (64 tokens over 1096 to 4096 keys at 8B 71.5 -> 65.4 us, 128 verify rounds of 29 over 548 to 2048 at 7B 128 -> 111; with
-// equal lengths the count costs 0.5 us for 64 and 2.4 us for 128 sequences, of 67 and 56). A sequence's rank is how many go
-// before it, counted by as many threads as there are for each.
-FG_DEVICE Work ranked_work(const PagedAttn& a, int idx, unsigned char* scratch, int* pick) {
-  const int i = threadIdx.x;
-  int* const keys = (int*)scratch;
-  int4* const spans = (int4*)(scratch + kMaxRanked * 4);
-  int k = -1;
-  if (i < a.batch) {
-    const Span s = span_of(a, i);
-    k = s.fresh ? keys_of(a, s) : 0;
-    spans[i] = make_int4(s.committed, s.fresh, s.row, i);
-  }
-  keys[i] = k;
-  __syncthreads();
-  int each = 0;  // log2 of the threads that count for a sequence
-  while (each < 6 && (a.batch << (each + 1)) <= kMaxRanked) ++each;
-  const int j = i >> each;
-  k = keys[j];
-  int r = 0;
-  for (int c = (i - (j << each)) * 4; c < a.batch; c += 4 << each) {
-    const int4 x = *(const int4*)(keys + c);
-    r += (x.x > k - (c < j)) + (x.y > k - (c + 1 < j)) + (x.z > k - (c + 2 < j)) + (x.w > k - (c + 3 < j));
-  }
-  for (int x = 1; x < 1 << each; x <<= 1) r += __shfl_xor(r, x, 64);
-  if (i == j << each && j < a.batch && r == idx) *(int4*)pick = spans[j];
-  __syncthreads();  // (after it the tiles may lie where these lay)
-  const int4 x = *(const int4*)pick;
-  const Span s = {x.x, x.y, x.z};
-  return {s, x.w, 0, keys_of(a, s), 0};
+// The largest lane's value, in lane 63.
+FG_DEVICE int scan_max(int x) {
+#define FG_MOVED(ctrl, rows) __builtin_amdgcn_update_dpp(x, x, ctrl, rows, 0xf, false)
+  x = max(x, FG_MOVED(0x111, 0xf));
+  x = max(x, FG_MOVED(0x112, 0xf));
+  x = max(x, FG_MOVED(0x114, 0xf));
+  x = max(x, FG_MOVED(0x118, 0xf));
+  x = max(x, FG_MOVED(0x142, 0xa));
+  x = max(x, FG_MOVED(0x143, 0xc));
+#undef FG_MOVED
+  return x;
 }
 
-// The work of workgroup idx of a kv head and row tile (the same in all its threads). A workgroup has kMaxRanked
-// threads and at least 20 bytes of scratch for each.
+// The idx-th sequence, long ones first: up to twice as many workgroups as CUs go in that order, so that no long one begins when
+// the others end. Sequences are sorted into eight classes by length, a thread a sequence, by ballots; within a class they keep
+// their order. 64 tokens over 1096 to 4096 keys at 8B 71 -> 66 us, 128 verify rounds of 29 over 548 to 2048 at 7B 131 -> 112, 4 x
+// 1024 tokens 106 -> 100; equal lengths lose 0.5 to 1 us. More workgroups even out by themselves: 128 tokens over 2096 to 4096 at
+// 14B, 1024 of them, take 153.5 us unsorted and 157.5 sorted, 256 over 200 to 2000 at 8B 118 and 126. (A sequence's rank by
+// comparing it with each other one: 151 in the last case.)
+struct Order {
+  int4 spans[kThreads];
+  uint64_t members[8][kThreads / 64];  // of a class among a wave's sequences
+  int top[kThreads / 64];
+};
+FG_DEVICE Work ordered_work(const PagedAttn& a, int idx, Order& at) {
+  static_assert(kThreads == 512 && 2 * kCUs <= kThreads, "eight waves and classes: a lane each; a thread a sequence");
+  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+  int keys = -1;
+  if (i < a.batch) {
+    const Span s = span_of(a, i);
+    keys = s.fresh ? keys_of(a, s) : 0;
+    at.spans[i] = make_int4(s.committed, s.fresh, s.row, keys);
+  }
+  const int top = scan_max(keys);
+  if (lane == 63) at.top[wave] = top;
+  __syncthreads();
+  const int4 x = *(const int4*)at.top, y = *(const int4*)(at.top + 4);
+  const float most = (float)(max(max(max(x.x, x.y), max(x.z, x.w)), max(max(y.x, y.y), max(y.z, y.w))) + 1);
+  const int its = keys < 0 ? 8 : 7 - min((int)((float)keys * (8.0f / most)), 7);
+  uint64_t mine = 0;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint64_t m = __ballot(its == c);
+    mine = lane == c ? m : mine;
+  }
+  if (lane < 8) at.members[lane][wave] = mine;
+  __syncthreads();
+  const uint64_t m = (&at.members[0][0])[lane];
+  const int count = __popcll(m), upto = scan_add(count);
+  const int l = __builtin_ctzll(__ballot((unsigned)(idx - (upto - count)) < (unsigned)count));
+  const int rest = idx - __builtin_amdgcn_readlane(upto - count, l);
+  const uint64_t one = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(m >> 32), l) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)m, l);
+  const int b = l % 8 * 64 + __builtin_ctzll(__ballot((one >> lane & 1) && __popcll(one & low_bits(lane)) == rest));
+  const int4 s = at.spans[b];
+  return {{s.x, s.y, s.z}, b, 0, s.w, 0};
+}
+
+// The work of workgroup idx of a kv head and row tile (the same in all its threads). A workgroup has kThreads
+// threads.
 template <int TILE>
-FG_DEVICE Work work_of(const PagedAttn& a, int idx, unsigned char* scratch, int* pick) {
+FG_DEVICE Work work_of(const PagedAttn& a, int idx, Order& order) {
   if (a.slots) return cut_work<TILE>(a, idx);
-  if (gridDim.x > kCUs && a.batch <= kMaxRanked) return ranked_work(a, idx, scratch, pick);
+  if (gridDim.x > kCUs && gridDim.x <= 2 * kCUs) return ordered_work(a, idx, order);
   const Span s = span_of(a, idx);
   return {s, idx, 0, keys_of(a, s), 0};
 }
@@ -284,8 +309,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   __shared__ int gone_any[3][KW], odd_any;  // whether there are any; whether V was kept at 0 where it is not finite
 
   const Pages& pg = a.pages;
-  static_assert(KW * T == kMaxRanked && sizeof(lds) >= 20 * kMaxRanked, "threads and LDS of work_of");
-  __shared__ __attribute__((aligned(16))) int pick[4];
+  static_assert(KW * T == kThreads, "threads of work_of");
+  __shared__ __attribute__((aligned(16))) Order order;
   int unit = blockIdx.x / m_tiles, mt = blockIdx.x % m_tiles;
   if (gridDim.x > kCUs) {
     // The row tiles of a unit on one XCD (workgroups go to the eight in turn), those with the most keys first: 4 x 1024 tokens
@@ -295,7 +320,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     mt = m_tiles - 1 - mt;
   }
   const int hkv = unit % pg.kv_heads;
-  const Work work = work_of<KB>(a, unit / pg.kv_heads, lds, pick);
+  const Work work = work_of<KB>(a, unit / pg.kv_heads, order);
   const int b = scalar(work.b);
   if (b < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
@@ -708,10 +733,10 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   constexpr int MERGE = W * NQ * 16 * (OROW * 4 + 8);
   __shared__ __attribute__((aligned(16))) unsigned char lds[W * VTILE > MERGE ? W * VTILE : MERGE];
   const Pages& pg = a.pages;
-  static_assert(W * 64 == kMaxRanked && sizeof(lds) >= 20 * kMaxRanked, "threads and LDS of work_of");
-  __shared__ __attribute__((aligned(16))) int pick[4];
+  static_assert(W * 64 == kThreads, "threads of work_of");
+  __shared__ __attribute__((aligned(16))) Order order;
   const int hkv = blockIdx.x % pg.kv_heads;
-  const Work work = work_of<32>(a, blockIdx.x / pg.kv_heads, lds, pick);
+  const Work work = work_of<32>(a, blockIdx.x / pg.kv_heads, order);
   const int b = scalar(work.b);
   if (b < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gq = lane >> 4, i16 = lane & 15;
