@@ -333,7 +333,7 @@ int fg_kv_read_paged(const fg_kv_pages* pages, int batch, const int32_t* start, 
  * (num_nodes <= 64), or, anc NULL, to new tokens 0..n (num_nodes <= 8192). new_len as in fg_rope_kv_write_paged: rows from
  * new_len[b] on are not written, and no row sees their tokens. Tokens without a page are not seen; a row that sees nothing is
  * 0. Infinities and NaN of tokens that a row does not see do not reach it. Scores, softmax sums and O in fp32, the weights
- * rounded to bf16 before they meet V. Where few rows meet many tokens, a sequence's tokens are split over
+ * in two bf16 parts that hold them but for 2^-18. Where few rows meet many tokens, a sequence's tokens are split over
  * workgroups whose parts are merged by a second launch; that needs workspace >= fg_paged_attention_workspace(...) bytes (capacity:
  * table_width * page_size; 0 when nothing is split), 16-byte aligned and one call's at a time; a null or smaller one runs unsplit. */
 size_t fg_paged_attention_workspace(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int capacity);

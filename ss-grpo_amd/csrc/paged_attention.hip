@@ -17,7 +17,6 @@ using fg::kPageE4M3;
 using fg::Pages;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -260,9 +259,10 @@ FG_DEVICE float v_element(const Pages& pg, int page, int r, int d) {
   return x[0] * fg::mx_scale(pg.vs[pg.scales_at(page) + (int64_t)r * (D / fg::kMxBlock) + d / fg::kMxBlock]);
 }
 
-// Infinities and NaN of V at tokens that only some rows see (the new tokens' tiles). The loops keep them at 0 there, since p = 0
-// times them would be NaN, and here, once, they are added for the rows that see them: p > 0 times an infinity or a NaN is
-// that. `add(page, row, token)` is called for each such token in [from, end).
+// Infinities and NaN of V. The loops keep them at 0 where not every row sees them (the new tokens' tiles), since p = 0 times
+// them would be NaN, and in bf16 everywhere, since P's lower part, which is 0 or negative too, would make NaN of infinities.
+// Here, once, they are added for the rows that see them: p > 0 times an infinity or a NaN is that. `add(page, row, token)` is
+// called for each such token in [from, end).
 template <int FMT, int D, typename F>
 FG_DEVICE void each_unusual(const Pages& pg, const const_i32* trow, int hkv, int lane, int from, int end, F add) {
   constexpr int PER = D / 64;  // elements of a lane
@@ -289,19 +289,22 @@ FG_DEVICE void wave_barrier() {  // a wave's LDS operations are done in order; t
 // tokens, which lie in one page, so that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their
 // way to one of two LDS stages, while the tile in the other is multiplied; one barrier per tile. S^T = K Q^T puts a query into
 // a lane: the softmax needs one exchange with the other half-wave, and P^T goes from the accumulators straight into O^T += V^T
-// P^T, rounded to bf16 once (2^-9 of each weight in the mean, the error of the bf16 output again); the sum is that of the
-// rounded weights. The groups merge their (m, l, O) at the end through LDS, the parts by a second kernel.
+// P^T, in two bf16 parts (hi + lo, p but for 2^-18 of it), so that the products with V are made twice and nothing but the output's
+// own rounding is left: 1.7e-3 from 64 bits, where one part leaves 2.3e-3. The groups merge their (m, l, O) at the end through LDS,
+// the parts by a second kernel.
 //
-// What bounds it: the matrix units and what stands in their way. 64 rounds of 29 nodes over 2048 keys at 7B (203 of 256 rows)
-// take 76 us, 720 TFLOP/s; the padded rows alone would take 57 at the 1215 TFLOP/s of a large product. Without fetching and
-// expanding it takes 67, without the barrier too 63, without reading the fragments 57. 4 x 1024 tokens at 8B: 100 us, 655 TFLOP/s.
-// Slower: two workgroups of four waves per CU (85 us), halves of the waves a phase apart (83), 32-key steps with the next
-// fragments read ahead (81), tiles of 128 keys (87); 3 or 4 tiles in flight took the same.
+// What bounds it: products, reads of fragments, exponentials and expansion, which a SIMD's two waves overlap in part. 64 rounds
+// of 29 nodes over 2048 keys at 7B (203 of 256 rows) take 93 us; the products of the padded rows, V's twice, would take 86 at the
+// 1215 TFLOP/s of a large product. 4 x 1024 tokens at 8B: 122 us. With one part of P: 74 and 100, of which the first were
+// 67 without fetching and expanding, 63 without the barrier too, 57 without reading the fragments.
+// Slower, with one part: two workgroups of four waves per CU (85 us), halves of the waves a phase apart (83), 32-key steps with the next
+// fragments read ahead (81), tiles of 128 keys (87); 3 or 4 tiles in flight took the same. With two: all of P before V (93 to 97),
+// 16 keys at a time (95).
 //
 // SHARED, for five or six 32-row blocks: waves w and w + 4 sit on one SIMD, so that a fifth block doubles the time of a tile.
 // Two waves take 32 keys each of every tile for such a block instead, and join their results at the end (32 verify rounds of 29
-// over 3096 to 4096 keys at 14B, 145 rows: 124 -> 114 us, on bf16 pages 130 -> 124). Steps of 32 keys cost rows that are not
-// shared 2 to 5 % (203 rows 77.3 -> 79.3, 4 x 1024 tokens 101 -> 106).
+// over 3096 to 4096 keys at 14B, 145 rows, with one part of P: 124 -> 116 us, on bf16 pages 128 -> 124). Steps of 32 keys cost rows
+// that are not shared 2 to 5 % (203 rows 77.3 -> 79.3, 4 x 1024 tokens 101 -> 106).
 template <int FMT, int D, int RW, int KW, int KB, bool SHARED>
 __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a, int m_tiles) {
   constexpr int T = RW * 64, ROWS = RW * 32;
@@ -315,7 +318,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   constexpr int MERGE = KW > 1 ? RW * KW * 32 * ((D + 4) * 4 + 8) : SHARED ? RW * 32 * (D * 4 + 16) : 0;
   __shared__ __attribute__((aligned(16))) unsigned char lds[KW * 2 * TILE > MERGE ? KW * 2 * TILE : MERGE];
   __shared__ uint64_t no_page[3][KW];  // a tile's keys without a page
-  __shared__ int gone_any[3][KW], odd_any;  // whether there are any; whether V was kept at 0 where it is not finite
+  __shared__ int gone_any[3][KW];      // whether there are any
+  __shared__ int odd_from, odd_to;     // the tokens among which V was kept at 0 where it is not finite
 
   const Pages& pg = a.pages;
   static_assert(KW * T == kThreads, "threads of work_of");
@@ -415,7 +419,6 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;
   const float sl2 = a.scale * 1.44269504088896341f;
-  const bf16x2 ones2 = __builtin_bit_cast(bf16x2, 0x3f803f80u);
 
   const uint32_t k_lane = (uint32_t)(l32 * KROW + g * 16);
   // V^T fragments by transposed reads: lane 16 gq + i addresses key 4 (gq / 2) + i / 4 and d 32 db + 16 (gq % 2) + 4 (i % 4),
@@ -431,8 +434,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       v_lane[db] = (uint32_t)(KB * KROW + key * VROW + (((4 * db + low) ^ v_swizzle(key)) * 16) + 8 * (i & 1));
   }
 
-  // V is 0 behind the part's end and without a page and, in the tiles that reach the new tokens, where it is not finite; K's rows
-  // there may be anything, their scores are masked.
+  // V is 0 behind the part's end and without a page and, in the tiles that reach the new tokens (bf16: in all), where it is not
+  // finite; K's rows there may be anything, their scores are masked.
   uint32_t k_put[NU], v_put[NU];  // where this thread's pieces go
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
@@ -442,20 +445,32 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   }
   auto put = [&](int key0, int buf, int slot, Loads& x) __attribute__((always_inline)) {
     unsigned char* const at = group + buf * TILE;
-    if (key0 + KB > clear || key0 + KB > end || x.paged != (1u << NU) - 1u) {  // the last tiles, and the rare ones
+    bool look = key0 + KB > end || x.paged != (1u << NU) - 1u;  // the last tiles, and the rare ones
+    if constexpr (FMT == kPageE4M3) {
+      look |= key0 + KB > clear;
+    } else {
+      uint32_t most = 0;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) most = max_u16x2(most, largest_u16(x.vp[u]));
+      look |= __any((most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u);
+    }
+    if (look) {
       uint64_t gone = 0;
       bool odd = false;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const int j0 = (u * RW + rw) * KPW;
         const bool ok = ((x.paged >> u) & 1u) && key0 + j0 + lane / CPK < end;
-        const bool bad = ok && key0 + KB > clear && (FMT == kPageE4M3 ? x.vsc[u] == 255u : not_finite(x.vp[u]));
+        const bool bad = ok && (FMT == kPageE4M3 ? key0 + KB > clear && x.vsc[u] == 255u : not_finite(x.vp[u]));
         odd |= bad;
         if (!((x.paged >> u) & 1u)) gone |= low_bits(KPW) << j0;
         if (bad || !ok) x.vp[u] = FMT == kPageE4M3 || !ok ? u32x4(0) : finite_part(x.vp[u]);  // (e4m3: all of a block's 32)
         if (FMT == kPageE4M3 && (bad || !ok)) x.vsc[u] = 127u;
       }
-      if (__any(odd) && lane == 0) odd_any = 1;
+      if (__any(odd) && lane == 0) {
+        atomicMin(&odd_from, key0);
+        atomicMax(&odd_to, min(key0 + KB, end));
+      }
       if (gone && lane == 0) {
         atomicOr((unsigned long long*)&no_page[slot][kw], gone);
         gone_any[slot][kw] = 1;
@@ -529,37 +544,39 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       m_run = m_new;
     }
     const float m_sub = m_run == -INFINITY ? 0.0f : m_run;
-    float psum = l_run;
-    bf16x8 pf[NB][2];
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
+    for (int kb = 0; kb < NB; ++kb) {
+      bf16x8 hi[2], lo[2];  // p = hi + lo but for 2^-18 of it
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        uint32_t packed[4];
+        uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j], sl2, -m_sub));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j + 1], sl2, -m_sub));
-          packed[j / 2] = fg::pack_bf16x2(p0, p1);
-          psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
+        for (int j = 0; j < 4; ++j) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + 2 * j], sl2, -m_sub));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + 2 * j + 1], sl2, -m_sub));
+          l_run += p0 + p1;
+          ph[j] = fg::pack_bf16x2(p0, p1);
+          pl[j] = fg::pack_bf16x2(p0 - __uint_as_float(ph[j] << 16), p1 - __uint_as_float(ph[j] & 0xffff0000u));
         }
-        pf[kb][ks] = __builtin_bit_cast(bf16x8, u32x4{packed[0], packed[1], packed[2], packed[3]});
+        hi[ks] = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
+        lo[ks] = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
       }
-    l_run = psum;
 #pragma unroll
-    for (int ks = 0; ks < 2 * NB; ++ks)
+      for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int db = 0; db < ND; ++db) {
-        const unsigned char* p0 = v_base + v_lane[db] + ks * 16 * VROW;
-        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
-        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[ks >> 1][ks & 1], o[db], 0, 0, 0);
-      }
+        for (int db = 0; db < ND; ++db) {
+          const unsigned char* p0 = v_base + v_lane[db] + (2 * kb + ks) * 16 * VROW;
+          const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
+          const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, hi[ks], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo[ks], o[db], 0, 0, 0);
+        }
+    }
   };
 
   if (tid < 3 * KW) (&no_page[0][0])[tid] = 0, (&gone_any[0][0])[tid] = 0;
-  if (tid == 0) odd_any = 0;
+  if (tid == 0) odd_from = end, odd_to = 0;
   __syncthreads();
   if (tiles) {
     if (mine > 0) put(key_of(0), 0, 0, ring[0]);
@@ -592,8 +609,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     if (t == turns) break;
     turn(t++, ring[0]);
   }
-  if (odd_any && row0 < M)
-    each_unusual<FMT, D>(pg, trow, hkv, lane, max(begin, clear - KB), end, [&](int page, int row, int key) {
+  if (odd_from < odd_to && row0 < M)
+    each_unusual<FMT, D>(pg, trow, hkv, lane, odd_from, odd_to, [&](int page, int row, int key) {
       // (the waves that met the key: the others' m may be -inf)
       if (KW > 1 ? (key - begin) / KB % KW != kw : (key - begin) % KB * sharers / KB != share) return;
       const bool sees = key < s0 || (a.anc ? (bits >> (key - s0)) & 1ull : key - s0 <= qn);
@@ -841,8 +858,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
   for (int t = 0; t < mine; ++t) {
     const int first = key_of(t);
     // ---------------- V to LDS
-    // As in put() above, but that V in bf16 is looked at in every tile: P's lower part is 0 or negative too, which would make
-    // NaN of infinities.
+    // As in put() above.
     bool look = first + 32 > end || cur.there != 3;
     if constexpr (FMT == kPageE4M3) {
       look |= first + 32 > s0;
