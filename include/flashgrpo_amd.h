@@ -328,7 +328,7 @@ int fg_rope_kv_write_paged_parts(const float* part, int splits, const void* bias
 int fg_kv_read_paged(const fg_kv_pages* pages, int batch, const int32_t* start, int count, const int32_t* row_map,
                      void* k_out, void* v_out, int dtype, void* stream);
 
-/* fg_tree_attention over pages (bf16 q and out [batch, num_nodes, q_heads, head_dim]): node n of sequence b attends to tokens
+/* fg_tree_attention over pages (scale positive and finite; bf16 q and out [batch, num_nodes, q_heads, head_dim]): node n of sequence b attends to tokens
  * [0, seq_len[b]) of cache row row_map[b] and to new tokens seq_len[b] + m for every bit m of anc[b * anc_batch_stride + n]
  * (num_nodes <= 64), or, anc NULL, to new tokens 0..n (num_nodes <= 8192). new_len as in fg_rope_kv_write_paged: rows from
  * new_len[b] on are not written, and no row sees their tokens. Tokens without a page are not seen; a row that sees nothing is

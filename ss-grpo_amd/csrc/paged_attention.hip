@@ -42,6 +42,7 @@ struct PagedAttn {
 };
 
 constexpr float kRescaleSlack = 8.0f;  // log2 units
+constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kMinPartKeys = 256;      // a part of a sequence's keys is at least so long
 constexpr int kCUs = 256;
 constexpr int kThreads = 512;          // of a workgroup of the attention kernels; sequences that are put in order
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;
-  const float sl2 = a.scale * 1.44269504088896341f;
+  const float sl2 = a.scale * kLog2e;
 
   const uint32_t k_lane = (uint32_t)(l32 * KROW + g * 16);
   // V^T fragments by transposed reads: lane 16 gq + i addresses key 4 (gq / 2) + i / 4 and d 32 db + 16 (gq % 2) + 4 (i % 4),
@@ -846,7 +847,7 @@ __global__ void __launch_bounds__(kStreamWaves * 64, 2) paged_stream_kernel(Page
 #pragma unroll
     for (int db = 0; db < ND; ++db) o[c][db] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  const float sl2 = a.scale * 1.44269504088896341f;
+  const float sl2 = a.scale * kLog2e;
   // V^T fragments (16 d x 32 keys): lane 16 gq + i addresses key 4 gq + i / 4 (+ 16) and d 16 db + 4 (i % 4), and receives keys
   // 4 gq + j (and 16 + ..) of d = 16 db + i: the keys of S^T's accumulators. Chunks of 16 bytes are swizzled by their key, so that
   // the four keys of a 16-lane read meet different banks.
@@ -1184,6 +1185,8 @@ extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* p
   FG_REQUIRE(!anc || num_nodes <= 64, "fg_paged_attention: num_nodes must be in [1, 64] with masks, [1, 8192] for a chain");
   FG_REQUIRE(sizes_ok(batch, num_nodes, q_heads, pages->kv_heads, pages->head_dim), "fg_paged_attention: bad shape");
   FG_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0, "fg_paged_attention: q must start 16-byte aligned, out 8-byte");
+  // Masked scores are minus infinity before they are scaled, and the largest score has to be the largest scaled one.
+  FG_REQUIRE(scale > 0.0f && scale * kLog2e < INFINITY, "fg_paged_attention: scale must be positive and finite (times log2 e too)");
   a.q = q;
   a.out = out;
   a.seq_len = seq_len;

@@ -1270,7 +1270,7 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
     """``tree_attention`` over pages (``fg_paged_attention``): q bf16 [B, N, Hq, d] contiguous; anc int64 [B, N] or [N] (bits of
     the new tokens that a node sees), or None for a causal chain. ``new_len`` int32 [B]: the rows of nodes from new_len[b] on
     stay as they were in ``out`` (bf16, q's shape, apart from q), and nobody sees their tokens. A row that sees no token is 0, and
-    infinities and NaN of tokens that it does not see do not reach it."""
+    infinities and NaN of tokens that it does not see do not reach it. ``scale``: positive and finite (None: head_dim^-0.5)."""
     _paged_sizes("paged_attention", pages, kv_heads, head_dim)
     dev, shape, at = pages.device, q.shape, q.data_ptr()
     given = out is not None
@@ -1283,7 +1283,7 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
     ok = (q.dtype is _BF16 is out.dtype and shape == (B, num_nodes, q_heads, head_dim) == out.shape and q.is_contiguous()
           and out.is_contiguous() and q.get_device() == dev == out.get_device() and not at & 15 and not into & 7
           and _held(seq_len, dev, B) and (new_len is None or _held(new_len, dev, B)) and (row_map is None or _held(row_map, dev, B))
-          and not (given and at < into + 2 * size and into < at + 2 * size and size))
+          and not (given and at < into + 2 * size and into < at + 2 * size and size) and (scale is None or 0.0 < scale < math.inf))
     if ok and anc is not None:
         if anc.dtype is not torch.int64:
             raise TypeError("anc must be int64 (bit pattern of the uint64 masks)")
@@ -1297,6 +1297,8 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
             raise ValueError(f"{what}: anc must be [{B}, {num_nodes}] or [{num_nodes}] with unit stride on the pages' device")
         if q.dtype is not _BF16 or shape != (B, num_nodes, q_heads, head_dim) or not q.is_contiguous() or at & 15 or q.get_device() != dev:
             raise ValueError(f"{what}: q must be contiguous 16-byte aligned bf16 [B, {num_nodes}, {q_heads}, {head_dim}] on the pages' device")
+        if not (scale is None or 0.0 < scale < math.inf):
+            raise ValueError(f"{what}: scale must be positive and finite")
         raise ValueError(f"{what}: out must be a contiguous 8-byte aligned bf16 tensor of q's shape, apart from it")
     if size == 0:
         return out
