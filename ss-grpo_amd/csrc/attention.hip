@@ -624,6 +624,9 @@ extern "C" int fg_tree_attention(const void* q, void* out, const void* k_cache, 
                    cache_head_stride % 8 == 0 && cache_batch_stride % 8 == 0,
                "fg_tree_attention: 16-byte alignment");
     FG_REQUIRE((int64_t)capacity * kD * 2 < (1ll << 31), "fg_tree_attention: capacity too large");
+    // Masked scores are minus infinity before they are scaled, and the largest score has to be the largest scaled one.
+    FG_REQUIRE(scale > 0.0f && scale * 1.44269504088896341f < INFINITY,
+               "fg_tree_attention: bf16 path: scale must be positive and finite (times log2 e too)");
     const int M = (q_heads / kv_heads) * num_nodes;
     const int splits = attn_splits(batch, num_nodes, q_heads, kv_heads, capacity);
     const bool split = splits > 1 && workspace &&

@@ -328,7 +328,8 @@ def rope_kv_write(qkv, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len
 def tree_attention(q, k_cache, v_cache, *, seq_len, anc, num_nodes, q_heads, kv_heads, head_dim, out=None,
                    row_map=None, scale=None):
     """q [B, N, Hq, d]; caches [Bc, Hkv, S, d]; anc uint64 as int64 [B, N] or [N], or None for a
-    causal chain of new keys (node n sees new keys 0..n)."""
+    causal chain of new keys (node n sees new keys 0..n). scale: of the scores (None: d^-0.5),
+    positive and finite where q is bf16."""
     _dev(q, k_cache, v_cache, seq_len, anc, row_map)
     _i32(seq_len, "seq_len")
     if anc is not None and anc.dtype != torch.int64:
