@@ -23,6 +23,7 @@ Replaces the Hugging Face decoder the reference drives through
 from __future__ import annotations
 
 import math
+import weakref
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -218,7 +219,8 @@ class PagedKVCache(KVCache):
     ``table`` [batch, width] int32 the page of every ``page_size`` tokens of a row, -1 where it has none. ``seq_len`` as in
     ``KVCache``. The page numbers are kept on the host too; ``reserve``, ``release`` and ``repeat_rows`` change them there and
     copy the table to the device, in order with the current stream. ``pages``: how many the pool has (None: enough for every
-    row to fill ``capacity``)."""
+    row to fill ``capacity``). Containers of one storage (``container_copy``) have lengths of their own but one table: a row that
+    one of them releases, or makes a repeat, has the new length in all of them."""
 
     def __init__(self, cfg: TargetConfig, batch: int, capacity: int, *, device, kv_format: str = "e4m3", page_size: int = 64,
                  pages: int | None = None):
@@ -246,6 +248,7 @@ class PagedKVCache(KVCache):
         self._rows = np.full((self.batch, width), -1, np.int32)  # the table, on the host
         self._uses = np.zeros(n, np.int64)                        # rows that hold a page
         self._free = list(range(n - 1, -1, -1))
+        self._sharing = weakref.WeakSet((self,))                  # the containers of these rows
         self._make_views()
 
     def _make_views(self):
@@ -354,12 +357,15 @@ class PagedKVCache(KVCache):
 
     def release(self, rows) -> None:
         """Gives the pages of the given cache rows back (their committed lengths become 0)."""
-        for r in self._checked(rows):
+        rows = self._checked(rows)
+        for r in rows:
             for p in self._rows[r][self._rows[r] >= 0]:
                 self._drop(int(p))
             self._rows[r] = -1
-            self.seq_len[int(r)] = 0
         self._upload()
+        rows = torch.as_tensor(rows, device=self.device)
+        for c in self._sharing:
+            c.seq_len.index_fill_(0, rows, 0)
 
     def gather_path(self, seq_len, acc_nodes, acc_len, tree_nodes, *, row_map=None, err_flag=None):
         K.kv_path_gather_paged(self._layers[0], seq_len=seq_len, acc_nodes=acc_nodes, acc_len=acc_len, tree_nodes=tree_nodes,
@@ -395,8 +401,10 @@ class PagedKVCache(KVCache):
                 copies.append((int(self._rows[s, whole]), int(self._rows[r, whole])))
         self._copy_pages(copies)
         self._upload()
-        self.seq_len.index_copy_(0, torch.as_tensor(dst, device=self.device),
-                                 self.seq_len.index_select(0, torch.as_tensor(src, device=self.device)))
+        src, dst = (torch.as_tensor(x, device=self.device) for x in (src, dst))
+        new = self.seq_len.index_select(0, src)
+        for c in self._sharing:
+            c.seq_len.index_copy_(0, dst, new)
 
     def select_rows(self, rows: torch.Tensor, capacity: int | None = None) -> "PagedKVCache":
         """A new cache, with a pool of its own, holding copies of the given rows' committed tokens (in that order)."""
@@ -418,8 +426,14 @@ class PagedKVCache(KVCache):
         out.seq_len.copy_(torch.from_numpy(lens.astype(np.int32)))
         return out
 
+    def container_copy(self) -> "PagedKVCache":
+        c = super().container_copy()
+        self._sharing.add(c)
+        return c
+
     def deep_copy(self) -> "PagedKVCache":
-        out = self.container_copy()
+        out = super().container_copy()
+        out._sharing = weakref.WeakSet((out,))
         out.codes = (self.codes.view(torch.uint8).clone().view(torch.float8_e4m3fn) if self.kv_format == "e4m3"
                      else self.codes.clone())
         out.scales = None if self.scales is None else self.scales.clone()
