@@ -320,7 +320,8 @@ class PagedKVCache(KVCache):
     def reserve(self, lengths, *, rows=None, first=None) -> None:
         """Gives the cache rows ``rows`` (None: all) pages for their first ``lengths`` tokens. Of the tokens from ``first`` on
         (None: the tokens that get new pages), which the caller is about to write, a page that other rows share is replaced
-        by a copy of it. Raises RuntimeError, with nothing changed, when the pool has too few pages."""
+        by a copy of it. Raises, with nothing changed, RuntimeError when the pool has too few pages, ValueError where committed
+        tokens before ``first`` have none."""
         rows = np.arange(self.batch) if rows is None else self._checked(rows, distinct=True)
         lengths = np.broadcast_to(np.asarray(lengths, np.int64), rows.shape)
         first = None if first is None else np.broadcast_to(np.asarray(first, np.int64), rows.shape)
@@ -328,7 +329,7 @@ class PagedKVCache(KVCache):
             raise ValueError("PagedKVCache: lengths and first must not be negative")
         if (lengths > self.capacity).any():
             raise ValueError(f"PagedKVCache: {int(lengths.max())} tokens exceed the cache capacity {self.capacity}")
-        need, P = [], self.page_size
+        need, early, P = [], [], self.page_size
         uses = self._uses.copy()
         for i, (r, n) in enumerate(zip(rows, lengths)):
             held = self._rows[r]
@@ -341,6 +342,12 @@ class PagedKVCache(KVCache):
                     uses[p] -= 1  # the last row that asks keeps the page itself
             if first is not None:  # tokens before it
                 need += [(r, slot, -1) for slot in range(min(int(first[i]) // P, -(-int(n) // P))) if held[slot] < 0]
+                early += [(r, P * slot) for slot in range(min(-(-int(first[i]) // P), held.size)) if held[slot] < 0]
+        if early:
+            lens = self.seq_len.cpu().numpy()
+            for r, token in early:
+                if token < lens[r]:
+                    raise ValueError(f"PagedKVCache: some of the {lens[r]} committed tokens of row {r} have no page")
         if not need:
             return
         if len(need) > len(self._free):

@@ -63,3 +63,21 @@ def test_containers_are_not_kept():
     assert len(c._sharing) == 1
     c.release([0])
     assert c.seq_len.tolist() == [0, 20, 3]
+
+
+def test_reserve_behind_committed_tokens_without_a_page():
+    """Tokens that are committed but have no page are not given one, which would hold anything: refused, with nothing changed."""
+    c = cache([20, 0, 40])
+    c.seq_len[1] = 20              # never written
+    c._drop(int(c._rows[2, 1]))    # tokens 16 .. 31 lost
+    c._rows[2, 1] = -1
+    before, free = c._rows.copy(), c.free_pages
+    for call in (lambda: c.reserve(24, rows=[1], first=20), lambda: c.reserve([24, 24, 24], first=[20, 20, 40]), lambda: c.reserve(50, rows=[2], first=40),
+                 lambda: c.reserve(50, rows=[2], first=17)):
+        with pytest.raises(ValueError, match="committed tokens of row . have no page"):
+            call()
+        assert (c._rows == before).all() and c.free_pages == free
+    c.reserve(50, rows=[2], first=16)  # what is about to be written needs no page yet
+    c.reserve(24, rows=[1], first=0)
+    c.reserve(30, rows=[0], first=25)  # a gap behind the committed tokens
+    assert holds_its_tokens(c)
