@@ -311,8 +311,8 @@ typedef struct fg_kv_pages {
  * seq_len[b] + n of cache row row_map[b] (NULL: b). new_len (NULL: num_nodes): the tokens of sequence b from new_len[b] on
  * are left out, their q_out rows and slots as they were. A slot without a page is not written and sets err_flag bit 8 (so does
  * a cache row outside the table; q_out is written). bf16 pages and q get fg_rope_kv_write's values, bit for bit. e4m3 pages:
- * q is rotated in fp32 by angles taken in 64 bits and rounded once; K is rotated in 64 bits, and K and V are quantised from there
- * as fg_mx_quantize does it. num_nodes at most 8192, rows 8-byte aligned with a stride ld_qkv that is a multiple of 4.
+ * q is rotated in fp32 by angles taken in 64 bits and rounded once; K is rotated in 64 bits and rounded to fp32, and K and V are
+ * quantised from there as fg_mx_quantize does it. num_nodes at most 8192, rows 8-byte aligned with a stride ld_qkv that is a multiple of 4.
  * Two tokens of one call must not have one slot (cache rows that share a page must not both write to it). */
 int fg_rope_kv_write_paged(const void* qkv, int64_t ld_qkv, int batch, int num_nodes, int q_heads,
                            const fg_kv_pages* pages, const int32_t* seq_len, const int32_t* pos_offset,

@@ -90,10 +90,10 @@ FG_DEVICE uint32_t amax4(const float (&v)[4]) {
 }
 
 // One workgroup per token: position seq_len[b] + pos_offset, slot seq_len[b] + n. bf16 pages get the values of
-// fg_rope_kv_write (every product and sum rounded to bf16, cos and sin too). e4m3 pages: nothing is rounded between the
-// projected row and the codes: q is rotated in fp32 and rounded once; the angles are taken in 64 bits (of an angle of
-// 10^5 radians fp32 keeps 2 decimals), and so is K's rotation (512 elements a token, hidden behind the row's loads), because
-// a code next to a tie follows the last bit.
+// fg_rope_kv_write (every product and sum rounded to bf16, cos and sin too). e4m3 pages: q is rotated in fp32 and rounded once; the
+// angles are taken in 64 bits (of an angle of 10^5 radians fp32 keeps 2 decimals), and so is K's rotation (512 elements a
+// token, hidden behind the row's loads), which is rounded to fp32 and quantised from there: codes are those of the 64-bit
+// definition but where a value is within half an fp32 step of a tie, which it then falls on.
 // Memory bounds it: 2944 tokens at 8B (66 MB) 16 us, 4.2 TB/s of the 4.9 that a large copy reaches; 64 x 29 at 7B (32 MB) 8.8 us;
 // one token 2.7 us, its length, its page and its row one after the other.
 template <int FMT, int D, bool PARTS>

@@ -1202,8 +1202,8 @@ def _write_paged(name, lead, pages, batch, num_nodes, q_heads, head_dim, seq_len
 def rope_kv_write_paged(qkv, pages, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out,
                         new_len=None, row_map=None, err_flag=None):
     """``rope_kv_write`` into pages (``fg_rope_kv_write_paged``): bf16 qkv rows; K and V go to slots seq_len[b] + n of cache
-    row row_map[b], in the pages' format. e4m3 pages: q is rotated in fp32 and rounded once, K and V are quantised from what the
-    formula gives, angles and K in 64 bits; bf16 pages and their q: ``rope_kv_write``'s values. ``new_len`` int32 [batch]:
+    row row_map[b], in the pages' format. e4m3 pages: q is rotated in fp32 and rounded once, K in 64 bits (angles too) and rounded
+    to fp32, from which it is quantised; bf16 pages and their q: ``rope_kv_write``'s values. ``new_len`` int32 [batch]:
     tokens from new_len[b] on are left out (their q_out rows and slots stay as they were). A slot without a page sets
     err_flag bit 8. Cache rows that share a page must not both write to it."""
     _paged_sizes("rope_kv_write_paged", pages, kv_heads, head_dim)
