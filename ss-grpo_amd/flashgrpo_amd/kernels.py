@@ -1062,7 +1062,7 @@ class KVPages:
     makes its block NaN). ``table``: int32 [rows, width]. The tensors are kept and their contents may change."""
 
     __slots__ = ("k", "v", "k_scales", "v_scales", "table", "format", "pages", "page_size", "kv_heads", "head_dim", "rows",
-                 "width", "device", "address", "_c")
+                 "width", "device", "address", "_spans", "_table", "_c")
 
     def __init__(self, k, v, k_scales, v_scales, table):
         fmt = PAGE_FORMATS.get(k.dtype)
@@ -1098,7 +1098,14 @@ class KVPages:
         self.k, self.v, self.k_scales, self.v_scales, self.table = k, v, k_scales, v_scales, table
         self.format, self.pages, self.page_size, self.kv_heads, self.head_dim = fmt, n, size, heads, d
         self.rows, self.width, self.device = rows, width, dev
-        self._c = _lib.KvPages(at, at_v, at_ks, at_vs, table.data_ptr(), first, scale_first or 0, row if rows > 1 else width, fmt, n, size,
+        held = ((n - 1) * first + heads * size * d) * (1 + fmt)
+        self._spans = (at, held), (at_v, held)  # (address, bytes) from the first page to the end of the last
+        if fmt == 0:
+            held = (n - 1) * scale_first + page
+            self._spans += (at_ks, held), (at_vs, held)
+        at_table = table.data_ptr()
+        self._table = at_table, 4 * ((rows - 1) * row + width)
+        self._c = _lib.KvPages(at, at_v, at_ks, at_vs, at_table, first, scale_first or 0, row if rows > 1 else width, fmt, n, size,
                                heads, d, rows, width)
         self.address = C.addressof(self._c)
 
@@ -1191,12 +1198,14 @@ def _write_paged(name, lead, pages, batch, num_nodes, q_heads, head_dim, seq_len
             raise ValueError(f"{what}: inv_freq must be a contiguous fp32 tensor of {head_dim // 2} entries on the pages' device")
         raise ValueError(f"{what}: q_out must be a contiguous 8-byte aligned bf16 [batch * num_nodes, q_heads, d] tensor on the pages' device")
     if size:
-        for a, n in read:
-            if a < at + 2 * size and at < a + n:
-                raise ValueError(f"{name[3:]}: q_out overlaps an operand")
-        _call_on(dev, name, *lead, batch, num_nodes, q_heads, pages.address, seq_len.data_ptr(), pos_offset.data_ptr(), pos_stride,
-                 inv_freq.data_ptr(), None if new_len is None else new_len.data_ptr(), None if row_map is None else row_map.data_ptr(),
-                 at, None if err_flag is None else err_flag.data_ptr())
+        lens, pos, freq, few = seq_len.data_ptr(), pos_offset.data_ptr(), inv_freq.data_ptr(), 4 * batch
+        new, rows = None if new_len is None else new_len.data_ptr(), None if row_map is None else row_map.data_ptr()
+        what, out = name[3:], (at, 2 * size)
+        _apart(what, (out, *pages._spans), read)
+        _apart(what, (out,), (*pages._spans, pages._table, (lens, few), (pos, 4 * (batch * pos_stride or num_nodes)), (freq, 2 * head_dim),
+                              (new or 0, few), (rows or 0, few)))
+        _call_on(dev, name, *lead, batch, num_nodes, q_heads, pages.address, lens, pos, pos_stride, freq, new, rows, at,
+                 None if err_flag is None else err_flag.data_ptr())
 
 
 def rope_kv_write_paged(qkv, pages, *, batch, num_nodes, q_heads, kv_heads, head_dim, seq_len, pos_offset, inv_freq, q_out,
@@ -1270,7 +1279,7 @@ def _paged_workspace_bytes(batch, num_nodes, q_heads, kv_heads, head_dim, capaci
 def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, head_dim, out=None, new_len=None, row_map=None, scale=None):
     """``tree_attention`` over pages (``fg_paged_attention``): q bf16 [B, N, Hq, d] contiguous; anc int64 [B, N] or [N] (bits of
     the new tokens that a node sees), or None for a causal chain. ``new_len`` int32 [B]: the rows of nodes from new_len[b] on
-    stay as they were in ``out`` (bf16, q's shape, apart from q), and nobody sees their tokens. A row that sees no token is 0, and
+    stay as they were in ``out`` (bf16, q's shape, apart from what is read), and nobody sees their tokens. A row that sees no token is 0, and
     infinities and NaN of tokens that it does not see do not reach it. ``scale``: positive and finite (None: head_dim^-0.5)."""
     _paged_sizes("paged_attention", pages, kv_heads, head_dim)
     dev, shape, at = pages.device, q.shape, q.data_ptr()
@@ -1284,7 +1293,7 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
     ok = (q.dtype is _BF16 is out.dtype and shape == (B, num_nodes, q_heads, head_dim) == out.shape and q.is_contiguous()
           and out.is_contiguous() and q.get_device() == dev == out.get_device() and not at & 15 and not into & 7
           and _held(seq_len, dev, B) and (new_len is None or _held(new_len, dev, B)) and (row_map is None or _held(row_map, dev, B))
-          and not (given and at < into + 2 * size and into < at + 2 * size and size) and (scale is None or 0.0 < scale < math.inf))
+          and (scale is None or 0.0 < scale < math.inf))
     if ok and anc is not None:
         if anc.dtype is not torch.int64:
             raise TypeError("anc must be int64 (bit pattern of the uint64 masks)")
@@ -1300,15 +1309,19 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
             raise ValueError(f"{what}: q must be contiguous 16-byte aligned bf16 [B, {num_nodes}, {q_heads}, {head_dim}] on the pages' device")
         if not (scale is None or 0.0 < scale < math.inf):
             raise ValueError(f"{what}: scale must be positive and finite")
-        raise ValueError(f"{what}: out must be a contiguous 8-byte aligned bf16 tensor of q's shape, apart from it")
+        raise ValueError(f"{what}: out must be a contiguous 8-byte aligned bf16 tensor of q's shape")
     if size == 0:
         return out
+    lens, few = seq_len.data_ptr(), 4 * B
+    new, rows = None if new_len is None else new_len.data_ptr(), None if row_map is None else row_map.data_ptr()
+    masks = None if anc is None else anc.data_ptr()
+    if given:
+        _apart("paged_attention", ((into, 2 * size),), (*pages._spans, pages._table, (at, 2 * size), (lens, few), (new or 0, few), (rows or 0, few),
+                                                        (masks or 0, 8 * ((B - 1) * anc_stride + num_nodes))))
     n = _paged_workspace_bytes(B, num_nodes, q_heads, kv_heads, head_dim, pages.width * pages.page_size)
     ws = torch.empty(n, dtype=_U8, device=q.device) if n else None  # the call's own, as in _mx_workspace
-    _call_on(dev, "fg_paged_attention", at, into, pages.address, B, num_nodes, q_heads, seq_len.data_ptr(),
-             None if new_len is None else new_len.data_ptr(), None if row_map is None else row_map.data_ptr(),
-             None if anc is None else anc.data_ptr(), anc_stride, head_dim ** -0.5 if scale is None else scale,
-             None if ws is None else ws.data_ptr(), n)
+    _call_on(dev, "fg_paged_attention", at, into, pages.address, B, num_nodes, q_heads, lens, new, rows, masks, anc_stride,
+             head_dim ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), n)
     return out
 
 
