@@ -1051,20 +1051,13 @@ def mx_plan(rows, cols, k, *, fmt="e4m3", gate_up=False) -> MXPlan:
 PAGE_FORMATS = {torch.float8_e4m3fn: 0, torch.bfloat16: 1}  # struct fg_kv_pages' format
 
 
-class KVPages:
-    """One layer's K and V in pages (struct ``fg_kv_pages``), checked once: token t of cache row r lies in page
-    ``table[r, t // page_size]``, slot ``t % page_size`` (a page number outside [0, pages): no page).
-
-    ``k``, ``v``: bf16 or float8_e4m3fn [pages, kv_heads, page_size, head_dim] views of the same strides, each page
-    contiguous and 16-byte aligned (a pool may hold a page's layers side by side), head_dim 64 or 128, page_size a power of
-    two from 16 on. float8_e4m3fn pages hold MX rows: ``k_scales``, ``v_scales`` uint8 [pages, kv_heads, page_size, head_dim /
-    32], as ``mx_quantize`` makes them but a row's scales side by side (codes 0x7f and 0xff must not occur; a scale of 255
-    makes its block NaN). ``table``: int32 [rows, width]. The tensors are kept and their contents may change."""
+class _Pages:
+    """``KVPages`` until they are filled."""
 
     __slots__ = ("k", "v", "k_scales", "v_scales", "table", "format", "pages", "page_size", "kv_heads", "head_dim", "rows",
                  "width", "device", "address", "_spans", "_table", "_c")
 
-    def __init__(self, k, v, k_scales, v_scales, table):
+    def _fill(self, k, v, k_scales, v_scales, table):
         fmt = PAGE_FORMATS.get(k.dtype)
         shape, stride, dev = k.shape, k.stride(), k.get_device()  # (-1: on the host, which no call takes)
         if fmt is None or v.dtype is not k.dtype or table.dtype is not _I32 or len(shape) != 4 or table.dim() != 2:
@@ -1146,6 +1139,32 @@ class KVPages:
     def capacity(self) -> int:
         """Tokens that a cache row's table has entries for."""
         return self.width * self.page_size
+
+
+class KVPages(_Pages):
+    """One layer's K and V in pages (struct ``fg_kv_pages``), checked once: token t of cache row r lies in page
+    ``table[r, t // page_size]``, slot ``t % page_size`` (a page number outside [0, pages): no page).
+
+    ``k``, ``v``: bf16 or float8_e4m3fn [pages, kv_heads, page_size, head_dim] views of the same strides, each page
+    contiguous and 16-byte aligned (a pool may hold a page's layers side by side), head_dim 64 or 128, page_size a power of
+    two from 16 on. float8_e4m3fn pages hold MX rows: ``k_scales``, ``v_scales`` uint8 [pages, kv_heads, page_size, head_dim /
+    32], as ``mx_quantize`` makes them but a row's scales side by side (codes 0x7f and 0xff must not occur; a scale of 255
+    makes its block NaN). ``table``: int32 [rows, width]. The tensors are kept and their contents may change; the attributes may
+    not."""
+
+    __slots__ = ()
+
+    def __new__(cls, k, v, k_scales, v_scales, table):
+        self = object.__new__(_Pages)
+        self._fill(k, v, k_scales, v_scales, table)
+        self.__class__ = cls  # (from here on its attributes are fixed)
+        return self
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"KVPages are checked once, {name} is fixed: make new ones")
+
+    def __delattr__(self, name):
+        self.__setattr__(name, None)
 
 
 def _page_stride(t, what):
