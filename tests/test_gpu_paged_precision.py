@@ -58,3 +58,12 @@ def test_weights_of_parts_keep_their_bits(group, n):
     held = Held(2, 46, 64, 1, 128, "e4m3", seed=3)
     q = queries(2, n, group, 128, n)
     close(attend(held, q, committed, None), exact_weights(held, q, committed, None, 128 ** -0.5), [n, n])
+
+
+def test_parts_that_the_slots_limit():
+    """A fixed number of parts is shared by the sequences of a call in proportion to their keys: one of 3000 keys is cut into more
+    beside a short sequence than beside one of 2500, which changes the order of its sums (not the bound)."""
+    held = Held(2, 47, 64, 16, 64, "e4m3", seed=5)
+    q = queries(2, 1, 32, 64, 1)
+    for committed in ([3000, 2500], [3000, 10], [3000, 3000], [2990, 1]):
+        close(attend(held, q, committed, None), exact_weights(held, q, committed, None, 64 ** -0.5), [1, 1])
