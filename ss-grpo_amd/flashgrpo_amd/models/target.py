@@ -254,7 +254,8 @@ class PagedKVCache(KVCache):
     def _make_views(self):
         c, s = self.codes, self.scales
         part = lambda l, i: None if s is None else s[:, l, i]
-        self._layers = [K.KVPages(c[:, l, 0], c[:, l, 1], part(l, 0), part(l, 1), self.table) for l in range(self.cfg.num_layers)]
+        table = self.table if self.batch else self.table.new_full((1, self.table.shape[1]), -1)
+        self._layers = [K.KVPages(c[:, l, 0], c[:, l, 1], part(l, 0), part(l, 1), table) for l in range(self.cfg.num_layers)]
 
     @property
     def kv(self) -> torch.Tensor:
@@ -269,10 +270,10 @@ class PagedKVCache(KVCache):
 
     def k(self, layer: int) -> torch.Tensor:
         """The values of K, [batch, Hkv, capacity, d] bf16: a copy, 0 where a row has no page."""
-        return K.kv_read_paged(self._layers[layer], count=self.capacity)[0]
+        return K.kv_read_paged(self._layers[layer], count=self.capacity, batch=self.batch)[0]
 
     def v(self, layer: int) -> torch.Tensor:
-        return K.kv_read_paged(self._layers[layer], count=self.capacity)[1]
+        return K.kv_read_paged(self._layers[layer], count=self.capacity, batch=self.batch)[1]
 
     @property
     def free_pages(self) -> int:

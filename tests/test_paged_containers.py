@@ -81,3 +81,15 @@ def test_reserve_behind_committed_tokens_without_a_page():
     c.reserve(24, rows=[1], first=0)
     c.reserve(30, rows=[0], first=25)  # a gap behind the committed tokens
     assert holds_its_tokens(c)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_no_rows(fmt):
+    """A cache of no rows, as the contiguous one has it: what is left when every sequence has ended."""
+    c = cache([20, 0, 40], kv_format=fmt)
+    none = W.select_cache_batch(c, torch.tensor([], dtype=torch.long))
+    assert none.batch == 0 and none.seq_len.numel() == 0 and tuple(none.table.shape) == (0, 4)
+    none.reserve(16)
+    none.release([])
+    none.repeat_rows(torch.tensor([], dtype=torch.long), torch.tensor([], dtype=torch.long))
+    assert none.select_rows(torch.tensor([], dtype=torch.long)).batch == 0 and none.container_copy().deep_copy().batch == 0
