@@ -1336,8 +1336,9 @@ def forward_tree(causal_lm: TargetModel, ids: torch.Tensor, mask4d: torch.Tensor
     if int(seq.max()) + N > pkv.capacity:
         raise ValueError(f"forward_tree: {N} tree nodes after {int(seq.max())} committed tokens exceed the "
                          f"cache capacity {pkv.capacity}")
-    committed = pkv.seq_len.cpu().numpy()
-    pkv.reserve(committed + N, first=committed)
+    if isinstance(pkv, PagedKVCache):
+        committed = pkv.seq_len.cpu().numpy()
+        pkv.reserve(committed + N, first=committed)
     anc, offset = native_tree_inputs(mask4d, pos, pkv.seq_len)
     tree_cache = pkv.container_copy() if clone_past else pkv
     err = torch.zeros(1, dtype=torch.int32, device=dev)
