@@ -287,8 +287,8 @@ int fg_mx_plan(int gate_up, int rows, int cols, int hidden, int x_format, int pl
  * e4m3, codes of 8 bits (no NaN codes; a NaN block is told by its scale), with scales [kv_heads][page_size][head_dim / 32], bytes,
  * `scale_stride` bytes behind those of the page before (fg_mx_quantize's blocks, a row's scales side by side); 1: bf16. head_dim
  * 64 or 128, page_size a power of two from 16 to 2^20, table_width * page_size less than 2^31 - 65536 tokens per row, a page (one
- * layer's K) less than 2^30 elements, page_stride less than 2^31. Pages 16-byte and scales 4-byte aligned. A host struct of device addresses, read during the call. No counterpart in the reference, whose
- * cache is DynamicCache. */
+ * layer's K) less than 2^30 elements, page_stride less than 2^31. Pages 16-byte and scales 4-byte aligned. A host struct of device
+ * addresses, read during the call. No counterpart in the reference, whose cache is DynamicCache. */
 typedef struct fg_kv_pages {
   void* k;
   void* v;
@@ -335,11 +335,18 @@ int fg_kv_read_paged(const fg_kv_pages* pages, int batch, const int32_t* start, 
  * 0. Infinities and NaN of tokens that a row does not see do not reach it. Scores, softmax sums and O in fp32, the weights
  * in two bf16 parts that hold them but for 2^-18. Where few rows meet many tokens, a sequence's tokens are split over
  * workgroups whose parts are merged by a second launch; that needs workspace >= fg_paged_attention_workspace(...) bytes (capacity:
- * table_width * page_size; 0 when nothing is split), 16-byte aligned and one call's at a time; a null or smaller one runs unsplit. */
+ * table_width * page_size; 0 when nothing is split), 16-byte aligned and one call's at a time; a null or smaller one runs unsplit. Equal
+ * calls give equal bits; where tokens are split, those of a sequence depend on the lengths of the others too (the order of its sums). */
 size_t fg_paged_attention_workspace(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, int capacity);
 int fg_paged_attention(const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes, int q_heads,
                        const int32_t* seq_len, const int32_t* new_len, const int32_t* row_map, const uint64_t* anc,
                        int64_t anc_batch_stride, float scale, void* workspace, size_t workspace_bytes, void* stream);
+/* The same with the weights rounded to bf16 once before they meet V, and their sum that of the rounded ones (as in
+ * fg_tree_attention), where more than 32 rows share a kv head: a fifth to a quarter less time. */
+int fg_paged_attention_bf16_weights(const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes,
+                                    int q_heads, const int32_t* seq_len, const int32_t* new_len,
+                                    const int32_t* row_map, const uint64_t* anc, int64_t anc_batch_stride, float scale,
+                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* fg_kv_path_gather over pages, for `layers` layers in one launch: `pages` describes the first, the others lie layer_stride
  * elements (scale_layer_stride bytes) behind each other. Moves tokens seq_len[b] + acc_nodes[b, j] to seq_len[b] + j for

@@ -17,6 +17,7 @@ using fg::kPageE4M3;
 using fg::Pages;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -43,7 +44,7 @@ struct PagedAttn {
 
 constexpr float kRescaleSlack = 8.0f;  // log2 units
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr int kMinPartKeys = 256;      // a part of a sequence's keys is at least so long
+constexpr int kMinPartKeys = 256;      // a sequence has at most one part for each so many keys that it begins
 constexpr int kCUs = 256;
 constexpr int kThreads = 512;          // of a workgroup of the attention kernels; sequences that are put in order
 constexpr int kMaxCut = 64;            // sequences that are cut: a lane each
@@ -108,8 +109,9 @@ FG_DEVICE T scan_add(T x) {
 }
 
 // Which part of which sequence is slot idx, from lengths that only the device knows. A sequence of k keys gets
-// 1 + floor((k - 1) f) parts of equal length, f the same for all: as large as the slots allow (all of them over all keys, else
-// five steps of bisection down to slots - batch, with which the parts always fit). Every wave works that out for itself, a lane a sequence;
+// 1 + floor((k - 1) f) parts of equal length, f the same for all: 1 / kMinPartKeys, or as large as the slots allow (all of them
+// over all keys, else five steps of bisection down to slots - batch, with which the parts always fit). So the order of a sequence's
+// sums follows from the other sequences' lengths too, where the slots do not suffice. Every wave works that out for itself, a lane a sequence;
 // the first workgroup leaves the shares for the kernel that joins the parts. (A token over 65536 keys beside seven over 1000,
 // at 8B: 44 us, with the same number of parts for each sequence 102; 3 verify rounds of 29 over 1096 to 4096 at 14B: 31 and 40.
 // What it costs: 0.3 us of 9.6 for a few tokens over short lengths.)
@@ -261,7 +263,7 @@ FG_DEVICE float v_element(const Pages& pg, int page, int r, int d) {
 }
 
 // Infinities and NaN of V. The loops keep them at 0 where not every row sees them (the new tokens' tiles), since p = 0 times
-// them would be NaN, and in bf16 everywhere, since P's lower part, which is 0 or negative too, would make NaN of infinities.
+// them would be NaN, and in bf16 everywhere where P has a lower part, which is 0 or negative too and would make NaN of infinities.
 // Here, once, they are added for the rows that see them: p > 0 times an infinity or a NaN is that. `add(page, row, token)` is
 // called for each such token in [from, end).
 template <int FMT, int D, typename F>
@@ -290,14 +292,16 @@ FG_DEVICE void wave_barrier() {  // a wave's LDS operations are done in order; t
 // tokens, which lie in one page, so that pages are looked up by the scalar unit. Codes are expanded to bf16 (exactly) on their
 // way to one of two LDS stages, while the tile in the other is multiplied; one barrier per tile. S^T = K Q^T puts a query into
 // a lane: the softmax needs one exchange with the other half-wave, and P^T goes from the accumulators straight into O^T += V^T
-// P^T, in two bf16 parts (hi + lo, p but for 2^-18 of it), so that the products with V are made twice and nothing but the output's
-// own rounding is left: 1.7e-3 from 64 bits, where one part leaves 2.3e-3. The groups merge their (m, l, O) at the end through LDS,
-// the parts by a second kernel.
+// P^T. The groups merge their (m, l, O) at the end through LDS, the parts of the keys by a second kernel.
+//
+// PARTS 2: P in two bf16 parts (hi + lo, p but for 2^-18 of it), so that the products with V are made twice and nothing but the
+// output's own rounding is left, 1.7e-3 from 64 bits. 1, for callers who ask for it: rounded to bf16 once (2^-9 of each weight in the
+// mean, the error of the bf16 output again: 2.3e-3), the sum that of the rounded weights, as in the contiguous cache's attention.
 //
 // What bounds it: products, reads of fragments, exponentials and expansion, which a SIMD's two waves overlap in part. 64 rounds
-// of 29 nodes over 2048 keys at 7B (203 of 256 rows) take 93 us; the products of the padded rows, V's twice, would take 86 at the
-// 1215 TFLOP/s of a large product. 4 x 1024 tokens at 8B: 122 us. With one part of P: 74 and 100, of which the first were
-// 67 without fetching and expanding, 63 without the barrier too, 57 without reading the fragments.
+// of 29 nodes over 2048 keys at 7B (203 of 256 rows) take 93 us with two parts, 74 with one; the products of the padded rows alone
+// would take 86 and 57 at the 1215 TFLOP/s of a large product. Of the 74, 67 are left without fetching and expanding, 63 without
+// the barrier too, 57 without reading the fragments. 4 x 1024 tokens at 8B: 122 and 100 us.
 // Slower, with one part: two workgroups of four waves per CU (85 us), halves of the waves a phase apart (83), 32-key steps with the next
 // fragments read ahead (81), tiles of 128 keys (87); 3 or 4 tiles in flight took the same. With two: all of P before V (93 to 97),
 // 16 keys at a time (95).
@@ -306,7 +310,7 @@ FG_DEVICE void wave_barrier() {  // a wave's LDS operations are done in order; t
 // Two waves take 32 keys each of every tile for such a block instead, and join their results at the end (32 verify rounds of 29
 // over 3096 to 4096 keys at 14B, 145 rows, with one part of P: 124 -> 116 us, on bf16 pages 128 -> 124). Steps of 32 keys cost rows
 // that are not shared 2 to 5 % (203 rows 77.3 -> 79.3, 4 x 1024 tokens 101 -> 106).
-template <int FMT, int D, int RW, int KW, int KB, bool SHARED>
+template <int FMT, int D, int RW, int KW, int KB, bool SHARED, int PARTS>
 __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a, int m_tiles) {
   constexpr int T = RW * 64, ROWS = RW * 32;
   constexpr int CPK = D * fg::page_elem_bytes<FMT> / 16;  // 16-byte pieces of a K or V row
@@ -435,8 +439,8 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       v_lane[db] = (uint32_t)(KB * KROW + key * VROW + (((4 * db + low) ^ v_swizzle(key)) * 16) + 8 * (i & 1));
   }
 
-  // V is 0 behind the part's end and without a page and, in the tiles that reach the new tokens (bf16: in all), where it is not
-  // finite; K's rows there may be anything, their scores are masked.
+  // V is 0 behind the part's end and without a page and, in the tiles that reach the new tokens (bf16 and two parts of P: in all),
+  // where it is not finite; K's rows there may be anything, their scores are masked.
   uint32_t k_put[NU], v_put[NU];  // where this thread's pieces go
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   auto put = [&](int key0, int buf, int slot, Loads& x) __attribute__((always_inline)) {
     unsigned char* const at = group + buf * TILE;
     bool look = key0 + KB > end || x.paged != (1u << NU) - 1u;  // the last tiles, and the rare ones
-    if constexpr (FMT == kPageE4M3) {
+    if constexpr (FMT == kPageE4M3 || PARTS == 1) {
       look |= key0 + KB > clear;
     } else {
       uint32_t most = 0;
@@ -462,7 +466,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       for (int u = 0; u < NU; ++u) {
         const int j0 = (u * RW + rw) * KPW;
         const bool ok = ((x.paged >> u) & 1u) && key0 + j0 + lane / CPK < end;
-        const bool bad = ok && (FMT == kPageE4M3 ? key0 + KB > clear && x.vsc[u] == 255u : not_finite(x.vp[u]));
+        const bool bad = ok && (key0 + KB > clear || (FMT == kPageBF16 && PARTS == 2)) && (FMT == kPageE4M3 ? x.vsc[u] == 255u : not_finite(x.vp[u]));
         odd |= bad;
         if (!((x.paged >> u) & 1u)) gone |= low_bits(KPW) << j0;
         if (bad || !ok) x.vp[u] = FMT == kPageE4M3 || !ok ? u32x4(0) : finite_part(x.vp[u]);  // (e4m3: all of a block's 32)
@@ -545,33 +549,64 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
       m_run = m_new;
     }
     const float m_sub = m_run == -INFINITY ? 0.0f : m_run;
+    if constexpr (PARTS == 2) {
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
-      bf16x8 hi[2], lo[2];  // p = hi + lo but for 2^-18 of it
+      for (int kb = 0; kb < NB; ++kb) {
+        bf16x8 hi[2], lo[2];  // p = hi + lo but for 2^-18 of it
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        uint32_t ph[4], pl[4];
+        for (int ks = 0; ks < 2; ++ks) {
+          uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + 2 * j], sl2, -m_sub));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + 2 * j + 1], sl2, -m_sub));
-          l_run += p0 + p1;
-          ph[j] = fg::pack_bf16x2(p0, p1);
-          pl[j] = fg::pack_bf16x2(p0 - __uint_as_float(ph[j] << 16), p1 - __uint_as_float(ph[j] & 0xffff0000u));
+          for (int j = 0; j < 4; ++j) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + 2 * j], sl2, -m_sub));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + 2 * j + 1], sl2, -m_sub));
+            l_run += p0 + p1;
+            ph[j] = fg::pack_bf16x2(p0, p1);
+            pl[j] = fg::pack_bf16x2(p0 - __uint_as_float(ph[j] << 16), p1 - __uint_as_float(ph[j] & 0xffff0000u));
+          }
+          hi[ks] = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
+          lo[ks] = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
         }
-        hi[ks] = __builtin_bit_cast(bf16x8, u32x4{ph[0], ph[1], ph[2], ph[3]});
-        lo[ks] = __builtin_bit_cast(bf16x8, u32x4{pl[0], pl[1], pl[2], pl[3]});
-      }
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int db = 0; db < ND; ++db) {
+            const unsigned char* p0 = v_base + v_lane[db] + (2 * kb + ks) * 16 * VROW;
+            const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
+            const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, hi[ks], o[db], 0, 0, 0);
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo[ks], o[db], 0, 0, 0);
+          }
+      }
+    } else {
+      float psum = l_run;
+      bf16x8 pf[NB][2];
+      const bf16x2 ones2 = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          uint32_t packed[4];
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j], sl2, -m_sub));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][ks * 8 + j + 1], sl2, -m_sub));
+            packed[j / 2] = fg::pack_bf16x2(p0, p1);
+            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, packed[j / 2]), ones2, psum, false);
+          }
+          pf[kb][ks] = __builtin_bit_cast(bf16x8, u32x4{packed[0], packed[1], packed[2], packed[3]});
+        }
+      l_run = psum;
+#pragma unroll
+      for (int ks = 0; ks < 2 * NB; ++ks)
 #pragma unroll
         for (int db = 0; db < ND; ++db) {
-          const unsigned char* p0 = v_base + v_lane[db] + (2 * kb + ks) * 16 * VROW;
+          const unsigned char* p0 = v_base + v_lane[db] + ks * 16 * VROW;
           const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p0);
           const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p0 + 8 * VROW));
           const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, hi[ks], o[db], 0, 0, 0);
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo[ks], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[ks >> 1][ks & 1], o[db], 0, 0, 0);
         }
     }
   };
@@ -1122,8 +1157,8 @@ Plan plan_of(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim, 
   const int64_t each = kv_heads * ((m + p.rows() - 1) / p.rows());  // workgroups of a sequence that is not cut
   // Parts where every sequence gets two at least (20 tokens over 2048 keys at 8B, 160 workgroups: whole 19.5 us, in 320 parts 28),
   // and no more workgroups than CUs, which would take two rounds (3 over 8192: 264 workgroups 22.5 us, 256 17.6). Few rows stay
-  // whole in short caches, where the second launch costs more (one over 600 keys at 8B: 8.2 us whole, 10.5 in parts; 4 over 1000
-  // at most: 11.4 and 10.3).
+  // whole in caches whose table is short, where the second launch costs more (one over 600 keys at 8B: 8.2 us whole, 10.5 in parts; 4
+  // over 1000 at most: 11.4 and 10.3). Lengths are on the device: as few keys in a wide table are cut.
   if (batch <= kMaxCut && 2 * batch * each <= kCUs && (m > 32 || capacity >= 1024)) {
     const int64_t most = std::max<int64_t>(1, capacity / kMinPartKeys);
     p.slots = (int)std::min<int64_t>(kCUs / each, batch * most);
@@ -1136,7 +1171,7 @@ int64_t workspace_of(const Plan& p, int batch, int num_nodes, int q_heads, int h
   return p.slots ? (int64_t)p.slots * num_nodes * q_heads * (head_dim * 4 + 8) + batch * 8ll : 0;
 }
 
-template <int FMT, int D>
+template <int FMT, int D, int PARTS>
 void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   const int64_t m = (int64_t)(a.Hq / a.pages.kv_heads) * a.N;
   const int m_tiles = (int)((m + p.rows() - 1) / p.rows());
@@ -1146,13 +1181,13 @@ void launch(const PagedAttn& a, const Plan& p, hipStream_t s) {
   else if (m <= 32)
     hipLaunchKernelGGL((paged_stream_kernel<FMT, D, 2>), grid, block, 0, s, a);
   else if (p.rw == 2)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 4, 32, false>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, 4, 32, false, PARTS>), grid, block, 0, s, a, m_tiles);
   else if (D == 64 || p.rw == 4)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 2, 64, false>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, 2, 64, false, PARTS>), grid, block, 0, s, a, m_tiles);
   else if (m <= 192)
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, true>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, true, PARTS>), grid, block, 0, s, a, m_tiles);
   else
-    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, false>), grid, block, 0, s, a, m_tiles);
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, 128, 8, 1, 64, false, PARTS>), grid, block, 0, s, a, m_tiles);
   if (a.slots) {
     const int64_t rows = (int64_t)a.batch * a.N * a.Hq;
     if (p.wide(a.batch, rows))
@@ -1167,26 +1202,19 @@ bool sizes_ok(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim)
          (head_dim == 64 || head_dim == 128) && (int64_t)batch * num_nodes < (1ll << 31) / q_heads;
 }
 
-}  // namespace
-
-extern "C" size_t fg_paged_attention_workspace(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim,
-                                               int capacity) {
-  if (!sizes_ok(batch, num_nodes, q_heads, kv_heads, head_dim) || capacity <= 0) return 0;
-  return (size_t)workspace_of(plan_of(batch, num_nodes, q_heads, kv_heads, head_dim, capacity), batch, num_nodes, q_heads, head_dim);
-}
-
-extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes,
-                                  int q_heads, const int32_t* seq_len, const int32_t* new_len, const int32_t* row_map,
-                                  const uint64_t* anc, int64_t anc_batch_stride, float scale, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+template <int PARTS>
+int attend(const char* what, const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes, int q_heads,
+           const int32_t* seq_len, const int32_t* new_len, const int32_t* row_map, const uint64_t* anc,
+           int64_t anc_batch_stride, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const std::string w(what);
   PagedAttn a;
-  if (int rc = fg::pages_of(pages, "fg_paged_attention", a.pages)) return rc;
-  FG_REQUIRE(q && out && seq_len, "fg_paged_attention: null pointer");
-  FG_REQUIRE(!anc || num_nodes <= 64, "fg_paged_attention: num_nodes must be in [1, 64] with masks, [1, 8192] for a chain");
-  FG_REQUIRE(sizes_ok(batch, num_nodes, q_heads, pages->kv_heads, pages->head_dim), "fg_paged_attention: bad shape");
-  FG_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0, "fg_paged_attention: q must start 16-byte aligned, out 8-byte");
+  if (int rc = fg::pages_of(pages, what, a.pages)) return rc;
+  FG_REQUIRE(q && out && seq_len, w + ": null pointer");
+  FG_REQUIRE(!anc || num_nodes <= 64, w + ": num_nodes must be in [1, 64] with masks, [1, 8192] for a chain");
+  FG_REQUIRE(sizes_ok(batch, num_nodes, q_heads, pages->kv_heads, pages->head_dim), w + ": bad shape");
+  FG_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 7) == 0, w + ": q must start 16-byte aligned, out 8-byte");
   // Masked scores are minus infinity before they are scaled, and the largest score has to be the largest scaled one.
-  FG_REQUIRE(scale > 0.0f && scale * kLog2e < INFINITY, "fg_paged_attention: scale must be positive and finite (times log2 e too)");
+  FG_REQUIRE(scale > 0.0f && scale * kLog2e < INFINITY, w + ": scale must be positive and finite (times log2 e too)");
   a.q = q;
   a.out = out;
   a.seq_len = seq_len;
@@ -1203,7 +1231,7 @@ extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* p
   if (need && (!workspace || workspace_bytes < (size_t)need || ((uintptr_t)workspace & 15))) p.slots = 0;
   const int64_t m = (int64_t)(q_heads / pages->kv_heads) * num_nodes;
   FG_REQUIRE((int64_t)batch * pages->kv_heads * ((m + p.rows() - 1) / p.rows()) < (1ll << 31),
-             "fg_paged_attention: bad shape (too many workgroups)");
+             w + ": bad shape (too many workgroups)");
   a.slots = p.slots;
   a.most = p.wide(batch, (int64_t)batch * num_nodes * q_heads) ? 256 : pages->head_dim / 4;
   a.o_part = (float*)workspace;
@@ -1211,8 +1239,33 @@ extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* p
   a.shares = (int2*)(a.ml_part + (int64_t)p.slots * num_nodes * q_heads);
   hipStream_t s = (hipStream_t)stream;
   if (pages->format == kPageE4M3)
-    pages->head_dim == 128 ? launch<kPageE4M3, 128>(a, p, s) : launch<kPageE4M3, 64>(a, p, s);
+    pages->head_dim == 128 ? launch<kPageE4M3, 128, PARTS>(a, p, s) : launch<kPageE4M3, 64, PARTS>(a, p, s);
   else
-    pages->head_dim == 128 ? launch<kPageBF16, 128>(a, p, s) : launch<kPageBF16, 64>(a, p, s);
-  return fg::check_launch("fg_paged_attention");
+    pages->head_dim == 128 ? launch<kPageBF16, 128, PARTS>(a, p, s) : launch<kPageBF16, 64, PARTS>(a, p, s);
+  return fg::check_launch(what);
+}
+
+}  // namespace
+
+extern "C" size_t fg_paged_attention_workspace(int batch, int num_nodes, int q_heads, int kv_heads, int head_dim,
+                                               int capacity) {
+  if (!sizes_ok(batch, num_nodes, q_heads, kv_heads, head_dim) || capacity <= 0) return 0;
+  return (size_t)workspace_of(plan_of(batch, num_nodes, q_heads, kv_heads, head_dim, capacity), batch, num_nodes, q_heads, head_dim);
+}
+
+extern "C" int fg_paged_attention(const void* q, void* out, const fg_kv_pages* pages, int batch, int num_nodes,
+                                  int q_heads, const int32_t* seq_len, const int32_t* new_len,
+                                  const int32_t* row_map, const uint64_t* anc, int64_t anc_batch_stride,
+                                  float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  return attend<2>("fg_paged_attention", q, out, pages, batch, num_nodes, q_heads, seq_len, new_len, row_map, anc,
+                   anc_batch_stride, scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" int fg_paged_attention_bf16_weights(const void* q, void* out, const fg_kv_pages* pages, int batch,
+                                               int num_nodes, int q_heads, const int32_t* seq_len,
+                                               const int32_t* new_len, const int32_t* row_map,
+                                               const uint64_t* anc, int64_t anc_batch_stride, float scale,
+                                               void* workspace, size_t workspace_bytes, void* stream) {
+  return attend<1>("fg_paged_attention_bf16_weights", q, out, pages, batch, num_nodes, q_heads, seq_len, new_len, row_map,
+                   anc, anc_batch_stride, scale, workspace, workspace_bytes, stream);
 }

@@ -77,6 +77,7 @@ SIGNATURES = {
     "fg_kv_read_paged": (_I, [_P, _I, _P, _I, _P, _P, _P, _I, _P]),
     "fg_paged_attention_workspace": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "fg_paged_attention": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I64, _F, _P, _SZ, _P]),
+    "fg_paged_attention_bf16_weights": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I64, _F, _P, _SZ, _P]),
     "fg_kv_path_gather_paged": (_I, [_P, _I, _I64, _I64, _I, _P, _P, _P, _I, _P, _I, _P, _P]),
     "fg_sample_workspace": (_SZ, [_I]),
     "fg_sample_tokens": (_I, [_P, _I, _I64, _I, _I, _P, _P, _P, _I, _I, _U64, _U64, _P, _I, _F, _I, _I, _U32, _P,

@@ -1295,11 +1295,14 @@ def _paged_workspace_bytes(batch, num_nodes, q_heads, kv_heads, head_dim, capaci
     return _lib.load().fg_paged_attention_workspace(batch, num_nodes, q_heads, kv_heads, head_dim, capacity)
 
 
-def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, head_dim, out=None, new_len=None, row_map=None, scale=None):
+def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, head_dim, out=None, new_len=None, row_map=None, scale=None,
+                    bf16_weights=False):
     """``tree_attention`` over pages (``fg_paged_attention``): q bf16 [B, N, Hq, d] contiguous; anc int64 [B, N] or [N] (bits of
     the new tokens that a node sees), or None for a causal chain. ``new_len`` int32 [B]: the rows of nodes from new_len[b] on
     stay as they were in ``out`` (bf16, q's shape, apart from what is read), and nobody sees their tokens. A row that sees no token is 0, and
-    infinities and NaN of tokens that it does not see do not reach it. ``scale``: positive and finite (None: head_dim^-0.5)."""
+    infinities and NaN of tokens that it does not see do not reach it. ``scale``: positive and finite (None: head_dim^-0.5).
+    ``bf16_weights``: the softmax's weights may be rounded to bf16, as ``tree_attention`` rounds them
+    (``fg_paged_attention_bf16_weights``: faster where more than 32 rows share a kv head); otherwise they keep 17 bits."""
     _paged_sizes("paged_attention", pages, kv_heads, head_dim)
     dev, shape, at = pages.device, q.shape, q.data_ptr()
     given = out is not None
@@ -1339,8 +1342,8 @@ def paged_attention(q, pages, *, seq_len, anc, num_nodes, q_heads, kv_heads, hea
                                                         (masks or 0, 8 * ((B - 1) * anc_stride + num_nodes))))
     n = _paged_workspace_bytes(B, num_nodes, q_heads, kv_heads, head_dim, pages.width * pages.page_size)
     ws = torch.empty(n, dtype=_U8, device=q.device) if n else None  # the call's own, as in _mx_workspace
-    _call_on(dev, "fg_paged_attention", at, into, pages.address, B, num_nodes, q_heads, lens, new, rows, masks, anc_stride,
-             head_dim ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), n)
+    _call_on(dev, "fg_paged_attention_bf16_weights" if bf16_weights else "fg_paged_attention", at, into, pages.address, B, num_nodes, q_heads,
+             lens, new, rows, masks, anc_stride, head_dim ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), n)
     return out
 
 
