@@ -645,8 +645,9 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
     if (t == turns) break;
     turn(t++, ring[0]);
   }
-  if (odd_from < odd_to && row0 < M)
-    each_unusual<FMT, D>(pg, trow, hkv, lane, odd_from, odd_to, [&](int page, int row, int key) {
+  const int unusual = scalar(odd_from), until = scalar(odd_to);
+  if (unusual < until && row0 < M)
+    each_unusual<FMT, D>(pg, trow, hkv, lane, unusual, until, [&](int page, int row, int key) {
       // (the waves that met the key: the others' m may be -inf)
       if (KW > 1 ? (key - begin) / KB % KW != kw : (key - begin) % KB * sharers / KB != share) return;
       const bool sees = key < s0 || (a.anc ? (bits >> (key - s0)) & 1ull : key - s0 <= qn);
