@@ -4,7 +4,8 @@
 //
 //   out[q] = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q . k_j - m),  m the running maximum, one pass over the keys
 //
-// A row that sees no key is 0. The G = q heads / kv heads rows of a node share every K and V row that is read.
+// A row that sees no key is 0. The G = q heads / kv heads rows of a node share every K and V row that is read. Times of more than 32
+// rows of a kv head are those of one bf16 part of P, unless two are named (paged_attn_kernel).
 #include "fg_paged.h"
 
 #include <algorithm>
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(RW * KW * 64, 2) paged_attn_kernel(PagedAttn a
   int unit = blockIdx.x / m_tiles, mt = blockIdx.x % m_tiles;
   if (gridDim.x > kCUs) {
     // The row tiles of a unit on one XCD (workgroups go to the eight in turn), those with the most keys first: 4 x 1024 tokens
-    // 110.5 -> 105 us, on bf16 pages 136 -> 129.5, 8 x 512 at 7B's heads 225 -> 214.
+    // 110.5 -> 105 us, 8 x 512 at 7B's heads 225 -> 214.
     const int whole = gridDim.x / m_tiles & ~7u, turn = blockIdx.x / 8;
     if ((int)(blockIdx.x / m_tiles) < whole) unit = turn / m_tiles * 8 + blockIdx.x % 8, mt = turn % m_tiles;
     mt = m_tiles - 1 - mt;

@@ -142,7 +142,7 @@ class FlashMedusaConfig:
     graph_verify_forward: bool = True
     # The rollout's KV cache: "contiguous"; "paged": bf16 pages, a prompt's shared by its repeats; "paged_e4m3": 8-bit pages,
     # quantised as they are written (bf16 models with heads of 64 or 128; the rollout then samples from the model with that
-    # cache, exactly).
+    # cache, exactly). Pages for the whole length are taken when a rollout starts.
     kv_cache: str = "contiguous"
     kv_page_size: int = 64
     # tree_layout="sparse_asymmetric" (flashgrpo_b200/decoding/flash_medusa_decoder.py:65-73);
