@@ -1166,6 +1166,9 @@ class KVPages(_Pages):
     def __delattr__(self, name):
         self.__setattr__(name, None)
 
+    def __copy__(self):
+        return self
+
 
 def _page_stride(t, what):
     """Elements between pages of a [pages, heads, size, n] view whose pages are contiguous."""

@@ -330,7 +330,14 @@ class PagedKVCache(KVCache):
             raise ValueError("PagedKVCache: lengths and first must not be negative")
         if (lengths > self.capacity).any():
             raise ValueError(f"PagedKVCache: {int(lengths.max())} tokens exceed the cache capacity {self.capacity}")
-        need, early, P = [], [], self.page_size
+        need, P = [], self.page_size
+        if first is not None:
+            gone = (self._rows[rows] < 0) & (np.arange(self._rows.shape[1]) < -(-first // P)[:, None])
+            if gone.any():
+                lens = self.seq_len.cpu().numpy()[rows]
+                lost = gone.any(1) & (gone.argmax(1) * P < lens)
+                if lost.any():
+                    raise ValueError(f"PagedKVCache: some of the {lens[lost][0]} committed tokens of row {rows[lost][0]} have no page")
         uses = self._uses.copy()
         for i, (r, n) in enumerate(zip(rows, lengths)):
             held = self._rows[r]
@@ -341,14 +348,8 @@ class PagedKVCache(KVCache):
                 elif first is not None and uses[p] > 1:
                     need.append((r, slot, int(p)))
                     uses[p] -= 1  # the last row that asks keeps the page itself
-            if first is not None:  # tokens before it
+            if first is not None and gone[i].any():  # tokens before it
                 need += [(r, slot, -1) for slot in range(min(int(first[i]) // P, -(-int(n) // P))) if held[slot] < 0]
-                early += [(r, P * slot) for slot in range(min(-(-int(first[i]) // P), held.size)) if held[slot] < 0]
-        if early:
-            lens = self.seq_len.cpu().numpy()
-            for r, token in early:
-                if token < lens[r]:
-                    raise ValueError(f"PagedKVCache: some of the {lens[r]} committed tokens of row {r} have no page")
         if not need:
             return
         if len(need) > len(self._free):

@@ -41,3 +41,10 @@ def test_keywords_and_refusals_as_before():
         K.KVPages(p.k, p.v, None, None, table)
     with pytest.raises(TypeError):
         K.KVPages(p.k, p.v, table)
+
+
+def test_copies_are_the_same():
+    import copy
+
+    p, _ = made()
+    assert copy.copy(p) is p
